@@ -1,8 +1,9 @@
 /*
  * mi355_fused.h -- C ABI of the MI355X (gfx950) fused RMSNorm and SiLU-and-mul
  * kernels, the fused gate/up projections, the weight-only int8 (W8A16)
- * linear with its quantiser, and the 16-bit linear of the MLP's down
- * projection.
+ * linear with its quantiser, the 16-bit linear of the MLP's down projection,
+ * and what lies between an attention block's projections: rotary positions, a
+ * paged and quantised key/value cache, and attention over it.
  *
  * The reference has no FFI: its boundary is a pair of Python launchers that
  * hand torch tensors to Triton kernels.  Each entry point below replaces one of
@@ -296,6 +297,145 @@ int mi355_linear16_ws_fwd(const void* x, const void* weight, const void* bias, v
                           int dtype, int bias_dtype, int out_dtype,
                           void* workspace, int64_t workspace_bytes,
                           void* stream);
+
+/*
+ * Rotary positions of x [batch, tokens, heads, head_dim].  With R = rotary_dim
+ * and, for token (b, t) and pair j < R / 2,
+ *   a = positions[b, t] * inv_freq[j],  c = scale cos a,  s = scale sin a:
+ *   y0 = x0 c - x1 s,  y1 = x1 c + x0 s         (fp32, rounded once)
+ * for the pairs (x[j], x[j + R / 2]) (interleaved = 0, the layout of Qwen2 and
+ * Llama) or (x[2j], x[2j + 1]) (interleaved = 1); elements from R on are
+ * copied.  Angles are formed and reduced in 64 bits, so far positions lose
+ * nothing.  Longer contexts are a matter of inv_freq and scale.
+ *
+ *   x          dtype (fp32, fp16, bf16); strides in elements, head_dim
+ *              contiguous; any strides >= 0 and any alignment.
+ *   y          [batch, tokens, heads, head_dim] of dtype, contiguous; must not
+ *              overlap x.
+ *   positions  int64 by two strides (0 for one row of positions for all).
+ *   inv_freq   fp32 [R / 2]; R even, 0 <= R <= head_dim, R <= 256.
+ *   batch * tokens < 2^24, heads <= 65535, head_dim < 2^20
+ *   (MI355_ERR_UNSUPPORTED beyond).  Nothing to do for 0 elements.
+ */
+int mi355_rotary_fwd(const void* x, void* y, const int64_t* positions, const float* inv_freq,
+                     int64_t batch, int64_t tokens, int64_t heads, int64_t head_dim, int64_t rotary_dim,
+                     int64_t x_stride_b, int64_t x_stride_t, int64_t x_stride_h,
+                     int64_t pos_stride_b, int64_t pos_stride_t,
+                     float scale, int interleaved, int dtype, void* stream);
+
+/* Element formats of a key/value cache. */
+enum mi355_kv_format {
+  MI355_KV_16BIT = 0, /* values of the call's dtype, no scales */
+  MI355_KV_INT8 = 1,  /* int8 codes with a scale per token and head: value = code * scale */
+  MI355_KV_E4M3 = 2   /* 8-bit floats (4 exponent, 3 mantissa bits, largest 448), likewise */
+};
+
+/*
+ * A paged key/value cache.  The token in slot s of sequence b lies on page
+ * page_table[b * table_stride + s / page_size] at place s % page_size.  One
+ * page per sequence makes a static cache.  The library keeps nothing of the
+ * struct after a call.
+ *
+ * page_table and the lengths that calls take are device memory: their values
+ * are checked by the kernels.  A slot beyond the table, or on a page number
+ * outside [0, pages), has no place: it is not written, reads as zero and is
+ * not attended to.  A slot that two sequences share is theirs to keep whole.
+ */
+typedef struct mi355_kv_cache {
+  void* k;                   /* [pages, kv_heads, page_size, head_dim], contiguous, 16-byte aligned */
+  void* v;                   /* the same */
+  float* k_scale;            /* [pages, kv_heads, page_size], 16-byte aligned; NULL for 16-bit values */
+  float* v_scale;            /* the same */
+  const int32_t* page_table; /* [batch, table_stride], table_width of them in use */
+  int64_t table_stride;
+  int64_t table_width;       /* table_width * page_size < 2^31 - 256 */
+  int64_t pages;             /* < 2^31 */
+  int64_t kv_heads;          /* 1 .. 65535 */
+  int64_t page_size;         /* a multiple of 16 */
+  int64_t head_dim;          /* a multiple of 16, at most 256 */
+  int format;                /* enum mi355_kv_format */
+} mi355_kv_cache;
+
+/*
+ * Writes the keys and values of `tokens` new tokens per sequence into slots
+ * seq_lens[b] + t, rotating the keys (and queries, if given) on the way:
+ *   kr = rotary(k) (as mi355_rotary_fwd, kept in fp32)
+ *   scale = max(max|row| / top, 1e-8), code = round(row / scale)   per token and head,
+ * top = 127 (int8, ties to even) or 448 (e4m3); 16-bit caches round once.  A
+ * row that holds an infinity or a NaN reads back as NaN.  Tokens from
+ * new_lens[b] on (NULL: none) are padding and not written; their queries are
+ * rotated all the same.
+ *
+ *   k, v      [batch, tokens, kv_heads, head_dim] of dtype (fp16, bf16) by
+ *             three strides each (strides[0..2] of k: batch, token, head;
+ *             [3..5] of v; [6..8] of q), head_dim contiguous, rows 16-byte
+ *             aligned.
+ *   q, q_out  [batch, tokens, q_heads, head_dim] likewise, q_out contiguous;
+ *             both NULL (q_heads = 0) to rotate no queries.
+ *   inv_freq  NULL (rotary_dim = 0): nothing is rotated, positions is not read.
+ *   batch * tokens < 2^24.
+ */
+int mi355_kv_cache_append_fwd(const mi355_kv_cache* cache, const void* k, const void* v, const void* q, void* q_out,
+                              const int32_t* seq_lens, const int32_t* new_lens,
+                              const int64_t* positions, const float* inv_freq,
+                              int64_t batch, int64_t tokens, int64_t q_heads, int64_t rotary_dim,
+                              const int64_t* strides, int64_t pos_stride_b, int64_t pos_stride_t,
+                              float scale, int interleaved, int dtype, void* stream);
+
+/*
+ * Reads slots start[b] + i, i < tokens, as values of dtype (code * scale,
+ * rounded once) into k_out, v_out [batch, kv_heads, tokens, head_dim]
+ * (contiguous, 16-byte aligned); zeros from slot end[b] on.  start may be NULL (0).
+ */
+int mi355_kv_cache_read_fwd(const mi355_kv_cache* cache, void* k_out, void* v_out,
+                            const int32_t* start, const int32_t* end, int64_t batch, int64_t tokens,
+                            int dtype, void* stream);
+
+/*
+ * Moves kept tokens together: slot seq_lens[b] + i becomes what slot
+ * seq_lens[b] + kept[b, i] held before the call, for i < kept_lens[b] (NULL:
+ * max_kept) -- the accepted path of a tree of drafted tokens, in any order and
+ * with repeats.  Codes and scales are moved as they are.  A negative kept[b, i]
+ * or a slot without a place leaves its destination as it was.
+ *   kept int32 [batch, kept_stride], max_kept <= 128.
+ */
+int mi355_kv_cache_keep_fwd(const mi355_kv_cache* cache, const int32_t* seq_lens, const int32_t* kept,
+                            const int32_t* kept_lens, int64_t batch, int64_t max_kept, int64_t kept_stride,
+                            void* stream);
+
+/*
+ * Attention of `tokens` new tokens per sequence over the cache, which holds
+ * them already in slots seq_lens[b] + t (mi355_kv_cache_append_fwd).  Query
+ * head h reads key/value head h / (q_heads / kv_heads).  Token t sees every
+ * slot below seq_lens[b] and the new token j iff tree_mask[b, t, j] != 0
+ * (NULL: j <= t, a chain):
+ *   S[s] = scale * q . K[s],  out = sum_s exp(S[s]) V[s] / sum_s exp(S[s])
+ * over the slots it sees, with fp32 sums and one rounding.  What it does not
+ * see has no influence, NaN and infinities included.  A token that sees
+ * nothing, and padding (t >= new_lens[b]; NULL: none), gets zeros, as does
+ * one whose scores are all -infinity.
+ *
+ *   q     [batch, tokens, q_heads, head_dim] of dtype (fp16, bf16) by three
+ *         strides (batch, token, head), head_dim contiguous, rows 16-byte
+ *         aligned.   out: the same shape, contiguous, 16-byte aligned.
+ *   tree_mask  bytes [batch, tokens, tokens] by mask_stride_b (0: one tree for
+ *         all sequences) and mask_stride_t; the last dimension contiguous.
+ *   tokens <= 128, q_heads a multiple of kv_heads and at most 65535,
+ *   batch * tokens * q_heads < 2^24 (MI355_ERR_UNSUPPORTED beyond).
+ *
+ * The cache is split over workgroups where sequences are few or long, and
+ * joined by a second kernel.  mi355_tree_attention_workspace returns the bytes
+ * that this wants on the current device; `workspace` is 16-byte aligned device
+ * memory that no other work touches until the call's kernels end (its contents
+ * need no preparation).  NULL or less of it: each sequence and head is one
+ * workgroup's work.  Equal arguments give equal bits.
+ */
+int64_t mi355_tree_attention_workspace(const mi355_kv_cache* cache, int64_t batch, int64_t tokens, int64_t q_heads);
+int mi355_tree_attention_fwd(const mi355_kv_cache* cache, const void* q, void* out,
+                             const int32_t* seq_lens, const int32_t* new_lens,
+                             const uint8_t* tree_mask, int64_t mask_stride_b, int64_t mask_stride_t,
+                             int64_t batch, int64_t tokens, int64_t q_heads, const int64_t* q_strides,
+                             float scale, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

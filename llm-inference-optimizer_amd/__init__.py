@@ -31,6 +31,12 @@ The reference's weight-only int8 stage sits beside it: ``w8a16_linear`` /
 (int8 weights with per-output-channel scales, HIP quantiser and W8A16
 kernels), composable with the fused-kernel patch.
 
+Between an attention block's projections: ``fused_rotary`` (rotary positions,
+``rotary_frequencies`` for long contexts), ``KVCache`` with ``kv_cache_append``,
+``kv_cache_read`` and ``kv_cache_keep`` (a paged cache, quantised to int8 or
+e4m3 as it is written), and ``tree_attention`` (one new token, or a tree of
+drafted ones, over that cache).
+
 The kernels live in ``libmi355_fused.so`` (gfx950 HIP, C ABI in
 ``include/mi355_fused.h``), built by ``build.py``.
 """
@@ -41,7 +47,10 @@ from .engine.graphed_decode import GraphedGreedyDecoder
 from .kernels.fused_rmsnorm_hip import fused_add_rmsnorm, fused_rmsnorm, naive_rmsnorm_reference
 from .kernels.fused_gate_up_hip import GATE_UP_MAX_ROWS, fused_gate_up_silu, naive_gate_up_silu_reference
 from .kernels.fused_swiglu_hip import fused_silu_mul, naive_silu_mul_reference
+from .kernels.kv_cache_hip import KV_FORMATS, KVCache, kv_cache_append, kv_cache_keep, kv_cache_read
 from .kernels.linear16_hip import LINEAR16_MAX_ROWS, linear16
+from .kernels.rotary_hip import fused_rotary, rotary_frequencies
+from .kernels.tree_attention_hip import TREE_ATTENTION_MAX_TOKENS, tree_attention
 from .kernels.w8a16_matmul_hip import fused_gate_up_silu_w8a16, quantize_int8_weight, w8a16_linear, w8a16_reference
 from .quantization.int8 import QuantizedLinearInt8, quantize_model_int8
 
@@ -52,4 +61,6 @@ __all__ = [
     "fused_gate_up_silu", "naive_gate_up_silu_reference", "GATE_UP_MAX_ROWS",
     "w8a16_linear", "w8a16_reference", "quantize_int8_weight", "QuantizedLinearInt8", "quantize_model_int8",
     "fused_gate_up_silu_w8a16", "linear16", "LINEAR16_MAX_ROWS",
+    "fused_rotary", "rotary_frequencies", "KVCache", "KV_FORMATS", "kv_cache_append", "kv_cache_read",
+    "kv_cache_keep", "tree_attention", "TREE_ATTENTION_MAX_TOKENS",
 ]

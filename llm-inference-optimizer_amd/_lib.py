@@ -28,7 +28,21 @@ EXPORTED_SYMBOLS = ("mi355_abi_version", "mi355_last_error", "mi355_rmsnorm_fwd"
                     "mi355_silu_mul_fwd", "mi355_gate_up_silu_fwd", "mi355_w8a16_linear_fwd",
                     "mi355_quantize_int8_fwd", "mi355_gate_up_silu_w8a16_fwd", "mi355_linear16_fwd",
                     "mi355_w8a16_linear_workspace", "mi355_w8a16_linear_ws_fwd", "mi355_linear16_workspace",
-                    "mi355_linear16_ws_fwd")
+                    "mi355_linear16_ws_fwd", "mi355_rotary_fwd", "mi355_kv_cache_append_fwd",
+                    "mi355_kv_cache_read_fwd", "mi355_kv_cache_keep_fwd", "mi355_tree_attention_workspace",
+                    "mi355_tree_attention_fwd")
+
+# cache formats of the C ABI (enum mi355_kv_format)
+KV_16BIT, KV_INT8, KV_E4M3 = 0, 1, 2
+
+
+class KvCacheStruct(ctypes.Structure):
+    """``mi355_kv_cache``."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+                ("table_width", ctypes.c_int64), ("pages", ctypes.c_int64), ("kv_heads", ctypes.c_int64),
+                ("page_size", ctypes.c_int64), ("head_dim", ctypes.c_int64), ("format", ctypes.c_int)]
 
 
 class KernelLibraryMissing(RuntimeError):
@@ -82,6 +96,19 @@ def _declare(L: ctypes.CDLL, path: Path) -> ctypes.CDLL:
     L.mi355_w8a16_linear_ws_fwd.restype = i32
     L.mi355_linear16_ws_fwd.argtypes = [*L.mi355_linear16_fwd.argtypes[:-1], vp, i64, vp]
     L.mi355_linear16_ws_fwd.restype = i32
+    f32, cache, strides = ctypes.c_float, ctypes.POINTER(KvCacheStruct), ctypes.POINTER(i64)
+    L.mi355_rotary_fwd.argtypes = [vp, vp, vp, vp, *[i64] * 10, f32, i32, i32, vp]
+    L.mi355_kv_cache_append_fwd.argtypes = [cache, vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, strides, i64,
+                                            i64, f32, i32, i32, vp]
+    L.mi355_kv_cache_read_fwd.argtypes = [cache, vp, vp, vp, vp, i64, i64, i32, vp]
+    L.mi355_kv_cache_keep_fwd.argtypes = [cache, vp, vp, vp, i64, i64, i64, vp]
+    L.mi355_tree_attention_workspace.argtypes = [cache, i64, i64, i64]
+    L.mi355_tree_attention_workspace.restype = i64
+    L.mi355_tree_attention_fwd.argtypes = [cache, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, strides, f32, i32, vp,
+                                           i64, vp]
+    for name in ("mi355_rotary_fwd", "mi355_kv_cache_append_fwd", "mi355_kv_cache_read_fwd",
+                 "mi355_kv_cache_keep_fwd", "mi355_tree_attention_fwd"):
+        getattr(L, name).restype = i32
     ver = L.mi355_abi_version()
     if ver != ABI_VERSION:
         raise KernelLibraryMissing(f"{path} has ABI version {ver}, expected {ABI_VERSION}; rebuild it")

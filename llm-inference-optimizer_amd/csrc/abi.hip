@@ -1,14 +1,13 @@
 // C ABI entry points (include/mi355_fused.h): argument validation, the
 // per-thread error message and the per-device CU-count cache.  Kernels and
 // their launchers live in rmsnorm.hip, silu_mul.hip, gate_up_silu.hip,
-// w8a16.hip, quantize_int8.hip and linear16.hip.
+// w8a16.hip, quantize_int8.hip and linear16.hip.  The entry points of rotary
+// positions and the key/value cache are in abi_kv_cache.hip.
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
 
 #include "common.h"
-
-#define MI355_EXPORT extern "C" __attribute__((visibility("default")))
 
 namespace mi355 {
 
@@ -44,6 +43,8 @@ std::atomic<int> g_cu_count[kMaxDevices];
 }  // namespace
 
 bool valid_dtype(int d) { return d == MI355_F32 || d == MI355_F16 || d == MI355_BF16; }
+
+void clear_error() { g_error[0] = '\0'; }
 
 void set_error(const char* fmt, ...) {
   va_list ap;

@@ -1,5 +1,4 @@
-// Shared device helpers for the gfx950 fused RMSNorm / SiLU-and-mul kernels:
-// 16-byte packet types, fp16/bf16 <-> fp32 conversion through gfx950's packed
+// Shared helpers of the gfx950 kernels and their entry points: 16-byte packet types, fp16/bf16 <-> fp32 conversion through gfx950's packed
 // convert instructions, wave64 reductions and the launch status plumbing.
 #pragma once
 
@@ -7,6 +6,8 @@
 #include <stdint.h>
 
 #include "../../include/mi355_fused.h"
+
+#define MI355_EXPORT extern "C" __attribute__((visibility("default")))
 
 namespace mi355 {
 
@@ -423,6 +424,8 @@ __device__ __forceinline__ float load_dyn(const void* p, int64_t i, int dt) {
 // Host-side helpers shared by the launchers.
 // ---------------------------------------------------------------------------
 void set_error(const char* fmt, ...);
+void clear_error();             // this thread's message
+bool valid_dtype(int d);        // one of enum mi355_dtype
 int compute_units(int* out);  // CU count of the current device, cached per device
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -431,6 +434,13 @@ inline int hip_status(hipError_t e, const char* what) {
   if (e == hipSuccess) return MI355_OK;
   set_error("%s: %s", what, hipGetErrorString(e));
   return MI355_ERR_HIP;
+}
+
+// Launches a kernel of one argument, a struct by value.
+template <typename A>
+int launch(void (*kernel)(A), dim3 grid, int block, unsigned lds, const A& a, hipStream_t s, const char* what) {
+  void* args[] = {const_cast<A*>(&a)};
+  return hip_status(hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, dim3(block), args, lds, s), what);
 }
 
 }  // namespace mi355

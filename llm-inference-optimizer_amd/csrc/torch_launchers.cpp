@@ -412,6 +412,275 @@ at::Tensor gate_up_silu_w8a16(const at::Tensor& x, const at::Tensor& wq_gate, co
   return out.reshape(with_last(x.sizes(), N));
 }
 
+// -------------------------------------- rotary positions, key/value cache
+
+typedef c10::optional<at::Tensor> OptTensor;
+bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
+
+// x [batch, tokens, heads, d] by its strides; copied where d is strided or
+// (packets) a row does not start on 16 bytes.
+struct Heads4 {
+  at::Tensor t;  // 4-d
+  int64_t batch, tokens, heads, d;
+  int64_t strides[3];
+};
+Heads4 heads4(const char* what, const at::Tensor& x, bool packets) {
+  if (x.dim() != 4) fail_assert(std::string(what) + " must be [batch, tokens, heads, head_dim], got " + shape_str(x.sizes()));
+  Heads4 r{x, x.size(0), x.size(1), x.size(2), x.size(3), {0, 0, 0}};
+  bool fits = x.numel() == 0 || x.stride(3) == 1 || r.d == 1;
+  if (packets && x.numel() != 0) {
+    fits = fits && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+    for (int i = 0; i < 3; ++i) fits = fits && (x.size(i) == 1 || x.stride(i) % 8 == 0);
+  }
+  if (!fits) r.t = x.clone(at::MemoryFormat::Contiguous);
+  for (int i = 0; i < 3; ++i) r.strides[i] = r.t.size(i) == 1 ? 0 : r.t.stride(i);  // a lone row's stride says nothing
+  return r;
+}
+
+// The cache's tensors (pools [pages, kv_heads, page_size, head_dim]).
+struct Cache {
+  at::Tensor table;  // keeps a copy alive
+  mi355_kv_cache c;
+  at::ScalarType values;  // the dtype of a 16-bit cache
+};
+Cache cache_of(const at::Tensor& k, const at::Tensor& v, const at::Tensor& table, const OptTensor& k_scale,
+               const OptTensor& v_scale) {
+  if (!(k.is_cuda() && v.is_cuda() && table.is_cuda())) fail_assert("the cache must be on a ROCm GPU");
+  if (k.dim() != 4 || k.sizes() != v.sizes())
+    fail_assert("cache.k and cache.v must be [pages, kv_heads, page_size, head_dim], got " + shape_str(k.sizes()) +
+                " and " + shape_str(v.sizes()));
+  const at::ScalarType t = k.scalar_type();
+  if (t != v.scalar_type()) fail_assert("cache dtypes differ: " + dtype_str(t) + " and " + dtype_str(v.scalar_type()));
+  int format;
+  if (t == at::kHalf || t == at::kBFloat16) format = MI355_KV_16BIT;
+  else if (t == at::kChar) format = MI355_KV_INT8;
+  else if (t == at::kFloat8_e4m3fn) format = MI355_KV_E4M3;
+  else fail_assert("cache dtype must be fp16, bf16, int8 or float8_e4m3fn, got " + dtype_str(t));
+  if (!(k.is_contiguous() && v.is_contiguous())) fail_assert("cache.k and cache.v must be contiguous");
+  if (!(table.dim() == 2 && table.scalar_type() == at::kInt))
+    fail_assert("page_table must be int32 [batch, pages], got " + dtype_str(table.scalar_type()) + " " +
+                shape_str(table.sizes()));
+  const int dev = k.get_device();
+  if (v.get_device() != dev || table.get_device() != dev) fail_assert("the cache's tensors must share a device");
+  Cache r{table, {}, t};
+  if (table.numel() && (table.stride(1) != 1 || (table.size(0) > 1 && table.stride(0) < table.size(1))))
+    r.table = table.contiguous();
+  const bool quantised = format != MI355_KV_16BIT;
+  if (quantised != has(k_scale) || quantised != has(v_scale))
+    fail_assert(quantised ? "a quantised cache needs k_scale and v_scale" : "a 16-bit cache has no scales");
+  if (quantised) {
+    for (const OptTensor* s : {&k_scale, &v_scale}) {
+      const at::Tensor& x = **s;
+      if (!(x.is_cuda() && x.get_device() == dev && x.scalar_type() == at::kFloat && x.is_contiguous() &&
+            x.sizes() == k.sizes().slice(0, 3)))
+        fail_assert("the cache's scales must be contiguous float32 " + shape_str(k.sizes().slice(0, 3)) +
+                    " on its device, got " + dtype_str(x.scalar_type()) + " " + shape_str(x.sizes()));
+    }
+  }
+  r.c.k = ptr(k);
+  r.c.v = ptr(v);
+  r.c.k_scale = quantised ? static_cast<float*>(ptr(*k_scale)) : nullptr;
+  r.c.v_scale = quantised ? static_cast<float*>(ptr(*v_scale)) : nullptr;
+  r.c.page_table = static_cast<const int32_t*>(ptr(r.table));
+  r.c.table_width = r.table.size(1);
+  r.c.table_stride = r.table.size(0) > 1 ? r.table.stride(0) : r.table.size(1);
+  r.c.pages = k.size(0);
+  r.c.kv_heads = k.size(1);
+  r.c.page_size = k.size(2);
+  r.c.head_dim = k.size(3);
+  r.c.format = format;
+  return r;
+}
+
+// int32 [batch] on the cache's device, contiguous (copied if need be).
+at::Tensor lengths(const char* what, const at::Tensor& t, int64_t batch, int dev) {
+  if (!(t.is_cuda() && t.get_device() == dev && t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == batch))
+    fail_assert(std::string(what) + " must be int32 (" + std::to_string(batch) + ",) on the cache's device, got " +
+                dtype_str(t.scalar_type()) + " " + shape_str(t.sizes()));
+  return t.contiguous();
+}
+const int32_t* ints(const at::Tensor& t) { return t.defined() ? static_cast<const int32_t*>(ptr(t)) : nullptr; }
+
+// positions (int64, or int32 widened) broadcast to [batch, tokens].
+at::Tensor positions_of(const at::Tensor& p, int64_t batch, int64_t tokens, int dev) {
+  if (!(p.is_cuda() && p.get_device() == dev && (p.scalar_type() == at::kLong || p.scalar_type() == at::kInt)))
+    fail_assert("positions must be an int64 or int32 tensor on x's device, got " + dtype_str(p.scalar_type()));
+  const bool fits = p.dim() <= 2 && (p.dim() < 1 || p.size(-1) == tokens || p.size(-1) == 1) &&
+                    (p.dim() < 2 || p.size(0) == batch || p.size(0) == 1);
+  if (!fits)
+    fail_assert("positions " + shape_str(p.sizes()) + " do not broadcast to (" + std::to_string(batch) + ", " +
+                std::to_string(tokens) + ")");
+  return (p.scalar_type() == at::kLong ? p : p.to(at::kLong)).expand({batch, tokens});
+}
+at::Tensor frequencies(const at::Tensor& f, int64_t d, int dev) {
+  if (!(f.is_cuda() && f.get_device() == dev && f.scalar_type() == at::kFloat && f.dim() == 1))
+    fail_assert("inv_freq must be a 1-d float32 tensor on x's device, got " + dtype_str(f.scalar_type()) + " " +
+                shape_str(f.sizes()));
+  if (2 * f.size(0) > d)
+    fail_assert("inv_freq has " + std::to_string(f.size(0)) + " pairs, more than head_dim " + std::to_string(d) + " holds");
+  return f.contiguous();
+}
+
+at::Tensor rotary(const at::Tensor& x, const at::Tensor& positions, const at::Tensor& inv_freq, double scale,
+                  bool interleaved) {
+  if (!x.is_cuda()) fail_assert("x must be a ROCm GPU tensor");
+  const int code = code_of(x.scalar_type());
+  if (code < 0) fail_assert("unsupported dtype x=" + dtype_str(x.scalar_type()) + " (fp16, bf16, fp32)");
+  const Heads4 h = heads4("x", x, false);
+  const int dev = x.get_device();
+  const at::Tensor p = positions_of(positions, h.batch, h.tokens, dev), f = frequencies(inv_freq, h.d, dev);
+  at::Tensor out = at::empty(x.sizes(), x.options());
+  if (out.numel()) {
+    Launch l(dev);
+    check("mi355_rotary_fwd",
+          mi355_rotary_fwd(ptr(h.t), ptr(out), static_cast<const int64_t*>(ptr(p)), static_cast<const float*>(ptr(f)),
+                           h.batch, h.tokens, h.heads, h.d, 2 * f.size(0), h.strides[0], h.strides[1], h.strides[2],
+                           p.stride(0), p.stride(1), static_cast<float>(scale), interleaved, code, l.stream));
+  }
+  return out;
+}
+
+int check_new(const char* what, const at::Tensor& x, const Cache& cache, int dev) {
+  if (!(x.is_cuda() && x.get_device() == dev)) fail_assert(std::string(what) + " must be on the cache's GPU");
+  if (x.scalar_type() != at::kHalf && x.scalar_type() != at::kBFloat16)
+    fail_assert(std::string(what) + " must be fp16 or bf16, got " + dtype_str(x.scalar_type()));
+  if (cache.c.format == MI355_KV_16BIT && x.scalar_type() != cache.values)
+    fail_assert(std::string(what) + " is " + dtype_str(x.scalar_type()) + ", the cache " + dtype_str(cache.values));
+  return code_of(x.scalar_type());
+}
+
+OptTensor kv_append(const at::Tensor& ck, const at::Tensor& cv, const at::Tensor& table, const OptTensor& ks,
+                    const OptTensor& vs, const at::Tensor& k, const at::Tensor& v, const at::Tensor& seq_lens,
+                    const OptTensor& new_lens, const OptTensor& q, const OptTensor& positions,
+                    const OptTensor& inv_freq, double scale, bool interleaved) {
+  const Cache cache = cache_of(ck, cv, table, ks, vs);
+  const int dev = ck.get_device();
+  const int code = check_new("k", k, cache, dev);
+  if (k.sizes() != v.sizes()) fail_assert("k and v differ: " + shape_str(k.sizes()) + " vs " + shape_str(v.sizes()));
+  if (check_new("v", v, cache, dev) != code) fail_assert("k and v must share a dtype");
+  const Heads4 kh = heads4("k", k, true), vh = heads4("v", v, true);
+  if (kh.heads != cache.c.kv_heads || kh.d != cache.c.head_dim)
+    fail_assert("k has " + std::to_string(kh.heads) + " heads of " + std::to_string(kh.d) + ", the cache " +
+                std::to_string(cache.c.kv_heads) + " of " + std::to_string(cache.c.head_dim));
+  if (table.size(0) != kh.batch)
+    fail_assert("page_table has " + std::to_string(table.size(0)) + " sequences, k " + std::to_string(kh.batch));
+  if (has(positions) != has(inv_freq)) fail_assert("positions and inv_freq go together");
+  if (has(q) && !has(inv_freq)) fail_assert("q is given to be rotated: positions and inv_freq are missing");
+  Heads4 qh{};
+  at::Tensor out;
+  if (has(q)) {
+    if (check_new("q", *q, cache, dev) != code) fail_assert("q, k and v must share a dtype");
+    qh = heads4("q", *q, true);
+    if (qh.batch != kh.batch || qh.tokens != kh.tokens || qh.d != kh.d)
+      fail_assert("q " + shape_str(q->sizes()) + " does not fit k " + shape_str(k.sizes()));
+    out = at::empty(q->sizes(), q->options());
+  }
+  const at::Tensor lens = lengths("seq_lens", seq_lens, kh.batch, dev);
+  const at::Tensor fresh = has(new_lens) ? lengths("new_lens", *new_lens, kh.batch, dev) : at::Tensor();
+  at::Tensor p, f;
+  if (has(inv_freq)) {
+    p = positions_of(*positions, kh.batch, kh.tokens, dev);
+    f = frequencies(*inv_freq, kh.d, dev);
+  }
+  if (kh.batch && kh.tokens) {
+    const int64_t strides[9] = {kh.strides[0], kh.strides[1], kh.strides[2], vh.strides[0], vh.strides[1],
+                                vh.strides[2], qh.strides[0], qh.strides[1], qh.strides[2]};
+    Launch l(dev);
+    check("mi355_kv_cache_append_fwd",
+          mi355_kv_cache_append_fwd(&cache.c, ptr(kh.t), ptr(vh.t), has(q) ? ptr(qh.t) : nullptr,
+                                    has(q) ? ptr(out) : nullptr, ints(lens), ints(fresh),
+                                    p.defined() ? static_cast<const int64_t*>(ptr(p)) : nullptr,
+                                    f.defined() ? static_cast<const float*>(ptr(f)) : nullptr, kh.batch, kh.tokens,
+                                    qh.heads, f.defined() ? 2 * f.size(0) : 0, strides,
+                                    p.defined() ? p.stride(0) : 0, p.defined() ? p.stride(1) : 0,
+                                    static_cast<float>(scale), interleaved, code, l.stream));
+  }
+  if (!has(q)) return c10::nullopt;
+  return out;
+}
+
+std::tuple<at::Tensor, at::Tensor> kv_read(const at::Tensor& ck, const at::Tensor& cv, const at::Tensor& table,
+                                           const OptTensor& ks, const OptTensor& vs, const at::Tensor& end,
+                                           int64_t tokens, const OptTensor& start, at::ScalarType dtype) {
+  const Cache cache = cache_of(ck, cv, table, ks, vs);
+  const int dev = ck.get_device();
+  if (dtype != at::kHalf && dtype != at::kBFloat16) fail_assert("dtype must be fp16 or bf16, got " + dtype_str(dtype));
+  if (cache.c.format == MI355_KV_16BIT && dtype != cache.values)
+    fail_assert("dtype is " + dtype_str(dtype) + ", the cache " + dtype_str(cache.values));
+  if (tokens < 0) fail_assert("tokens must be >= 0");
+  const int64_t batch = table.size(0);
+  const at::Tensor e = lengths("end", end, batch, dev);
+  const at::Tensor s = has(start) ? lengths("start", *start, batch, dev) : at::Tensor();
+  const auto options = ck.options().dtype(dtype);
+  at::Tensor k = at::empty({batch, cache.c.kv_heads, tokens, cache.c.head_dim}, options);
+  at::Tensor v = at::empty(k.sizes(), options);
+  if (batch && tokens) {
+    Launch l(dev);
+    check("mi355_kv_cache_read_fwd", mi355_kv_cache_read_fwd(&cache.c, ptr(k), ptr(v), ints(s), ints(e), batch, tokens,
+                                                             code_of(dtype), l.stream));
+  }
+  return {k, v};
+}
+
+void kv_keep(const at::Tensor& ck, const at::Tensor& cv, const at::Tensor& table, const OptTensor& ks,
+             const OptTensor& vs, const at::Tensor& seq_lens, const at::Tensor& kept, const OptTensor& kept_lens) {
+  const Cache cache = cache_of(ck, cv, table, ks, vs);
+  const int dev = ck.get_device();
+  const int64_t batch = table.size(0);
+  if (!(kept.is_cuda() && kept.get_device() == dev && kept.scalar_type() == at::kInt && kept.dim() == 2 &&
+        kept.size(0) == batch))
+    fail_assert("kept must be int32 [" + std::to_string(batch) + ", n] on the cache's device, got " +
+                dtype_str(kept.scalar_type()) + " " + shape_str(kept.sizes()));
+  const at::Tensor lens = lengths("seq_lens", seq_lens, batch, dev);
+  const at::Tensor n = has(kept_lens) ? lengths("kept_lens", *kept_lens, batch, dev) : at::Tensor();
+  const at::Tensor kc = kept.contiguous();
+  if (batch && kept.size(1)) {
+    Launch l(dev);
+    check("mi355_kv_cache_keep_fwd", mi355_kv_cache_keep_fwd(&cache.c, ints(lens), ints(kc), ints(n), batch,
+                                                             kc.size(1), kc.size(1), l.stream));
+  }
+}
+
+at::Tensor tree_attention(const at::Tensor& q, const at::Tensor& ck, const at::Tensor& cv, const at::Tensor& table,
+                          const OptTensor& ks, const OptTensor& vs, const at::Tensor& seq_lens,
+                          const OptTensor& new_lens, const OptTensor& tree_mask, double scale) {
+  const Cache cache = cache_of(ck, cv, table, ks, vs);
+  const int dev = ck.get_device();
+  const int code = check_new("q", q, cache, dev);
+  const Heads4 h = heads4("q", q, true);
+  if (h.d != cache.c.head_dim || h.heads % std::max<int64_t>(1, cache.c.kv_heads) != 0)
+    fail_assert("q has " + std::to_string(h.heads) + " heads of " + std::to_string(h.d) + ", the cache " +
+                std::to_string(cache.c.kv_heads) + " of " + std::to_string(cache.c.head_dim));
+  if (table.size(0) != h.batch)
+    fail_assert("page_table has " + std::to_string(table.size(0)) + " sequences, q " + std::to_string(h.batch));
+  const at::Tensor lens = lengths("seq_lens", seq_lens, h.batch, dev);
+  const at::Tensor fresh = has(new_lens) ? lengths("new_lens", *new_lens, h.batch, dev) : at::Tensor();
+  at::Tensor mask;
+  if (has(tree_mask)) {
+    mask = *tree_mask;
+    const bool fits = (mask.dim() == 2 || (mask.dim() == 3 && (mask.size(0) == h.batch || mask.size(0) == 1))) &&
+                      mask.size(-1) == h.tokens && mask.size(-2) == h.tokens;
+    if (!(mask.is_cuda() && mask.get_device() == dev && mask.scalar_type() == at::kBool && fits))
+      fail_assert("tree_mask must be bool [tokens, tokens] or [batch, tokens, tokens] on q's device, got " +
+                  dtype_str(mask.scalar_type()) + " " + shape_str(mask.sizes()));
+    if (mask.dim() == 2) mask = mask.unsqueeze(0);
+    if (mask.numel() && mask.stride(2) != 1 && mask.size(2) != 1) mask = mask.contiguous();
+  }
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  if (out.numel()) {
+    Launch l(dev);
+    const at::Tensor work = workspace(mi355_tree_attention_workspace(&cache.c, h.batch, h.tokens, h.heads), q);
+    check("mi355_tree_attention_fwd",
+          mi355_tree_attention_fwd(&cache.c, ptr(h.t), ptr(out), ints(lens), ints(fresh),
+                                   mask.defined() ? static_cast<const uint8_t*>(ptr(mask)) : nullptr,
+                                   mask.defined() && mask.size(0) > 1 ? mask.stride(0) : 0,
+                                   mask.defined() && mask.size(1) > 1 ? mask.stride(1) : 0, h.batch, h.tokens, h.heads,
+                                   h.strides, static_cast<float>(scale), code,
+                                   work.defined() ? ptr(work) : nullptr, work.defined() ? work.numel() : 0, l.stream));
+  }
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_mi355_torch, m) {
@@ -430,4 +699,16 @@ PYBIND11_MODULE(_mi355_torch, m) {
         py::arg("out_f32"));
   m.def("gate_up_silu_w8a16", &gate_up_silu_w8a16, py::arg("x"), py::arg("wq_gate"), py::arg("scale_gate"),
         py::arg("wq_up"), py::arg("scale_up"), py::arg("out_f32"));
+  m.def("rotary", &rotary, py::arg("x"), py::arg("positions"), py::arg("inv_freq"), py::arg("scale"),
+        py::arg("interleaved"));
+  m.def("kv_append", &kv_append, py::arg("cache_k"), py::arg("cache_v"), py::arg("page_table"), py::arg("k_scale"),
+        py::arg("v_scale"), py::arg("k"), py::arg("v"), py::arg("seq_lens"), py::arg("new_lens"), py::arg("q"),
+        py::arg("positions"), py::arg("inv_freq"), py::arg("scale"), py::arg("interleaved"));
+  m.def("kv_read", &kv_read, py::arg("cache_k"), py::arg("cache_v"), py::arg("page_table"), py::arg("k_scale"),
+        py::arg("v_scale"), py::arg("end"), py::arg("tokens"), py::arg("start"), py::arg("dtype"));
+  m.def("kv_keep", &kv_keep, py::arg("cache_k"), py::arg("cache_v"), py::arg("page_table"), py::arg("k_scale"),
+        py::arg("v_scale"), py::arg("seq_lens"), py::arg("kept"), py::arg("kept_lens"));
+  m.def("tree_attention", &tree_attention, py::arg("q"), py::arg("cache_k"), py::arg("cache_v"),
+        py::arg("page_table"), py::arg("k_scale"), py::arg("v_scale"), py::arg("seq_lens"), py::arg("new_lens"),
+        py::arg("tree_mask"), py::arg("scale"));
 }

@@ -1,0 +1,190 @@
+"""What rotary positions, the cache and attention over it refuse before any GPU work, and their host-side parts."""
+import ctypes
+import importlib
+
+import pytest
+import torch
+
+P = 0x10000  # a fake, never-dereferenced, 16-byte aligned device address
+
+
+@pytest.fixture(scope="module")
+def L():
+    return importlib.import_module("llm-inference-optimizer_amd._lib")
+
+
+@pytest.fixture(scope="module")
+def lib(L):
+    return L.load()
+
+
+def _cache(L, **kw):
+    args = dict(k=P, v=P, k_scale=P, v_scale=P, page_table=P, table_stride=8, table_width=8, pages=10, kv_heads=2,
+                page_size=16, head_dim=64, format=L.KV_INT8)
+    args.update(kw)
+    return ctypes.byref(L.KvCacheStruct(**args))
+
+
+def _strides(*v):
+    return (ctypes.c_int64 * len(v))(*v)
+
+
+def _expect(lib, status, code, message):
+    assert status == code
+    assert message in lib.mi355_last_error().decode()
+
+
+@pytest.mark.parametrize("kw,code,message", [
+    (dict(dtype=7), -1, "unknown dtype"), (dict(batch=-1), -1, "sizes"), (dict(d=0), -1, "sizes"),
+    (dict(sb=-8), -1, "strides"), (dict(r=3), -1, "rotary_dim must be even"), (dict(r=66), -1, "rotary_dim must be even"),
+    (dict(d=512, r=258), -2, "at most 256"), (dict(pos=0), -1, "positions"), (dict(freq=0), -1, "inv_freq"),
+    (dict(batch=1 << 12, tokens=1 << 12), -2, "limits"), (dict(batch=1 << 40, tokens=1 << 40), -2, "limits"),
+    (dict(heads=65536), -2, "limits"), (dict(d=1 << 20), -2, "limits"), (dict(x=0), -1, "null"), (dict(y=0), -1, "null")])
+def test_rotary_abi_rejects(lib, kw, code, message):
+    a = dict(x=P, y=P, pos=P, freq=P, batch=1, tokens=2, heads=3, d=64, r=64, sb=0, dtype=1)
+    a.update(kw)
+    _expect(lib, lib.mi355_rotary_fwd(a["x"], a["y"], a["pos"], a["freq"], a["batch"], a["tokens"], a["heads"], a["d"],
+                                      a["r"], a["sb"], 64, 64, 0, 1, 1.0, 0, a["dtype"], None), code, message)
+
+
+def test_rotary_abi_empty_is_noop(lib):
+    for sizes in ((0, 2, 3), (2, 0, 3), (2, 3, 0)):
+        assert lib.mi355_rotary_fwd(0, 0, P, P, *sizes, 64, 64, 0, 0, 0, 0, 0, 1.0, 0, 1, None) == 0
+        assert lib.mi355_last_error().decode() == ""
+
+
+BAD_CACHES = [
+    (dict(format=3), -1, "format"), (dict(pages=-1), -1, "sizes"), (dict(kv_heads=0), -1, "sizes"),
+    (dict(table_stride=7), -1, "sizes"), (dict(head_dim=72), -2, "head_dim"), (dict(head_dim=272), -2, "head_dim"),
+    (dict(page_size=24), -2, "page_size"), (dict(kv_heads=65536), -2, "limits"), (dict(pages=1 << 31), -2, "limits"),
+    (dict(table_width=1 << 27, table_stride=1 << 27), -2, "limits"), (dict(k=0), -1, "null"),
+    (dict(page_table=0), -1, "null"), (dict(v=P + 8), -1, "aligned"), (dict(k_scale=0), -1, "scales"),
+    (dict(v_scale=P + 4), -1, "aligned")]
+
+
+@pytest.mark.parametrize("kw,code,message", BAD_CACHES)
+def test_cache_calls_reject_a_bad_cache(L, lib, kw, code, message):
+    """Every call that takes a cache checks it, before any GPU work."""
+    c, s9 = _cache(L, **kw), _strides(*[64] * 9)
+    heads = 2 * max(1, kw.get("kv_heads", 2))
+    if heads > 65535:
+        heads = kw["kv_heads"]
+    _expect(lib, lib.mi355_kv_cache_append_fwd(c, P, P, None, None, P, None, None, None, 1, 1, 0, 0, s9, 0, 0, 1.0, 0, 1,
+                                               None), code, message)
+    _expect(lib, lib.mi355_kv_cache_read_fwd(c, P, P, None, P, 1, 1, 1, None), code, message)
+    _expect(lib, lib.mi355_kv_cache_keep_fwd(c, P, P, None, 1, 1, 1, None), code, message)
+    _expect(lib, lib.mi355_tree_attention_fwd(c, P, P, P, None, None, 0, 0, 1, 1, heads, s9, 1.0, 1, None, 0, None),
+            code, message)
+
+
+def test_null_cache(lib):
+    _expect(lib, lib.mi355_kv_cache_read_fwd(None, P, P, None, P, 1, 1, 1, None), -1, "null cache")
+    assert lib.mi355_tree_attention_workspace(None, 1, 1, 2) == 0
+
+
+@pytest.mark.parametrize("kw,code,message", [
+    (dict(dtype=0), -2, "fp16 or bf16"), (dict(dtype=9), -1, "unknown dtype"), (dict(tokens=-1), -1, "sizes"),
+    (dict(r=2, pos=0), -1, "positions"), (dict(r=66), -1, "rotary_dim"), (dict(batch=1 << 20, tokens=1 << 20), -2, "limits"),
+    (dict(qh=65536), -2, "limits"), (dict(k=0), -1, "null"), (dict(lens=0), -1, "null"), (dict(qh=2, q=0), -1, "null"),
+    (dict(k=P + 2), -2, "aligned"), (dict(strides=[64, 64, 60] + [64] * 6), -2, "multiples of 8"),
+    (dict(strides=[-64, 64, 64] + [64] * 6), -1, "strides")])
+def test_append_abi_rejects(L, lib, kw, code, message):
+    a = dict(k=P, q=P, lens=P, pos=P, batch=1, tokens=2, qh=0, r=0, strides=[64] * 9, dtype=1)
+    a.update(kw)
+    _expect(lib, lib.mi355_kv_cache_append_fwd(_cache(L), a["k"], P, a["q"], P, a["lens"], None, a["pos"], P, a["batch"],
+                                               a["tokens"], a["qh"], a["r"], _strides(*a["strides"]), 0, 1, 1.0, 0,
+                                               a["dtype"], None), code, message)
+
+
+@pytest.mark.parametrize("kw,code,message", [
+    (dict(dtype=0), -2, "fp16 or bf16"), (dict(tokens=129), -2, "tokens <= 128"), (dict(heads=3), -1, "multiple of kv_heads"),
+    (dict(batch=1 << 18, tokens=64), -2, "limits"), (dict(q=0), -1, "null"), (dict(q=P + 8), -2, "aligned"),
+    (dict(strides=[64, 64, 4]), -2, "multiples of 8"), (dict(strides=[64, -64, 64]), -1, "strides"),
+    (dict(work=P + 8, bytes=64), -1, "workspace"), (dict(work=P, bytes=-1), -1, "workspace")])
+def test_attention_abi_rejects(L, lib, kw, code, message):
+    a = dict(q=P, batch=1, tokens=2, heads=4, strides=[64] * 3, dtype=1, work=None, bytes=0)
+    a.update(kw)
+    _expect(lib, lib.mi355_tree_attention_fwd(_cache(L), a["q"], P, P, None, None, 0, 0, a["batch"], a["tokens"],
+                                              a["heads"], _strides(*a["strides"]), 1.0, a["dtype"], a["work"], a["bytes"],
+                                              None), code, message)
+
+
+def test_read_and_keep_abi_rejects(L, lib):
+    c = _cache(L)
+    for args, code, message in [((c, P, P, None, P, 1, 1, 0, None), -2, "fp16 or bf16"),
+                                ((c, P, P, None, P, -1, 1, 1, None), -1, "sizes"),
+                                ((c, P, P, None, P, 1 << 20, 1 << 7, 1, None), -2, "limits"),
+                                ((c, P, P, None, 0, 1, 1, 1, None), -1, "null"),
+                                ((c, P + 2, P, None, P, 1, 1, 1, None), -1, "aligned")]:
+        _expect(lib, lib.mi355_kv_cache_read_fwd(*args), code, message)
+    for args, code, message in [((c, P, P, None, 1, 129, 129, None), -2, "max_kept"),
+                                ((c, P, P, None, 1 << 24, 1, 1, None), -2, "limits"),
+                                ((c, P, 0, None, 1, 1, 1, None), -1, "null"),
+                                ((c, P, P, None, 1, -1, 1, None), -1, "sizes")]:
+        _expect(lib, lib.mi355_kv_cache_keep_fwd(*args), code, message)
+
+
+def test_empty_calls_are_noops(L, lib):
+    c, s9 = _cache(L), _strides(*[64] * 9)
+    assert lib.mi355_kv_cache_append_fwd(c, 0, 0, None, None, 0, None, None, None, 0, 5, 0, 0, s9, 0, 0, 1.0, 0, 1, None) == 0
+    assert lib.mi355_kv_cache_read_fwd(c, 0, 0, None, 0, 3, 0, 1, None) == 0
+    assert lib.mi355_kv_cache_keep_fwd(c, 0, 0, None, 3, 0, 0, None) == 0
+    assert lib.mi355_tree_attention_fwd(c, 0, 0, 0, None, None, 0, 0, 2, 0, 4, s9, 1.0, 1, None, 0, None) == 0
+    assert lib.mi355_last_error().decode() == ""
+
+
+def test_launchers_refuse_host_tensors(pkg):
+    x, lens = torch.zeros((1, 2, 2, 64), dtype=torch.float16), torch.zeros(1, dtype=torch.int32)
+    cache = pkg.KVCache.allocate(1, 32, 2, 64, "int8", device="cpu")
+    with pytest.raises(AssertionError, match="ROCm GPU"):
+        pkg.fused_rotary(x, torch.zeros((1, 2), dtype=torch.long), torch.zeros(32))
+    for call in (lambda: pkg.kv_cache_append(cache, x, x, lens), lambda: pkg.kv_cache_read(cache, lens, 3),
+                 lambda: pkg.kv_cache_keep(cache, lens, lens[:, None]), lambda: pkg.tree_attention(x, cache, lens)):
+        with pytest.raises(AssertionError, match="ROCm GPU"):
+            call()
+
+
+def test_allocate(pkg):
+    c = pkg.KVCache.allocate(3, 100, 2, 64, "int8", device="cpu")
+    assert c.k.shape == (3, 2, 112, 64) and c.k.dtype == torch.int8 and c.capacity == 112
+    assert c.page_table.tolist() == [[0], [1], [2]] and c.k_scale.shape == (3, 2, 112)
+    assert c.num_bytes() == 2 * 3 * 2 * 112 * 68
+    c = pkg.KVCache.allocate(2, 100, 2, 64, "16bit", torch.bfloat16, "cpu", page_size=32)
+    assert c.k.shape == (8, 2, 32, 64) and c.k.dtype == torch.bfloat16 and c.k_scale is None and c.capacity == 128
+    assert c.page_table.tolist() == [[0, 1, 2, 3], [4, 5, 6, 7]]
+    assert pkg.KVCache.allocate(1, 0, 1, 16, "e4m3", device="cpu").v.dtype == torch.float8_e4m3fn
+    for kw in (dict(kv_format="int4"), dict(page_size=24), dict(head_dim=72), dict(head_dim=512)):
+        with pytest.raises(ValueError):
+            pkg.KVCache.allocate(**{**dict(batch=1, max_len=8, kv_heads=1, head_dim=64, device="cpu"), **kw})
+
+
+@pytest.mark.parametrize("d,theta,scaling", [
+    (128, 1e6, None), (64, 1e4, {"rope_type": "linear", "factor": 4.0}),
+    (128, 1e6, {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32768}),
+    (128, 1e4, {"rope_type": "yarn", "factor": 16.0, "original_max_position_embeddings": 4096, "beta_fast": 24,
+                "beta_slow": 2, "attention_factor": 1.5}),
+    (128, 5e5, {"rope_type": "llama3", "factor": 8.0, "original_max_position_embeddings": 8192,
+                "low_freq_factor": 1.0, "high_freq_factor": 4.0})])
+def test_frequencies_are_those_of_hf_models(pkg, d, theta, scaling):
+    """Against the rotary module of an HF model with the same settings (32-bit there: 1e-6 relative)."""
+    transformers = pytest.importorskip("transformers")
+    from transformers.models.llama.modeling_llama import LlamaRotaryEmbedding
+    rope = {"rope_theta": theta, **(scaling or {"rope_type": "default"})}
+    cfg = transformers.LlamaConfig(hidden_size=2 * d, num_attention_heads=2, max_position_embeddings=131072,
+                                   rope_parameters=rope)
+    hf = LlamaRotaryEmbedding(cfg)
+    freq, scale = pkg.rotary_frequencies(d, theta, scaling)
+    assert freq.dtype == torch.float32 and freq.shape == (d // 2,)
+    torch.testing.assert_close(freq, hf.inv_freq, rtol=2e-6, atol=0)
+    assert scale == pytest.approx(hf.attention_scaling, rel=1e-6)
+
+
+def test_frequencies_ntk_and_refusals(pkg):
+    f, scale = pkg.rotary_frequencies(64, 1e4, {"rope_type": "ntk", "factor": 4.0})
+    base, _ = pkg.rotary_frequencies(64, 1e4)
+    assert scale == 1.0 and f[0] == base[0] == 1.0
+    assert f[-1].item() == pytest.approx(base[-1].item() / 4, rel=1e-6)
+    assert pkg.rotary_frequencies(2, 1e4, {"rope_type": "ntk", "factor": 4.0})[0].tolist() == [1.0]
+    for args in ((3,), (0,), (64, 1e4, {"rope_type": "dynamic", "factor": 2.0})):
+        with pytest.raises(ValueError):
+            pkg.rotary_frequencies(*args)

@@ -1,0 +1,101 @@
+"""fused_rotary on the GPU against its 64-bit form, and its refusals."""
+import pytest
+import torch
+
+import kv_oracle as K
+
+pytestmark = pytest.mark.gpu
+
+
+def _freq(pairs, theta=1e6):
+    return (theta ** (-torch.arange(pairs, dtype=torch.float64) / max(1, pairs))).float()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("batch,tokens,heads,d,rotary", [
+    (1, 1, 1, 64, 64), (3, 5, 12, 128, 128), (2, 7, 14, 64, 32), (1, 9, 3, 96, 24), (2, 2, 5, 80, 40),
+    (1, 3, 2, 256, 256), (1, 4, 2, 36, 36), (2, 3, 3, 7, 6), (1, 2, 2, 300, 2), (1, 1100, 2, 64, 64),
+    (1, 2, 20, 128, 0), (1, 5, 3, 128, 74)])
+def test_matches_64_bit_form(pkg, cuda, dtype, interleaved, batch, tokens, heads, d, rotary):
+    g = torch.Generator().manual_seed(d + rotary)
+    x = torch.randn((batch, tokens, heads, d), generator=g).to(dtype)
+    pos = torch.randint(-5, 1_000_000, (batch, tokens), generator=g)
+    f = _freq(rotary // 2)
+    y = pkg.fused_rotary(x.to(cuda), pos.to(cuda), f.to(cuda), scale=1.1386, interleaved=interleaved)
+    assert y.shape == x.shape and y.dtype == dtype and y.is_contiguous()
+    K.close(y, *K.rotary(x, pos, f, 1.1386, interleaved))
+    assert torch.equal(y[..., rotary:].cpu(), x[..., rotary:])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_strided_views_and_broadcast_positions(pkg, cuda, dtype):
+    """q as a slice of a fused projection, heads before tokens, every second element, an offset that no packet starts
+    on, a broadcast batch; positions of one row, of one token, int32."""
+    f = _freq(32)
+    base = torch.randn((2, 6, 10 * 64 + 3), generator=torch.Generator().manual_seed(1)).to(dtype)
+    views = [base[..., :640].view(2, 6, 10, 64)[:, :, 2:7], base[..., 1:641].unflatten(-1, (10, 64)),
+             base[..., :640].view(2, 6, 10, 64).transpose(1, 2), base[..., :640].view(2, 6, 5, 128)[..., ::2],
+             base[:1, :, :640].view(1, 6, 10, 64).expand(3, 6, 10, 64), base[..., :640].view(2, 6, 10, 64)[1:, 3:4]]
+    for x in views:
+        t = x.shape[1]
+        for pos in (torch.arange(t) * 1001, torch.arange(t, dtype=torch.int32)[None] + 7, torch.tensor([[123456]]),
+                    torch.tensor(9)):
+            xg = x.to(cuda) if x.is_contiguous() else base.to(cuda).as_strided(x.shape, x.stride(), x.storage_offset())
+            y = pkg.fused_rotary(xg, pos.to(cuda), f.to(cuda))
+            K.close(y, *K.rotary(x, pos.expand(x.shape[:2]), f))
+
+
+def test_far_positions_keep_their_angle(pkg, cuda):
+    """Positions near 2^28: the 64-bit product is exact, an fp32 one would be off by whole turns."""
+    x = torch.randn((1, 64, 2, 128), generator=torch.Generator().manual_seed(3))
+    pos = (1 << 28) - 1 - 977 * torch.arange(64)[None]
+    f = _freq(64, 1e4)
+    K.close(pkg.fused_rotary(x.to(cuda), pos.to(cuda), f.to(cuda)), *K.rotary(x, pos, f))
+
+
+def test_turning_back(pkg, cuda):
+    """The rotation by the opposite positions undoes it (fp32: twice the bound)."""
+    x = torch.randn((2, 9, 3, 128), generator=torch.Generator().manual_seed(4)).to(cuda)
+    pos, f = torch.arange(9, device=cuda) * 12345, _freq(64).to(cuda)
+    y = pkg.fused_rotary(pkg.fused_rotary(x, pos, f), -pos, f)
+    assert (y - x).abs().max().item() <= 2 * 4e-7 * 2 * 1.5 * x.abs().max().item()
+
+
+def test_empty_tensors(pkg, cuda):
+    f = _freq(32).to(cuda)
+    for shape in ((0, 3, 2, 64), (2, 0, 2, 64), (2, 3, 0, 64)):
+        assert pkg.fused_rotary(torch.empty(shape, device=cuda), torch.zeros((1, 1), device=cuda).long(), f).shape == shape
+
+
+def test_other_stream_and_graph(pkg, cuda):
+    x = torch.randn((3, 4, 6, 128), generator=torch.Generator().manual_seed(5)).half().to(cuda)
+    pos, f = torch.arange(4, device=cuda) + 100, _freq(64).to(cuda)
+    want = pkg.fused_rotary(x, pos, f)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert torch.equal(pkg.fused_rotary(x, pos, f), want)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = pkg.fused_rotary(x, pos, f)
+    for seed in range(3):
+        x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(seed)).half())
+        pos.add_(17)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, pkg.fused_rotary(x, pos, f))
+
+
+def test_refusals(pkg, cuda):
+    x, p, f = torch.zeros((1, 2, 3, 64), device=cuda), torch.zeros((1, 2), dtype=torch.long, device=cuda), _freq(32).to(cuda)
+    for args, message in [((x.cpu(), p, f), "ROCm GPU"), ((x.int(), p, f), "unsupported dtype"),
+                          ((x[0], p, f), r"\[batch, tokens"), ((x, p.float(), f), "positions"),
+                          ((x, p.expand(2, 2), f), "broadcast"), ((x, p[:, :1].expand(1, 3), f), "broadcast"),
+                          ((x, p.cpu(), f), "positions"), ((x, p, f.double()), "inv_freq"),
+                          ((x, p, f[None]), "inv_freq"), ((x, p, torch.zeros(33, device=cuda)), "more than head_dim")]:
+        with pytest.raises(AssertionError, match=message):
+            pkg.fused_rotary(*args)
+    with pytest.raises(Exception, match="rotary_dim must be at most 256"):
+        pkg.fused_rotary(torch.zeros((1, 1, 1, 300), device=cuda), p[:, :1], torch.zeros(129, device=cuda))

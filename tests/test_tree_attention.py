@@ -1,0 +1,234 @@
+"""tree_attention on the GPU against its 64-bit form: lengths from nothing to long, masks that leave rows empty, and
+values in places that nobody sees."""
+import pytest
+import torch
+
+import kv_oracle as K
+
+pytestmark = pytest.mark.gpu
+
+FORMATS = ["16bit", "int8", "e4m3"]
+
+
+def _q(shape, dtype, seed, std=2.0):
+    return (std * torch.randn(shape, generator=torch.Generator().manual_seed(seed))).to(dtype)
+
+
+def _case(pkg, kind, dtype, batch, tokens, hq, kvh, d, page, lens, seed=1):
+    per = max(1, (max(lens) + tokens + page - 1) // page)
+    table, pages = K.shuffled_table(batch, per, 2, seed)
+    cache = K.make_cache(pkg, kind, dtype, (pages, kvh, page, d), table, seed + 1)
+    return cache, _q((batch, tokens, hq, d), dtype, seed + 2).cuda()
+
+
+@pytest.mark.parametrize("kind", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("batch,tokens,hq,kvh,d,page,lens,tree", [
+    (1, 1, 1, 1, 64, 16, [0], False),
+    (1, 1, 12, 2, 128, 16, [777], False),
+    (4, 1, 14, 2, 64, 16, [0, 1, 31, 300], False),
+    (3, 5, 28, 4, 128, 48, [0, 47, 130], True),
+    (2, 17, 6, 3, 96, 32, [64, 9], True),
+    (2, 33, 10, 5, 80, 64, [63, 200], False),
+    (1, 64, 8, 1, 256, 16, [40], True),
+    (2, 128, 4, 4, 16, 256, [250, 0], True),
+    (5, 3, 40, 8, 128, 16, [16, 32, 48, 15, 17], False),
+    (1, 2, 32, 32, 32, 16, [1030], False)])
+def test_matches_64_bit_form(pkg, cuda, kind, dtype, batch, tokens, hq, kvh, d, page, lens, tree):
+    cache, q = _case(pkg, kind, dtype, batch, tokens, hq, kvh, d, page, lens)
+    mask = K.random_tree(batch, tokens, 3) if tree else None
+    out = pkg.tree_attention(q, cache, K.ints(lens), tree_mask=None if mask is None else mask.to(cuda))
+    assert out.shape == q.shape and out.dtype == dtype
+    K.close(out, *K.attention(q, cache, lens, mask=mask))
+    again = pkg.tree_attention(q, cache, K.ints(lens), tree_mask=None if mask is None else mask.to(cuda))
+    assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("kind", FORMATS)
+@pytest.mark.parametrize("lens,batch_pad", [([20011], 0), ([9000, 3, 511, 0], 0)])
+def test_long_and_unequal_contexts(pkg, cuda, kind, lens, batch_pad):
+    """Contexts that are split over workgroups, beside ones that are not."""
+    cache, q = _case(pkg, kind, torch.bfloat16, len(lens), 2, 8, 2, 128, 64, lens)
+    K.close(pkg.tree_attention(q, cache, K.ints(lens)), *K.attention(q, cache, lens))
+
+
+@pytest.mark.parametrize("kind", FORMATS)
+def test_rows_that_see_nothing_and_padding(pkg, cuda, kind):
+    """Empty mask rows without a context get zeros; with one, the context alone; padding gets zeros."""
+    lens, new = [0, 0, 37, 5], [6, 3, 6, 0]
+    cache, q = _case(pkg, kind, torch.float16, 4, 6, 4, 2, 64, 16, lens)
+    mask = K.random_tree(4, 6, 4)
+    mask[0, 2] = False
+    mask[2, 3] = False
+    mask[1] = False
+    out = pkg.tree_attention(q, cache, K.ints(lens), new_lens=K.ints(new), tree_mask=mask.to(cuda))
+    K.close(out, *K.attention(q, cache, lens, new, mask))
+    assert not out[0, 2].any() and not out[1].any() and not out[3].any() and out[2, 3].any()
+
+
+@pytest.mark.parametrize("kind", FORMATS)
+@pytest.mark.parametrize("d", [64, 128])
+def test_unseen_values_have_no_influence(pkg, cuda, kind, d):
+    """NaN, infinities and largest values in slots behind the last token, in padding tokens, and in drafted tokens of
+    other branches -- keys, values and scales -- leave a row's bits as they are."""
+    batch, tokens, lens, new = 2, 6, [37, 3], [6, 4]
+    cache, q = _case(pkg, kind, torch.float16, batch, tokens, 6, 2, d, 16, lens)
+    mask = torch.eye(tokens, dtype=torch.bool).expand(batch, tokens, tokens).clone()
+    mask[:, 1:, 0] = True   # token 0 is everyone's parent but token 5's; nobody else sees tokens 1 .. 5
+    mask[:, 5] = False
+    mask[:, 5, 5] = True
+    args = dict(new_lens=K.ints(new), tree_mask=mask.to(cuda))
+    want = pkg.tree_attention(q, cache, K.ints(lens), **args)
+    K.close(want, *K.attention(q, cache, lens, new, mask))
+    for bad in (float("nan"), float("inf"), float("-inf"), 65504.0):
+        hit = pkg.KVCache(*(None if t is None else t.clone() for t in cache.tensors()))
+        for b in range(batch):
+            for s in [lens[b] + 1, lens[b] + 3] + list(range(lens[b] + new[b], lens[b] + 16)):
+                at = K.place(cache, b, s)
+                if at is None:
+                    continue
+                for pool, scale in ((hit.k, hit.k_scale), (hit.v, hit.v_scale)):
+                    if kind == "16bit":
+                        pool[at[0], :, at[1], ::3] = bad
+                    else:
+                        scale[at[0], :, at[1]] = bad
+                        if kind == "e4m3":
+                            pool.view(torch.uint8)[at[0], :, at[1], ::3] = 0x7f  # e4m3's NaN
+        got = pkg.tree_attention(q, hit, K.ints(lens), **args)
+        ok = torch.ones((batch, tokens), dtype=torch.bool, device=cuda)
+        ok[:, [1, 3]] = False  # they see themselves
+        assert torch.equal(got[ok], want[ok]), bad
+        assert not got[ok].isnan().any()
+        if bad != bad:
+            assert got[0, 1].isnan().any(-1).all() and got[0, 3].isnan().any(-1).all()
+
+
+def test_seen_values_that_are_not_finite(pkg, cuda):
+    """A visible NaN key makes its rows NaN, a visible NaN value its column; rows whose scores are all -infinity get
+    zeros."""
+    cache, q = _case(pkg, "16bit", torch.float16, 1, 2, 2, 1, 64, 16, [5])
+    p, at = K.place(cache, 0, 6)
+    for pool, rows in ((cache.k, slice(None)), (cache.v, 7)):
+        was = pool[p, 0, at, 7].item()
+        pool[p, 0, at, 7] = float("nan")
+        out = pkg.tree_attention(q, cache, K.ints([5]))
+        assert out[0, 1][:, rows].isnan().all() and not out[0, 0].isnan().any()
+        if rows == 7:
+            assert out[0, 1].isnan().sum() == 2
+        pool[p, 0, at, 7] = was
+    q[:] = 1.0
+    cache.k[:] = float("-inf")
+    assert not pkg.tree_attention(q, cache, K.ints([5])).any()
+
+
+@pytest.mark.parametrize("kind", FORMATS)
+def test_pages_that_are_not_there(pkg, cuda, kind):
+    """Pages of -1 or beyond the pool are not attended to, nor are slots beyond the table."""
+    table = torch.tensor([[0, -1, 2, 5], [99, 1, 3, -1], [-1, -1, -1, -1]])
+    cache = K.make_cache(pkg, kind, torch.bfloat16, (6, 2, 16, 64), table, 3)
+    q = _q((3, 4, 4, 64), torch.bfloat16, 5).to(cuda)
+    for lens in ([60, 60, 60], [62, 10, 0], [64, 1000, 2**31 - 1], [-5, 0, -2**31]):
+        K.close(pkg.tree_attention(q, cache, K.ints(lens)), *K.attention(q, cache, lens))
+
+
+def test_large_scores_and_scale(pkg, cuda):
+    """Scores of some hundreds: the exponentials' range, a running maximum that keeps rising, a scale of its own."""
+    lens = [600, 100]
+    cache, q = _case(pkg, "int8", torch.float16, 2, 3, 6, 2, 64, 32, lens)
+    q *= 8
+    ramp = torch.linspace(0.01, 3, cache.k_scale.shape[2], device=cuda)
+    cache.k_scale *= ramp
+    for scale in (1.0, 0.01, -0.5):
+        K.close(pkg.tree_attention(q, cache, K.ints(lens), scale=scale), *K.attention(q, cache, lens, scale=scale))
+
+
+def test_strided_queries_and_masks(pkg, cuda):
+    lens = [20, 50]
+    cache, _ = _case(pkg, "int8", torch.float16, 2, 5, 6, 2, 64, 16, lens)
+    qkv = _q((2, 5, 10, 64), torch.float16, 9).to(cuda)
+    odd = _q((2, 5, 6 * 64 + 1), torch.float16, 10).to(cuda)[..., 1:].unflatten(-1, (6, 64))
+    one = K.random_tree(1, 5, 6)
+    masks = [one.to(cuda), one[0].to(cuda), one[0].T.contiguous().T.to(cuda), one.to(cuda).expand(2, 5, 5),
+             torch.nn.functional.pad(one, (0, 3)).to(cuda)[..., :5]]
+    for q in (qkv[:, :, 2:8], odd, qkv[:, :, :6].transpose(1, 2).contiguous().transpose(1, 2)):
+        want = pkg.tree_attention(q.contiguous(), cache, K.ints(lens), tree_mask=one.expand(2, 5, 5).contiguous().to(cuda))
+        for mask in masks:
+            assert torch.equal(pkg.tree_attention(q, cache, K.ints(lens), tree_mask=mask), want)
+
+
+def test_offsets_beyond_32_bits(pkg, cuda):
+    pages, page = 300_000, 16
+    cache = pkg.KVCache(*(torch.zeros((pages, 8, page, 128), dtype=torch.uint8, device=cuda).view(torch.int8)
+                          for _ in range(2)), K.ints([[pages - 1, pages - 2, pages - 3]]),
+                        *(torch.zeros((pages, 8, page), device=cuda) for _ in range(2)))
+    x = _q((1, 40, 8, 128), torch.float16, 30, 1.0).to(cuda)
+    small = pkg.KVCache.allocate(1, 48, 8, 128, "int8", device=cuda, page_size=16)
+    for c in (cache, small):
+        pkg.kv_cache_append(c, x, x, K.ints([0]))
+    q = _q((1, 2, 16, 128), torch.float16, 31).to(cuda)
+    assert torch.equal(pkg.tree_attention(q, cache, K.ints([38])), pkg.tree_attention(q, small, K.ints([38])))
+    del cache
+    torch.cuda.empty_cache()
+
+
+def test_graphs_share_a_pool_and_other_streams(pkg, cuda):
+    """Two captured steps of different sizes in one memory pool, replayed in turn with other lengths and contents, and
+    eager calls on a side stream at the same time."""
+    cases = [_case(pkg, "int8", torch.float16, 2, 1, 12, 2, 128, 16, [4000, 4000]),
+             _case(pkg, "e4m3", torch.bfloat16, 1, 7, 14, 2, 64, 32, [3000], seed=5)]
+    lens = [K.ints([4000, 4000]), K.ints([3000])]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for (c, q), n in zip(cases, lens):
+            pkg.tree_attention(q, c, n)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs, outs, pool = [], [], None
+    for (c, q), n in zip(cases, lens):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            outs.append(pkg.tree_attention(q, c, n))
+        pool = graph.pool()
+        graphs.append(graph)
+    for i in range(4):
+        lens[0].copy_(K.ints([1 + 1333 * i, 4000 - 900 * i]))
+        lens[1].copy_(K.ints([3000 - 999 * i]))
+        for (c, q), n in zip(cases, lens):
+            q.copy_(_q(q.shape, q.dtype, 70 + i))
+        for which in ((0, 1), (1, 0))[i % 2]:
+            graphs[which].replay()
+            torch.cuda.synchronize()
+            (c, q), n = cases[which], lens[which]
+            want = pkg.tree_attention(q, c, n)
+            assert torch.equal(outs[which], want)
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                other = pkg.tree_attention(q, c, n)
+            here = pkg.tree_attention(q, c, n)
+            torch.cuda.synchronize()
+            assert torch.equal(other, want) and torch.equal(here, want)
+
+
+def test_empty_calls(pkg, cuda):
+    cache = pkg.KVCache.allocate(2, 32, 2, 64, "int8", device=cuda)
+    q = torch.empty((2, 0, 4, 64), dtype=torch.float16, device=cuda)
+    assert pkg.tree_attention(q, cache, K.ints([0, 0])).shape == q.shape
+
+
+def test_refusals(pkg, cuda):
+    cache = pkg.KVCache.allocate(2, 32, 2, 64, "int8", device=cuda)
+    q, lens = torch.zeros((2, 3, 4, 64), dtype=torch.float16, device=cuda), K.ints([0, 0])
+    mask = torch.zeros((3, 3), dtype=torch.bool, device=cuda)
+    for args, kw, message in [
+            ((q.cpu(), cache, lens), {}, "GPU"), ((q.float(), cache, lens), {}, "fp16 or bf16"),
+            ((q[0], cache, lens), {}, r"\[batch"), ((q[..., :32], cache, lens), {}, "heads"),
+            ((q[:, :, :3], cache, lens), {}, "heads"), ((q[:1], cache, lens[:1]), {}, "sequences"),
+            ((q, cache, lens.long()), {}, "int32"), ((q, cache, lens), {"new_lens": lens[:1]}, "new_lens"),
+            ((q, cache, lens), {"tree_mask": mask.int()}, "tree_mask"), ((q, cache, lens), {"tree_mask": mask[:2]}, "tree_mask"),
+            ((q, cache, lens), {"tree_mask": mask.expand(3, 3, 3)}, "tree_mask"),
+            ((q, cache, lens), {"tree_mask": mask.cpu()}, "tree_mask")]:
+        with pytest.raises(AssertionError, match=message):
+            pkg.tree_attention(*args, **kw)
+    with pytest.raises(Exception, match="tokens <= 128"):
+        pkg.tree_attention(torch.zeros((2, 129, 4, 64), dtype=torch.float16, device=cuda), cache, lens)

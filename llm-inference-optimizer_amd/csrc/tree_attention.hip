@@ -1,9 +1,58 @@
-// Attention of a few new tokens per sequence over a paged cache (simple form:
-// a wave per query row, one cache slot after the other).
+// Attention of a few new tokens per sequence (one, a chain or a tree of drafted
+// ones) over a paged cache of 16-bit values or one-byte codes, for gfx950.
+//
+//   S[s] = scale q . K[s],   out = sum_s exp(S[s] - m) V[s] / sum_s exp(S[s] - m)
+//
+// over the slots s that a token sees: one pass over the cache with a running
+// maximum m and sum.  A decode step reads every key and value once for a few
+// rows of q, so it is bound by HBM: the T q_heads / kv_heads rows that share a
+// key/value head are taken together.
+//
+// Products on MFMA (v_mfma_f32_16x16x32), without LDS: a wave takes tiles of
+// 32 slots and computes
+//   S^T = K Q^T   A = K: lane (r = l % 16, quad = l / 16) holds 8 elements of
+//                 the key in slot r of a 16-slot unit; B = Q^T: the lane's
+//                 column is query row l % 16.  A lane gets S of its query row
+//                 for the slots 4 quad .. 4 quad + 3 of both units -- which is
+//                 what the next product wants from it:
+//   O^T = V^T P^T B = P^T: its 8 weights; A = V^T: 8 slots of one element d.
+// The order of the summed index is free as long as A and B agree, and so is the
+// order of rows: row r of V^T tile x is element d = NV r + x (NV = DP / 16), so
+// that a lane loads NV consecutive elements of each of its 8 values, whole
+// cache lines per row, and an output row lies in consecutive registers.
+// Softmax statistics of a query row stay in its lane's column; they meet other
+// lanes only where the maximum moves, and at the end.
+//
+// Precision: codes are exact in 16 bits, so S is an fp32 sum of exact products
+// times the key's scale.  Weights times the value's scale go to the second
+// product as two bf16 parts (fp16 for an fp16 cache), high and rest: 16
+// significant bits where one part would have 8.  It costs a second MFMA, of
+// which a decode step has plenty to spare.  The maximum moves only when a score
+// passes it by 2^8, so most tiles do not rescale O; weights then are at most 2^8.
+//
+// Split: the tiles of all sequences, heads and row blocks form one line, of
+// which every workgroup takes an equal share, whatever the contexts' lengths;
+// the four waves take its tiles in turn and join in LDS.  A (sequence, head,
+// row block) that one workgroup holds whole is written at once; the pieces of
+// the others go to the workspace and tree_attention_join adds them in order.
+//
+// What may not be read: the buffer descriptor of each 16-slot unit ends with
+// the last slot in use (and is empty for a page that is not there), so that
+// loads beyond return zeros in hardware.  Slots that some rows see and others
+// do not (drafted tokens) are taken out of the second product where they hold
+// NaN or infinities, and added by themselves to the rows that see them.
+#include <type_traits>
+
 #include "kv_cache.h"
 
 namespace mi355 {
 namespace {
+
+constexpr int kTile = 32;            // slots of a tile: two units of 16
+constexpr int kWaves = 4;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLow = -1e30f;       // the running maximum before any score
+constexpr float kSlack = 8.0f;       // log2 of how far scores may pass it
 
 struct TreeArgs {
   KvCache c;
@@ -13,84 +62,714 @@ struct TreeArgs {
   const uint8_t* mask;  // [batch, tokens, tokens] by strides, or null: a chain
   int64_t mask_b, mask_t;
   int64_t qb, qt, qh;
-  int64_t rows;
-  int tokens, q_heads;
-  float scale;
+  float* partial;       // [2 workgroups][rows of a block][d], then (max, sum) [2 workgroups][rows]; null: no split
+  float2* stats;
+  int batch, tokens, q_heads, group;  // group = q_heads / kv_heads
+  int blocks;                         // row blocks of 16 MT rows
+  int grid;                           // workgroups of the first kernel
+  uint32_t page_mul, page_shift;      // unit / units per page = unit * page_mul >> page_shift
+  float scale;                        // times log2 e
 };
 
-template <typename T, int FMT> __device__ __forceinline__ float cache_elem(const void* pool, const float* scales, int64_t row, int d, int i) {
-  if constexpr (FMT == KV_16BIT) return load_elem<T>(pool, row * d + i);
-  else {
-    const uint32_t code = static_cast<const uint8_t*>(pool)[row * d + i];
-    float f[4];
-    decode4<FMT>(code, f);
-    return f[0] * scales[row];
+// One sequence: its place on the line of tiles.
+struct Seq {
+  int len, fresh, end, tiles;  // context, new tokens, slots in use, tiles per head and row block
+  __device__ __forceinline__ Seq(const TreeArgs& a, int b) {
+    const int cap = a.c.capacity();
+    len = max(0, min(a.lens[b], cap));
+    fresh = max(0, min(a.new_lens ? a.new_lens[b] : a.tokens, a.tokens));
+    end = min(len + fresh, cap);
+    tiles = max(1, (end + kTile - 1) / kTile);
+  }
+};
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// The line: sequence b has Seq::tiles * heads * blocks tiles, (head, block)
+// outermost.  `total` tiles; the first tile of sequence b is start(b).
+__device__ __forceinline__ int line_total(const TreeArgs& a, int upto) {
+  int sum = 0;
+  for (int b = threadIdx.x & 63; b < upto; b += 64) sum += Seq(a, b).tiles;
+  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+  return uniform(sum) * a.c.heads * a.blocks;
+}
+
+// The sequence that tile `at` (< total) belongs to, and its first tile.
+__device__ __forceinline__ int line_find(const TreeArgs& a, int at, int* start) {
+  const int lane = threadIdx.x & 63, hm = a.c.heads * a.blocks;
+  int before = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    const int mine = b0 + lane < a.batch ? Seq(a, b0 + lane).tiles * hm : 0;
+    int upto = mine;
+    for (int d = 1; d < 64; d *= 2) {
+      const int o = __shfl_up(upto, d);
+      if (lane >= d) upto += o;
+    }
+    const uint64_t past = __builtin_amdgcn_ballot_w64(before + upto > at);
+    if (past) {
+      const int i = __builtin_ctzll(past);
+      *start = before + uniform(__shfl(upto - mine, i));
+      return b0 + i;
+    }
+    before += uniform(__shfl(upto, 63));
+  }
+  *start = before;
+  return a.batch;
+}
+
+// Tiles per workgroup: equal shares, a whole number of tiles for each wave.
+__device__ __forceinline__ int line_share(int total, int grid) {
+  return ((total + grid - 1) / grid + kWaves - 1) / kWaves * kWaves;
+}
+
+template <int FMT> __device__ __forceinline__ constexpr int elem_bytes() { return FMT == KV_16BIT ? 2 : 1; }
+
+// The 16 slots of a unit: descriptors that end with its last slot in use.
+template <int FMT> struct Unit {
+  rsrc_t k, v, ks, vs;
+  bool whole;  // 16 slots, all there
+  __device__ __forceinline__ Unit(const TreeArgs& a, int h, int slot, int end, int page) {
+    const int upp = a.c.page_size / 16;
+    const int u = slot / 16;
+    const int in_page = u - static_cast<int>((static_cast<uint64_t>(u) * a.page_mul) >> a.page_shift) * upp;
+    int n = max(0, min(end - slot, 16));
+    if (page < 0 || page >= a.c.pages) n = 0;
+    whole = n == 16;
+    const int64_t row = n ? (static_cast<int64_t>(page) * a.c.heads + h) * a.c.page_size + 16 * in_page : 0;
+    const uint32_t bytes = static_cast<uint32_t>(n * a.c.d * elem_bytes<FMT>());
+    k = make_rsrc(static_cast<const uint8_t*>(a.c.k) + row * a.c.d * elem_bytes<FMT>(), bytes);
+    v = make_rsrc(static_cast<const uint8_t*>(a.c.v) + row * a.c.d * elem_bytes<FMT>(), bytes);
+    if constexpr (FMT != KV_16BIT) {
+      ks = make_rsrc(a.c.k_scale + row, static_cast<uint32_t>(4 * n));
+      vs = make_rsrc(a.c.v_scale + row, static_cast<uint32_t>(4 * n));
+    }
+  }
+};
+
+// Page of a unit, or -1.
+__device__ __forceinline__ int page_of(const TreeArgs& a, const int32_t* table, int slot, int end) {
+  if (slot >= end) return -1;
+  const int u = slot / 16;
+  return table[(static_cast<uint64_t>(u) * a.page_mul) >> a.page_shift];
+}
+
+// Four codes of a dword, as MFMA operands of T: two dwords.
+template <typename T, int FMT> __device__ __forceinline__ u32x2 widen_codes(uint32_t d) {
+  if constexpr (FMT == KV_INT8) {
+    return widen_i8x4<T>(d);
+  } else if constexpr (T::code == MI355_F16) {
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d, 1.0f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d, 1.0f, true))};
+  } else {
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(d, 1.0f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(d, 1.0f, true))};
   }
 }
 
-template <typename T, int FMT> __global__ __launch_bounds__(64) void tree_attention_rows(TreeArgs a) {
-  const int64_t r = blockIdx.x;
-  const int lane = threadIdx.x;
-  const int h = r % a.q_heads, kvh = h / (a.q_heads / a.c.heads);
-  const int64_t bt = r / a.q_heads, b = bt / a.tokens;
-  const int t = bt % a.tokens;
-  const int cap = a.c.capacity();
-  const int len = max(0, min(a.lens[b], cap));
-  const int fresh = max(0, min(a.new_lens ? a.new_lens[b] : a.tokens, a.tokens));
-  const int last = t < fresh ? min(len + fresh, cap) : 0;
-  float q[4], o[4] = {0, 0, 0, 0}, m = -INFINITY, sum = 0;
-  for (int i = 0; i < 4; ++i) {
-    const int d = lane + 64 * i;
-    q[i] = d < a.c.d ? load_elem<T>(a.q, b * a.qb + t * a.qt + h * a.qh + d) : 0.f;
+__device__ __forceinline__ float max_quads(float v) {  // over the 4 lanes of a column
+  {
+    const uint32_t b = as_u32(v);
+    auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    const uint32_t lo = r[0], hi = r[1];
+    v = fmaxf(as_f32(lo), as_f32(hi));
   }
-  for (int s = 0; s < last; ++s) {
-    if (s >= len) {
-      const int j = s - len;
-      if (a.mask ? a.mask[b * a.mask_b + t * a.mask_t + j] == 0 : j > t) continue;
+  {
+    const uint32_t b = as_u32(v);
+    auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    const uint32_t lo = r[0], hi = r[1];
+    v = fmaxf(as_f32(lo), as_f32(hi));
+  }
+  return v;
+}
+__device__ __forceinline__ float sum_quads(float v) {
+  {
+    const uint32_t b = as_u32(v);
+    auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    const uint32_t lo = r[0], hi = r[1];
+    v = as_f32(lo) + as_f32(hi);
+  }
+  {
+    const uint32_t b = as_u32(v);
+    auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    const uint32_t lo = r[0], hi = r[1];
+    v = as_f32(lo) + as_f32(hi);
+  }
+  return v;
+}
+
+// The keys, values and scales of a tile in a lane's registers.
+//   keys    unit u, load i: slot l % 16, elements (8-bit) 64 i + 16 quad .. + 15
+//           or (16-bit) 32 i + 8 quad .. + 7
+//   values  unit u, slot 4 quad + j, elements NV (l % 16) .. + NV - 1
+//   scales  unit u, slots 4 quad .. 4 quad + 3
+template <typename T, int FMT, int DP> struct Tile {
+  static constexpr int ES = FMT == KV_16BIT ? 2 : 1;
+  static constexpr int NV = DP / 16;
+  static constexpr int KL = DP * ES / 64;     // 16-byte key loads per unit
+  static constexpr int VD = NV * ES / 4;      // dwords of a value per lane
+  u32x4 k[2][KL];
+  uint32_t v[2][4][VD];
+  f32x4 ks[2], vs[2];
+
+  __device__ __forceinline__ void load_keys(const Unit<FMT>& u0, const Unit<FMT>& u1, int d) {
+    const int lane = threadIdx.x & 63, r = lane & 15, quad = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < KL; ++i) {
+      const int byte = 64 * i + 16 * quad;
+      const uint32_t off = byte < d * ES ? static_cast<uint32_t>(r * d * ES + byte) : kOob;
+      k[0][i] = buf_load16_cached(u0.k, off);
+      k[1][i] = buf_load16_cached(u1.k, off);
     }
-    const int64_t row = a.c.row(b, s, kvh);
-    if (row < 0) continue;
-    float dot = 0;
-    for (int i = 0; i < 4; ++i) {
-      const int d = lane + 64 * i;
-      if (d < a.c.d) dot += q[i] * cache_elem<T, FMT>(a.c.k, a.c.k_scale, row, a.c.d, d);
-    }
-    const float score = wave_allreduce_sum(dot) * a.scale;
-    if (score == -INFINITY) continue;
-    const float top = fmaxf(m, score);
-    const float was = expf(m - top), p = expf(score - top);
-    m = top;
-    sum = sum * was + p;
-    for (int i = 0; i < 4; ++i) {
-      const int d = lane + 64 * i;
-      if (d < a.c.d) o[i] = o[i] * was + p * cache_elem<T, FMT>(a.c.v, a.c.v_scale, row, a.c.d, d);
+    if constexpr (FMT != KV_16BIT) {
+      ks[0] = __builtin_bit_cast(f32x4, buf_load16_cached(u0.ks, 16u * quad));
+      ks[1] = __builtin_bit_cast(f32x4, buf_load16_cached(u1.ks, 16u * quad));
     }
   }
-  for (int i = 0; i < 4; ++i) {
-    const int d = lane + 64 * i;
-    if (d < a.c.d) store_elem<T>(a.out, r * a.c.d + d, sum == 0.f ? 0.f : o[i] / sum);
+
+  __device__ __forceinline__ void load_values(const Unit<FMT>& u0, const Unit<FMT>& u1, int d) {
+    const int lane = threadIdx.x & 63, r = lane & 15, quad = lane >> 4;
+    if constexpr (FMT != KV_16BIT) {
+      vs[0] = __builtin_bit_cast(f32x4, buf_load16_cached(u0.vs, 16u * quad));
+      vs[1] = __builtin_bit_cast(f32x4, buf_load16_cached(u1.vs, 16u * quad));
+    }
+    const uint32_t first = NV * r < d ? static_cast<uint32_t>((4 * quad * d + NV * r) * ES) : kOob;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const rsrc_t rsrc = u ? u1.v : u0.v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = j * d * ES;  // uniform: the scalar offset of the load
+        if constexpr (VD == 1) {
+          v[u][j][0] = __builtin_amdgcn_raw_buffer_load_b32(rsrc, first, at, 0);
+        } else if constexpr (VD == 2) {
+          const u32x2 t = __builtin_amdgcn_raw_buffer_load_b64(rsrc, first, at, 0);
+          v[u][j][0] = t[0];
+          v[u][j][1] = t[1];
+        } else {
+#pragma unroll
+          for (int w = 0; w < VD / 4; ++w) {
+            const u32x4 t = __builtin_amdgcn_raw_buffer_load_b128(rsrc, first + 16 * w, at, 0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[u][j][4 * w + e] = t[e];
+          }
+        }
+      }
+    }
+  }
+
+  // MFMA k-step n (32 of the DP elements) of unit u's keys.
+  __device__ __forceinline__ u32x4 keys(int u, int n) const {
+    if constexpr (FMT == KV_16BIT) {
+      return k[u][n];
+    } else {
+      const u32x2 lo = widen_codes<T, FMT>(k[u][n / 2][2 * (n & 1)]), hi = widen_codes<T, FMT>(k[u][n / 2][2 * (n & 1) + 1]);
+      return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    }
+  }
+
+  // Elements x (even) and x + 1 of the 8 values: two V^T operands.
+  __device__ __forceinline__ void values2(int x, u32x4& even, u32x4& odd) const {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {  // the slot pairs of a k-step
+      const int u = p >> 1, j = 2 * (p & 1);
+      if constexpr (FMT == KV_16BIT) {
+        const uint32_t a = v[u][j][x / 2], b = v[u][j + 1][x / 2];
+        even[p] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+        odd[p] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+      } else if constexpr (FMT == KV_E4M3) {
+        const uint32_t a8 = v[u][j][x / 4], b8 = v[u][j + 1][x / 4];
+        uint32_t a, b;
+        if (x & 2) {
+          a = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a8, 1.0f, true));
+          b = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b8, 1.0f, true));
+        } else {
+          a = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a8, 1.0f, false));
+          b = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b8, 1.0f, false));
+        }
+        even[p] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+        odd[p] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+      } else {
+        // the upper half of an fp32 integer below 2^8 is its bf16 pattern
+        const uint32_t a8 = v[u][j][x / 4] >> (8 * (x & 3)), b8 = v[u][j + 1][x / 4] >> (8 * (x & 3));
+        even[p] = __builtin_amdgcn_perm(as_u32(static_cast<float>(static_cast<int8_t>(b8 & 0xff))),
+                                        as_u32(static_cast<float>(static_cast<int8_t>(a8 & 0xff))), 0x07060302u);
+        odd[p] = __builtin_amdgcn_perm(as_u32(static_cast<float>(static_cast<int8_t>((b8 >> 8) & 0xff))),
+                                       as_u32(static_cast<float>(static_cast<int8_t>((a8 >> 8) & 0xff))), 0x07060302u);
+      }
+    }
+  }
+
+  // Slots of this lane's 8 (bit 4 u + j) whose value has a NaN or an infinity
+  // in any lane; those are zeroed.
+  __device__ __forceinline__ uint32_t take_out_non_finite() {
+    uint32_t bad = 0;
+    if constexpr (FMT == KV_INT8) return 0;
+    const int quad = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        bool hit = false;
+#pragma unroll
+        for (int w = 0; w < VD; ++w) {
+          const uint32_t e = v[u][j][w];
+          if constexpr (FMT == KV_E4M3) {
+#pragma unroll
+            for (int b = 0; b < 32; b += 8) hit |= ((e >> b) & 0x7f) == 0x7f;
+          } else {
+            constexpr uint32_t ex = T::code == MI355_F16 ? 0x7c00u : 0x7f80u;
+            hit |= (e & ex) == ex || ((e >> 16) & ex) == ex;
+          }
+        }
+        const uint64_t any = __builtin_amdgcn_ballot_w64(hit);
+        if ((any >> (16 * quad)) & 0xffff) {
+          bad |= 1u << (4 * u + j);
+#pragma unroll
+          for (int w = 0; w < VD; ++w) v[u][j][w] = 0;
+        }
+      }
+    }
+    return bad;
+  }
+};
+
+template <int FMT, int DP, int MT> constexpr int min_waves() { return MT == 1 && DP <= 128 ? 3 : DP * MT <= 256 ? 2 : 1; }
+
+template <typename T, int FMT, int DP, int MT>
+__global__ __launch_bounds__(64 * kWaves, (min_waves<FMT, DP, MT>())) void tree_attention_split(TreeArgs a) {
+  typedef typename T::bits bits;
+  typedef Tile<T, FMT, DP> KvTile;
+  constexpr int NV = KvTile::NV, NQ = DP / 32, ROWS = 16 * MT, PITCH = DP + 4;
+  // the weights' type in the second product: codes and bf16 values are exact in bf16
+  typedef typename std::conditional<FMT == KV_16BIT, T, BF16>::type VT;
+  __shared__ float joined[kWaves][ROWS][PITCH];
+  __shared__ float wave_max[kWaves][ROWS], wave_sum[kWaves][ROWS];
+
+  const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+  const int wave = uniform(threadIdx.x >> 6);
+  const int d = a.c.d, hm_count = a.c.heads * a.blocks;
+
+  // this workgroup's tiles [at, last) of the line, or one (head, block) of one sequence
+  int at, last, b, start;
+  if (a.partial) {
+    const int share = line_share(line_total(a, a.batch), a.grid);
+    at = static_cast<int>(blockIdx.x) * share;
+    last = at + share;
+    b = line_find(a, at, &start);
+  } else {
+    b = blockIdx.x / hm_count;
+    start = 0;
+    at = (blockIdx.x % hm_count) * uniform(Seq(a, b).tiles);
+    last = at + 1;  // the first tile; widened to the whole below
+  }
+  const int line_first = at;
+
+  while (b < a.batch && at < last) {
+    const Seq s(a, b);
+    const int len = uniform(s.len), fresh = uniform(s.fresh), tiles = uniform(s.tiles), end = uniform(s.end);
+    const int hm = (at - start) / tiles, t0 = at - start - hm * tiles;
+    if (hm >= hm_count) {
+      start += tiles * hm_count;
+      ++b;
+      continue;
+    }
+    if (!a.partial) last = at + tiles;
+    const int t1 = min(tiles, t0 + last - at);
+    const int h = hm / a.blocks, row0 = (hm % a.blocks) * ROWS;
+    const int rows = min(ROWS, a.tokens * a.group - row0);
+    const int32_t* table = a.c.table + static_cast<int64_t>(b) * a.c.table_stride;
+
+    // Q^T operands: 16-byte packets of this lane's query rows, elements as the keys'
+    u32x4 q[MT][NQ];
+    int token[MT];  // of the lane's query row; fresh or more: none
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int r = row0 + 16 * m + col;
+      const int t = r / a.group, g = r - t * a.group;
+      token[m] = t;
+      const bool in = 16 * m + col < rows && t < fresh;
+      const bits* qr = static_cast<const bits*>(a.q) + b * a.qb + t * a.qt + (static_cast<int64_t>(h) * a.group + g) * a.qh;
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        const int e = FMT == KV_16BIT ? 32 * n + 8 * quad : 64 * (n / 2) + 16 * quad + 8 * (n & 1);
+        q[m][n] = in && e < d ? *reinterpret_cast<const u32x4*>(qr + e) : u32x4{0, 0, 0, 0};
+      }
+    }
+
+    f32x4 o[MT][NV];
+    float top[MT], sum[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      top[m] = kLow;
+      sum[m] = 0.f;
+#pragma unroll
+      for (int x = 0; x < NV; ++x) o[m][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    KvTile kv;
+    int tile = t0 + wave;
+    // nothing is loaded for tiles from t1 on: their units are empty
+    const int stop = min(end, t1 * kTile);
+    int p0 = page_of(a, table, tile * kTile, stop), p1 = page_of(a, table, tile * kTile + 16, stop);
+    bool whole;
+    {
+      const Unit<FMT> u0(a, h, tile * kTile, stop, p0), u1(a, h, tile * kTile + 16, stop, p1);
+      whole = u0.whole && u1.whole;
+      kv.load_keys(u0, u1, d);
+      kv.load_values(u0, u1, d);
+    }
+    bool there0 = p0 >= 0 && p0 < a.c.pages, there1 = p1 >= 0 && p1 < a.c.pages;
+    p0 = page_of(a, table, (tile + kWaves) * kTile, stop);
+    p1 = page_of(a, table, (tile + kWaves) * kTile + 16, stop);
+
+    for (; tile < t1; tile += kWaves) {
+      f32x4 sc[MT][2];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) sc[m][0] = sc[m][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        const u32x4 k0 = kv.keys(0, n), k1 = kv.keys(1, n);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          sc[m][0] = mfma16<T>(k0, q[m][n], sc[m][0]);
+          sc[m][1] = mfma16<T>(k1, q[m][n], sc[m][1]);
+        }
+      }
+      float kscale[2][4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) kscale[u][j] = FMT == KV_16BIT ? a.scale : a.scale * kv.ks[u][j];
+
+      // the next tile's keys, while this one's weights are computed
+      const Unit<FMT> n0(a, h, (tile + kWaves) * kTile, stop, p0), n1(a, h, (tile + kWaves) * kTile + 16, stop, p1);
+      kv.load_keys(n0, n1, d);
+
+      const bool masked = !whole || (tile + 1) * kTile > len;
+      uint32_t seen[MT], bad = 0;  // bit 4 u + j
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        seen[m] = 0xff;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sc[m][u][j] *= kscale[u][j];
+      }
+      if (masked) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          seen[m] = 0;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int slot = tile * kTile + 16 * u + 4 * quad + j, i = slot - len;
+              bool see = u ? there1 : there0;
+              if (i >= 0)
+                see = see && i < fresh && token[m] < fresh &&
+                      (a.mask ? a.mask[b * a.mask_b + token[m] * a.mask_t + i] != 0 : i <= token[m]);
+              if (see) seen[m] |= 1u << (4 * u + j);
+              else sc[m][u][j] = -INFINITY;
+            }
+          }
+        }
+        bad = kv.take_out_non_finite();
+      }
+
+      u32x4 hi[MT], lo[MT];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        float most = fmaxf(fmaxf(fmaxf(sc[m][0][0], sc[m][0][1]), fmaxf(sc[m][0][2], sc[m][0][3])),
+                           fmaxf(fmaxf(sc[m][1][0], sc[m][1][1]), fmaxf(sc[m][1][2], sc[m][1][3])));
+        if (__builtin_amdgcn_ballot_w64(most > top[m] + kSlack)) {
+          const float now = fmaxf(top[m], max_quads(most));
+          const float f = __builtin_amdgcn_exp2f(top[m] - now);
+          top[m] = now;
+          sum[m] *= f;
+#pragma unroll
+          for (int x = 0; x < NV; ++x)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[m][x][i] *= f;
+        }
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          w[e] = __builtin_amdgcn_exp2f(sc[m][e >> 2][e & 3] - top[m]);
+          sum[m] += w[e];
+          if constexpr (FMT != KV_16BIT) w[e] *= kv.vs[e >> 2][e & 3];
+        }
+        if (masked) {  // a scale that nobody sees may be anything
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e] = (seen[m] >> e) & 1 ? w[e] : 0.f;
+        }
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          hi[m][p] = narrow2<VT>(f32x2{w[2 * p], w[2 * p + 1]});
+          const f32x2 back = widen2<VT>(hi[m][p]);
+          lo[m][p] = narrow2<VT>(f32x2{w[2 * p] - back.x, w[2 * p + 1] - back.y});
+        }
+        if (masked && __builtin_amdgcn_ballot_w64(bad != 0)) {
+          // values that are not finite, for the rows that see them: element by element
+#pragma unroll 1
+          for (int e = 0; e < 32; ++e) {
+            const int from = 16 * (e >> 3) + col;  // the lane with this slot's weight: quad e / 8, bit e % 8
+            if (!uniform(__shfl(static_cast<int>(bad >> (e & 7)), 16 * (e >> 3)) & 1)) continue;
+            float we = w[0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) we = (e & 7) == i ? w[i] : we;
+            we = __shfl(we, from);
+            const bool see = (__shfl(static_cast<int>(seen[m] >> (e & 7)), from) & 1) != 0;
+            const int slot = tile * kTile + 16 * ((e >> 2) & 1) + 4 * (e >> 3) + (e & 3);
+            const int64_t row = a.c.row(b, slot, h);
+            if (row < 0 || !see) continue;
+#pragma unroll
+            for (int x = 0; x < NV; ++x)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int el = NV * (4 * quad + i) + x;
+                if (el >= d) continue;
+                float val;
+                if constexpr (FMT == KV_16BIT) {
+                  val = load_elem<T>(a.c.v, row * d + el);
+                } else {
+                  float f[4];
+                  decode4<FMT>(static_cast<const uint8_t*>(a.c.v)[row * d + el], f);
+                  val = f[0];
+                }
+                o[m][x][i] = fmaf(we, val, o[m][x][i]);
+              }
+          }
+        }
+      }
+
+#pragma unroll
+      for (int x = 0; x < NV; x += 2) {
+        u32x4 even, odd;
+        kv.values2(x, even, odd);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          o[m][x] = mfma16<VT>(even, hi[m], o[m][x]);
+          o[m][x] = mfma16<VT>(even, lo[m], o[m][x]);
+          o[m][x + 1] = mfma16<VT>(odd, hi[m], o[m][x + 1]);
+          o[m][x + 1] = mfma16<VT>(odd, lo[m], o[m][x + 1]);
+        }
+      }
+      kv.load_values(n0, n1, d);
+      whole = n0.whole && n1.whole;
+      there0 = p0 >= 0 && p0 < a.c.pages;
+      there1 = p1 >= 0 && p1 < a.c.pages;
+      p0 = page_of(a, table, (tile + 2 * kWaves) * kTile, stop);
+      p1 = page_of(a, table, (tile + 2 * kWaves) * kTile + 16, stop);
+    }
+
+    // join the waves: common maximum, scaled sums
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      sum[m] = sum_quads(sum[m]);
+      if (quad == 0) {
+        wave_max[wave][16 * m + col] = top[m];
+        wave_sum[wave][16 * m + col] = sum[m];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int r = 16 * m + col;
+      const float f = __builtin_amdgcn_exp2f(
+          top[m] - fmaxf(fmaxf(wave_max[0][r], wave_max[1][r]), fmaxf(wave_max[2][r], wave_max[3][r])));
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int x = 0; x < NV; x += 4)
+          *reinterpret_cast<f32x4*>(&joined[wave][r][NV * (4 * quad + i) + x]) =
+              f32x4{o[m][x][i] * f, o[m][x + 1][i] * f, o[m][x + 2][i] * f, o[m][x + 3][i] * f};
+    }
+    __syncthreads();
+    const bool cut = t0 > 0 || t1 < tiles;
+    const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (at == line_first ? 0 : 1);
+    for (int e = threadIdx.x; e < rows * (d / 4); e += 64 * kWaves) {
+      const int r = e / (d / 4), c = 4 * (e - r * (d / 4));
+      const float most = fmaxf(fmaxf(wave_max[0][r], wave_max[1][r]), fmaxf(wave_max[2][r], wave_max[3][r]));
+      float total = 0.f;
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        total += wave_sum[w][r] * __builtin_amdgcn_exp2f(wave_max[w][r] - most);
+        v += *reinterpret_cast<const f32x4*>(&joined[w][r][c]);
+      }
+      if (cut) {
+        *reinterpret_cast<f32x4*>(a.partial + (slot * ROWS + r) * d + c) = v;
+        if (c == 0) a.stats[slot * ROWS + r] = float2{most, total};
+      } else {
+        const int t = (row0 + r) / a.group, g = row0 + r - t * a.group;
+        const float inv = 1.0f / total;
+        const bool none = t >= fresh || total == 0.f;
+        bits* out = static_cast<bits*>(a.out) +
+                    ((static_cast<int64_t>(b) * a.tokens + t) * a.q_heads + h * a.group + g) * d + c;
+        *reinterpret_cast<u32x2*>(out) = none ? u32x2{0, 0} : u32x2{narrow2<T>(f32x2{v[0] * inv, v[1] * inv}),
+                                                                     narrow2<T>(f32x2{v[2] * inv, v[3] * inv})};
+      }
+    }
+    __syncthreads();
+    at += t1 - t0;
   }
 }
 
-template <typename T> int tree_typed(const TreeArgs& a, int fmt, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>(a.rows));
+// Adds the pieces of one query row that was cut: workgroups of the first
+// kernel in order, 8 groups of lanes taking every eighth piece.
+template <typename T>
+__global__ __launch_bounds__(256) void tree_attention_join(TreeArgs a, int block_rows) {
+  typedef typename T::bits bits;
+  const int64_t qrow = blockIdx.x;
+  const int hq = static_cast<int>(qrow % a.q_heads);
+  const int64_t bt = qrow / a.q_heads;
+  const int b = static_cast<int>(bt / a.tokens), t = static_cast<int>(bt % a.tokens);
+  const int h = hq / a.group, r = t * a.group + hq - h * a.group;
+  const int block = r / block_rows, rr = r - block * block_rows;
+  const Seq s(a, b);
+  const int tiles = uniform(s.tiles);
+  const int share = line_share(line_total(a, a.batch), a.grid);
+  const int first = line_total(a, b) + (h * a.blocks + block) * tiles;
+  const int w0 = first / share, w1 = (first + tiles - 1) / share;
+  if (w0 == w1) return;  // written by the first kernel
+
+  __shared__ f32x4 acc[8][64];
+  __shared__ float group_sum[8];
+  float most = kLow;
+  for (int w = w0; w <= w1; ++w) {
+    const int64_t slot = 2 * static_cast<int64_t>(w) + (max(first, w * share) == w * share ? 0 : 1);
+    most = fmaxf(most, a.stats[slot * block_rows + rr].x);
+  }
+  const int part = threadIdx.x / 32;
+  f32x4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  float total = 0.f;
+  for (int w = w0 + part; w <= w1; w += 8) {
+    const int64_t slot = 2 * static_cast<int64_t>(w) + (max(first, w * share) == w * share ? 0 : 1);
+    const float2 st = a.stats[slot * block_rows + rr];
+    const float f = __builtin_amdgcn_exp2f(st.x - most);
+    total += st.y * f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int c = 4 * (threadIdx.x % 32 + 32 * i);
+      if (c < a.c.d) {
+        const f32x4 p = *reinterpret_cast<const f32x4*>(a.partial + (slot * block_rows + rr) * a.c.d + c);
+        v[i] += p * f;
+      }
+    }
+  }
+  acc[part][threadIdx.x % 32] = v[0];
+  acc[part][32 + threadIdx.x % 32] = v[1];
+  if (threadIdx.x % 32 == 0) group_sum[part] = total;
+  __syncthreads();
+  const int c = 4 * threadIdx.x;
+  if (c >= a.c.d) return;
+  f32x4 o = acc[0][threadIdx.x];
+  total = group_sum[0];
+#pragma unroll
+  for (int p = 1; p < 8; ++p) {
+    o += acc[p][threadIdx.x];
+    total += group_sum[p];
+  }
+  const float inv = 1.0f / total;
+  const bool none = t >= s.fresh || total == 0.f;
+  *reinterpret_cast<u32x2*>(static_cast<bits*>(a.out) + qrow * a.c.d + c) =
+      none ? u32x2{0, 0} : u32x2{narrow2<T>(f32x2{o[0] * inv, o[1] * inv}), narrow2<T>(f32x2{o[2] * inv, o[3] * inv})};
+}
+
+// Row blocks and grid of a call.
+struct Plan {
+  int mt, blocks, grid;
+  int64_t partial_bytes, bytes;  // of the workspace; 0: no split
+};
+
+Plan plan(const mi355_kv_cache& c, int64_t batch, int64_t tokens, int64_t q_heads, int cus) {
+  Plan p{};
+  const int64_t rows = tokens * (q_heads / c.kv_heads);
+  p.mt = rows <= 16 ? 1 : rows <= 32 || c.head_dim > 128 ? 2 : 4;
+  p.blocks = static_cast<int>((rows + 16 * p.mt - 1) / (16 * p.mt));
+  const int64_t pieces = batch * c.kv_heads * p.blocks;
+  const int64_t tiles = (c.table_width * c.page_size + kTile - 1) / kTile;  // of the longest possible context
+  p.grid = static_cast<int>(pieces);
+  if (tiles <= 2 * kWaves || pieces * tiles > 0x7fffffff - 65536 * kWaves) return p;
+  const int64_t wanted = (pieces * tiles + kWaves - 1) / kWaves;
+  const int64_t most = static_cast<int64_t>(cus) * (p.mt == 1 && c.head_dim <= 128 ? 3 : c.head_dim * p.mt <= 256 ? 2 : 1);
+  p.grid = static_cast<int>(wanted < most ? wanted : most);
+  p.partial_bytes = 2 * int64_t{p.grid} * 16 * p.mt * c.head_dim * 4;
+  p.bytes = p.partial_bytes + 2 * int64_t{p.grid} * 16 * p.mt * 8;
+  return p;
+}
+
+template <typename T, int FMT> int tree_typed(const TreeArgs& a, const Plan& p, hipStream_t s) {
   static const char* what = "tree_attention launch";
-  if (fmt == KV_INT8) return launch(tree_attention_rows<T, KV_INT8>, grid, 64, 0, a, s, what);
-  if (fmt == KV_E4M3) return launch(tree_attention_rows<T, KV_E4M3>, grid, 64, 0, a, s, what);
-  return launch(tree_attention_rows<T, KV_16BIT>, grid, 64, 0, a, s, what);
+  const dim3 grid(static_cast<unsigned>(p.grid));
+  constexpr int block = 64 * kWaves;
+#define MI355_TREE(DP, MT) return launch(tree_attention_split<T, FMT, DP, MT>, grid, block, 0, a, s, what)
+  if (a.c.d <= 64) {
+    if (p.mt == 1) MI355_TREE(64, 1);
+    if (p.mt == 2) MI355_TREE(64, 2);
+    MI355_TREE(64, 4);
+  }
+  if (a.c.d <= 128) {
+    if (p.mt == 1) MI355_TREE(128, 1);
+    if (p.mt == 2) MI355_TREE(128, 2);
+    MI355_TREE(128, 4);
+  }
+  if (p.mt == 1) MI355_TREE(256, 1);
+  MI355_TREE(256, 2);
+#undef MI355_TREE
 }
 
 }  // namespace
 
-int64_t tree_attention_workspace(const mi355_kv_cache&, int64_t, int64_t, int64_t) { return 0; }
+int64_t tree_attention_workspace(const mi355_kv_cache& cache, int64_t batch, int64_t tokens, int64_t q_heads) {
+  int cus = 0;
+  if (compute_units(&cus) != MI355_OK) return 0;
+  return plan(cache, batch, tokens, q_heads, cus).bytes;
+}
 
 int tree_attention_launch(const mi355_kv_cache& cache, const void* q, void* out, const int32_t* lens,
                           const int32_t* new_lens, const uint8_t* mask, int64_t mask_b, int64_t mask_t, int64_t batch,
-                          int tokens, int q_heads, const int64_t* q_strides, float scale, int dtype, void*, int64_t,
-                          hipStream_t stream) {
-  const TreeArgs a{kv_cache_args(cache), q, out, lens, new_lens, mask, mask_b, mask_t, q_strides[0], q_strides[1],
-                   q_strides[2], batch * tokens * q_heads, tokens, q_heads, scale};
-  return dtype == MI355_F16 ? tree_typed<F16>(a, cache.format, stream) : tree_typed<BF16>(a, cache.format, stream);
+                          int tokens, int q_heads, const int64_t* q_strides, float scale, int dtype, void* work,
+                          int64_t work_bytes, hipStream_t stream) {
+  int cus = 0;
+  const int st = compute_units(&cus);
+  if (st != MI355_OK) return st;
+  Plan p = plan(cache, batch, tokens, q_heads, cus);
+  TreeArgs a{kv_cache_args(cache), q, out, lens, new_lens, mask, mask_b, mask_t, q_strides[0], q_strides[1],
+             q_strides[2], nullptr, nullptr, static_cast<int>(batch), tokens, q_heads,
+             q_heads / static_cast<int>(cache.kv_heads), p.blocks, 0, 0, 0, scale * kLog2e};
+  if (p.bytes > 0 && work != nullptr && work_bytes >= p.bytes) {
+    a.partial = static_cast<float*>(work);
+    a.stats = reinterpret_cast<float2*>(static_cast<uint8_t*>(work) + p.partial_bytes);
+  } else {
+    p.grid = static_cast<int>(batch * cache.kv_heads * p.blocks);
+  }
+  a.grid = p.grid;
+  // unit / units_per_page for unit < 2^27: ceil(2^(31 + L) / u) with L = ceil(log2 u) fits 32 bits, and the product
+  // is off by less than 2^L in 2^(31 + L), too little to reach the next integer
+  const uint32_t upp = static_cast<uint32_t>(cache.page_size / 16);
+  uint32_t log = 0;
+  while ((uint64_t{1} << log) < upp) ++log;
+  a.page_mul = static_cast<uint32_t>(((uint64_t{1} << (31 + log)) + upp - 1) / upp);
+  a.page_shift = 31 + log;
+  int r;
+  if (dtype == MI355_F16) {
+    r = cache.format == KV_INT8   ? tree_typed<F16, KV_INT8>(a, p, stream)
+        : cache.format == KV_E4M3 ? tree_typed<F16, KV_E4M3>(a, p, stream)
+                                  : tree_typed<F16, KV_16BIT>(a, p, stream);
+  } else {
+    r = cache.format == KV_INT8   ? tree_typed<BF16, KV_INT8>(a, p, stream)
+        : cache.format == KV_E4M3 ? tree_typed<BF16, KV_E4M3>(a, p, stream)
+                                  : tree_typed<BF16, KV_16BIT>(a, p, stream);
+  }
+  if (r != MI355_OK || a.partial == nullptr) return r;
+  const int block_rows = 16 * p.mt;
+  void* args[] = {&a, const_cast<int*>(&block_rows)};
+  const void* join = dtype == MI355_F16 ? reinterpret_cast<const void*>(tree_attention_join<F16>)
+                                        : reinterpret_cast<const void*>(tree_attention_join<BF16>);
+  return hip_status(hipLaunchKernel(join, dim3(static_cast<unsigned>(batch * tokens * q_heads)), dim3(256), args, 0,
+                                    stream),
+                    "tree_attention join launch");
 }
 
 }  // namespace mi355

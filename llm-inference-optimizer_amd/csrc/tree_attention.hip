@@ -39,8 +39,9 @@
 // What may not be read: the buffer descriptor of each 16-slot unit ends with
 // the last slot in use (and is empty for a page that is not there), so that
 // loads beyond return zeros in hardware.  Slots that some rows see and others
-// do not (drafted tokens) are taken out of the second product where they hold
-// NaN or infinities, and added by themselves to the rows that see them.
+// do not (drafted tokens) keep NaN and infinities out of the second product,
+// which would spread them to every row; the rows that see them get them added
+// at the end.
 #include <type_traits>
 
 #include "kv_cache.h"
@@ -62,60 +63,103 @@ struct TreeArgs {
   const uint8_t* mask;  // [batch, tokens, tokens] by strides, or null: a chain
   int64_t mask_b, mask_t;
   int64_t qb, qt, qh;
-  float* partial;       // [2 workgroups][rows of a block][d], then (max, sum) [2 workgroups][rows]; null: no split
-  float2* stats;
+  float* partial;       // [2 workgroups][rows of a block][d]; null: no split
+  float2* stats;        // [2 workgroups][rows of a block]: maximum and sum
+  int32_t* starts;      // [1 + batch]: the workgroups' share of tiles, the first tile of each sequence
   int batch, tokens, q_heads, group;  // group = q_heads / kv_heads
-  int blocks;                         // row blocks of 16 MT rows
+  int mt, blocks;                     // row blocks of 16 mt rows
   int grid;                           // workgroups of the first kernel
   uint32_t page_mul, page_shift;      // unit / units per page = unit * page_mul >> page_shift
   float scale;                        // times log2 e
 };
 
-// One sequence: its place on the line of tiles.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Scalar load of read-only memory at a uniform index: counted apart from the
+// vector loads in flight, which a vector load of a page number would wait for.
+__device__ __forceinline__ int32_t scalar_load(const int32_t* p, int64_t i) {
+  typedef const __attribute__((address_space(4))) int32_t* constant_ptr;
+  return reinterpret_cast<constant_ptr>(reinterpret_cast<uintptr_t>(p))[i];
+}
+
+// One sequence: its context, new tokens, slots in use, and tiles per head and
+// row block.
 struct Seq {
-  int len, fresh, end, tiles;  // context, new tokens, slots in use, tiles per head and row block
-  __device__ __forceinline__ Seq(const TreeArgs& a, int b) {
+  int len, fresh, end, tiles;
+  __device__ __forceinline__ Seq(const TreeArgs& a, int len_, int fresh_) {
     const int cap = a.c.capacity();
-    len = max(0, min(a.lens[b], cap));
-    fresh = max(0, min(a.new_lens ? a.new_lens[b] : a.tokens, a.tokens));
+    len = max(0, min(len_, cap));
+    fresh = max(0, min(fresh_, a.tokens));
     end = min(len + fresh, cap);
     tiles = max(1, (end + kTile - 1) / kTile);
   }
+  // by a scalar b
+  static __device__ __forceinline__ Seq of(const TreeArgs& a, int b) {
+    return Seq(a, scalar_load(a.lens, b), a.new_lens ? scalar_load(a.new_lens, b) : a.tokens);
+  }
+  // the tiles of sequence b0 + lane, 0 beyond the last
+  static __device__ __forceinline__ int of_lane(const TreeArgs& a, int b0) {
+    const int b = b0 + static_cast<int>(threadIdx.x & 63);
+    return b < a.batch ? Seq(a, a.lens[b], a.new_lens ? a.new_lens[b] : a.tokens).tiles : 0;
+  }
 };
 
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-
-// The line: sequence b has Seq::tiles * heads * blocks tiles, (head, block)
-// outermost.  `total` tiles; the first tile of sequence b is start(b).
-__device__ __forceinline__ int line_total(const TreeArgs& a, int upto) {
-  int sum = 0;
-  for (int b = threadIdx.x & 63; b < upto; b += 64) sum += Seq(a, b).tiles;
-  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
-  return uniform(sum) * a.c.heads * a.blocks;
+template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_add(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+// Sum of v over this lane and those before it.
+__device__ __forceinline__ int wave_scan(int v) {
+  v = dpp_add<0x111, 0xf>(v);  // row_shr:1
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  v = dpp_add<0x118, 0xf>(v);
+  v = dpp_add<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+  v = dpp_add<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
+  return v;
 }
 
-// The sequence that tile `at` (< total) belongs to, and its first tile.
-__device__ __forceinline__ int line_find(const TreeArgs& a, int at, int* start) {
-  const int lane = threadIdx.x & 63, hm = a.c.heads * a.blocks;
-  int before = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    const int mine = b0 + lane < a.batch ? Seq(a, b0 + lane).tiles * hm : 0;
-    int upto = mine;
-    for (int d = 1; d < 64; d *= 2) {
-      const int o = __shfl_up(upto, d);
-      if (lane >= d) upto += o;
-    }
-    const uint64_t past = __builtin_amdgcn_ballot_w64(before + upto > at);
-    if (past) {
-      const int i = __builtin_ctzll(past);
-      *start = before + uniform(__shfl(upto - mine, i));
-      return b0 + i;
-    }
-    before += uniform(__shfl(upto, 63));
+// The line of tiles: sequence b has Seq::tiles of them for each of its heads
+// and row blocks, head and block outermost.
+struct Line {
+  int first;  // tiles per head and block, of this lane's sequence among the first 64 and those before
+  int total;  // of all sequences
+  __device__ __forceinline__ explicit Line(const TreeArgs& a) {
+    first = wave_scan(Seq::of_lane(a, 0));
+    total = __builtin_amdgcn_readlane(first, 63);
+    for (int b0 = 64; b0 < a.batch; b0 += 64) total += __builtin_amdgcn_readlane(wave_scan(Seq::of_lane(a, b0)), 63);
+    total *= a.c.heads * a.blocks;
   }
-  *start = before;
-  return a.batch;
-}
+  // The sequence that tile `at` belongs to (batch: none) and its first tile.
+  __device__ __forceinline__ int find(const TreeArgs& a, int at, int* start) const {
+    const int hm = a.c.heads * a.blocks;
+    int before = 0, upto = first;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+      if (b0) upto = wave_scan(Seq::of_lane(a, b0));
+      const uint64_t past = __builtin_amdgcn_ballot_w64((before + upto) * hm > at);
+      if (past) {
+        const int i = uniform(__builtin_ctzll(past));
+        *start = (before + (i ? __builtin_amdgcn_readlane(upto, i - 1) : 0)) * hm;
+        return b0 + i;
+      }
+      before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    *start = before * hm;
+    return a.batch;
+  }
+  // For the join: the share, then the first tile of every sequence.
+  __device__ __forceinline__ void write(const TreeArgs& a, int share, int32_t* to) const {
+    const int lane = threadIdx.x & 63;
+    if (lane == 0) to[0] = share;
+    int before = 0, upto = first;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+      if (b0) upto = wave_scan(Seq::of_lane(a, b0));
+      const int b = b0 + lane + 1;
+      if (b < a.batch) to[1 + b] = (before + upto) * a.c.heads * a.blocks;
+      before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    if (lane == 0) to[1] = 0;
+  }
+};
 
 // Tiles per workgroup: equal shares, a whole number of tiles for each wave.
 __device__ __forceinline__ int line_share(int total, int grid) {
@@ -146,11 +190,12 @@ template <int FMT> struct Unit {
   }
 };
 
-// Page of a unit, or -1.
+// Page of a unit, or -1.  In a scalar register, as the descriptors made from
+// it have to be (a vector one would make each load a loop over the lanes).
 __device__ __forceinline__ int page_of(const TreeArgs& a, const int32_t* table, int slot, int end) {
   if (slot >= end) return -1;
   const int u = slot / 16;
-  return table[(static_cast<uint64_t>(u) * a.page_mul) >> a.page_shift];
+  return scalar_load(table, static_cast<int64_t>((static_cast<uint64_t>(u) * a.page_mul) >> a.page_shift));
 }
 
 // Four codes of a dword, as MFMA operands of T: two dwords.
@@ -299,39 +344,68 @@ template <typename T, int FMT, int DP> struct Tile {
     }
   }
 
-  // Slots of this lane's 8 (bit 4 u + j) whose value has a NaN or an infinity
-  // in any lane; those are zeroed.
-  __device__ __forceinline__ uint32_t take_out_non_finite() {
-    uint32_t bad = 0;
-    if constexpr (FMT == KV_INT8) return 0;
-    const int quad = (threadIdx.x & 63) >> 4;
+  // Zeroes the elements of the values that are NaN or infinite; whether any
+  // lane had one.
+  __device__ __forceinline__ bool take_out_non_finite() {
+    if constexpr (FMT == KV_INT8) return false;
+    bool hit = false;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        bool hit = false;
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int w = 0; w < VD; ++w) {
           const uint32_t e = v[u][j][w];
+          uint32_t drop = 0;
           if constexpr (FMT == KV_E4M3) {
-#pragma unroll
-            for (int b = 0; b < 32; b += 8) hit |= ((e >> b) & 0x7f) == 0x7f;
+            // a byte of 0x7f behind its sign: adding 1 carries into the sign bit
+            const uint32_t full = ((e & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+            drop = (full >> 7) * 0xffu;
           } else {
             constexpr uint32_t ex = T::code == MI355_F16 ? 0x7c00u : 0x7f80u;
-            hit |= (e & ex) == ex || ((e >> 16) & ex) == ex;
+            if ((e & ex) == ex) drop = 0xffffu;
+            if ((e >> 16 & ex) == ex) drop |= 0xffff0000u;
           }
+          hit |= drop != 0;
+          v[u][j][w] = e & ~drop;
         }
-        const uint64_t any = __builtin_amdgcn_ballot_w64(hit);
-        if ((any >> (16 * quad)) & 0xffff) {
-          bad |= 1u << (4 * u + j);
-#pragma unroll
-          for (int w = 0; w < VD; ++w) v[u][j][w] = 0;
+    return __builtin_amdgcn_ballot_w64(hit) != 0;
+  }
+};
+
+// Adds the NaN and infinities that take_out_non_finite left out of one wave's
+// tiles to the output rows that see them: rare, and slow.  In LDS, where rows
+// and elements can be indexed.  Weights do not matter to them.
+template <typename T, int FMT, int PITCH>
+__device__ __forceinline__ void add_non_finite(const TreeArgs& a, float (*acc)[PITCH], int b, int h, int row0, int rows,
+                                               int len, int fresh, int first, int last) {
+  const int lane = threadIdx.x & 63;
+  for (int tile = first; tile < last; tile += kWaves) {
+#pragma unroll 1
+    for (int slot = tile * kTile; slot < (tile + 1) * kTile; ++slot) {
+      const int64_t at = slot < len + fresh ? a.c.row(b, slot, h) : -1;
+      if (at < 0) continue;
+#pragma unroll 1
+      for (int e = lane; e < a.c.d; e += 64) {
+        float v;
+        if constexpr (FMT == KV_16BIT) {
+          v = load_elem<T>(a.c.v, at * a.c.d + e);
+        } else {
+          float f[4];
+          decode4<FMT>(static_cast<const uint8_t*>(a.c.v)[at * a.c.d + e], f);
+          v = f[0];
+        }
+        if (v - v == 0.f) continue;
+#pragma unroll 1
+        for (int r = 0; r < rows; ++r) {
+          const int t = (row0 + r) / a.group, i = slot - len;
+          const bool see = i < 0 || (t < fresh && (a.mask ? a.mask[b * a.mask_b + t * a.mask_t + i] != 0 : i <= t));
+          if (see) acc[r][e] += v;
         }
       }
     }
-    return bad;
   }
-};
+}
 
 template <int FMT, int DP, int MT> constexpr int min_waves() { return MT == 1 && DP <= 128 ? 3 : DP * MT <= 256 ? 2 : 1; }
 
@@ -352,21 +426,23 @@ __global__ __launch_bounds__(64 * kWaves, (min_waves<FMT, DP, MT>())) void tree_
   // this workgroup's tiles [at, last) of the line, or one (head, block) of one sequence
   int at, last, b, start;
   if (a.partial) {
-    const int share = line_share(line_total(a, a.batch), a.grid);
+    const Line line(a);
+    const int share = line_share(line.total, a.grid);
     at = static_cast<int>(blockIdx.x) * share;
     last = at + share;
-    b = line_find(a, at, &start);
+    b = line.find(a, at, &start);
+    if (blockIdx.x == 0 && wave == 0) line.write(a, share, a.starts);
   } else {
     b = blockIdx.x / hm_count;
     start = 0;
-    at = (blockIdx.x % hm_count) * uniform(Seq(a, b).tiles);
+    at = (blockIdx.x % hm_count) * Seq::of(a, b).tiles;
     last = at + 1;  // the first tile; widened to the whole below
   }
   const int line_first = at;
 
   while (b < a.batch && at < last) {
-    const Seq s(a, b);
-    const int len = uniform(s.len), fresh = uniform(s.fresh), tiles = uniform(s.tiles), end = uniform(s.end);
+    const Seq s = Seq::of(a, b);
+    const int len = s.len, fresh = s.fresh, tiles = s.tiles, end = s.end;
     const int hm = (at - start) / tiles, t0 = at - start - hm * tiles;
     if (hm >= hm_count) {
       start += tiles * hm_count;
@@ -407,6 +483,7 @@ __global__ __launch_bounds__(64 * kWaves, (min_waves<FMT, DP, MT>())) void tree_
     }
 
     KvTile kv;
+    bool left_out = false;
     int tile = t0 + wave;
     // nothing is loaded for tiles from t1 on: their units are empty
     const int stop = min(end, t1 * kTile);
@@ -446,7 +523,7 @@ __global__ __launch_bounds__(64 * kWaves, (min_waves<FMT, DP, MT>())) void tree_
       kv.load_keys(n0, n1, d);
 
       const bool masked = !whole || (tile + 1) * kTile > len;
-      uint32_t seen[MT], bad = 0;  // bit 4 u + j
+      uint32_t seen[MT];  // bit 4 u + j
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         seen[m] = 0xff;
@@ -458,22 +535,19 @@ __global__ __launch_bounds__(64 * kWaves, (min_waves<FMT, DP, MT>())) void tree_
       if (masked) {
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          seen[m] = 0;
+          const int t = min(token[m], a.tokens - 1);
+          uint32_t bits8 = 0;
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int slot = tile * kTile + 16 * u + 4 * quad + j, i = slot - len;
-              bool see = u ? there1 : there0;
-              if (i >= 0)
-                see = see && i < fresh && token[m] < fresh &&
-                      (a.mask ? a.mask[b * a.mask_b + token[m] * a.mask_t + i] != 0 : i <= token[m]);
-              if (see) seen[m] |= 1u << (4 * u + j);
-              else sc[m][u][j] = -INFINITY;
-            }
+          for (int e = 0; e < 8; ++e) {
+            const int i = tile * kTile + 16 * (e >> 2) + 4 * quad + (e & 3) - len;  // the new token in this slot
+            const bool edge = a.mask ? a.mask[b * a.mask_b + t * a.mask_t + max(0, min(i, a.tokens - 1))] != 0 : i <= t;
+            const bool see = (e < 4 ? there0 : there1) & ((i < 0) | ((i < fresh) & (token[m] < fresh) & edge));
+            bits8 |= static_cast<uint32_t>(see) << e;
+            sc[m][e >> 2][e & 3] = see ? sc[m][e >> 2][e & 3] : -INFINITY;
           }
+          seen[m] = bits8;
         }
-        bad = kv.take_out_non_finite();
+        left_out |= kv.take_out_non_finite();
       }
 
       u32x4 hi[MT], lo[MT];
@@ -507,38 +581,6 @@ __global__ __launch_bounds__(64 * kWaves, (min_waves<FMT, DP, MT>())) void tree_
           hi[m][p] = narrow2<VT>(f32x2{w[2 * p], w[2 * p + 1]});
           const f32x2 back = widen2<VT>(hi[m][p]);
           lo[m][p] = narrow2<VT>(f32x2{w[2 * p] - back.x, w[2 * p + 1] - back.y});
-        }
-        if (masked && __builtin_amdgcn_ballot_w64(bad != 0)) {
-          // values that are not finite, for the rows that see them: element by element
-#pragma unroll 1
-          for (int e = 0; e < 32; ++e) {
-            const int from = 16 * (e >> 3) + col;  // the lane with this slot's weight: quad e / 8, bit e % 8
-            if (!uniform(__shfl(static_cast<int>(bad >> (e & 7)), 16 * (e >> 3)) & 1)) continue;
-            float we = w[0];
-#pragma unroll
-            for (int i = 1; i < 8; ++i) we = (e & 7) == i ? w[i] : we;
-            we = __shfl(we, from);
-            const bool see = (__shfl(static_cast<int>(seen[m] >> (e & 7)), from) & 1) != 0;
-            const int slot = tile * kTile + 16 * ((e >> 2) & 1) + 4 * (e >> 3) + (e & 3);
-            const int64_t row = a.c.row(b, slot, h);
-            if (row < 0 || !see) continue;
-#pragma unroll
-            for (int x = 0; x < NV; ++x)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int el = NV * (4 * quad + i) + x;
-                if (el >= d) continue;
-                float val;
-                if constexpr (FMT == KV_16BIT) {
-                  val = load_elem<T>(a.c.v, row * d + el);
-                } else {
-                  float f[4];
-                  decode4<FMT>(static_cast<const uint8_t*>(a.c.v)[row * d + el], f);
-                  val = f[0];
-                }
-                o[m][x][i] = fmaf(we, val, o[m][x][i]);
-              }
-          }
         }
       }
 
@@ -584,6 +626,7 @@ __global__ __launch_bounds__(64 * kWaves, (min_waves<FMT, DP, MT>())) void tree_
           *reinterpret_cast<f32x4*>(&joined[wave][r][NV * (4 * quad + i) + x]) =
               f32x4{o[m][x][i] * f, o[m][x + 1][i] * f, o[m][x + 2][i] * f, o[m][x + 3][i] * f};
     }
+    if (left_out) add_non_finite<T, FMT>(a, joined[wave], b, h, row0, rows, len, fresh, t0 + wave, t1);
     __syncthreads();
     const bool cut = t0 > 0 || t1 < tiles;
     const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (at == line_first ? 0 : 1);
@@ -615,71 +658,88 @@ __global__ __launch_bounds__(64 * kWaves, (min_waves<FMT, DP, MT>())) void tree_
   }
 }
 
-// Adds the pieces of one query row that was cut: workgroups of the first
-// kernel in order, 8 groups of lanes taking every eighth piece.
-template <typename T>
-__global__ __launch_bounds__(256) void tree_attention_join(TreeArgs a, int block_rows) {
+// Adds the pieces of one query row that was cut, in order: lanes 0 - 31 and
+// 32 - 63 of each of WAVES waves take every 2 WAVES-th piece, 4 (and, beyond
+// 128, 4 more) elements per lane.  One wave per row, or four where pieces per
+// row are many.
+template <typename T, int WAVES>
+__global__ __launch_bounds__(256) void tree_attention_join(TreeArgs a) {
   typedef typename T::bits bits;
-  const int64_t qrow = blockIdx.x;
-  const int hq = static_cast<int>(qrow % a.q_heads);
-  const int64_t bt = qrow / a.q_heads;
-  const int b = static_cast<int>(bt / a.tokens), t = static_cast<int>(bt % a.tokens);
+  constexpr int PARTS = 2 * WAVES, PER = kWaves / WAVES;  // rows of a workgroup
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int qrow = static_cast<int>(blockIdx.x) * PER + wave / WAVES;
+  const int row_count = a.batch * a.tokens * a.q_heads;
+  const int hq = qrow % a.q_heads, bt = qrow / a.q_heads;
+  const int t = bt % a.tokens, b = min(bt / a.tokens, a.batch - 1);
+  const int block_rows = 16 * a.mt;
   const int h = hq / a.group, r = t * a.group + hq - h * a.group;
   const int block = r / block_rows, rr = r - block * block_rows;
-  const Seq s(a, b);
-  const int tiles = uniform(s.tiles);
-  const int share = line_share(line_total(a, a.batch), a.grid);
-  const int first = line_total(a, b) + (h * a.blocks + block) * tiles;
-  const int w0 = first / share, w1 = (first + tiles - 1) / share;
-  if (w0 == w1) return;  // written by the first kernel
+  const Seq s = Seq::of(a, b);
+  const int share = scalar_load(a.starts, 0);
+  const int first = scalar_load(a.starts, 1 + b) + (h * a.blocks + block) * s.tiles;
+  const int w0 = first / share, w1 = (first + s.tiles - 1) / share;
+  const bool mine = qrow < row_count && w0 != w1;  // else written by the first kernel
+  if (WAVES == kWaves && !mine) return;
 
-  __shared__ f32x4 acc[8][64];
-  __shared__ float group_sum[8];
+  // where workgroup w left its piece: the first of its tiles, or the last
+  const auto slot = [&](int w) {
+    return (2 * static_cast<int64_t>(w) + (w * share >= first ? 0 : 1)) * block_rows + rr;
+  };
   float most = kLow;
-  for (int w = w0; w <= w1; ++w) {
-    const int64_t slot = 2 * static_cast<int64_t>(w) + (max(first, w * share) == w * share ? 0 : 1);
-    most = fmaxf(most, a.stats[slot * block_rows + rr].x);
-  }
-  const int part = threadIdx.x / 32;
+  for (int w = w0 + lane; mine && w <= w1; w += 64) most = fmaxf(most, a.stats[slot(w)].x);
+  for (int i = 1; i < 64; i *= 2) most = fmaxf(most, __shfl_xor(most, i));
+
+  const int part = 2 * (wave % WAVES) + lane / 32;
   f32x4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
   float total = 0.f;
-  for (int w = w0 + part; w <= w1; w += 8) {
-    const int64_t slot = 2 * static_cast<int64_t>(w) + (max(first, w * share) == w * share ? 0 : 1);
-    const float2 st = a.stats[slot * block_rows + rr];
+  const int c0 = 4 * (lane % 32);
+#pragma unroll 4
+  for (int w = w0 + part; mine && w <= w1; w += PARTS) {
+    const int64_t at = slot(w);
+    const float2 st = a.stats[at];
     const float f = __builtin_amdgcn_exp2f(st.x - most);
     total += st.y * f;
+    const float* p = a.partial + at * a.c.d;
+    if (c0 < a.c.d) v[0] += *reinterpret_cast<const f32x4*>(p + c0) * f;
+    if (c0 + 128 < a.c.d) v[1] += *reinterpret_cast<const f32x4*>(p + c0 + 128) * f;
+  }
+  total += __shfl_xor(total, 32);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int c = 4 * (threadIdx.x % 32 + 32 * i);
-      if (c < a.c.d) {
-        const f32x4 p = *reinterpret_cast<const f32x4*>(a.partial + (slot * block_rows + rr) * a.c.d + c);
-        v[i] += p * f;
-      }
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[i][e] += __shfl_xor(v[i][e], 32);
+
+  if constexpr (WAVES > 1) {
+    __shared__ f32x4 acc[WAVES][64];
+    __shared__ float sums[WAVES];
+    if (lane < 32) {
+      acc[wave][lane] = v[0];
+      acc[wave][32 + lane] = v[1];
+    }
+    if (lane == 0) sums[wave] = total;
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) {
+      v[0] += acc[w][lane % 32];
+      v[1] += acc[w][32 + lane % 32];
+      total += sums[w];
     }
   }
-  acc[part][threadIdx.x % 32] = v[0];
-  acc[part][32 + threadIdx.x % 32] = v[1];
-  if (threadIdx.x % 32 == 0) group_sum[part] = total;
-  __syncthreads();
-  const int c = 4 * threadIdx.x;
-  if (c >= a.c.d) return;
-  f32x4 o = acc[0][threadIdx.x];
-  total = group_sum[0];
-#pragma unroll
-  for (int p = 1; p < 8; ++p) {
-    o += acc[p][threadIdx.x];
-    total += group_sum[p];
-  }
+  if (!mine) return;
   const float inv = 1.0f / total;
   const bool none = t >= s.fresh || total == 0.f;
-  *reinterpret_cast<u32x2*>(static_cast<bits*>(a.out) + qrow * a.c.d + c) =
+  const int c = c0 + 128 * (lane / 32);  // lanes 32 - 63 hold the same sums and write the second half
+  if (c >= a.c.d) return;
+  const f32x4 o = lane < 32 ? v[0] : v[1];
+  *reinterpret_cast<u32x2*>(static_cast<bits*>(a.out) + static_cast<int64_t>(qrow) * a.c.d + c) =
       none ? u32x2{0, 0} : u32x2{narrow2<T>(f32x2{o[0] * inv, o[1] * inv}), narrow2<T>(f32x2{o[2] * inv, o[3] * inv})};
 }
 
 // Row blocks and grid of a call.
 struct Plan {
   int mt, blocks, grid;
-  int64_t partial_bytes, bytes;  // of the workspace; 0: no split
+  int64_t partial_bytes, stats_bytes, bytes;  // of the workspace; 0: no split
 };
 
 Plan plan(const mi355_kv_cache& c, int64_t batch, int64_t tokens, int64_t q_heads, int cus) {
@@ -695,7 +755,8 @@ Plan plan(const mi355_kv_cache& c, int64_t batch, int64_t tokens, int64_t q_head
   const int64_t most = static_cast<int64_t>(cus) * (p.mt == 1 && c.head_dim <= 128 ? 3 : c.head_dim * p.mt <= 256 ? 2 : 1);
   p.grid = static_cast<int>(wanted < most ? wanted : most);
   p.partial_bytes = 2 * int64_t{p.grid} * 16 * p.mt * c.head_dim * 4;
-  p.bytes = p.partial_bytes + 2 * int64_t{p.grid} * 16 * p.mt * 8;
+  p.stats_bytes = 2 * int64_t{p.grid} * 16 * p.mt * 8;
+  p.bytes = p.partial_bytes + p.stats_bytes + 4 * (batch + 1);
   return p;
 }
 
@@ -719,6 +780,16 @@ template <typename T, int FMT> int tree_typed(const TreeArgs& a, const Plan& p, 
 #undef MI355_TREE
 }
 
+template <typename T> int tree_join(const TreeArgs& a, const Plan& p, hipStream_t s) {
+  static const char* what = "tree_attention join launch";
+  const int64_t rows = int64_t{a.batch} * a.tokens * a.q_heads;
+  // a workgroup per row where most rows have more than 8 pieces
+  if (p.grid > 8 * int64_t{a.batch} * a.c.heads * a.blocks)
+    return launch(tree_attention_join<T, kWaves>, dim3(static_cast<unsigned>(rows)), 64 * kWaves, 0, a, s, what);
+  return launch(tree_attention_join<T, 1>, dim3(static_cast<unsigned>((rows + kWaves - 1) / kWaves)), 64 * kWaves, 0, a,
+                s, what);
+}
+
 }  // namespace
 
 int64_t tree_attention_workspace(const mi355_kv_cache& cache, int64_t batch, int64_t tokens, int64_t q_heads) {
@@ -736,11 +807,12 @@ int tree_attention_launch(const mi355_kv_cache& cache, const void* q, void* out,
   if (st != MI355_OK) return st;
   Plan p = plan(cache, batch, tokens, q_heads, cus);
   TreeArgs a{kv_cache_args(cache), q, out, lens, new_lens, mask, mask_b, mask_t, q_strides[0], q_strides[1],
-             q_strides[2], nullptr, nullptr, static_cast<int>(batch), tokens, q_heads,
-             q_heads / static_cast<int>(cache.kv_heads), p.blocks, 0, 0, 0, scale * kLog2e};
+             q_strides[2], nullptr, nullptr, nullptr, static_cast<int>(batch), tokens, q_heads,
+             q_heads / static_cast<int>(cache.kv_heads), p.mt, p.blocks, 0, 0, 0, scale * kLog2e};
   if (p.bytes > 0 && work != nullptr && work_bytes >= p.bytes) {
     a.partial = static_cast<float*>(work);
     a.stats = reinterpret_cast<float2*>(static_cast<uint8_t*>(work) + p.partial_bytes);
+    a.starts = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(work) + p.partial_bytes + p.stats_bytes);
   } else {
     p.grid = static_cast<int>(batch * cache.kv_heads * p.blocks);
   }
@@ -763,13 +835,7 @@ int tree_attention_launch(const mi355_kv_cache& cache, const void* q, void* out,
                                   : tree_typed<BF16, KV_16BIT>(a, p, stream);
   }
   if (r != MI355_OK || a.partial == nullptr) return r;
-  const int block_rows = 16 * p.mt;
-  void* args[] = {&a, const_cast<int*>(&block_rows)};
-  const void* join = dtype == MI355_F16 ? reinterpret_cast<const void*>(tree_attention_join<F16>)
-                                        : reinterpret_cast<const void*>(tree_attention_join<BF16>);
-  return hip_status(hipLaunchKernel(join, dim3(static_cast<unsigned>(batch * tokens * q_heads)), dim3(256), args, 0,
-                                    stream),
-                    "tree_attention join launch");
+  return dtype == MI355_F16 ? tree_join<F16>(a, p, stream) : tree_join<BF16>(a, p, stream);
 }
 
 }  // namespace mi355

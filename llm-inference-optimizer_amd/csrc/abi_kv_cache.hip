@@ -67,6 +67,7 @@ int check_cache(const char* fn, const mi355_kv_cache* c) {
 // The pointers of a cache that a call is about to use.
 int check_pools(const char* fn, const mi355_kv_cache* c) {
   if (c->k == nullptr || c->v == nullptr || c->page_table == nullptr) return bad(fn, "null pointer in the cache");
+  if (c->pages < 1 || c->table_width < 1) return bad(fn, "a cache without pages");
   if (!aligned16(c->k) || !aligned16(c->v)) return bad(fn, "the cache's pools must be 16-byte aligned");
   if (c->format != MI355_KV_16BIT) {
     if (c->k_scale == nullptr || c->v_scale == nullptr) return bad(fn, "a quantised cache needs its scales");

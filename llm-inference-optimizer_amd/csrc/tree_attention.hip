@@ -50,7 +50,11 @@ namespace mi355 {
 namespace {
 
 constexpr int kTile = 32;            // slots of a tile: two units of 16
-constexpr int kWaves = 4;
+
+constexpr int kWaves = 4;            // of a workgroup
+
+// Waves that a SIMD holds at the registers of a kernel.
+constexpr int simd_waves(int dp, int mt) { return mt == 1 && dp <= 64 ? 4 : mt == 1 && dp <= 128 ? 3 : dp * mt <= 256 ? 2 : 1; }
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLow = -1e30f;       // the running maximum before any score
 constexpr float kSlack = 8.0f;       // log2 of how far scores may pass it
@@ -121,13 +125,22 @@ __device__ __forceinline__ int wave_scan(int v) {
 // The line of tiles: sequence b has Seq::tiles of them for each of its heads
 // and row blocks, head and block outermost.
 struct Line {
-  int first;  // tiles per head and block, of this lane's sequence among the first 64 and those before
-  int total;  // of all sequences
+  int len, fresh;  // of this lane's sequence among the first 64
+  int first;       // tiles per head and block, of it and those before
+  int total;       // of all sequences
+  Line() = default;
   __device__ __forceinline__ explicit Line(const TreeArgs& a) {
-    first = wave_scan(Seq::of_lane(a, 0));
+    const int b = min(static_cast<int>(threadIdx.x & 63), a.batch - 1);
+    len = a.lens[b];
+    fresh = a.new_lens ? a.new_lens[b] : a.tokens;
+    first = wave_scan(static_cast<int>(threadIdx.x & 63) < a.batch ? Seq(a, len, fresh).tiles : 0);
     total = __builtin_amdgcn_readlane(first, 63);
     for (int b0 = 64; b0 < a.batch; b0 += 64) total += __builtin_amdgcn_readlane(wave_scan(Seq::of_lane(a, b0)), 63);
     total *= a.c.heads * a.blocks;
+  }
+  // Sequence b < 64.
+  __device__ __forceinline__ Seq seq(const TreeArgs& a, int b) const {
+    return Seq(a, __builtin_amdgcn_readlane(len, b), __builtin_amdgcn_readlane(fresh, b));
   }
   // The sequence that tile `at` belongs to (batch: none) and its first tile.
   __device__ __forceinline__ int find(const TreeArgs& a, int at, int* start) const {
@@ -193,9 +206,9 @@ template <int FMT> struct Unit {
 // Page of a unit, or -1.  In a scalar register, as the descriptors made from
 // it have to be (a vector one would make each load a loop over the lanes).
 __device__ __forceinline__ int page_of(const TreeArgs& a, const int32_t* table, int slot, int end) {
-  if (slot >= end) return -1;
-  const int u = slot / 16;
-  return scalar_load(table, static_cast<int64_t>((static_cast<uint64_t>(u) * a.page_mul) >> a.page_shift));
+  const int u = max(0, min(slot, end - 1)) / 16;  // without a branch: a table has a page at least
+  const int page = scalar_load(table, static_cast<int64_t>((static_cast<uint64_t>(u) * a.page_mul) >> a.page_shift));
+  return slot < end ? page : -1;
 }
 
 // Four codes of a dword, as MFMA operands of T: two dwords.
@@ -247,7 +260,7 @@ __device__ __forceinline__ float sum_quads(float v) {
 //           or (16-bit) 32 i + 8 quad .. + 7
 //   values  unit u, slot 4 quad + j, elements NV (l % 16) .. + NV - 1
 //   scales  unit u, slots 4 quad .. 4 quad + 3
-template <typename T, int FMT, int DP> struct Tile {
+template <typename T, int FMT, int DP, int AUX> struct Tile {
   static constexpr int ES = FMT == KV_16BIT ? 2 : 1;
   static constexpr int NV = DP / 16;
   static constexpr int KL = DP * ES / 64;     // 16-byte key loads per unit
@@ -262,20 +275,20 @@ template <typename T, int FMT, int DP> struct Tile {
     for (int i = 0; i < KL; ++i) {
       const int byte = 64 * i + 16 * quad;
       const uint32_t off = byte < d * ES ? static_cast<uint32_t>(r * d * ES + byte) : kOob;
-      k[0][i] = buf_load16_cached(u0.k, off);
-      k[1][i] = buf_load16_cached(u1.k, off);
+      k[0][i] = __builtin_amdgcn_raw_buffer_load_b128(u0.k, off, 0, AUX);
+      k[1][i] = __builtin_amdgcn_raw_buffer_load_b128(u1.k, off, 0, AUX);
     }
     if constexpr (FMT != KV_16BIT) {
-      ks[0] = __builtin_bit_cast(f32x4, buf_load16_cached(u0.ks, 16u * quad));
-      ks[1] = __builtin_bit_cast(f32x4, buf_load16_cached(u1.ks, 16u * quad));
+      ks[0] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(u0.ks, 16u * quad, 0, AUX));
+      ks[1] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(u1.ks, 16u * quad, 0, AUX));
     }
   }
 
   __device__ __forceinline__ void load_values(const Unit<FMT>& u0, const Unit<FMT>& u1, int d) {
     const int lane = threadIdx.x & 63, r = lane & 15, quad = lane >> 4;
     if constexpr (FMT != KV_16BIT) {
-      vs[0] = __builtin_bit_cast(f32x4, buf_load16_cached(u0.vs, 16u * quad));
-      vs[1] = __builtin_bit_cast(f32x4, buf_load16_cached(u1.vs, 16u * quad));
+      vs[0] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(u0.vs, 16u * quad, 0, AUX));
+      vs[1] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(u1.vs, 16u * quad, 0, AUX));
     }
     const uint32_t first = NV * r < d ? static_cast<uint32_t>((4 * quad * d + NV * r) * ES) : kOob;
 #pragma unroll
@@ -285,15 +298,15 @@ template <typename T, int FMT, int DP> struct Tile {
       for (int j = 0; j < 4; ++j) {
         const int at = j * d * ES;  // uniform: the scalar offset of the load
         if constexpr (VD == 1) {
-          v[u][j][0] = __builtin_amdgcn_raw_buffer_load_b32(rsrc, first, at, 0);
+          v[u][j][0] = __builtin_amdgcn_raw_buffer_load_b32(rsrc, first, at, AUX);
         } else if constexpr (VD == 2) {
-          const u32x2 t = __builtin_amdgcn_raw_buffer_load_b64(rsrc, first, at, 0);
+          const u32x2 t = __builtin_amdgcn_raw_buffer_load_b64(rsrc, first, at, AUX);
           v[u][j][0] = t[0];
           v[u][j][1] = t[1];
         } else {
 #pragma unroll
           for (int w = 0; w < VD / 4; ++w) {
-            const u32x4 t = __builtin_amdgcn_raw_buffer_load_b128(rsrc, first + 16 * w, at, 0);
+            const u32x4 t = __builtin_amdgcn_raw_buffer_load_b128(rsrc, first + 16 * w, at, AUX);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[u][j][4 * w + e] = t[e];
           }
@@ -407,12 +420,11 @@ __device__ __forceinline__ void add_non_finite(const TreeArgs& a, float (*acc)[P
   }
 }
 
-template <int FMT, int DP, int MT> constexpr int min_waves() { return MT == 1 && DP <= 128 ? 3 : DP * MT <= 256 ? 2 : 1; }
-
 template <typename T, int FMT, int DP, int MT>
-__global__ __launch_bounds__(64 * kWaves, (min_waves<FMT, DP, MT>())) void tree_attention_split(TreeArgs a) {
+__global__ __launch_bounds__(64 * kWaves, simd_waves(DP, MT)) void tree_attention_split(TreeArgs a) {
   typedef typename T::bits bits;
-  typedef Tile<T, FMT, DP> KvTile;
+  // rows that fit one block read the cache once; more blocks meet it in the L2
+  typedef Tile<T, FMT, DP, MT == 4 ? 0 : kStreamAux> KvTile;
   constexpr int NV = KvTile::NV, NQ = DP / 32, ROWS = 16 * MT, PITCH = DP + 4;
   // the weights' type in the second product: codes and bf16 values are exact in bf16
   typedef typename std::conditional<FMT == KV_16BIT, T, BF16>::type VT;
@@ -425,8 +437,9 @@ __global__ __launch_bounds__(64 * kWaves, (min_waves<FMT, DP, MT>())) void tree_
 
   // this workgroup's tiles [at, last) of the line, or one (head, block) of one sequence
   int at, last, b, start;
+  Line line;
   if (a.partial) {
-    const Line line(a);
+    line = Line(a);
     const int share = line_share(line.total, a.grid);
     at = static_cast<int>(blockIdx.x) * share;
     last = at + share;
@@ -441,7 +454,7 @@ __global__ __launch_bounds__(64 * kWaves, (min_waves<FMT, DP, MT>())) void tree_
   const int line_first = at;
 
   while (b < a.batch && at < last) {
-    const Seq s = Seq::of(a, b);
+    const Seq s = a.partial && b < 64 ? line.seq(a, b) : Seq::of(a, b);
     const int len = s.len, fresh = s.fresh, tiles = s.tiles, end = s.end;
     const int hm = (at - start) / tiles, t0 = at - start - hm * tiles;
     if (hm >= hm_count) {
@@ -454,6 +467,11 @@ __global__ __launch_bounds__(64 * kWaves, (min_waves<FMT, DP, MT>())) void tree_
     const int h = hm / a.blocks, row0 = (hm % a.blocks) * ROWS;
     const int rows = min(ROWS, a.tokens * a.group - row0);
     const int32_t* table = a.c.table + static_cast<int64_t>(b) * a.c.table_stride;
+    int tile = t0 + wave;
+    // nothing is loaded for tiles from t1 on: their units are empty
+    const int stop = min(end, t1 * kTile);
+    const int p0_first = page_of(a, table, tile * kTile, stop), p1_first = page_of(a, table, tile * kTile + 16, stop);
+    int p0 = page_of(a, table, (tile + kWaves) * kTile, stop), p1 = page_of(a, table, (tile + kWaves) * kTile + 16, stop);
 
     // Q^T operands: 16-byte packets of this lane's query rows, elements as the keys'
     u32x4 q[MT][NQ];
@@ -484,20 +502,14 @@ __global__ __launch_bounds__(64 * kWaves, (min_waves<FMT, DP, MT>())) void tree_
 
     KvTile kv;
     bool left_out = false;
-    int tile = t0 + wave;
-    // nothing is loaded for tiles from t1 on: their units are empty
-    const int stop = min(end, t1 * kTile);
-    int p0 = page_of(a, table, tile * kTile, stop), p1 = page_of(a, table, tile * kTile + 16, stop);
     bool whole;
     {
-      const Unit<FMT> u0(a, h, tile * kTile, stop, p0), u1(a, h, tile * kTile + 16, stop, p1);
+      const Unit<FMT> u0(a, h, tile * kTile, stop, p0_first), u1(a, h, tile * kTile + 16, stop, p1_first);
       whole = u0.whole && u1.whole;
       kv.load_keys(u0, u1, d);
       kv.load_values(u0, u1, d);
     }
-    bool there0 = p0 >= 0 && p0 < a.c.pages, there1 = p1 >= 0 && p1 < a.c.pages;
-    p0 = page_of(a, table, (tile + kWaves) * kTile, stop);
-    p1 = page_of(a, table, (tile + kWaves) * kTile + 16, stop);
+    bool there0 = p0_first >= 0 && p0_first < a.c.pages, there1 = p1_first >= 0 && p1_first < a.c.pages;
 
     for (; tile < t1; tile += kWaves) {
       f32x4 sc[MT][2];
@@ -617,8 +629,10 @@ __global__ __launch_bounds__(64 * kWaves, (min_waves<FMT, DP, MT>())) void tree_
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       const int r = 16 * m + col;
-      const float f = __builtin_amdgcn_exp2f(
-          top[m] - fmaxf(fmaxf(wave_max[0][r], wave_max[1][r]), fmaxf(wave_max[2][r], wave_max[3][r])));
+      float most = wave_max[0][r];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) most = fmaxf(most, wave_max[w][r]);
+      const float f = __builtin_amdgcn_exp2f(top[m] - most);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -632,7 +646,9 @@ __global__ __launch_bounds__(64 * kWaves, (min_waves<FMT, DP, MT>())) void tree_
     const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (at == line_first ? 0 : 1);
     for (int e = threadIdx.x; e < rows * (d / 4); e += 64 * kWaves) {
       const int r = e / (d / 4), c = 4 * (e - r * (d / 4));
-      const float most = fmaxf(fmaxf(wave_max[0][r], wave_max[1][r]), fmaxf(wave_max[2][r], wave_max[3][r]));
+      float most = wave_max[0][r];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) most = fmaxf(most, wave_max[w][r]);
       float total = 0.f;
       f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -659,79 +675,91 @@ __global__ __launch_bounds__(64 * kWaves, (min_waves<FMT, DP, MT>())) void tree_
 }
 
 // Adds the pieces of one query row that was cut, in order: lanes 0 - 31 and
-// 32 - 63 of each of WAVES waves take every 2 WAVES-th piece, 4 (and, beyond
-// 128, 4 more) elements per lane.  One wave per row, or four where pieces per
-// row are many.
+// 32 - 63 of each of WAVES waves take every 2 WAVES-th piece with a running
+// maximum, 4 (and, beyond 128, 4 more) elements per lane.  Latency is all there
+// is to it: one wave per row, or eight where pieces per row are many, so that
+// most pieces are in flight at once.
+constexpr int kJoinWaves = 8;
+
 template <typename T, int WAVES>
-__global__ __launch_bounds__(256) void tree_attention_join(TreeArgs a) {
+__global__ __launch_bounds__(64 * kJoinWaves) void tree_attention_join(TreeArgs a) {
   typedef typename T::bits bits;
-  constexpr int PARTS = 2 * WAVES, PER = kWaves / WAVES;  // rows of a workgroup
+  constexpr int PARTS = 2 * WAVES, PER = kJoinWaves / WAVES;  // rows of a workgroup
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int qrow = static_cast<int>(blockIdx.x) * PER + wave / WAVES;
   const int row_count = a.batch * a.tokens * a.q_heads;
   const int hq = qrow % a.q_heads, bt = qrow / a.q_heads;
   const int t = bt % a.tokens, b = min(bt / a.tokens, a.batch - 1);
+  const int share = scalar_load(a.starts, 0), start = scalar_load(a.starts, 1 + b);
+  const Seq s = Seq::of(a, b);
   const int block_rows = 16 * a.mt;
   const int h = hq / a.group, r = t * a.group + hq - h * a.group;
   const int block = r / block_rows, rr = r - block * block_rows;
-  const Seq s = Seq::of(a, b);
-  const int share = scalar_load(a.starts, 0);
-  const int first = scalar_load(a.starts, 1 + b) + (h * a.blocks + block) * s.tiles;
+  const int first = start + (h * a.blocks + block) * s.tiles;
   const int w0 = first / share, w1 = (first + s.tiles - 1) / share;
   const bool mine = qrow < row_count && w0 != w1;  // else written by the first kernel
-  if (WAVES == kWaves && !mine) return;
-
-  // where workgroup w left its piece: the first of its tiles, or the last
-  const auto slot = [&](int w) {
-    return (2 * static_cast<int64_t>(w) + (w * share >= first ? 0 : 1)) * block_rows + rr;
-  };
-  float most = kLow;
-  for (int w = w0 + lane; mine && w <= w1; w += 64) most = fmaxf(most, a.stats[slot(w)].x);
-  for (int i = 1; i < 64; i *= 2) most = fmaxf(most, __shfl_xor(most, i));
+  if (WAVES > 1 && !mine) return;
 
   const int part = 2 * (wave % WAVES) + lane / 32;
-  f32x4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-  float total = 0.f;
   const int c0 = 4 * (lane % 32);
+  const bool in0 = c0 < a.c.d, in1 = c0 + 128 < a.c.d;
+  f32x4 v0 = {0.f, 0.f, 0.f, 0.f}, v1 = v0;
+  float most = kLow, total = 0.f;
 #pragma unroll 4
-  for (int w = w0 + part; mine && w <= w1; w += PARTS) {
-    const int64_t at = slot(w);
+  for (int w = w0 + part; w <= w1; w += PARTS) {
+    // where workgroup w left its piece: the first of its tiles, or the last
+    const int64_t at = (2 * static_cast<int64_t>(w) + (w * share >= first ? 0 : 1)) * block_rows + rr;
+    if (!mine) break;
     const float2 st = a.stats[at];
-    const float f = __builtin_amdgcn_exp2f(st.x - most);
-    total += st.y * f;
-    const float* p = a.partial + at * a.c.d;
-    if (c0 < a.c.d) v[0] += *reinterpret_cast<const f32x4*>(p + c0) * f;
-    if (c0 + 128 < a.c.d) v[1] += *reinterpret_cast<const f32x4*>(p + c0 + 128) * f;
+    const float* p = a.partial + at * a.c.d + c0;
+    const f32x4 p0 = in0 ? *reinterpret_cast<const f32x4*>(p) : f32x4{0.f, 0.f, 0.f, 0.f};
+    const f32x4 p1 = in1 ? *reinterpret_cast<const f32x4*>(p + 128) : f32x4{0.f, 0.f, 0.f, 0.f};
+    const float now = fmaxf(most, st.x);
+    const float was = __builtin_amdgcn_exp2f(most - now), f = __builtin_amdgcn_exp2f(st.x - now);
+    most = now;
+    total = total * was + st.y * f;
+    v0 = v0 * was + p0 * f;
+    v1 = v1 * was + p1 * f;
   }
-  total += __shfl_xor(total, 32);
+  // lanes l and l + 32
+  {
+    const float other = __shfl_xor(most, 32), now = fmaxf(most, other);
+    const float f = __builtin_amdgcn_exp2f(most - now);
+    most = now;
+    total *= f;
+    total += __shfl_xor(total, 32);
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[i][e] += __shfl_xor(v[i][e], 32);
-
+    for (int e = 0; e < 4; ++e) {
+      v0[e] *= f;
+      v1[e] *= f;
+      v0[e] += __shfl_xor(v0[e], 32);
+      v1[e] += __shfl_xor(v1[e], 32);
+    }
+  }
   if constexpr (WAVES > 1) {
     __shared__ f32x4 acc[WAVES][64];
-    __shared__ float sums[WAVES];
-    if (lane < 32) {
-      acc[wave][lane] = v[0];
-      acc[wave][32 + lane] = v[1];
-    }
-    if (lane == 0) sums[wave] = total;
+    __shared__ float2 sums[WAVES];
+    acc[wave][lane] = lane < 32 ? v0 : v1;
+    if (lane == 0) sums[wave] = float2{most, total};
     __syncthreads();
     if (wave) return;
+    for (int w = 1; w < WAVES; ++w) most = fmaxf(most, sums[w].x);
+    v0 = f32x4{0.f, 0.f, 0.f, 0.f};
+    total = 0.f;
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) {
-      v[0] += acc[w][lane % 32];
-      v[1] += acc[w][32 + lane % 32];
-      total += sums[w];
+    for (int w = 0; w < WAVES; ++w) {
+      const float f = __builtin_amdgcn_exp2f(sums[w].x - most);
+      v0 += acc[w][lane] * f;
+      total += sums[w].y * f;
     }
+    v1 = v0;
   }
   if (!mine) return;
   const float inv = 1.0f / total;
   const bool none = t >= s.fresh || total == 0.f;
-  const int c = c0 + 128 * (lane / 32);  // lanes 32 - 63 hold the same sums and write the second half
+  const int c = c0 + 128 * (lane / 32);  // lanes 32 - 63 write the second half
   if (c >= a.c.d) return;
-  const f32x4 o = lane < 32 ? v[0] : v[1];
+  const f32x4 o = lane < 32 ? v0 : v1;
   *reinterpret_cast<u32x2*>(static_cast<bits*>(a.out) + static_cast<int64_t>(qrow) * a.c.d + c) =
       none ? u32x2{0, 0} : u32x2{narrow2<T>(f32x2{o[0] * inv, o[1] * inv}), narrow2<T>(f32x2{o[2] * inv, o[3] * inv})};
 }
@@ -750,9 +778,10 @@ Plan plan(const mi355_kv_cache& c, int64_t batch, int64_t tokens, int64_t q_head
   const int64_t pieces = batch * c.kv_heads * p.blocks;
   const int64_t tiles = (c.table_width * c.page_size + kTile - 1) / kTile;  // of the longest possible context
   p.grid = static_cast<int>(pieces);
+  const int dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
   if (tiles <= 2 * kWaves || pieces * tiles > 0x7fffffff - 65536 * kWaves) return p;
   const int64_t wanted = (pieces * tiles + kWaves - 1) / kWaves;
-  const int64_t most = static_cast<int64_t>(cus) * (p.mt == 1 && c.head_dim <= 128 ? 3 : c.head_dim * p.mt <= 256 ? 2 : 1);
+  const int64_t most = static_cast<int64_t>(cus) * simd_waves(dp, p.mt);
   p.grid = static_cast<int>(wanted < most ? wanted : most);
   p.partial_bytes = 2 * int64_t{p.grid} * 16 * p.mt * c.head_dim * 4;
   p.stats_bytes = 2 * int64_t{p.grid} * 16 * p.mt * 8;
@@ -763,8 +792,7 @@ Plan plan(const mi355_kv_cache& c, int64_t batch, int64_t tokens, int64_t q_head
 template <typename T, int FMT> int tree_typed(const TreeArgs& a, const Plan& p, hipStream_t s) {
   static const char* what = "tree_attention launch";
   const dim3 grid(static_cast<unsigned>(p.grid));
-  constexpr int block = 64 * kWaves;
-#define MI355_TREE(DP, MT) return launch(tree_attention_split<T, FMT, DP, MT>, grid, block, 0, a, s, what)
+#define MI355_TREE(DP, MT) return launch(tree_attention_split<T, FMT, DP, MT>, grid, 64 * kWaves, 0, a, s, what)
   if (a.c.d <= 64) {
     if (p.mt == 1) MI355_TREE(64, 1);
     if (p.mt == 2) MI355_TREE(64, 2);
@@ -783,11 +811,10 @@ template <typename T, int FMT> int tree_typed(const TreeArgs& a, const Plan& p, 
 template <typename T> int tree_join(const TreeArgs& a, const Plan& p, hipStream_t s) {
   static const char* what = "tree_attention join launch";
   const int64_t rows = int64_t{a.batch} * a.tokens * a.q_heads;
-  // a workgroup per row where most rows have more than 8 pieces
-  if (p.grid > 8 * int64_t{a.batch} * a.c.heads * a.blocks)
-    return launch(tree_attention_join<T, kWaves>, dim3(static_cast<unsigned>(rows)), 64 * kWaves, 0, a, s, what);
-  return launch(tree_attention_join<T, 1>, dim3(static_cast<unsigned>((rows + kWaves - 1) / kWaves)), 64 * kWaves, 0, a,
-                s, what);
+  if (p.grid > 8 * int64_t{a.batch} * a.c.heads * a.blocks)  // most rows have more than 8 pieces
+    return launch(tree_attention_join<T, kJoinWaves>, dim3(static_cast<unsigned>(rows)), 64 * kJoinWaves, 0, a, s, what);
+  return launch(tree_attention_join<T, 1>, dim3(static_cast<unsigned>((rows + kJoinWaves - 1) / kJoinWaves)),
+                64 * kJoinWaves, 0, a, s, what);
 }
 
 }  // namespace

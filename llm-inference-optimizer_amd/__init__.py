@@ -35,11 +35,15 @@ Between an attention block's projections: ``fused_rotary`` (rotary positions,
 ``rotary_frequencies`` for long contexts), ``KVCache`` with ``kv_cache_append``,
 ``kv_cache_read`` and ``kv_cache_keep`` (a paged cache, quantised to int8 or
 e4m3 as it is written), and ``tree_attention`` (one new token, or a tree of
-drafted ones, over that cache).
+drafted ones, over that cache).  ``patch_model_with_fused_kernels(...,
+fuse_attention=True)`` installs ``CachedAttention``, with which
+``GraphedGreedyDecoder(..., kv_cache="int8")`` decodes over such a cache, and
+with ``draft_tokens=n`` verifies drafted trees.
 
 The kernels live in ``libmi355_fused.so`` (gfx950 HIP, C ABI in
 ``include/mi355_fused.h``), built by ``build.py``.
 """
+from .engine.cached_attention import ATTENTION_CLASS_NAMES, CachedAttention, DecoderCache
 from .engine.fused_norm_activation_patch import (DECODER_LAYER_CLASS_NAMES, MLP_CLASS_NAMES, RMSNORM_CLASS_NAMES,
                                                  FusedDecoderLayer, FusedMLP, FusedRMSNorm,
                                                  patch_model_with_fused_kernels)
@@ -62,5 +66,6 @@ __all__ = [
     "w8a16_linear", "w8a16_reference", "quantize_int8_weight", "QuantizedLinearInt8", "quantize_model_int8",
     "fused_gate_up_silu_w8a16", "linear16", "LINEAR16_MAX_ROWS",
     "fused_rotary", "rotary_frequencies", "KVCache", "KV_FORMATS", "kv_cache_append", "kv_cache_read",
-    "kv_cache_keep", "tree_attention", "TREE_ATTENTION_MAX_TOKENS",
+    "kv_cache_keep", "tree_attention", "TREE_ATTENTION_MAX_TOKENS", "CachedAttention", "DecoderCache",
+    "ATTENTION_CLASS_NAMES",
 ]

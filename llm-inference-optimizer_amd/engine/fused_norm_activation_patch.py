@@ -34,7 +34,10 @@ FusedMLP's down projection on the HIP 16-bit linear (``linear16``: weight
 streaming on MFMA) for inputs of at most ``LINEAR16_MAX_ROWS`` rows, where
 torch's linear is far from HBM bandwidth; its fp32 sums run in another order
 than hipBLASLt's, so outputs may differ in the last bit.  The count appears as
-``"down"``.
+``"down"``.  ``fuse_attention=True`` (off by default) replaces attention modules
+by ``CachedAttention``, which the decoder's quantised cache needs
+(``GraphedGreedyDecoder(..., kv_cache="int8")``); with any other cache they run
+their original forward.  The count appears as ``"attention"``.
 """
 from __future__ import annotations
 
@@ -46,6 +49,7 @@ from ..kernels.fused_swiglu_hip import fused_silu_mul
 from ..kernels.linear16_hip import LINEAR16_MAX_ROWS, linear16
 from ..kernels.w8a16_matmul_hip import fused_gate_up_silu_w8a16
 from ..quantization.int8 import QuantizedLinearInt8
+from .cached_attention import CachedAttention, cacheable
 
 __all__ = ["RMSNORM_CLASS_NAMES", "MLP_CLASS_NAMES", "DECODER_LAYER_CLASS_NAMES", "FusedRMSNorm", "FusedMLP",
            "FusedDecoderLayer", "patch_model_with_fused_kernels"]
@@ -186,7 +190,8 @@ class FusedDecoderLayer(torch.nn.Module):
 
 def patch_model_with_fused_kernels(model: torch.nn.Module, patch_norm: bool = True,
                                    patch_mlp: bool = True, fuse_residual: bool = False,
-                                   fuse_gate_up: bool = False, hip_down: bool = False) -> dict:
+                                   fuse_gate_up: bool = False, hip_down: bool = False,
+                                   fuse_attention: bool = False) -> dict:
     """Replace matching RMSNorm and/or MLP child modules in place (setattr on
     the parent).  Returns ``{"rmsnorm": count, "mlp": count}``.
     ``patch_norm`` / ``patch_mlp`` enable each kernel independently.
@@ -195,7 +200,9 @@ def patch_model_with_fused_kernels(model: torch.nn.Module, patch_norm: bool = Tr
     ``fuse_gate_up`` builds each FusedMLP with ``fuse_gate_up=True`` and adds
     ``"gate_up": count`` (the MLPs whose projections the fused kernel can
     read).  ``hip_down`` builds each FusedMLP with ``hip_down=True`` and adds
-    ``"down": count`` (the MLPs whose down projection ``linear16`` can run)."""
+    ``"down": count`` (the MLPs whose down projection ``linear16`` can run).
+    ``fuse_attention`` replaces matching attention modules by ``CachedAttention``
+    and adds ``"attention": count``."""
     counts = {"rmsnorm": 0, "mlp": 0}
     if fuse_gate_up:
         counts["gate_up"] = 0
@@ -217,6 +224,13 @@ def patch_model_with_fused_kernels(model: torch.nn.Module, patch_norm: bool = Tr
                     counts["gate_up"] += 1
                 if fused.hip_down:
                     counts["down"] += 1
+    if fuse_attention:
+        counts["attention"] = 0
+        for parent in list(model.modules()):
+            for child_name, child in list(parent.named_children()):
+                if cacheable(child):
+                    setattr(parent, child_name, CachedAttention(child))
+                    counts["attention"] += 1
     if fuse_residual:
         counts["add_rmsnorm"] = 0
         for parent in list(model.modules()):

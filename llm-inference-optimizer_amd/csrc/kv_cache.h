@@ -61,15 +61,23 @@ template <int FMT> __device__ __forceinline__ void decode4(uint32_t d, float (&f
   }
 }
 
-// fp32 values divided by their scale (|f| <= the format's largest code, up to
-// the division's rounding) -> four codes, rounded to nearest, ties to even.
+// x / scale, correctly rounded, for rc = 1 / scale correctly rounded: the
+// remainder of the first quotient is exact in one fma.  A third of a division's
+// instructions.
+__device__ __forceinline__ float quotient(float x, float scale, float rc) {
+  const float q = x * rc;
+  return __builtin_fmaf(__builtin_fmaf(-q, scale, x), rc, q);
+}
+
+// Quotients (at most the format's largest code, up to their rounding) -> four
+// codes, rounded to nearest, ties to even.
 template <int FMT> __device__ __forceinline__ uint32_t encode4(const float (&f)[4]) {
   if constexpr (FMT == KV_INT8) {
-    uint32_t d = 0;
+    // 1.5 * 2^23 + f has f, rounded to an integer, in its low bits
+    uint32_t t[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      d |= (static_cast<uint32_t>(static_cast<int>(__builtin_rintf(f[i]))) & 0xffu) << (8 * i);
-    return d;
+    for (int i = 0; i < 4; ++i) t[i] = as_u32(f[i] + 12582912.0f);
+    return __builtin_amdgcn_perm(t[1], t[0], 0x0c0c0400u) | __builtin_amdgcn_perm(t[3], t[2], 0x04000c0cu);
   } else {
     int d = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
     d = __builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], d, true);

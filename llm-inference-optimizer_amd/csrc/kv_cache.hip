@@ -3,7 +3,8 @@
 //
 // All three are bound by HBM on long inputs and by launch and load latency on
 // a decode step's few rows.  A row (one token and head, head_dim elements) is
-// held by 4 to 32 lanes of one 8-element packet each.
+// held by 4 to 32 lanes of one 8-element packet each; a wave of the append
+// takes a token, or with few tokens a pass over some of its rows.
 //
 //   append  per row of new keys (rotated, in fp32) and values:
 //             amax = max |x|,  scale = max(amax / top, 1e-8),  top = 127 | 448
@@ -51,80 +52,111 @@ struct AppendArgs {
   void* q_out;
   const int32_t *lens, *new_lens;
   Strides ks, vs, qs;
-  int64_t tokens;
-  int q_heads, lanes, rows_per_wg;
+  int rows, tokens, q_heads, lanes;  // rows = batch * tokens
+  // heads per wave; from which blockIdx.y on it takes keys and values
+  int q_per_wave, kv_per_wave, kv_from;
 };
 
-template <typename T, int FMT> __global__ __launch_bounds__(256) void append_rows(AppendArgs a) {
+constexpr int kAhead = 2;  // query rows of a lane in flight
+constexpr int kWaves = 4;  // of a workgroup, each for itself
+
+template <typename T, int FMT, int MODE> __global__ __launch_bounds__(64 * kWaves) void append_rows(AppendArgs a) {
   typedef typename T::bits bits;
-  __shared__ float cs[2 * kMaxPairs];
-  const int64_t b = blockIdx.x / a.tokens, t = blockIdx.x % a.tokens;
-  if (a.rot.rotary) {
-    rotary_angles(cs, a.rot, a.rot.positions[b * a.rot.pos_stride_b + t * a.rot.pos_stride_t]);
-    __syncthreads();
-  }
-  const int64_t slot = a.lens[b] + t;
+  __shared__ float angles[kWaves][2 * kMaxPairs];
+  const int index = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int token = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(wave);
+  if (token >= a.rows) return;
+  float* cs = angles[wave];
+  const int b = token / a.tokens, t = token - b * a.tokens;
+  const int64_t position = MODE == ROTARY_NONE ? 0 : a.rot.positions[b * a.rot.pos_stride_b + t * a.rot.pos_stride_t];
+  const int64_t slot = static_cast<int64_t>(a.lens[b]) + t;
   const bool stored = a.new_lens == nullptr || t < a.new_lens[b];
-  const int d0 = (threadIdx.x % a.lanes) * 8;
-  const bool in = d0 < a.c.d;
-  // rows of a token: its query heads, then its keys', then its values'
-  const int rows = a.q_heads + 2 * a.c.heads;
-  const int first = blockIdx.y * a.rows_per_wg;
-  for (int r = first + threadIdx.x / a.lanes; r < min(rows, first + a.rows_per_wg); r += 256 / a.lanes) {
-    RotaryPacket<T> p;
-    float y[8];
-    if (r < a.q_heads) {
-      if (in) {
-        const bits* row = static_cast<const bits*>(a.q) + b * a.qs.b + t * a.qs.t + r * a.qs.h;
-        p.load(row, d0, a.rot);
-        p.rotate(y, row, d0, a.rot, cs);
-        Packet<T> o;
-        o.pack(y);
-        bits* out = static_cast<bits*>(a.q_out) + (static_cast<int64_t>(blockIdx.x) * a.q_heads + r) * a.c.d;
-        *reinterpret_cast<u32x4*>(out + d0) = o.raw;
-      }
-      continue;
-    }
-    const bool key = r < a.q_heads + a.c.heads;
-    const int h = r - a.q_heads - (key ? 0 : a.c.heads);
-    const int64_t at = stored ? a.c.row(b, slot, h) : -1;
-    if (at < 0) continue;  // the same for all lanes of a row
-    uint32_t top = 0;
-    if (in) {
-      const bits* row = key ? static_cast<const bits*>(a.k) + b * a.ks.b + t * a.ks.t + h * a.ks.h
-                            : static_cast<const bits*>(a.v) + b * a.vs.b + t * a.vs.t + h * a.vs.h;
-      RotaryArgs rot = a.rot;
-      if (!key) rot.rotary = 0;
-      p.load(row, d0, rot);
-      p.rotate(y, row, d0, rot, cs);
+  RotaryLane<T, MODE> lane(a.rot, (index % a.lanes) * 8);
+  const bool in = lane.d0 < a.c.d;
+  const int step = 64 / a.lanes, mine = index / a.lanes;
+
+  // Rows of a token: its query heads, then its keys' and values'.  The grid's
+  // y takes passes of `step` rows: query passes first.
+  const int q_last = in ? min(a.q_heads, (static_cast<int>(blockIdx.y) + 1) * a.q_per_wave) : 0;
+  int h = blockIdx.y * a.q_per_wave + mine;
+  const bits* q = static_cast<const bits*>(a.q) + b * a.qs.b + t * a.qs.t + h * a.qs.h;
+  bits* q_out = static_cast<bits*>(a.q_out) + (static_cast<int64_t>(token) * a.q_heads + h) * a.c.d + lane.d0;
+  RotaryPacket<T, MODE> p[kAhead];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, as_u32(y[i]) & 0x7fffffffu);
+  for (int u = 0; u < kAhead; ++u)
+    if (h + u * step < q_last) p[u].load(q + u * step * a.qs.h, lane);
+
+  const int kv_rows = 2 * a.c.heads;
+  const int kv_first = (static_cast<int>(blockIdx.y) - a.kv_from) * a.kv_per_wave;
+  // a wave of queries, and one of padding, has no rows of keys and values
+  const int kv_last = kv_first < 0 || !stored ? 0 : min(kv_rows, kv_first + a.kv_per_wave);
+  int r = max(kv_first, 0) + mine;
+  const auto kv_row = [&](int i) {
+    return i < a.c.heads ? static_cast<const bits*>(a.k) + b * a.ks.b + t * a.ks.t + i * a.ks.h
+                         : static_cast<const bits*>(a.v) + b * a.vs.b + t * a.vs.t + (i - a.c.heads) * a.vs.h;
+  };
+  RotaryPacket<T, MODE> kv;
+  if (in && r < kv_last) kv.load(kv_row(r), lane);
+  const int64_t first = kv_last > 0 ? a.c.row(b, slot, 0) : -1;  // of head 0
+
+  if constexpr (MODE != ROTARY_NONE) {
+    rotary_angles(cs, a.rot, position, index, 64);  // while the rows are on their way
+    wave_sync();
+    lane.angles(a.rot, cs);
+  }
+
+  while (h < q_last) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (h >= q_last) break;
+      float y[8];
+      lane.turn(y, p[u].own, p[u].other, q, a.rot, cs);
+      Packet<T> o;
+      o.pack(y);
+      if (h + kAhead * step < q_last) p[u].load(q + kAhead * step * a.qs.h, lane);
+      *reinterpret_cast<u32x4*>(q_out) = o.raw;
+      h += step;
+      q += step * a.qs.h;
+      q_out += step * a.c.d;
     }
+  }
+
+  if (first < 0) return;  // padding, or a slot without a place
+  for (; r < kv_last; r += step) {
+    const bool key = r < a.c.heads;
+    const int64_t at = first + static_cast<int64_t>(key ? r : r - a.c.heads) * a.c.page_size;
     void* pool = key ? a.c.k : a.c.v;
+    float y[8];
+    if (in) {
+      if (key) lane.turn(y, kv.own, kv.other, kv_row(r), a.rot, cs);
+      else kv.own.unpack(y);
+      if (r + step < kv_last) kv.load(kv_row(r + step), lane);
+    }
     if constexpr (FMT == KV_16BIT) {
-      if (in) {
-        Packet<T> o;
-        o.pack(y);
-        *reinterpret_cast<u32x4*>(static_cast<bits*>(pool) + at * a.c.d + d0) = o.raw;
-      }
+      Packet<T> o;
+      o.pack(y);
+      if (in) *reinterpret_cast<u32x4*>(static_cast<bits*>(pool) + at * a.c.d + lane.d0) = o.raw;
     } else {
+      uint32_t top = 0;
+      if (in) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, as_u32(y[e]) & 0x7fffffffu);
+      }
       top = row_max(top, a.lanes);
       const bool finite = top < 0x7f800000u;
       const float scale = finite ? fmaxf(as_f32(top) / kv_top<FMT>(), 1e-8f) : as_f32(top);
       if (in) {
-        u32x2 code = {0, 0};
-        if (finite) {
-          float lo[4], hi[4];
+        const float rc = 1.0f / scale;
+        float lo[4], hi[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            lo[i] = y[i] / scale;
-            hi[i] = y[4 + i] / scale;
-          }
-          code = u32x2{encode4<FMT>(lo), encode4<FMT>(hi)};
+        for (int e = 0; e < 4; ++e) {
+          lo[e] = quotient(y[e], scale, rc);
+          hi[e] = quotient(y[4 + e], scale, rc);
         }
-        *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(pool) + at * a.c.d + d0) = code;
+        const u32x2 code = {encode4<FMT>(lo), encode4<FMT>(hi)};
+        *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(pool) + at * a.c.d + lane.d0) = finite ? code : u32x2{0, 0};
       }
-      if (d0 == 0) (key ? a.c.k_scale : a.c.v_scale)[at] = scale;
+      if (lane.d0 == 0) (key ? a.c.k_scale : a.c.v_scale)[at] = scale;
     }
   }
 }
@@ -133,42 +165,50 @@ struct ReadArgs {
   KvCache c;
   void *k_out, *v_out;  // [batch, heads, tokens, d]
   const int32_t *start, *end;
-  int64_t tokens, rows;  // rows = batch * heads * tokens
+  int64_t rows;  // batch * heads * tokens
+  uint32_t tokens;
   int lanes;
 };
 
+// A lane's packet of a row's keys and values; every load of a row is issued
+// before any of its stores.
 template <typename T, int FMT> __global__ __launch_bounds__(256) void read_rows(ReadArgs a) {
   typedef typename T::bits bits;
   const int64_t r = static_cast<int64_t>(blockIdx.x) * (256 / a.lanes) + threadIdx.x / a.lanes;
   const int d0 = (threadIdx.x % a.lanes) * 8;
   if (r >= a.rows || d0 >= a.c.d) return;
-  const int64_t bh = r / a.tokens, i = r % a.tokens, b = bh / a.c.heads;
-  const int64_t slot = (a.start ? a.start[b] : 0) + i;
-  const int64_t at = slot < a.end[b] ? a.c.row(b, slot, static_cast<int>(bh % a.c.heads)) : -1;
+  // 32 bits hold a row: fewer than 2^27 of them
+  const uint32_t bh = static_cast<uint32_t>(r) / a.tokens, i = static_cast<uint32_t>(r) - bh * a.tokens;
+  const uint32_t b = bh / a.c.heads, h = bh - b * a.c.heads;
+  const int64_t slot = static_cast<int64_t>(a.start ? a.start[b] : 0) + i;
+  const int64_t at = slot < a.end[b] ? a.c.row(b, slot, static_cast<int>(h)) : -1;
+  Packet<T> o[2];
+  o[0].raw = o[1].raw = u32x4{0, 0, 0, 0};
+  if (at >= 0) {
+    if constexpr (FMT == KV_16BIT) {
+      o[0].raw = *reinterpret_cast<const u32x4*>(static_cast<const bits*>(a.c.k) + at * a.c.d + d0);
+      o[1].raw = *reinterpret_cast<const u32x4*>(static_cast<const bits*>(a.c.v) + at * a.c.d + d0);
+    } else {
+      u32x2 code[2];
+      code[0] = *reinterpret_cast<const u32x2*>(static_cast<const uint8_t*>(a.c.k) + at * a.c.d + d0);
+      code[1] = *reinterpret_cast<const u32x2*>(static_cast<const uint8_t*>(a.c.v) + at * a.c.d + d0);
+      const float scale[2] = {a.c.k_scale[at], a.c.v_scale[at]};
 #pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    Packet<T> o;
-    o.raw = u32x4{0, 0, 0, 0};
-    const void* pool = side ? a.c.v : a.c.k;
-    if (at >= 0) {
-      if constexpr (FMT == KV_16BIT) {
-        o.raw = *reinterpret_cast<const u32x4*>(static_cast<const bits*>(pool) + at * a.c.d + d0);
-      } else {
-        const u32x2 code = *reinterpret_cast<const u32x2*>(static_cast<const uint8_t*>(pool) + at * a.c.d + d0);
-        const float scale = (side ? a.c.v_scale : a.c.k_scale)[at];
+      for (int side = 0; side < 2; ++side) {
         float lo[4], hi[4], f[8];
-        decode4<FMT>(code[0], lo);
-        decode4<FMT>(code[1], hi);
+        decode4<FMT>(code[side][0], lo);
+        decode4<FMT>(code[side][1], hi);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          f[j] = lo[j] * scale;
-          f[4 + j] = hi[j] * scale;
+          f[j] = lo[j] * scale[side];
+          f[4 + j] = hi[j] * scale[side];
         }
-        o.pack(f);
+        o[side].pack(f);
       }
     }
-    *reinterpret_cast<u32x4*>(static_cast<bits*>(side ? a.v_out : a.k_out) + r * a.c.d + d0) = o.raw;
   }
+  *reinterpret_cast<u32x4*>(static_cast<bits*>(a.k_out) + r * a.c.d + d0) = o[0].raw;
+  *reinterpret_cast<u32x4*>(static_cast<bits*>(a.v_out) + r * a.c.d + d0) = o[1].raw;
 }
 
 struct KeepArgs {
@@ -211,11 +251,20 @@ __global__ __launch_bounds__(256) void keep_rows(KeepArgs a) {
   }
 }
 
-template <typename T> int append_typed(const AppendArgs& a, int fmt, dim3 grid, hipStream_t s) {
+template <typename T, int FMT> int append_format(const AppendArgs& a, dim3 grid, hipStream_t s) {
   static const char* what = "kv_cache_append launch";
-  if (fmt == KV_INT8) return launch(append_rows<T, KV_INT8>, grid, 256, 0, a, s, what);
-  if (fmt == KV_E4M3) return launch(append_rows<T, KV_E4M3>, grid, 256, 0, a, s, what);
-  return launch(append_rows<T, KV_16BIT>, grid, 256, 0, a, s, what);
+  switch (rotary_mode(a.rot, 8)) {
+    case ROTARY_NONE: return launch(append_rows<T, FMT, ROTARY_NONE>, grid, 256, 0, a, s, what);
+    case ROTARY_HALF: return launch(append_rows<T, FMT, ROTARY_HALF>, grid, 256, 0, a, s, what);
+    case ROTARY_PAIRS: return launch(append_rows<T, FMT, ROTARY_PAIRS>, grid, 256, 0, a, s, what);
+    default: return launch(append_rows<T, FMT, ROTARY_SINGLE>, grid, 256, 0, a, s, what);
+  }
+}
+
+template <typename T> int append_typed(const AppendArgs& a, int fmt, dim3 grid, hipStream_t s) {
+  if (fmt == KV_INT8) return append_format<T, KV_INT8>(a, grid, s);
+  if (fmt == KV_E4M3) return append_format<T, KV_E4M3>(a, grid, s);
+  return append_format<T, KV_16BIT>(a, grid, s);
 }
 
 template <typename T> int read_typed(const ReadArgs& a, int fmt, dim3 grid, hipStream_t s) {
@@ -232,20 +281,28 @@ int kv_append_launch(const mi355_kv_cache& cache, const RotaryArgs& rot, const v
                      int64_t tokens, int q_heads, int dtype, hipStream_t stream) {
   AppendArgs a{kv_cache_args(cache), rot, k, v, q, q_out, lens, new_lens,
                {strides[0], strides[1], strides[2]}, {strides[3], strides[4], strides[5]},
-               {strides[6], strides[7], strides[8]}, tokens, q_heads, 0, 0};
-  const int rows = q_heads + 2 * a.c.heads;
-  a.lanes = row_lanes(a.c.d / 8);
-  // one pass over rows per workgroup until the tokens alone fill the chip
-  a.rows_per_wg = batch * tokens < 1024 ? 256 / a.lanes : rows;
-  const dim3 grid(static_cast<unsigned>(batch * tokens),
-                  static_cast<unsigned>((rows + a.rows_per_wg - 1) / a.rows_per_wg));
+               {strides[6], strides[7], strides[8]}, static_cast<int>(batch * tokens),
+               static_cast<int>(tokens), q_heads, row_lanes(cache.head_dim / 8),
+               0, 0, 0};
+  const int step = 64 / a.lanes, kv_rows = 2 * a.c.heads;
+  const int q_passes = (q_heads + step - 1) / step, kv_passes = (kv_rows + step - 1) / step;
+  dim3 grid(static_cast<unsigned>((batch * tokens + kWaves - 1) / kWaves));
+  if (batch * tokens < 1024) {  // a pass per wave until the tokens alone fill the chip
+    a.q_per_wave = a.kv_per_wave = step;
+    a.kv_from = q_passes;
+    grid.y = static_cast<unsigned>(q_passes + kv_passes);
+  } else {
+    a.q_per_wave = q_heads;
+    a.kv_per_wave = kv_rows;
+  }
   return dtype == MI355_F16 ? append_typed<F16>(a, cache.format, grid, stream)
                             : append_typed<BF16>(a, cache.format, grid, stream);
 }
 
 int kv_read_launch(const mi355_kv_cache& cache, void* k_out, void* v_out, const int32_t* start, const int32_t* end,
                    int64_t batch, int64_t tokens, int dtype, hipStream_t stream) {
-  ReadArgs a{kv_cache_args(cache), k_out, v_out, start, end, tokens, batch * cache.kv_heads * tokens, 0};
+  ReadArgs a{kv_cache_args(cache), k_out, v_out, start, end, batch * cache.kv_heads * tokens,
+             static_cast<uint32_t>(tokens), 0};
   a.lanes = row_lanes(a.c.d / 8);
   const int per = 256 / a.lanes;
   const dim3 grid(static_cast<unsigned>((a.rows + per - 1) / per));

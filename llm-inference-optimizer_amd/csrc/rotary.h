@@ -12,8 +12,8 @@
 // fp32 frequency is exact; it is reduced to a fraction of a turn in 64 bits,
 // and only that fraction (|t| <= 1/2) goes to 32 bits for the sine and cosine:
 // at most 2^-26 turns, 10^-7 radians.  64-bit operations run at half the
-// 32-bit rate on this chip, and a workgroup computes a token's R/2 angles once
-// for all of its heads (through LDS).
+// 32-bit rate on this chip, and a wave computes a token's R/2 angles once for
+// all of its heads (through LDS).
 #pragma once
 
 #include "common.h"
@@ -31,10 +31,10 @@ struct RotaryArgs {
   int interleaved;  // 0: half layout
 };
 
-// Fills cs[j] = scale cos(p f_j), cs[kMaxPairs + j] = scale sin(p f_j); every
-// thread of the workgroup calls it, then a barrier.
-__device__ __forceinline__ void rotary_angles(float* cs, const RotaryArgs& a, int64_t p) {
-  for (int j = threadIdx.x; j < a.rotary / 2; j += blockDim.x) {
+// Fills cs[j] = scale cos(p f_j), cs[kMaxPairs + j] = scale sin(p f_j) with
+// `count` threads, this one the `index`-th; a barrier among them follows.
+__device__ __forceinline__ void rotary_angles(float* cs, const RotaryArgs& a, int64_t p, int index, int count) {
+  for (int j = index; j < a.rotary / 2; j += count) {
     const double turns = static_cast<double>(p) * static_cast<double>(a.inv_freq[j]) * 0.15915494309189533577;
     const float t = static_cast<float>(turns - __builtin_rint(turns));
     float s, c;
@@ -43,55 +43,96 @@ __device__ __forceinline__ void rotary_angles(float* cs, const RotaryArgs& a, in
     cs[kMaxPairs + j] = a.scale * s;
   }
 }
+// For one wave: LDS operations of a wave are done in order.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 
-// Elements d0 .. d0 + W - 1 of one head, loaded with what rotates into them.
-// `row` is the head's first element, 16-byte aligned; d0 a multiple of W.
-template <typename T> struct RotaryPacket {
+// How a lane's packet of elements meets its pairs.
+enum RotaryMode {
+  ROTARY_NONE,    // nothing is rotated
+  ROTARY_HALF,    // half layout, whole packets of partners
+  ROTARY_PAIRS,   // interleaved, whole packets of pairs
+  ROTARY_SINGLE   // element by element: R / 2 (or, interleaved, R) is no multiple of a packet
+};
+inline RotaryMode rotary_mode(const RotaryArgs& a, int width) {
+  if (a.rotary == 0) return ROTARY_NONE;
+  if (a.interleaved) return a.rotary % width == 0 ? ROTARY_PAIRS : ROTARY_SINGLE;
+  return a.rotary / 2 % width == 0 ? ROTARY_HALF : ROTARY_SINGLE;
+}
+
+// A lane's elements d0 .. d0 + W - 1 of every head turn by the same angles:
+//   y[i] = x[i] c[i] + (partner of x[i]) s[i]
+// with the sine's sign in s.  Held in registers over the heads of a token.
+template <typename T, int MODE> struct RotaryLane {
   static constexpr int W = pack_width<T>::value;
-  Packet<T> own, other;
+  float c[W], s[W];
+  int d0, partner;  // first element of the packet that holds the partners
+  bool turned;
 
-  __device__ __forceinline__ void load(const void* row, int d0, const RotaryArgs& a) {
-    const typename T::bits* r = static_cast<const typename T::bits*>(row);
-    own.raw = *reinterpret_cast<const u32x4*>(r + d0);
+  __device__ __forceinline__ RotaryLane(const RotaryArgs& a, int d0_) : d0(d0_) {
     const int half = a.rotary / 2;
-    // half layout with whole packets of partners; single elements otherwise
-    if (!a.interleaved && half % W == 0 && d0 < a.rotary)
-      other.raw = *reinterpret_cast<const u32x4*>(r + (d0 < half ? d0 + half : d0 - half));
+    turned = MODE != ROTARY_NONE && d0 < a.rotary;
+    partner = MODE != ROTARY_HALF || !turned ? d0 : d0 < half ? d0 + half : d0 - half;
   }
-
-  __device__ __forceinline__ void rotate(float (&y)[W], const void* row, int d0, const RotaryArgs& a,
-                                         const float* cs) const {
-    const float* sn = cs + kMaxPairs;
-    const int half = a.rotary / 2;
-    own.unpack(y);
-    if (d0 >= a.rotary) return;
-    if (a.interleaved) {
+  __device__ __forceinline__ void angles(const RotaryArgs& a, const float* cs) {
+    if constexpr (MODE == ROTARY_HALF || MODE == ROTARY_PAIRS) {
+      if (!turned) return;
+      const int half = a.rotary / 2;
 #pragma unroll
-      for (int i = 0; i < W; i += 2) {
-        if (d0 + i >= a.rotary) break;
-        const int j = (d0 + i) / 2;
-        const float x0 = y[i], x1 = y[i + 1];
-        y[i] = x0 * cs[j] - x1 * sn[j];
-        y[i + 1] = x1 * cs[j] + x0 * sn[j];
+      for (int i = 0; i < W; ++i) {
+        const int j = MODE == ROTARY_PAIRS ? (d0 + i) / 2 : (d0 < half ? d0 : d0 - half) + i;
+        const bool first = MODE == ROTARY_PAIRS ? (i & 1) == 0 : d0 < half;
+        c[i] = cs[j];
+        s[i] = first ? -cs[kMaxPairs + j] : cs[kMaxPairs + j];
       }
-    } else if (half % W == 0) {
+    }
+  }
+  // The packet `own` of a head and, in the half layout, its partners'.
+  __device__ __forceinline__ void turn(float (&y)[W], const Packet<T>& own, const Packet<T>& other, const void* row,
+                                       const RotaryArgs& a, const float* cs) const {
+    own.unpack(y);
+    if (!turned) return;
+    if constexpr (MODE == ROTARY_HALF) {
       float o[W];
       other.unpack(o);
-      const int j = d0 < half ? d0 : d0 - half;
-      const float sign = d0 < half ? -1.0f : 1.0f;
 #pragma unroll
-      for (int i = 0; i < W; ++i) y[i] = y[i] * cs[j + i] + sign * (o[i] * sn[j + i]);
-    } else {
+      for (int i = 0; i < W; ++i) y[i] = y[i] * c[i] + o[i] * s[i];
+    } else if constexpr (MODE == ROTARY_PAIRS) {
 #pragma unroll
+      for (int i = 0; i < W; i += 2) {
+        const float x0 = y[i], x1 = y[i + 1];
+        y[i] = x0 * c[i] + x1 * s[i];
+        y[i + 1] = x1 * c[i + 1] + x0 * s[i + 1];
+      }
+    } else if constexpr (MODE == ROTARY_SINGLE) {
+      const float* sn = cs + kMaxPairs;
+      const int half = a.rotary / 2;
+#pragma unroll 1
       for (int i = 0; i < W; ++i) {
         const int d = d0 + i;
         if (d >= a.rotary) break;
-        const bool lo = d < half;
-        const float o = load_elem<T>(row, lo ? d + half : d - half);
-        const int j = lo ? d : d - half;
-        y[i] = y[i] * cs[j] + (lo ? -(o * sn[j]) : o * sn[j]);
+        const bool first = a.interleaved ? (d & 1) == 0 : d < half;
+        const int j = a.interleaved ? d / 2 : first ? d : d - half;
+        const float x = load_elem<T>(row, d);
+        const float o = load_elem<T>(row, a.interleaved ? d ^ 1 : first ? d + half : d - half);
+        const float v = x * cs[j] + (first ? -(o * sn[j]) : o * sn[j]);
+#pragma unroll
+        for (int e = 0; e < W; ++e) y[e] = e == i ? v : y[e];
       }
     }
+  }
+};
+
+// A head's packet and its partners', on their way.
+template <typename T, int MODE> struct RotaryPacket {
+  Packet<T> own, other;
+  __device__ __forceinline__ void load(const void* row, const RotaryLane<T, MODE>& lane) {
+    const typename T::bits* r = static_cast<const typename T::bits*>(row);
+    own.raw = *reinterpret_cast<const u32x4*>(r + lane.d0);
+    if constexpr (MODE == ROTARY_HALF) other.raw = *reinterpret_cast<const u32x4*>(r + lane.partner);
   }
 };
 

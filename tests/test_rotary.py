@@ -16,7 +16,7 @@ def _freq(pairs, theta=1e6):
 @pytest.mark.parametrize("batch,tokens,heads,d,rotary", [
     (1, 1, 1, 64, 64), (3, 5, 12, 128, 128), (2, 7, 14, 64, 32), (1, 9, 3, 96, 24), (2, 2, 5, 80, 40),
     (1, 3, 2, 256, 256), (1, 4, 2, 36, 36), (2, 3, 3, 7, 6), (1, 2, 2, 300, 2), (1, 1100, 2, 64, 64),
-    (1, 2, 20, 128, 0), (1, 5, 3, 128, 74)])
+    (1, 2, 20, 128, 0), (1, 5, 3, 128, 74), (1, 3, 2, 512, 256), (2, 2, 3, 2048, 64)])
 def test_matches_64_bit_form(pkg, cuda, dtype, interleaved, batch, tokens, heads, d, rotary):
     g = torch.Generator().manual_seed(d + rotary)
     x = torch.randn((batch, tokens, heads, d), generator=g).to(dtype)

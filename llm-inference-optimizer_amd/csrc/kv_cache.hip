@@ -84,7 +84,7 @@ template <typename T, int FMT, int MODE> __global__ __launch_bounds__(64 * kWave
   RotaryPacket<T, MODE> p[kAhead];
 #pragma unroll
   for (int u = 0; u < kAhead; ++u)
-    if (h + u * step < q_last) p[u].load(q + u * step * a.qs.h, lane);
+    if (h + u * step < q_last) p[u].load(q + u * step * a.qs.h, lane, a.rot);
 
   const int kv_rows = 2 * a.c.heads;
   const int kv_first = (static_cast<int>(blockIdx.y) - a.kv_from) * a.kv_per_wave;
@@ -96,7 +96,7 @@ template <typename T, int FMT, int MODE> __global__ __launch_bounds__(64 * kWave
                          : static_cast<const bits*>(a.v) + b * a.vs.b + t * a.vs.t + (i - a.c.heads) * a.vs.h;
   };
   RotaryPacket<T, MODE> kv;
-  if (in && r < kv_last) kv.load(kv_row(r), lane);
+  if (in && r < kv_last) kv.load(kv_row(r), lane, a.rot);
   const int64_t first = kv_last > 0 ? a.c.row(b, slot, 0) : -1;  // of head 0
 
   if constexpr (MODE != ROTARY_NONE) {
@@ -110,10 +110,10 @@ template <typename T, int FMT, int MODE> __global__ __launch_bounds__(64 * kWave
     for (int u = 0; u < kAhead; ++u) {
       if (h >= q_last) break;
       float y[8];
-      lane.turn(y, p[u].own, p[u].other, q, a.rot, cs);
+      p[u].turn(y, lane);
       Packet<T> o;
       o.pack(y);
-      if (h + kAhead * step < q_last) p[u].load(q + kAhead * step * a.qs.h, lane);
+      if (h + kAhead * step < q_last) p[u].load(q + kAhead * step * a.qs.h, lane, a.rot);
       *reinterpret_cast<u32x4*>(q_out) = o.raw;
       h += step;
       q += step * a.qs.h;
@@ -128,9 +128,9 @@ template <typename T, int FMT, int MODE> __global__ __launch_bounds__(64 * kWave
     void* pool = key ? a.c.k : a.c.v;
     float y[8];
     if (in) {
-      if (key) lane.turn(y, kv.own, kv.other, kv_row(r), a.rot, cs);
+      if (key) kv.turn(y, lane);
       else kv.own.unpack(y);
-      if (r + step < kv_last) kv.load(kv_row(r + step), lane);
+      if (r + step < kv_last) kv.load(kv_row(r + step), lane, a.rot);
     }
     if constexpr (FMT == KV_16BIT) {
       Packet<T> o;
@@ -257,7 +257,7 @@ template <typename T, int FMT> int append_format(const AppendArgs& a, dim3 grid,
     case ROTARY_NONE: return launch(append_rows<T, FMT, ROTARY_NONE>, grid, 256, 0, a, s, what);
     case ROTARY_HALF: return launch(append_rows<T, FMT, ROTARY_HALF>, grid, 256, 0, a, s, what);
     case ROTARY_PAIRS: return launch(append_rows<T, FMT, ROTARY_PAIRS>, grid, 256, 0, a, s, what);
-    default: return launch(append_rows<T, FMT, ROTARY_SINGLE>, grid, 256, 0, a, s, what);
+    default: return launch(append_rows<T, FMT, ROTARY_ODD>, grid, 256, 0, a, s, what);
   }
 }
 

@@ -52,87 +52,79 @@ __device__ __forceinline__ void wave_sync() {
 
 // How a lane's packet of elements meets its pairs.
 enum RotaryMode {
-  ROTARY_NONE,    // nothing is rotated
-  ROTARY_HALF,    // half layout, whole packets of partners
-  ROTARY_PAIRS,   // interleaved, whole packets of pairs
-  ROTARY_SINGLE   // element by element: R / 2 (or, interleaved, R) is no multiple of a packet
+  ROTARY_NONE,   // nothing is rotated
+  ROTARY_HALF,   // half layout, whole packets of partners
+  ROTARY_PAIRS,  // interleaved
+  ROTARY_ODD     // half layout, R / 2 no multiple of a packet: partners one by one
 };
 inline RotaryMode rotary_mode(const RotaryArgs& a, int width) {
   if (a.rotary == 0) return ROTARY_NONE;
-  if (a.interleaved) return a.rotary % width == 0 ? ROTARY_PAIRS : ROTARY_SINGLE;
-  return a.rotary / 2 % width == 0 ? ROTARY_HALF : ROTARY_SINGLE;
+  if (a.interleaved) return ROTARY_PAIRS;
+  return a.rotary / 2 % width == 0 ? ROTARY_HALF : ROTARY_ODD;
 }
 
 // A lane's elements d0 .. d0 + W - 1 of every head turn by the same angles:
-//   y[i] = x[i] c[i] + (partner of x[i]) s[i]
+//   y[i] = x[i] c[i] + (partner of x[i]) s[i]     for i < turned, x[i] beyond
 // with the sine's sign in s.  Held in registers over the heads of a token.
 template <typename T, int MODE> struct RotaryLane {
   static constexpr int W = pack_width<T>::value;
   float c[W], s[W];
-  int d0, partner;  // first element of the packet that holds the partners
-  bool turned;
+  int d0, turned;
 
   __device__ __forceinline__ RotaryLane(const RotaryArgs& a, int d0_) : d0(d0_) {
+    turned = MODE == ROTARY_NONE ? 0 : max(0, min(a.rotary - d0, W));
+  }
+  // The element that rotates into element d of a half layout.
+  static __device__ __forceinline__ int partner(const RotaryArgs& a, int d) {
     const int half = a.rotary / 2;
-    turned = MODE != ROTARY_NONE && d0 < a.rotary;
-    partner = MODE != ROTARY_HALF || !turned ? d0 : d0 < half ? d0 + half : d0 - half;
+    return d < half ? d + half : d - half;
   }
   __device__ __forceinline__ void angles(const RotaryArgs& a, const float* cs) {
-    if constexpr (MODE == ROTARY_HALF || MODE == ROTARY_PAIRS) {
-      if (!turned) return;
-      const int half = a.rotary / 2;
+    const int half = a.rotary / 2;
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        const int j = MODE == ROTARY_PAIRS ? (d0 + i) / 2 : (d0 < half ? d0 : d0 - half) + i;
-        const bool first = MODE == ROTARY_PAIRS ? (i & 1) == 0 : d0 < half;
-        c[i] = cs[j];
-        s[i] = first ? -cs[kMaxPairs + j] : cs[kMaxPairs + j];
-      }
-    }
-  }
-  // The packet `own` of a head and, in the half layout, its partners'.
-  __device__ __forceinline__ void turn(float (&y)[W], const Packet<T>& own, const Packet<T>& other, const void* row,
-                                       const RotaryArgs& a, const float* cs) const {
-    own.unpack(y);
-    if (!turned) return;
-    if constexpr (MODE == ROTARY_HALF) {
-      float o[W];
-      other.unpack(o);
-#pragma unroll
-      for (int i = 0; i < W; ++i) y[i] = y[i] * c[i] + o[i] * s[i];
-    } else if constexpr (MODE == ROTARY_PAIRS) {
-#pragma unroll
-      for (int i = 0; i < W; i += 2) {
-        const float x0 = y[i], x1 = y[i + 1];
-        y[i] = x0 * c[i] + x1 * s[i];
-        y[i + 1] = x1 * c[i + 1] + x0 * s[i + 1];
-      }
-    } else if constexpr (MODE == ROTARY_SINGLE) {
-      const float* sn = cs + kMaxPairs;
-      const int half = a.rotary / 2;
-#pragma unroll 1
-      for (int i = 0; i < W; ++i) {
-        const int d = d0 + i;
-        if (d >= a.rotary) break;
-        const bool first = a.interleaved ? (d & 1) == 0 : d < half;
-        const int j = a.interleaved ? d / 2 : first ? d : d - half;
-        const float x = load_elem<T>(row, d);
-        const float o = load_elem<T>(row, a.interleaved ? d ^ 1 : first ? d + half : d - half);
-        const float v = x * cs[j] + (first ? -(o * sn[j]) : o * sn[j]);
-#pragma unroll
-        for (int e = 0; e < W; ++e) y[e] = e == i ? v : y[e];
-      }
+    for (int i = 0; i < W; ++i) {
+      if (i >= turned) break;
+      const int d = d0 + i;
+      const bool first = MODE == ROTARY_PAIRS ? (i & 1) == 0 : d < half;
+      const int j = MODE == ROTARY_PAIRS ? d / 2 : first ? d : d - half;
+      c[i] = cs[j];
+      s[i] = first ? -cs[kMaxPairs + j] : cs[kMaxPairs + j];
     }
   }
 };
 
-// A head's packet and its partners', on their way.
+// A head's packet and what rotates into it, on their way.
 template <typename T, int MODE> struct RotaryPacket {
+  static constexpr int W = pack_width<T>::value;
+  typedef typename T::bits bits;
   Packet<T> own, other;
-  __device__ __forceinline__ void load(const void* row, const RotaryLane<T, MODE>& lane) {
-    const typename T::bits* r = static_cast<const typename T::bits*>(row);
+  bits single[MODE == ROTARY_ODD ? W : 1];
+
+  __device__ __forceinline__ void load(const void* row, const RotaryLane<T, MODE>& lane, const RotaryArgs& a) {
+    const bits* r = static_cast<const bits*>(row);
     own.raw = *reinterpret_cast<const u32x4*>(r + lane.d0);
-    if constexpr (MODE == ROTARY_HALF) other.raw = *reinterpret_cast<const u32x4*>(r + lane.partner);
+    if constexpr (MODE == ROTARY_HALF)
+      other.raw = *reinterpret_cast<const u32x4*>(r + (lane.turned ? lane.partner(a, lane.d0) : lane.d0));
+    if constexpr (MODE == ROTARY_ODD) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) single[i] = r[i < lane.turned ? lane.partner(a, lane.d0 + i) : lane.d0];
+    }
+  }
+  __device__ __forceinline__ void turn(float (&y)[W], const RotaryLane<T, MODE>& lane) const {
+    own.unpack(y);
+    if constexpr (MODE == ROTARY_NONE) return;
+    float o[W];
+    if constexpr (MODE == ROTARY_HALF) other.unpack(o);
+    if constexpr (MODE == ROTARY_PAIRS) own.unpack(o);
+    if constexpr (MODE == ROTARY_ODD) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) o[i] = load_elem<T>(&single[i], 0);
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const float v = y[i] * lane.c[i] + o[MODE == ROTARY_PAIRS ? i ^ 1 : i] * lane.s[i];
+      y[i] = i < lane.turned ? v : y[i];
+    }
   }
 };
 

@@ -42,7 +42,7 @@ template <typename T, int MODE> __global__ __launch_bounds__(64 * kWaves) void r
   bits* y = static_cast<bits*>(a.y) + (static_cast<int64_t>(token) * a.heads + h) * a.d + lane.d0;
   RotaryPacket<T, MODE> p[kAhead];
   const auto load = [&](int u) {
-    if (h + u * step < last) p[u].load(x + u * step * a.sh, lane);
+    if (h + u * step < last) p[u].load(x + u * step * a.sh, lane, a.rot);
   };
 #pragma unroll
   for (int u = 0; u < kAhead; ++u) load(u);  // on their way while the angles are computed
@@ -56,10 +56,10 @@ template <typename T, int MODE> __global__ __launch_bounds__(64 * kWaves) void r
     for (int u = 0; u < kAhead; ++u) {
       if (h >= last) break;
       float v[W];
-      lane.turn(v, p[u].own, p[u].other, x, a.rot, cs);
+      p[u].turn(v, lane);
       Packet<T> o;
       o.pack(v);
-      if (h + kAhead * step < last) p[u].load(x + kAhead * step * a.sh, lane);
+      if (h + kAhead * step < last) p[u].load(x + kAhead * step * a.sh, lane, a.rot);
       *reinterpret_cast<u32x4*>(y) = o.raw;
       h += step;
       x += step * a.sh;
@@ -109,7 +109,7 @@ template <typename T> int rotary_typed(Args a, hipStream_t s) {
       case ROTARY_NONE: return launch(rotary_rows<T, ROTARY_NONE>, grid, 256, 0, a, s, what);
       case ROTARY_HALF: return launch(rotary_rows<T, ROTARY_HALF>, grid, 256, 0, a, s, what);
       case ROTARY_PAIRS: return launch(rotary_rows<T, ROTARY_PAIRS>, grid, 256, 0, a, s, what);
-      default: return launch(rotary_rows<T, ROTARY_SINGLE>, grid, 256, 0, a, s, what);
+      default: return launch(rotary_rows<T, ROTARY_ODD>, grid, 256, 0, a, s, what);
     }
   }
   return launch(rotary_generic<T>, grid, 256, 0, a, s, what);

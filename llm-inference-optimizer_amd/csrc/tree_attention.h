@@ -26,7 +26,7 @@ struct TreeArgs {
   int32_t* starts;      // [1 + batch]: the workgroups' share of tiles, the first tile of each sequence
   int batch, tokens, q_heads, group;  // group = q_heads / kv_heads
   int block_rows, blocks;             // row blocks
-  int tile;                           // slots of a tile on the line
+  int tile, pad;                      // slots of a tile on the line, tiles that a piece costs beside its own
   int grid;                           // workgroups of the first kernel
   uint32_t page_mul, page_shift;      // unit / units per page = unit * page_mul >> page_shift
   float scale;                        // |scale| log2 e
@@ -43,7 +43,9 @@ __device__ __forceinline__ int32_t scalar_load(const int32_t* p, int64_t i) {
 }
 
 // One sequence: its context, new tokens, slots in use, and tiles per head and
-// row block.
+// row block.  `pad` of those, the first, stand for what a piece costs besides
+// its tiles (queries to load, sums to join and write): a share that holds the
+// beginning of more pieces holds fewer tiles.
 struct Seq {
   int len, fresh, end, tiles;
   __device__ __forceinline__ Seq(const TreeArgs& a, int len_, int fresh_) {
@@ -51,7 +53,7 @@ struct Seq {
     len = max(0, min(len_, cap));
     fresh = max(0, min(fresh_, a.tokens));
     end = min(len + fresh, cap);
-    tiles = max(1, (end + a.tile - 1) / a.tile);
+    tiles = a.pad + max(1, (end + a.tile - 1) / a.tile);
   }
   // by a scalar b
   static __device__ __forceinline__ Seq of(const TreeArgs& a, int b) {
@@ -518,20 +520,20 @@ __device__ __forceinline__ void store_result(const TreeArgs& a, const Piece& p, 
 // vector registers would make each load a loop over the lanes.
 struct Share {
   Line line;
-  int at, last, b, start, first;
+  int at, last, b, start, first, size;
   // one piece
   Piece p;
-  int t0, t1, tiles;
+  int t0, t1, tiles;  // tiles [t0, t1) of `tiles`
+  int width;          // on the line
   const int32_t* table;
 
   __device__ __forceinline__ Share(const TreeArgs& a, int step) {
     if (a.partial) {
       line = Line(a);
-      const int share = line_share(line.total, a.grid, step);
-      at = static_cast<int>(blockIdx.x) * share;
-      last = at + share;
+      size = line_share(line.total, a.grid, step);
+      at = static_cast<int>(blockIdx.x) * size;
+      last = at + size;
       b = line.find(a, at, &start);
-      if (blockIdx.x == 0 && uniform(threadIdx.x >> 6) == 0) line.write(a, share, a.starts);
     } else {  // one (head, block) of one sequence
       const int hm_count = a.c.heads * a.blocks;
       b = blockIdx.x / hm_count;
@@ -545,16 +547,23 @@ struct Share {
     const int hm_count = a.c.heads * a.blocks;
     while (b < a.batch && at < last) {
       const Seq s = a.partial && b < 64 ? line.seq(a, b) : Seq::of(a, b);
-      tiles = uniform(s.tiles);
-      const int hm = uniform((at - start) / tiles);
+      const int hm = uniform((at - start) / s.tiles);
       if (hm >= hm_count) {
-        start = uniform(start + tiles * hm_count);
+        start = uniform(start + s.tiles * hm_count);
         b = uniform(b + 1);
         continue;
       }
-      t0 = uniform(at - start - hm * tiles);
-      if (!a.partial) last = uniform(at + tiles);
-      t1 = uniform(min(tiles, t0 + last - at));
+      const int v0 = uniform(at - start - hm * s.tiles);
+      if (!a.partial) last = uniform(at + s.tiles);
+      const int v1 = uniform(min(s.tiles, v0 + last - at));
+      tiles = uniform(s.tiles - a.pad);
+      t0 = max(0, v0 - a.pad);
+      t1 = v1 - a.pad;
+      width = v1 - v0;
+      if (t1 <= t0) {  // the share ends before the piece's first tile
+        done();
+        continue;
+      }
       const int h = uniform(hm / a.blocks), row0 = uniform((hm - h * a.blocks) * a.block_rows);
       p = Piece{b, h, row0, uniform(min(a.block_rows, a.tokens * a.group - row0)), uniform(s.len), uniform(s.fresh),
                 uniform(min(s.end, t1 * a.tile))};
@@ -563,10 +572,14 @@ struct Share {
     }
     return false;
   }
+  // For the join; last, since loads wait for the stores before them.
+  __device__ __forceinline__ void finish(const TreeArgs& a) const {
+    if (a.partial && blockIdx.x == 0 && uniform(threadIdx.x >> 6) == 0) line.write(a, size, a.starts);
+  }
   __device__ __forceinline__ bool cut() const { return t0 > 0 || t1 < tiles; }
   // where the piece goes in the workspace: the first of the share, or the last
   __device__ __forceinline__ int64_t slot() const { return 2 * static_cast<int64_t>(blockIdx.x) + (at == first ? 0 : 1); }
-  __device__ __forceinline__ void done() { at = uniform(at + t1 - t0); }
+  __device__ __forceinline__ void done() { at = uniform(at + width); }
 };
 
 }  // namespace mi355

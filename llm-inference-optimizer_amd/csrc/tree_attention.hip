@@ -216,6 +216,7 @@ __global__ __launch_bounds__(64 * kWaves, stream_waves(DP, MT)) void tree_attent
     __syncthreads();
     share.done();
   }
+  share.finish(a);
 }
 
 // More rows: the four waves of a workgroup take 16 MT rows each and share the
@@ -460,6 +461,7 @@ __global__ __launch_bounds__(64 * kWaves, wide_groups(DP, MT)) void tree_attenti
     }
     share.done();
   }
+  share.finish(a);
 }
 
 // Adds the pieces of one query row that was cut, in order: lanes 0 - 31 and
@@ -484,7 +486,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void tree_attention_join(TreeArgs 
   const int h = hq / a.group, r = t * a.group + hq - h * a.group;
   const int block = r / block_rows, rr = r - block * block_rows;
   const int first = start + (h * a.blocks + block) * s.tiles;
-  const int w0 = first / share, w1 = (first + s.tiles - 1) / share;
+  const int w0 = (first + a.pad) / share, w1 = (first + s.tiles - 1) / share;
   const bool mine = qrow < row_count && w0 != w1;  // else written by the first kernel
   if (WAVES > 1 && !mine) return;
 
@@ -555,7 +557,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void tree_attention_join(TreeArgs 
 // Kernel, row blocks and grid of a call.
 struct Plan {
   bool wide;
-  int mt, block_rows, blocks, tile, step, grid;
+  int mt, block_rows, blocks, tile, pad, step, grid;
   int64_t partial_bytes, stats_bytes, bytes;  // of the workspace; 0: no split
 };
 
@@ -569,10 +571,15 @@ Plan plan(const mi355_kv_cache& c, int64_t batch, int64_t tokens, int64_t q_head
   p.blocks = static_cast<int>((rows + p.block_rows - 1) / p.block_rows);
   p.tile = p.wide ? kWideTile : kStreamTile;
   p.step = p.wide ? 1 : kWaves;  // tiles of a workgroup's step
+  // What a piece costs beside its tiles, in tiles.  Measured (stream, wide): 0, 0
+  // / 4, 2 / 8, 4 / 16, 6 tiles give 37.9 / 36.4 / 34.6 / 36.5 us for 32 ragged
+  // contexts to 6000, 14.2 / 10.6 / 9.8 / 9.6 us for one of 777 and 65.7 / 61.2
+  // / 60.3 / 62.1 us for 8 trees of 48.
+  p.pad = p.wide ? 4 : 8;
   const int64_t pieces = batch * c.kv_heads * p.blocks;
-  const int64_t tiles = (c.table_width * c.page_size + p.tile - 1) / p.tile;  // of the longest possible context
+  const int64_t tiles = (c.table_width * c.page_size + p.tile - 1) / p.tile + p.pad;  // of the longest possible context
   p.grid = static_cast<int>(pieces);
-  if (tiles <= 2 * p.step || pieces * tiles > 0x7fffffff - 65536 * p.step) return p;
+  if (tiles - p.pad <= 2 * p.step || pieces * tiles > 0x7fffffff - 65536 * p.step) return p;
   const int64_t wanted = (pieces * tiles + p.step - 1) / p.step;
   const int64_t most = static_cast<int64_t>(cus) * (p.wide ? wide_groups(dp, p.mt) : stream_waves(dp, p.mt));
   p.grid = static_cast<int>(wanted < most ? wanted : most);
@@ -630,9 +637,10 @@ int tree_attention_launch(const mi355_kv_cache& cache, const void* q, void* out,
   Plan p = plan(cache, batch, tokens, q_heads, cus);
   TreeArgs a{kv_cache_args(cache), q, out, lens, new_lens, mask, mask_b, mask_t, q_strides[0], q_strides[1],
              q_strides[2], nullptr, nullptr, nullptr, static_cast<int>(batch), tokens, q_heads,
-             q_heads / static_cast<int>(cache.kv_heads), p.block_rows, p.blocks, p.tile, 0, 0, 0, __builtin_fabsf(scale) * kLog2e, scale < 0.f};
+             q_heads / static_cast<int>(cache.kv_heads), p.block_rows, p.blocks, p.tile, 0, 0, 0, 0, __builtin_fabsf(scale) * kLog2e, scale < 0.f};
   if (p.bytes > 0 && work != nullptr && work_bytes >= p.bytes) {
     a.partial = static_cast<float*>(work);
+    a.pad = p.pad;
     a.stats = reinterpret_cast<float2*>(static_cast<uint8_t*>(work) + p.partial_bytes);
     a.starts = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(work) + p.partial_bytes + p.stats_bytes);
   } else {

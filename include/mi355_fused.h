@@ -348,7 +348,7 @@ typedef struct mi355_kv_cache {
   float* v_scale;            /* the same */
   const int32_t* page_table; /* [batch, table_stride], table_width of them in use */
   int64_t table_stride;
-  int64_t table_width;       /* table_width * page_size < 2^31 - 256 */
+  int64_t table_width;       /* table_width * page_size < 2^30 */
   int64_t pages;             /* < 2^31 */
   int64_t kv_heads;          /* 1 .. 65535 */
   int64_t page_size;         /* a multiple of 16 */
@@ -373,7 +373,7 @@ typedef struct mi355_kv_cache {
  *   q, q_out  [batch, tokens, q_heads, head_dim] likewise, q_out contiguous;
  *             both NULL (q_heads = 0) to rotate no queries.
  *   inv_freq  NULL (rotary_dim = 0): nothing is rotated, positions is not read.
- *   batch * tokens < 2^24.
+ *   batch * tokens < 2^24, q_heads + 2 kv_heads <= 65535.
  */
 int mi355_kv_cache_append_fwd(const mi355_kv_cache* cache, const void* k, const void* v, const void* q, void* q_out,
                               const int32_t* seq_lens, const int32_t* new_lens,

@@ -59,8 +59,8 @@ int check_cache(const char* fn, const mi355_kv_cache* c) {
   }
   if (c->head_dim % 16 != 0 || c->head_dim > 256) return beyond(fn, "head_dim must be a multiple of 16, at most 256");
   if (c->page_size % 16 != 0) return beyond(fn, "page_size must be a multiple of 16");
-  if (c->kv_heads > 65535 || c->pages > 0x7fffffff || !product_below(c->table_width, c->page_size, 0x7fffffff - 256))
-    return beyond(fn, "cache beyond the kernels' limits (kv_heads <= 65535, pages < 2^31, table slots < 2^31 - 256)");
+  if (c->kv_heads > 65535 || c->pages > 0x7fffffff || !product_below(c->table_width, c->page_size, int64_t{1} << 30))
+    return beyond(fn, "cache beyond the kernels' limits (kv_heads <= 65535, pages < 2^31, table slots < 2^30)");
   return MI355_OK;
 }
 
@@ -143,8 +143,8 @@ MI355_EXPORT int mi355_kv_cache_append_fwd(const mi355_kv_cache* cache, const vo
   st = check_rotary(fn, rotary_dim, cache->head_dim, positions, inv_freq);
   if (st != MI355_OK) return st;
   if (batch == 0 || tokens == 0) return MI355_OK;
-  if (!product_below(batch, tokens, kMaxRows) || q_heads > 65535)
-    return beyond(fn, "size beyond the kernel's limits (batch * tokens < 2^24, q_heads <= 65535)");
+  if (!product_below(batch, tokens, kMaxRows) || q_heads > 65535 || q_heads + 2 * cache->kv_heads > 65535)
+    return beyond(fn, "size beyond the kernel's limits (batch * tokens < 2^24, q_heads + 2 kv_heads <= 65535)");
   if (k == nullptr || v == nullptr || seq_lens == nullptr || strides == nullptr ||
       (q_heads > 0 && (q == nullptr || q_out == nullptr)))
     return bad(fn, "null pointer");

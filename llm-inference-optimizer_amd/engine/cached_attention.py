@@ -30,11 +30,6 @@ ATTENTION_CLASS_NAMES = {"Qwen2Attention", "LlamaAttention", "MistralAttention"}
 _PARTS = ("q_proj", "k_proj", "v_proj", "o_proj", "head_dim", "layer_idx", "scaling")
 
 
-def _dynamic_cache():
-    from transformers import DynamicCache
-    return DynamicCache
-
-
 class DecoderCache:
     """What a decode step needs to know of the cache, for ``CachedAttention``:
     one ``KVCache`` per layer (they share a page table) and the step's static
@@ -61,9 +56,8 @@ class DecoderCache:
                              "patch_model_with_fused_kernels(model, fuse_attention=True)")
         rotary = model.model.rotary_emb
         p = next(model.parameters())
-        kv_heads = {b.k_proj.out_features // b.head_dim for b in blocks}
-        layers = [KVCache.allocate(batch_size, max_len, kv_heads.copy().pop(), b.head_dim, kv_format, p.dtype, p.device,
-                                   page_size) for b in blocks]
+        layers = [KVCache.allocate(batch_size, max_len, b.k_proj.out_features // b.head_dim, b.head_dim, kv_format,
+                                   p.dtype, p.device, page_size) for b in blocks]
         table = layers[0].page_table
         for c in layers:
             c.page_table = table
@@ -71,7 +65,9 @@ class DecoderCache:
 
     def as_past(self):
         """An HF cache object that carries this one."""
-        past = _dynamic_cache()()
+        from transformers import DynamicCache
+
+        past = DynamicCache()
         past.mi355_cache = self
         return past
 

@@ -57,7 +57,8 @@ BAD_CACHES = [
     (dict(format=3), -1, "format"), (dict(pages=-1), -1, "sizes"), (dict(kv_heads=0), -1, "sizes"),
     (dict(table_stride=7), -1, "sizes"), (dict(head_dim=72), -2, "head_dim"), (dict(head_dim=272), -2, "head_dim"),
     (dict(page_size=24), -2, "page_size"), (dict(kv_heads=65536), -2, "limits"), (dict(pages=1 << 31), -2, "limits"),
-    (dict(table_width=1 << 27, table_stride=1 << 27), -2, "limits"), (dict(k=0), -1, "null"),
+    (dict(table_width=1 << 26, table_stride=1 << 26), -2, "limits"),
+    (dict(pages=0), -1, "without pages"), (dict(table_width=0), -1, "without pages"), (dict(k=0), -1, "null"),
     (dict(page_table=0), -1, "null"), (dict(v=P + 8), -1, "aligned"), (dict(k_scale=0), -1, "scales"),
     (dict(v_scale=P + 4), -1, "aligned")]
 
@@ -85,7 +86,8 @@ def test_null_cache(lib):
 @pytest.mark.parametrize("kw,code,message", [
     (dict(dtype=0), -2, "fp16 or bf16"), (dict(dtype=9), -1, "unknown dtype"), (dict(tokens=-1), -1, "sizes"),
     (dict(r=2, pos=0), -1, "positions"), (dict(r=66), -1, "rotary_dim"), (dict(batch=1 << 20, tokens=1 << 20), -2, "limits"),
-    (dict(qh=65536), -2, "limits"), (dict(k=0), -1, "null"), (dict(lens=0), -1, "null"), (dict(qh=2, q=0), -1, "null"),
+    (dict(qh=65536), -2, "limits"), (dict(qh=65532), -2, "limits"), (dict(k=0), -1, "null"), (dict(lens=0), -1, "null"),
+    (dict(qh=2, q=0), -1, "null"),
     (dict(k=P + 2), -2, "aligned"), (dict(strides=[64, 64, 60] + [64] * 6), -2, "multiples of 8"),
     (dict(strides=[-64, 64, 64] + [64] * 6), -1, "strides")])
 def test_append_abi_rejects(L, lib, kw, code, message):

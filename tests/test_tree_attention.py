@@ -33,6 +33,9 @@ def _case(pkg, kind, dtype, batch, tokens, hq, kvh, d, page, lens, seed=1):
     (1, 64, 8, 1, 256, 16, [40], True),
     (2, 128, 4, 4, 16, 256, [250, 0], True),
     (5, 3, 40, 8, 128, 16, [16, 32, 48, 15, 17], False),
+    (1, 50, 28, 4, 128, 64, [100], True),
+    (2, 3, 8, 1, 256, 32, [70, 5], True),
+    (1, 20, 6, 1, 64, 32, [33], True),
     (1, 2, 32, 32, 32, 16, [1030], False)])
 def test_matches_64_bit_form(pkg, cuda, kind, dtype, batch, tokens, hq, kvh, d, page, lens, tree):
     cache, q = _case(pkg, kind, dtype, batch, tokens, hq, kvh, d, page, lens)
@@ -50,6 +53,56 @@ def test_long_and_unequal_contexts(pkg, cuda, kind, lens, batch_pad):
     """Contexts that are split over workgroups, beside ones that are not."""
     cache, q = _case(pkg, kind, torch.bfloat16, len(lens), 2, 8, 2, 128, 64, lens)
     K.close(pkg.tree_attention(q, cache, K.ints(lens)), *K.attention(q, cache, lens))
+
+
+@pytest.mark.parametrize("tokens,kind,d", [(20, "int8", 64), (12, "16bit", 128), (9, "e4m3", 256)])
+def test_long_contexts_of_many_rows(pkg, cuda, tokens, kind, d):
+    lens = [5000, 700]
+    cache, q = _case(pkg, kind, torch.float16, 2, tokens, 12, 2, d, 48, lens)
+    mask = K.random_tree(2, tokens, 9)
+    K.close(pkg.tree_attention(q, cache, K.ints(lens), tree_mask=mask.to(cuda)), *K.attention(q, cache, lens, mask=mask))
+
+
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_more_than_64_sequences(pkg, cuda, tokens):
+    """Contexts of 0 to 400 slots of 150 sequences: the plan goes over the lengths in several rounds."""
+    g = torch.Generator().manual_seed(5)
+    lens = torch.randint(0, 400, (150,), generator=g).tolist()
+    lens[:3], lens[63:66], lens[149] = [0, 0, 400], [1, 399, 0], 400
+    new = torch.randint(0, tokens + 1, (150,), generator=g).tolist()
+    cache, q = _case(pkg, "int8", torch.float16, 150, tokens, 2, 1, 32, 16, lens)
+    pick = [0, 1, 2, 63, 64, 65, 100, 128, 149]
+    out = pkg.tree_attention(q, cache, K.ints(lens), new_lens=K.ints(new))
+    part = pkg.KVCache(cache.k, cache.v, cache.page_table[pick], cache.k_scale, cache.v_scale)
+    K.close(out[pick], *K.attention(q[pick], part, [lens[i] for i in pick], [new[i] for i in pick]))
+    # all of them against the same sequences in batches of their own
+    for i in range(0, 150, 50):
+        part = pkg.KVCache(cache.k, cache.v, cache.page_table[i:i + 50], cache.k_scale, cache.v_scale)
+        one = pkg.tree_attention(q[i:i + 50], part, K.ints(lens[i:i + 50]), new_lens=K.ints(new[i:i + 50]))
+        # other splits of the same sums: fp32 rounding and one step of fp16
+        assert (one.float() - out[i:i + 50].float()).abs().max().item() <= 2.0 ** -9
+
+
+def test_without_a_workspace(pkg, cuda):
+    """The C call without scratch memory: every sequence and head in one workgroup, the same result up to the order of
+    the sums."""
+    import ctypes
+    import importlib
+    L = importlib.import_module("llm-inference-optimizer_amd._lib")
+    for tokens, lens in ((1, [3000, 17, 0]), (30, [900, 65, 0])):
+        cache, q = _case(pkg, "int8", torch.float16, 3, tokens, 6, 2, 128, 32, lens)
+        c = L.KvCacheStruct(cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
+                            cache.page_table.data_ptr(), cache.page_table.shape[1], cache.page_table.shape[1],
+                            *cache.k.shape, L.KV_INT8)
+        n = K.ints(lens)
+        lib = L.load()
+        assert lib.mi355_tree_attention_workspace(ctypes.byref(c), 3, tokens, 6) > 0
+        out = torch.full_like(q, float("nan"))
+        strides = (ctypes.c_int64 * 3)(*q.stride()[:3])
+        assert lib.mi355_tree_attention_fwd(ctypes.byref(c), q.data_ptr(), out.data_ptr(), n.data_ptr(), None, None, 0, 0,
+                                            3, tokens, 6, strides, 128 ** -0.5, L.F16, None, 0,
+                                            L.stream_handle(q.device)) == 0
+        K.close(out, *K.attention(q, cache, lens))
 
 
 @pytest.mark.parametrize("kind", FORMATS)

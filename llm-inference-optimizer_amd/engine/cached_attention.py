@@ -55,6 +55,9 @@ class DecoderCache:
             raise ValueError("kv_cache needs the model's attention patched: "
                              "patch_model_with_fused_kernels(model, fuse_attention=True)")
         rotary = model.model.rotary_emb
+        if getattr(rotary, "rope_type", "default") in ("dynamic", "longrope"):
+            raise ValueError(f"rope_type {rotary.rope_type!r} changes the frequencies as the text grows: cached keys "
+                             "would keep old ones")
         p = next(model.parameters())
         layers = [KVCache.allocate(batch_size, max_len, b.k_proj.out_features // b.head_dim, b.head_dim, kv_format,
                                    p.dtype, p.device, page_size) for b in blocks]
@@ -82,10 +85,12 @@ class DecoderCache:
 
 def cacheable(module: torch.nn.Module) -> bool:
     """Whether ``CachedAttention`` can run this attention module: grouped heads
-    of a width the cache takes, rotary over the whole head, no window and no
-    norms of queries and keys."""
+    of a width the cache takes, no window and no norms of queries and keys."""
+    # a module without a window of its own may take the model's
+    config = getattr(module, "config", None)
+    window = module.sliding_window if hasattr(module, "sliding_window") else getattr(config, "sliding_window", None)
     return (module.__class__.__name__ in ATTENTION_CLASS_NAMES and all(hasattr(module, p) for p in _PARTS)
-            and getattr(module, "sliding_window", None) is None and not hasattr(module, "q_norm")
+            and window is None and not hasattr(module, "q_norm")
             and module.head_dim % 16 == 0 and module.head_dim <= 256)
 
 

@@ -21,6 +21,12 @@ from .. import _lib
 
 __all__ = ["fused_rotary", "rotary_frequencies"]
 
+# what each rope_type reads
+_SCALING_KEYS = {
+    "default": set(), "linear": {"factor"}, "ntk": {"factor"},
+    "yarn": {"factor", "original_max_position_embeddings", "beta_fast", "beta_slow", "attention_factor"},
+    "llama3": {"factor", "original_max_position_embeddings", "low_freq_factor", "high_freq_factor"}}
+
 
 def fused_rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, scale: float = 1.0,
                  interleaved: bool = False) -> torch.Tensor:
@@ -52,12 +58,21 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: dict | 
       0.1 ln(factor) + 1.
     * ``{"rope_type": "llama3", "factor", "original_max_position_embeddings",
       "low_freq_factor", "high_freq_factor"}``: the same idea with a ramp over
-      the turns themselves, between low_freq_factor and high_freq_factor."""
+      the turns themselves, between low_freq_factor and high_freq_factor.
+
+    Other types and keys are refused (None values, "type" beside "rope_type" and
+    a "rope_theta" that is theta excepted)."""
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
     d, scale = rotary_dim, 1.0
     j = torch.arange(0, d, 2, dtype=torch.float64)
-    kind = (scaling or {}).get("rope_type", "default")
+    kind = scaling.get("rope_type", scaling.get("type")) if scaling else "default"
+    if kind not in _SCALING_KEYS:
+        raise ValueError(f"unknown rope_type {kind!r} ({', '.join(_SCALING_KEYS)})")
+    unknown = {k for k, v in (scaling or {}).items() if v is not None and not (k == "rope_theta" and v == theta)}
+    unknown -= _SCALING_KEYS[kind] | {"rope_type", "type"}
+    if unknown:
+        raise ValueError(f"rope_type {kind!r} does not take {', '.join(sorted(unknown))}")
     if kind == "ntk":
         theta = theta * scaling["factor"] ** (d / (d - 2)) if d > 2 else theta
     freq = theta ** (-j / d)
@@ -79,6 +94,4 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: dict | 
         low, high = scaling["low_freq_factor"], scaling["high_freq_factor"]
         keep = ((turns - low) / (high - low)).clamp(0, 1)
         freq = freq * keep + freq / scaling["factor"] * (1 - keep)
-    elif kind not in ("default", "ntk"):
-        raise ValueError(f"unknown rope_type {kind!r} (default, linear, ntk, yarn, llama3)")
     return freq.to(device=device, dtype=torch.float32), float(scale)

@@ -190,3 +190,39 @@ def test_frequencies_ntk_and_refusals(pkg):
     for args in ((3,), (0,), (64, 1e4, {"rope_type": "dynamic", "factor": 2.0})):
         with pytest.raises(ValueError):
             pkg.rotary_frequencies(*args)
+
+
+def test_frequencies_refuse_what_they_would_ignore(pkg):
+    yarn = {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 4096}
+    base, _ = pkg.rotary_frequencies(64, 1e4, yarn)
+    same = {"type": "yarn", "factor": 4.0, "original_max_position_embeddings": 4096, "rope_theta": 1e4, "beta_fast": None}
+    assert torch.equal(pkg.rotary_frequencies(64, 1e4, same)[0], base)
+    for other in ({**yarn, "mscale": 0.7}, {**yarn, "rope_theta": 1e6}, {"factor": 2.0}, {"rope_type": "default", "factor": 2.0}):
+        with pytest.raises(ValueError):
+            pkg.rotary_frequencies(64, 1e4, other)
+
+
+def _tiny(kind, **kw):
+    transformers = pytest.importorskip("transformers")
+    cfg = getattr(transformers, kind + "Config")(hidden_size=64, intermediate_size=64, num_hidden_layers=2, vocab_size=64,
+                                                 num_attention_heads=4, num_key_value_heads=2, **kw)
+    return getattr(transformers, kind + "ForCausalLM")(cfg)
+
+
+@pytest.mark.parametrize("kind,kw,count", [
+    ("Mistral", dict(sliding_window=64), 0), ("Mistral", dict(sliding_window=None), 2),
+    ("Qwen2", dict(use_sliding_window=True, max_window_layers=1, sliding_window=64), 1),
+    ("Qwen2", dict(use_sliding_window=False, sliding_window=64), 2), ("Llama", {}, 2)])
+def test_attention_with_a_window_is_left_alone(pkg, kind, kw, count):
+    model = _tiny(kind, **kw)
+    assert pkg.patch_model_with_fused_kernels(model, fuse_attention=True)["attention"] == count
+    if count < 2:
+        with pytest.raises(ValueError, match="patched"):
+            pkg.DecoderCache.allocate(model, 1, 32, "int8")
+
+
+def test_rotary_that_changes_with_the_length_is_refused(pkg):
+    model = _tiny("Llama", rope_parameters={"rope_theta": 1e4, "rope_type": "dynamic", "factor": 2.0})
+    pkg.patch_model_with_fused_kernels(model, fuse_attention=True)
+    with pytest.raises(ValueError, match="dynamic"):
+        pkg.DecoderCache.allocate(model, 1, 32, "int8")

@@ -29,8 +29,7 @@ struct TreeArgs {
   int tile, pad;                      // slots of a tile on the line, tiles that a piece costs beside its own
   int grid;                           // workgroups of the first kernel
   uint32_t page_mul, page_shift;      // unit / units per page = unit * page_mul >> page_shift
-  float scale;                        // |scale| log2 e
-  int negative;                       // scale is: queries change their sign
+  float scale;                        // times log2 e
 };
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -404,16 +403,15 @@ template <int NV> struct Rows {
       for (int i = 0; i < 4; ++i) o[x][i] *= f;
   }
 
-  // Scores of 8 slots (-infinity where not seen; times `unit`, log2) -> weights
-  // times the values' scales, as the two parts of a P^T operand of VT.
+  // Scores of 8 slots (log2; -infinity where not seen) -> weights times the
+  // values' scales, as the two parts of a P^T operand of VT.
   template <typename VT, bool SCALED>
-  __device__ __forceinline__ void weights(const f32x4 (&sc)[2], float unit, const f32x4& vs0, const f32x4& vs1,
-                                          bool masked, uint32_t seen, u32x4& hi, u32x4& lo) {
+  __device__ __forceinline__ void weights(const f32x4 (&sc)[2], const f32x4& vs0, const f32x4& vs1, bool masked,
+                                          uint32_t seen, u32x4& hi, u32x4& lo) {
     float w[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float s = sc[e >> 2][e & 3];
-      w[e] = __builtin_amdgcn_exp2f(SCALED ? s - top : __builtin_fmaf(s, unit, -top));
+      w[e] = __builtin_amdgcn_exp2f(sc[e >> 2][e & 3] - top);
       sum += w[e];
       if constexpr (SCALED) w[e] *= e < 4 ? vs0[e & 3] : vs1[e & 3];
     }
@@ -456,7 +454,6 @@ __device__ __forceinline__ void load_queries(const TreeArgs& a, const Piece& p, 
   for (int n = 0; n < NQ; ++n) {
     const int e = key_element<FMT>(n, quad);
     q[n] = in && e < a.c.d ? *reinterpret_cast<const u32x4*>(row + e) : u32x4{0, 0, 0, 0};
-    if (a.negative) q[n] ^= 0x80008000u;
   }
 }
 

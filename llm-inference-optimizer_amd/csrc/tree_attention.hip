@@ -64,7 +64,6 @@ __global__ __launch_bounds__(64 * kWaves, stream_waves(DP, MT)) void tree_attent
   // the weights' type in the second product: codes and bf16 values are exact in bf16
   typedef typename std::conditional<FMT == KV_16BIT, T, BF16>::type VT;
   constexpr bool SCALED = FMT != KV_16BIT;
-  const float unit = SCALED ? 1.0f : a.scale;  // of a score, log2: a quantised one is scaled with its key
   __shared__ float joined[kWaves][ROWS][PITCH];
   __shared__ float wave_max[kWaves][ROWS], wave_sum[kWaves][ROWS];
   const int col = threadIdx.x & 15, quad = (threadIdx.x & 63) >> 4;
@@ -114,16 +113,14 @@ __global__ __launch_bounds__(64 * kWaves, stream_waves(DP, MT)) void tree_attent
           sc[m][1] = mfma16<T>(k1, q[m][n], sc[m][1]);
         }
       }
-      if constexpr (SCALED) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float f = a.scale * kv[u].ks[j];
+        for (int j = 0; j < 4; ++j) {
+          const float f = SCALED ? a.scale * kv[u].ks[j] : a.scale;
 #pragma unroll
-            for (int m = 0; m < MT; ++m) sc[m][u][j] *= f;
-          }
-      }
+          for (int m = 0; m < MT; ++m) sc[m][u][j] *= f;
+        }
 
       const bool masked = !whole || (tile + 1) * TILE > p.len;
       uint32_t seen[MT];
@@ -150,9 +147,9 @@ __global__ __launch_bounds__(64 * kWaves, stream_waves(DP, MT)) void tree_attent
       u32x4 hi[MT], lo[MT];
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        const float most = Rows<NV>::largest(sc[m]) * unit;
+        const float most = Rows<NV>::largest(sc[m]);
         if (rows[m].passed(most)) rows[m].raise(most);
-        rows[m].template weights<VT, SCALED>(sc[m], a.scale, kv[0].vs, kv[1].vs, masked, seen[m], hi[m], lo[m]);
+        rows[m].template weights<VT, SCALED>(sc[m], kv[0].vs, kv[1].vs, masked, seen[m], hi[m], lo[m]);
       }
 #pragma unroll
       for (int x = 0; x < NV; x += 2) {
@@ -234,7 +231,6 @@ __global__ __launch_bounds__(64 * kWaves, wide_groups(DP, MT)) void tree_attenti
   constexpr int NV = Regs::NV, NQ = DP / 32, PITCH = DP + 4, TILE = kWideTile;
   typedef typename std::conditional<FMT == KV_16BIT, T, BF16>::type VT;
   constexpr bool SCALED = FMT != KV_16BIT;
-  const float unit = SCALED ? 1.0f : a.scale;  // of a score, log2: a quantised one is scaled with its key
   struct Stage {
     u32x4 k[4][NQ][64];      // unit, k-step, lane
     u32x2 v[2][NV][64][2];   // pair of units, element, lane, unit of the pair
@@ -362,15 +358,14 @@ __global__ __launch_bounds__(64 * kWaves, wide_groups(DP, MT)) void tree_attenti
             sc[pair][m][1] = mfma16<T>(k1, q[m][n], sc[pair][m][1]);
           }
         }
-        if constexpr (SCALED) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const f32x4 f = *reinterpret_cast<const f32x4*>(&s.ks[32 * pair + 16 * u + 4 * quad]) * a.scale;
+        for (int u = 0; u < 2; ++u) {
+          f32x4 f = {a.scale, a.scale, a.scale, a.scale};
+          if constexpr (SCALED) f *= *reinterpret_cast<const f32x4*>(&s.ks[32 * pair + 16 * u + 4 * quad]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+          for (int j = 0; j < 4; ++j)
 #pragma unroll
-              for (int m = 0; m < MT; ++m) sc[pair][m][u][j] *= f[j];
-          }
+            for (int m = 0; m < MT; ++m) sc[pair][m][u][j] *= f[j];
         }
         if (masked) {
 #pragma unroll
@@ -384,7 +379,7 @@ __global__ __launch_bounds__(64 * kWaves, wide_groups(DP, MT)) void tree_attenti
       bool passed = false;
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        most[m] = fmaxf(Rows<NV>::largest(sc[0][m]), Rows<NV>::largest(sc[1][m])) * unit;
+        most[m] = fmaxf(Rows<NV>::largest(sc[0][m]), Rows<NV>::largest(sc[1][m]));
         passed |= rows[m].passed(most[m]);
       }
       if (passed) {
@@ -401,7 +396,7 @@ __global__ __launch_bounds__(64 * kWaves, wide_groups(DP, MT)) void tree_attenti
         }
 #pragma unroll
         for (int m = 0; m < MT; ++m)
-          rows[m].template weights<VT, SCALED>(sc[pair][m], a.scale, vs0, vs1, masked, seen[m] >> (8 * pair), hi[pair][m],
+          rows[m].template weights<VT, SCALED>(sc[pair][m], vs0, vs1, masked, seen[m] >> (8 * pair), hi[pair][m],
                                                lo[pair][m]);
       }
 #pragma unroll
@@ -637,7 +632,7 @@ int tree_attention_launch(const mi355_kv_cache& cache, const void* q, void* out,
   Plan p = plan(cache, batch, tokens, q_heads, cus);
   TreeArgs a{kv_cache_args(cache), q, out, lens, new_lens, mask, mask_b, mask_t, q_strides[0], q_strides[1],
              q_strides[2], nullptr, nullptr, nullptr, static_cast<int>(batch), tokens, q_heads,
-             q_heads / static_cast<int>(cache.kv_heads), p.block_rows, p.blocks, p.tile, 0, 0, 0, 0, __builtin_fabsf(scale) * kLog2e, scale < 0.f};
+             q_heads / static_cast<int>(cache.kv_heads), p.block_rows, p.blocks, p.tile, 0, 0, 0, 0, scale * kLog2e};
   if (p.bytes > 0 && work != nullptr && work_bytes >= p.bytes) {
     a.partial = static_cast<float*>(work);
     a.pad = p.pad;

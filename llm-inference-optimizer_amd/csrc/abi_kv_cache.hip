@@ -174,8 +174,8 @@ MI355_EXPORT int mi355_kv_cache_read_fwd(const mi355_kv_cache* cache, void* k_ou
   if (batch < 0 || tokens < 0) return bad(fn, "sizes out of range");
   if (batch == 0 || tokens == 0) return MI355_OK;
   // a workgroup of 256 threads holds 8 rows at least
-  if (!product_below(batch, tokens, (8 * kMaxRows) / cache->kv_heads))
-    return beyond(fn, "size beyond the kernel's limits (batch * tokens * kv_heads < 2^27)");
+  if (!product_below(batch, tokens, (4 * kMaxRows) / cache->kv_heads))
+    return beyond(fn, "size beyond the kernel's limits (batch * tokens * kv_heads < 2^26)");
   if (k_out == nullptr || v_out == nullptr || end == nullptr) return bad(fn, "null pointer");
   if (!aligned16(k_out) || !aligned16(v_out)) return bad(fn, "k_out and v_out must be 16-byte aligned");
   st = check_pools(fn, cache);

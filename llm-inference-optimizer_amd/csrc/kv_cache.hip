@@ -177,7 +177,7 @@ template <typename T, int FMT> __global__ __launch_bounds__(256) void read_rows(
   const int64_t r = static_cast<int64_t>(blockIdx.x) * (256 / a.lanes) + threadIdx.x / a.lanes;
   const int d0 = (threadIdx.x % a.lanes) * 8;
   if (r >= a.rows || d0 >= a.c.d) return;
-  // 32 bits hold a row: fewer than 2^27 of them
+  // 32 bits hold a row: fewer than 2^26 of them
   const uint32_t bh = static_cast<uint32_t>(r) / a.tokens, i = static_cast<uint32_t>(r) - bh * a.tokens;
   const uint32_t b = bh / a.c.heads, h = bh - b * a.c.heads;
   const int64_t slot = static_cast<int64_t>(a.start ? a.start[b] : 0) + i;

@@ -7,10 +7,9 @@
 
 namespace mi355 {
 
-
 constexpr int kWaves = 4;            // of a workgroup
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLow = -1e30f;       // the running maximum before any score
+constexpr float kLow = -3.4028235e38f;  // the running maximum before any score: the lowest number
 constexpr float kSlack = 8.0f;       // log2 of how far scores may pass it
 
 struct TreeArgs {
@@ -408,6 +407,10 @@ template <int NV> struct Rows {
   template <typename VT, bool SCALED>
   __device__ __forceinline__ void weights(const f32x4 (&sc)[2], const f32x4& vs0, const f32x4& vs1, bool masked,
                                           uint32_t seen, u32x4& hi, u32x4& lo) {
+    // The score has been multiplied by the scale and rounded, as the maximum has:
+    // fused into the subtraction, the unrounded product of a large score would
+    // differ from the maximum made of it by more than the exponential holds.
+#pragma clang fp contract(off)
     float w[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -518,6 +521,7 @@ __device__ __forceinline__ void store_result(const TreeArgs& a, const Piece& p, 
 struct Share {
   Line line;
   int at, last, b, start, first, size;
+  int alone;  // without a split: head and block
   // one piece
   Piece p;
   int t0, t1, tiles;  // tiles [t0, t1) of `tiles`
@@ -534,9 +538,9 @@ struct Share {
     } else {  // one (head, block) of one sequence
       const int hm_count = a.c.heads * a.blocks;
       b = blockIdx.x / hm_count;
-      start = 0;
-      at = (blockIdx.x % hm_count) * Seq::of(a, b).tiles;
-      last = at + 1;  // widened to the whole in next()
+      alone = blockIdx.x - b * hm_count;
+      start = at = 0;
+      last = Seq::of(a, b).tiles;
     }
     first = at;
   }
@@ -544,14 +548,13 @@ struct Share {
     const int hm_count = a.c.heads * a.blocks;
     while (b < a.batch && at < last) {
       const Seq s = a.partial && b < 64 ? line.seq(a, b) : Seq::of(a, b);
-      const int hm = uniform((at - start) / s.tiles);
+      const int hm = a.partial ? uniform((at - start) / s.tiles) : alone;
       if (hm >= hm_count) {
         start = uniform(start + s.tiles * hm_count);
         b = uniform(b + 1);
         continue;
       }
-      const int v0 = uniform(at - start - hm * s.tiles);
-      if (!a.partial) last = uniform(at + s.tiles);
+      const int v0 = a.partial ? uniform(at - start - hm * s.tiles) : 0;
       const int v1 = uniform(min(s.tiles, v0 + last - at));
       tiles = uniform(s.tiles - a.pad);
       t0 = max(0, v0 - a.pad);

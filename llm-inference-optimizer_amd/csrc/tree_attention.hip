@@ -53,7 +53,9 @@ constexpr int kStreamTile = 32;  // slots of a wave's tile
 constexpr int kWideTile = 64;    // slots of a workgroup's tile
 
 // Waves that a SIMD holds at the registers of tree_attention_stream.
-constexpr int stream_waves(int dp, int mt) { return mt == 1 && dp <= 64 ? 4 : mt == 1 && dp <= 128 ? 3 : dp * mt <= 256 ? 2 : 1; }
+constexpr int stream_waves(int dp, int mt) {
+  return mt == 1 && dp <= 64 ? 4 : mt == 1 && dp <= 128 ? 3 : dp * mt <= 256 ? 2 : 1;
+}
 
 // Up to 16 MT = 32 query rows per key/value head: a wave for itself, tile by
 // tile, loads straight to MFMA operands.

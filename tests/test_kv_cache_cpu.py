@@ -115,7 +115,7 @@ def test_read_and_keep_abi_rejects(L, lib):
     c = _cache(L)
     for args, code, message in [((c, P, P, None, P, 1, 1, 0, None), -2, "fp16 or bf16"),
                                 ((c, P, P, None, P, -1, 1, 1, None), -1, "sizes"),
-                                ((c, P, P, None, P, 1 << 20, 1 << 7, 1, None), -2, "limits"),
+                                ((c, P, P, None, P, 1 << 19, 1 << 6, 1, None), -2, "limits"),
                                 ((c, P, P, None, 0, 1, 1, 1, None), -1, "null"),
                                 ((c, P + 2, P, None, P, 1, 1, 1, None), -1, "aligned")]:
         _expect(lib, lib.mi355_kv_cache_read_fwd(*args), code, message)

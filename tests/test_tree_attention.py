@@ -184,6 +184,49 @@ def test_pages_that_are_not_there(pkg, cuda, kind):
         K.close(pkg.tree_attention(q, cache, K.ints(lens)), *K.attention(q, cache, lens))
 
 
+@pytest.mark.parametrize("kind", FORMATS)
+@pytest.mark.parametrize("tokens", [3, 40])
+def test_scale_of_zero_and_below(pkg, cuda, kind, tokens):
+    """With a scale of 0 every slot that is seen weighs the same, and one that is not still nothing."""
+    lens = [70, 0, 33]
+    cache, q = _case(pkg, kind, torch.bfloat16, 3, tokens, 4, 2, 64, 16, lens)
+    for scale in (0.0, -0.0, -0.3):
+        K.close(pkg.tree_attention(q, cache, K.ints(lens), scale=scale), *K.attention(q, cache, lens, scale=scale))
+
+
+@pytest.mark.parametrize("kind", FORMATS)
+@pytest.mark.parametrize("tokens,length", [(1, 40), (1, 700), (20, 700), (70, 700)])
+def test_scores_near_the_lowest_number(pkg, cuda, kind, tokens, length):
+    """Scores of -10^33 and below are scores like others: the least negative one takes all the weight, and equal ones
+    share it -- a product that is rounded for the maximum has to be the same one in the exponent."""
+    cache, q = _case(pkg, kind, torch.bfloat16, 1, tokens, 2, 1, 64, 16, [length])
+    quantised = cache.k_scale is not None
+    unit = 1.0 if quantised else 1e17
+    q.zero_()
+    q[..., 0] = 1.7e17
+    rows = torch.zeros(cache.k.shape, dtype=torch.float32, device=cuda)
+    rows[..., 0] = -3 * unit
+    page, place = cache.page_table[0, 1].item(), 3  # slot 19, before the new tokens
+    rows[page, 0, place, 0] = -unit
+    cache.k.copy_(rows.to(cache.k.dtype))
+    if quantised:
+        cache.k_scale.fill_(1.1e17)
+        v = cache.v[page, 0, place].float() * cache.v_scale[page, 0, place]
+    else:
+        v = cache.v[page, 0, place].float()
+    out = pkg.tree_attention(q, cache, K.ints([length]), scale=0.3)
+    # weight 1, whose product with the scale is off by 2^-16 (two bf16 parts), and one rounding to bf16
+    assert ((out.float() - v).abs() <= v.abs() * (2.0 ** -8 + 2.0 ** -15)).all()
+    # the same score everywhere: the values' mean
+    cache.k.copy_((rows * 0 + (rows != 0) * (-unit)).to(cache.k.dtype))
+    first = torch.zeros((1, tokens, tokens), dtype=torch.bool, device=cuda)
+    out = pkg.tree_attention(q, cache, K.ints([length]), tree_mask=first, scale=0.3)
+    k, values = pkg.kv_cache_read(cache, K.ints([length]), length, dtype=torch.bfloat16)
+    mean, spread = values.double().mean(2)[:, :, None], values.double().abs().mean(2)[:, :, None]
+    # read rounds every value (2^-8), the weights are off by 2^-16, the sum by 700 * 2^-24, the result by 2^-8
+    assert ((out.double().transpose(1, 2) - mean).abs() <= 2.0 ** -8 * mean.abs() + 2.0 ** -7.9 * spread).all()
+
+
 def test_large_scores_and_scale(pkg, cuda):
     """Scores of some hundreds: the exponentials' range, a running maximum that keeps rising, a scale of its own."""
     lens = [600, 100]

@@ -19,6 +19,12 @@
 //           head, pool and 128 bytes of the rows, loads those of every kept
 //           row into LDS and then writes, so that any order and any overlap of
 //           slots is right.
+//
+// Measured: append of 3001 tokens of 4 sequences (bf16 to e4m3, queries and keys
+// rotated, 225 MB) 34.0 us, 6.6 TB/s; of 16 single tokens 4.6 us, of which a
+// launch takes half.  Read of 16 x 1 tokens 2.5 us.  Keep of 9 of 64 tokens of
+// 128 sequences (16-bit values, 10.5 MB) 7.0 us: the page table, the kept
+// numbers, the rows and the stores are four dependent trips.
 #include "kv_cache.h"
 #include "rotary.h"
 
@@ -287,7 +293,10 @@ int kv_append_launch(const mi355_kv_cache& cache, const RotaryArgs& rot, const v
   const int step = 64 / a.lanes, kv_rows = 2 * a.c.heads;
   const int q_passes = (q_heads + step - 1) / step, kv_passes = (kv_rows + step - 1) / step;
   dim3 grid(static_cast<unsigned>((batch * tokens + kWaves - 1) / kWaves));
-  if (batch * tokens < 1024) {  // a pass per wave until the tokens alone fill the chip
+  // a pass per wave until the tokens alone fill the chip (a pass against a token
+  // per wave: 8.7 / 9.55 us for 512 tokens of 28 + 2 x 4 heads, 18.0 / 14.2 us
+  // for 2048)
+  if (batch * tokens < 1024) {
     a.q_per_wave = a.kv_per_wave = step;
     a.kv_from = q_passes;
     grid.y = static_cast<unsigned>(q_passes + kv_passes);

@@ -8,6 +8,10 @@
 // half layout a lane also loads the packet that rotates into its own: the row
 // is in the L1 by then, so HBM sees it once.  The first heads' packets are
 // loaded before the angles are computed, which take about as long as the loads.
+//
+// Measured: 16384 tokens of 28 heads of 128 (bf16, 235 MB read and written)
+// 36.2 us, 6.5 TB/s, the rate of a plain copy of that size; 4 tokens of 12 heads
+// 2.5 us, a launch and two dependent round trips to memory.
 #include "rotary.h"
 
 namespace mi355 {
@@ -97,9 +101,12 @@ template <typename T> int rotary_typed(Args a, hipStream_t s) {
   constexpr int W = pack_width<T>::value;
   const int64_t es = sizeof(typename T::bits), rows = a.rows;
   // whole packets, and a wave's lanes for a row at most
-  const bool vec = a.d % W == 0 && a.d / W <= 64 && aligned16(a.x) && aligned16(a.y) && (a.sb * es | a.st * es | a.sh * es) % 16 == 0;
+  const bool vec = a.d % W == 0 && a.d / W <= 64 && aligned16(a.x) && aligned16(a.y) &&
+                   (a.sb * es | a.st * es | a.sh * es) % 16 == 0;
   a.lanes = vec ? row_lanes(a.d / W) : 64;
-  // one pass over heads per wave until the tokens alone fill the chip
+  // one pass over heads per wave until the tokens alone fill the chip (28 heads
+  // of 128, a pass against a token per wave: 4.31 / 4.64 us for 512 tokens, 5.88
+  // / 5.21 us for 1024)
   a.heads_per_wave = rows < 1024 ? 64 / a.lanes : a.heads;
   const dim3 grid(static_cast<unsigned>(vec ? (rows + kWaves - 1) / kWaves : rows),
                   static_cast<unsigned>((a.heads + a.heads_per_wave - 1) / a.heads_per_wave));

@@ -58,7 +58,15 @@ constexpr int stream_waves(int dp, int mt) {
 }
 
 // Up to 16 MT = 32 query rows per key/value head: a wave for itself, tile by
-// tile, loads straight to MFMA operands.
+// tile, loads straight to MFMA operands.  The next tile's keys are loaded as soon
+// as this one's scores are taken, its values after the second product: the
+// registers hold one tile, and the other waves of the SIMD cover the rest.
+// Bound by HBM where contexts are long: 2 of 120011 slots (28 / 4 heads of 128,
+// e4m3, 253 MB) 47.4 us, 6.2 TB/s behind some 6 us of start and end; 32 ragged
+// ones to 6000 (int8, 114 MB) 27.8 us, 4.1 TB/s with that start; one context of 777 slots 7.0 us, all
+// of it latency.  Loads are non-temporal: 55.6 against 59.7 us with the join on
+// the long contexts, which pass through the caches, and 36.9 against 33.4 us on
+// the 114 MB where they are still there from the call before.
 template <typename T, int FMT, int DP, int MT>
 __global__ __launch_bounds__(64 * kWaves, stream_waves(DP, MT)) void tree_attention_stream(TreeArgs a) {
   typedef UnitRegs<T, FMT, DP, kStreamAux> Regs;  // the cache is read once
@@ -225,6 +233,10 @@ __global__ __launch_bounds__(64 * kWaves, stream_waves(DP, MT)) void tree_attent
 // packet per lane as the operand is read back, so that neither side meets a
 // bank twice.  Two tiles in LDS: while one is used, the next is written and the
 // one after it is on its way to registers; one barrier per tile.
+// 8 trees of 48 tokens over ragged contexts to 4100 (28 / 4 heads of 128, 16-bit,
+// 45 MB): 51.2 us for 13.2 GFLOP, 20 with the low parts of the weights: per SIMD
+// the matrix unit is busy 24% of the time and the vector unit 42% (exponentials,
+// the split of the weights, masks), with two waves to overlap them.
 constexpr int wide_groups(int dp, int mt) { return dp <= 64 && mt == 1 ? 3 : dp <= 128 ? 2 : 1; }  // of a CU
 
 template <typename T, int FMT, int DP, int MT>
@@ -562,6 +574,12 @@ Plan plan(const mi355_kv_cache& c, int64_t batch, int64_t tokens, int64_t q_head
   Plan p{};
   const int dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
   const int64_t rows = tokens * (q_heads / c.kv_heads);
+  // The stream kernel to 32 rows (8 contexts of 4096, D 128, stream / wide: 28
+  // rows of int8 28.3 / 30.2 us, of 16 bits 31.1 / 29.0; 56 rows of int8 in 64-row
+  // tiles of the stream kernel 50.8 / 31).  Wide: 16 rows per wave while one block
+  // holds them all, then 32 (336 rows, blocks of 128 / 64: 81 / 90 us for 8
+  // contexts of 4096 of int8, 64.6 / 66.2 us for ragged ones of 16 bits); 256-wide
+  // heads have the registers for 16.
   p.wide = rows > 32;
   p.mt = p.wide ? (rows <= 64 || dp == 256 ? 1 : 2) : (rows <= 16 ? 1 : 2);
   p.block_rows = 16 * p.mt * (p.wide ? kWaves : 1);
@@ -609,7 +627,10 @@ template <typename T, int FMT> int tree_typed(const TreeArgs& a, const Plan& p, 
 template <typename T> int tree_join(const TreeArgs& a, const Plan& p, hipStream_t s) {
   static const char* what = "tree_attention join launch";
   const int64_t rows = int64_t{a.batch} * a.tokens * a.q_heads;
-  // more than 8 pieces for most rows, and too few rows to fill the chip with a wave each
+  // More than 8 pieces for most rows, and too few rows to fill the chip with a
+  // wave each: 8 waves against one per row, with the first kernel, 55.9 / 73.5 us
+  // for 56 rows of 2 long contexts; but 32.7 / 27.4 us for 24 trees of 9 tokens
+  // (3024 rows of few pieces).
   if (p.grid > 8 * int64_t{a.batch} * a.c.heads * a.blocks && rows <= 1024)
     return launch(tree_attention_join<T, kJoinWaves>, dim3(static_cast<unsigned>(rows)), 64 * kJoinWaves, 0, a, s, what);
   return launch(tree_attention_join<T, 1>, dim3(static_cast<unsigned>((rows + kJoinWaves - 1) / kJoinWaves)),

@@ -6,10 +6,13 @@ HF's own ``StaticCache`` instead of the reference's paged KV cache (paged
 attention is not on this path): every buffer the decode step touches is
 allocated once, the step reads only static tensors (the current tokens and
 the cache position), and after the first step the whole forward pass -- 28
-layers of attention, the fused RMSNorm / SiLU-and-mul kernels, GEMMs, LM head
-and argmax -- is one graph replay.  As in the reference (:129-147), the graph
+layers of attention, the fused RMSNorm / SiLU-and-mul kernels, GEMMs and LM
+head -- is one graph replay.  As in the reference (:129-147), the graph
 is replayed right after capture, so the first captured step also returns a
-computed result rather than whatever the capture pass left behind.
+computed result rather than whatever the capture pass left behind.  The argmax
+stays outside: over a vocabulary torch splits it over workgroups that count
+themselves in memory which a memset clears before, and a memset replayed as a
+graph node may not have cleared it -- then nobody writes the result.
 
 It works with the patched and the unpatched model alike; the fused kernels
 enqueue no allocation, sync or memset, so they capture cleanly.
@@ -76,7 +79,6 @@ class GraphedGreedyDecoder:
         self._pos = torch.zeros((1,), dtype=torch.long, device=self.device)
         self._pos0 = self._pos.view(())  # 0-d view for the cache's write counters
         self._pos_ids = torch.zeros((batch_size, 1), dtype=torch.long, device=self.device)
-        self._next = None
         self._logits = None
         self._graph = None
 
@@ -92,7 +94,6 @@ class GraphedGreedyDecoder:
             self._mask = torch.zeros((n, t, t), dtype=torch.bool, device=self.device)
             self._kept = torch.zeros((n, t), dtype=torch.int32, device=self.device)
             self._kept_lens = torch.zeros((n,), dtype=torch.int32, device=self.device)
-        self._next = None
         self._logits = None
         self._graph = None
 
@@ -103,19 +104,19 @@ class GraphedGreedyDecoder:
                          logits_to_keep=1 if prompt else 0)
         return out.logits
 
-    def _cached_step(self) -> tuple[torch.Tensor, torch.Tensor]:
+    def _cached_step(self) -> torch.Tensor:
         """One token per sequence, or a draft: first the last draft's accepted
         tokens move together and become part of the cache."""
         if not self.draft_tokens:
             logits = self._cached_forward(self._tok, self._pos_ids)[:, -1]
             self.cache.lens.add_(1)
-            return logits, logits.argmax(-1, keepdim=True)
+            return logits
         self.cache.keep(self._kept, self._kept_lens)
         self.cache.lens.add_(self._kept_lens)
-        logits = self._cached_forward(self._tok, self._pos_ids, self._new_lens, self._mask)
-        return logits, logits.argmax(-1)
+        return self._cached_forward(self._tok, self._pos_ids, self._new_lens, self._mask)
 
-    def _step(self) -> tuple[torch.Tensor, torch.Tensor]:
+    def _step_logits(self) -> torch.Tensor:
+        """What the graph holds."""
         if isinstance(self.cache, DecoderCache):
             return self._cached_step()
         # HF's StaticLayer writes at its own device-side counter
@@ -126,8 +127,14 @@ class GraphedGreedyDecoder:
         torch._foreach_copy_(counters, [self._pos0] * len(counters))
         out = self.model(input_ids=self._tok, past_key_values=self.cache, cache_position=self._pos,
                          position_ids=self._pos_ids, use_cache=True)
-        logits = out.logits[:, -1]
-        return logits, logits.argmax(-1, keepdim=True)
+        return out.logits[:, -1]
+
+    def _picks(self, logits: torch.Tensor) -> torch.Tensor:
+        return logits.argmax(-1, keepdim=not self.draft_tokens)
+
+    def _step(self) -> tuple[torch.Tensor, torch.Tensor]:
+        logits = self._step_logits()
+        return logits, self._picks(logits)
 
     def _capture(self) -> None:
         side = torch.cuda.Stream(device=self.device)
@@ -137,17 +144,17 @@ class GraphedGreedyDecoder:
             lens = self.cache.lens.clone()
             side.wait_stream(torch.cuda.current_stream(self.device))
         with torch.cuda.stream(side):
-            self._step()  # warm-up: kernel selection and lazy allocations happen outside the capture
+            self._step_logits()  # warm-up: kernel selection and lazy allocations happen outside the capture
         torch.cuda.current_stream(self.device).wait_stream(side)
         if cached:
             self.cache.lens.copy_(lens)
         torch.cuda.synchronize(self.device)
         self._graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self._graph):
-            self._logits, self._next = self._step()
+            self._logits = self._step_logits()
 
     def _run(self) -> tuple[torch.Tensor, torch.Tensor]:
-        """One step, replayed (captured at first) or eager; the graph's outputs
+        """One step, replayed (captured at first) or eager; the graph's logits
         are overwritten by the next."""
         self.steps += 1
         if not self.use_graph:
@@ -155,7 +162,7 @@ class GraphedGreedyDecoder:
         if self._graph is None:
             self._capture()
         self._graph.replay()
-        return self._logits, self._next
+        return self._logits, self._picks(self._logits)
 
     def _cached_prompt(self, input_ids: torch.Tensor) -> torch.Tensor:
         """The prompt into an empty cache; its last logits."""
@@ -240,7 +247,6 @@ class GraphedGreedyDecoder:
                 self._pos.fill_(S + i)
             self._pos_ids.fill_(S + i)
             logits, tok = self._run()
-            tok = tok.clone()
             toks.append(tok)
             if return_logits:
                 # a copy: the graph's output buffer is rewritten by the next replay

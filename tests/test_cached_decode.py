@@ -106,6 +106,20 @@ def test_drafts_that_are_accepted(pkg, cuda, draft):
     assert dec.steps < 149
 
 
+@pytest.mark.parametrize("kv,draft", [(None, None), ("16bit", None), ("int8", None), ("int8", 6)])
+def test_a_large_vocabulary(pkg, cuda, kv, draft):
+    """Many replays with a vocabulary over which an argmax takes more than one workgroup, and eager work between."""
+    model = _model(cuda, vocab=151936)
+    pkg.patch_model_with_fused_kernels(model, fuse_attention=kv is not None)
+    dec = pkg.GraphedGreedyDecoder(model, 1, 160, **({} if kv is None else dict(kv_cache=kv, draft_tokens=draft)))
+    for seed in (1, 2, 3):
+        ids = _prompt(cuda, 1, 50, seed=seed)
+        out, logits = dec.generate(ids, 40, return_logits=True)
+        assert torch.equal(logits.argmax(-1), out[:, 50:]) and out.min() >= 0 and out.max() < 151936
+        again = dec.generate(ids, 40)
+        assert torch.equal(again, out)
+
+
 def test_bf16_wide_heads_and_int8_weights(pkg, cuda):
     """Heads of 128, bf16, weights quantised after the patch (the attention's projections among them)."""
     model = _model(cuda, heads=4, kv_heads=1, hidden=512, dtype=torch.bfloat16)

@@ -31,7 +31,7 @@ import torch
 
 from ..kernels.tree_attention_hip import TREE_ATTENTION_MAX_TOKENS
 from .cached_attention import DecoderCache
-from .prompt_lookup import accept, draft_tree
+from .prompt_lookup import TextIndex, accept, draft_tree
 
 __all__ = ["GraphedGreedyDecoder"]
 
@@ -177,26 +177,26 @@ class GraphedGreedyDecoder:
         B, S = input_ids.shape
         t = self.draft_tokens
         logits = self._cached_prompt(input_ids)
-        seqs = input_ids.tolist()
+        seqs = [TextIndex(row) for row in input_ids.tolist()]
         for s, tok in zip(seqs, logits.argmax(-1).tolist()):
-            s.append(tok)
+            s.extend([tok])
         done = S + max_new_tokens
         kept_logits = [[row.to(torch.float32, copy=True)] for row in logits] if return_logits else None
         self._kept_lens.zero_()
         while any(len(s) < done for s in seqs):
             trees = [draft_tree(s, t) if len(s) < done else ([], []) for s in seqs]
-            tok, pos = torch.zeros((B, t), dtype=torch.long), torch.zeros((B, t), dtype=torch.long)
-            mask = torch.zeros((B, t, t), dtype=torch.bool)
+            tok, pos = [[0] * t for _ in seqs], [[0] * t for _ in seqs]
+            mask = [[[False] * t for _ in range(t)] for _ in seqs]
             for b, (nodes, parents) in enumerate(trees):
-                for i, (node, parent) in enumerate(zip(nodes, parents)):
+                tok[b][:len(nodes)] = nodes
+                for i, parent in enumerate(parents):
                     if i:
-                        mask[b, i] = mask[b, parent]
-                    mask[b, i, i] = True
-                    tok[b, i] = node
-                    pos[b, i] = len(seqs[b]) - 1 if i == 0 else pos[b, parent] + 1
-            self._tok.copy_(tok)
-            self._pos_ids.copy_(pos)
-            self._mask.copy_(mask)
+                        mask[b][i] = list(mask[b][parent])
+                    mask[b][i][i] = True
+                    pos[b][i] = len(seqs[b]) - 1 if i == 0 else pos[b][parent] + 1
+            self._tok.copy_(torch.tensor(tok))
+            self._pos_ids.copy_(torch.tensor(pos))
+            self._mask.copy_(torch.tensor(mask))
             self._new_lens.copy_(torch.tensor([len(n) for n, _ in trees], dtype=torch.int32))
             logits, picks = self._run()
             picks = picks.tolist()
@@ -207,7 +207,7 @@ class GraphedGreedyDecoder:
                 path = accept(nodes, parents, picks[b])[:done - len(seqs[b])]
                 kept[b, :len(path)] = torch.tensor(path, dtype=torch.int32)
                 counts[b] = len(path)
-                seqs[b] += [picks[b][i] for i in path]
+                seqs[b].extend([picks[b][i] for i in path])
                 if return_logits:
                     kept_logits[b] += [logits[b, i].to(torch.float32, copy=True) for i in path]
             self._kept.copy_(kept)
@@ -216,7 +216,7 @@ class GraphedGreedyDecoder:
         self.cache.keep(self._kept, self._kept_lens)
         self.cache.lens.add_(self._kept_lens)
         self._kept_lens.zero_()
-        ids = torch.tensor(seqs, dtype=torch.long, device=self.device)
+        ids = torch.tensor([s.tokens for s in seqs], dtype=torch.long, device=self.device)
         return (ids, torch.stack([torch.stack(r) for r in kept_logits])) if return_logits else ids
 
     @torch.inference_mode()

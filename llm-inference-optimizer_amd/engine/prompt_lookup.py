@@ -4,25 +4,51 @@ accepts what the model agrees with.  Host code, one sequence at a time.
 """
 from __future__ import annotations
 
-__all__ = ["draft_tree", "accept"]
+__all__ = ["TextIndex", "draft_tree", "accept"]
 
 
-def draft_tree(tokens: list[int], size: int, max_ngram: int = 3, branches: int = 4) -> tuple[list[int], list[int]]:
-    """A tree of at most ``size`` nodes that continues ``tokens``: (token of each
+class TextIndex:
+    """A text that grows, and where each of its n-grams (n <= ``max_ngram``)
+    begins, so that a step does not search the whole text for its last tokens."""
+
+    def __init__(self, tokens: list[int], max_ngram: int = 3):
+        self.tokens: list[int] = []
+        self.max_ngram = max_ngram
+        self._starts: list[dict[tuple, list[int]]] = [{} for _ in range(max_ngram)]
+        self.extend(tokens)
+
+    def __len__(self) -> int:
+        return len(self.tokens)
+
+    def extend(self, tokens: list[int]) -> None:
+        old = len(self.tokens)
+        self.tokens += tokens
+        for n, starts in enumerate(self._starts, 1):
+            for start in range(max(0, old - n + 1), len(self.tokens) - n + 1):
+                starts.setdefault(tuple(self.tokens[start:start + n]), []).append(start)
+
+    def earlier(self, n: int):
+        """Where the last ``n`` tokens occurred before, the latest first."""
+        starts = self._starts[n - 1][tuple(self.tokens[-n:])]
+        return (starts[i] for i in range(len(starts) - 2, -1, -1))
+
+
+def draft_tree(text: TextIndex | list[int], size: int, branches: int = 4) -> tuple[list[int], list[int]]:
+    """A tree of at most ``size`` nodes that continues ``text``: (token of each
     node, parent of each node).  Node 0 is the last token (parent -1); the rest
     are the tokens behind up to ``branches`` earlier occurrences of the last
-    ``max_ngram`` (then fewer) tokens, the latest occurrences first, merged where
+    ``text.max_ngram`` (then fewer) tokens, the latest occurrences first, merged where
     they begin alike.  Parents come before their children."""
+    if not isinstance(text, TextIndex):
+        text = TextIndex(text)
+    tokens = text.tokens
     nodes, parents = [tokens[-1]], [-1]
     children: dict[tuple[int, int], int] = {}  # (parent, token) -> node
     found = 0
-    for n in range(min(max_ngram, len(tokens) - 1), 0, -1):
-        suffix = tokens[-n:]
-        for start in range(len(tokens) - n - 1, -1, -1):
+    for n in range(min(text.max_ngram, len(tokens) - 1), 0, -1):
+        for start in text.earlier(n):
             if len(nodes) >= size or found >= branches:
                 return nodes, parents
-            if tokens[start:start + n] != suffix:
-                continue
             found += 1
             at = 0
             # half of the free nodes for each continuation but the last: room for others

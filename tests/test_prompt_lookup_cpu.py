@@ -49,6 +49,22 @@ def test_trees_are_trees_of_the_text(size):
             assert path in text
 
 
+def test_an_index_that_grows():
+    rng = random.Random(5)
+    for _ in range(100):
+        index, tokens = PL.TextIndex([]), []
+        for _ in range(rng.randint(1, 12)):
+            more = [rng.randrange(3) for _ in range(rng.randint(0, 5))]
+            tokens = tokens + more
+            index.extend(more)
+            assert index.tokens == tokens and len(index) == len(tokens)
+            for n in range(1, min(3, len(tokens)) + 1):
+                want = [i for i in range(len(tokens) - n - 1, -1, -1) if tokens[i:i + n] == tokens[-n:]]
+                assert list(index.earlier(n)) == want
+            if tokens:
+                assert PL.draft_tree(index, 9) == PL.draft_tree(tokens, 9)
+
+
 def test_accept_walks_the_picks():
     nodes, parents = [3, 5, 4, 6, 7], [-1, 0, 0, 1, 2]
     assert PL.accept(nodes, parents, [5, 6, 0, 9, 0]) == [0, 1, 3]

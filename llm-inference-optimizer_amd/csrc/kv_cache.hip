@@ -20,11 +20,12 @@
 //           row into LDS and then writes, so that any order and any overlap of
 //           slots is right.
 //
-// Measured: append of 3001 tokens of 4 sequences (bf16 to e4m3, queries and keys
-// rotated, 225 MB) 34.0 us, 6.6 TB/s; of 16 single tokens 4.6 us, of which a
-// launch takes half.  Read of 16 x 1 tokens 2.5 us.  Keep of 9 of 64 tokens of
-// 128 sequences (16-bit values, 10.5 MB) 7.0 us: the page table, the kept
-// numbers, the rows and the stores are four dependent trips.
+// Measured: append of 3001 tokens of 4 sequences, half of them padding (28 + 2 x
+// 4 heads of 128, bf16 to e4m3, queries and keys rotated, 200 MB) 34.0 us, 5.9
+// TB/s; of 16 single tokens 4.6 us, of which a launch takes half.  Read of the
+// former (32 MB) 8.0 us, of one token 2.5.  Keep of up to 9 of 64 tokens of 128
+// sequences (8 heads of 16-bit values, 5 MB) 7.0 us: lengths, kept numbers, page
+// table, rows and stores are dependent trips to memory.
 #include "kv_cache.h"
 #include "rotary.h"
 

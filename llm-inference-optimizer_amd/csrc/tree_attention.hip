@@ -234,7 +234,7 @@ __global__ __launch_bounds__(64 * kWaves, stream_waves(DP, MT)) void tree_attent
 // bank twice.  Two tiles in LDS: while one is used, the next is written and the
 // one after it is on its way to registers; one barrier per tile.
 // 8 trees of 48 tokens over ragged contexts to 4100 (28 / 4 heads of 128, 16-bit,
-// 45 MB): 51.2 us for 13.2 GFLOP, 20 with the low parts of the weights: per SIMD
+// 45 MB): 46.6 us for 13.2 GFLOP, 20 with the low parts of the weights: per SIMD
 // the matrix unit is busy 24% of the time and the vector unit 42% (exponentials,
 // the split of the weights, masks), with two waves to overlap them.
 constexpr int wide_groups(int dp, int mt) { return dp <= 64 && mt == 1 ? 3 : dp <= 128 ? 2 : 1; }  // of a CU

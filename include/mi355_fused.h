@@ -386,6 +386,7 @@ int mi355_kv_cache_append_fwd(const mi355_kv_cache* cache, const void* k, const 
  * Reads slots start[b] + i, i < tokens, as values of dtype (code * scale,
  * rounded once) into k_out, v_out [batch, kv_heads, tokens, head_dim]
  * (contiguous, 16-byte aligned); zeros from slot end[b] on.  start may be NULL (0).
+ * batch * tokens * kv_heads < 2^26.
  */
 int mi355_kv_cache_read_fwd(const mi355_kv_cache* cache, void* k_out, void* v_out,
                             const int32_t* start, const int32_t* end, int64_t batch, int64_t tokens,

@@ -476,16 +476,17 @@ __global__ __launch_bounds__(64 * kWaves, wide_groups(DP, MT)) void tree_attenti
 // Adds the pieces of one query row that was cut, in order: lanes 0 - 31 and
 // 32 - 63 of each of WAVES waves take every 2 WAVES-th piece with a running
 // maximum, 4 (and, beyond 128, 4 more) elements per lane.  Latency is all there
-// is to it: one wave per row, or eight where pieces per row are many, so that
-// most pieces are in flight at once.
-constexpr int kJoinWaves = 8;
+// is to it: the more waves a row has, the more of its pieces are in flight at
+// once.  A workgroup holds one row, or with one wave per row eight of them.
+constexpr int kJoinRows = 8;
 
 template <typename T, int WAVES>
-__global__ __launch_bounds__(64 * kJoinWaves) void tree_attention_join(TreeArgs a) {
+__global__ __launch_bounds__(64 * (WAVES == 1 ? kJoinRows : WAVES)) void tree_attention_join(TreeArgs a) {
   typedef typename T::bits bits;
-  constexpr int PARTS = 2 * WAVES, PER = kJoinWaves / WAVES;  // rows of a workgroup
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  const int qrow = static_cast<int>(blockIdx.x) * PER + wave / WAVES;
+  constexpr int PARTS = 2 * WAVES;
+  const int lane = threadIdx.x & 63, w_id = uniform(threadIdx.x >> 6);
+  const int wave = WAVES == 1 ? 0 : w_id;  // of the row's
+  const int qrow = WAVES == 1 ? static_cast<int>(blockIdx.x) * kJoinRows + w_id : static_cast<int>(blockIdx.x);
   const int row_count = a.batch * a.tokens * a.q_heads;
   const int hq = qrow % a.q_heads, bt = qrow / a.q_heads;
   const int t = bt % a.tokens, b = min(bt / a.tokens, a.batch - 1);
@@ -499,7 +500,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void tree_attention_join(TreeArgs 
   const bool mine = qrow < row_count && w0 != w1;  // else written by the first kernel
   if (WAVES > 1 && !mine) return;
 
-  const int part = 2 * (wave % WAVES) + lane / 32;
+  const int part = 2 * wave + lane / 32;
   const int c0 = 4 * (lane % 32);
   const bool in0 = c0 < a.c.d, in1 = c0 + 128 < a.c.d;
   f32x4 v0 = {0.f, 0.f, 0.f, 0.f}, v1 = v0;
@@ -627,14 +628,18 @@ template <typename T, int FMT> int tree_typed(const TreeArgs& a, const Plan& p, 
 template <typename T> int tree_join(const TreeArgs& a, const Plan& p, hipStream_t s) {
   static const char* what = "tree_attention join launch";
   const int64_t rows = int64_t{a.batch} * a.tokens * a.q_heads;
-  // More than 8 pieces for most rows, and too few rows to fill the chip with a
-  // wave each: 8 waves against one per row, with the first kernel, 55.9 / 73.5 us
-  // for 56 rows of 2 long contexts; but 32.7 / 27.4 us for 24 trees of 9 tokens
-  // (3024 rows of few pieces).
-  if (p.grid > 8 * int64_t{a.batch} * a.c.heads * a.blocks && rows <= 1024)
-    return launch(tree_attention_join<T, kJoinWaves>, dim3(static_cast<unsigned>(rows)), 64 * kJoinWaves, 0, a, s, what);
-  return launch(tree_attention_join<T, 1>, dim3(static_cast<unsigned>((rows + kJoinWaves - 1) / kJoinWaves)),
-                64 * kJoinWaves, 0, a, s, what);
+  const int64_t pieces = p.grid / (int64_t{a.batch} * a.c.heads * a.blocks);  // of a row, on average
+  // Twice as many waves per row while half a wave has more than one piece and
+  // the chip (8192 waves) holds them.  Against one wave per row: 56 rows of 96
+  // pieces 55.9 / 73.5 us with the first kernel; 896 rows of 6 3.96 / 4.84 us
+  // (4 waves / 1); 3024 rows of 16 7.2 / 7.9 (2 / 1; 8.7 with 4, 13.1 with 8);
+  // 10752 rows of 5 13.5 / 9.9 (2 / 1).
+  const auto fits = [&](int waves) { return pieces > 2 * waves && 2 * rows * waves <= 8192; };
+  const auto grid = [&](int64_t groups) { return dim3(static_cast<unsigned>(groups)); };
+  if (fits(4)) return launch(tree_attention_join<T, 8>, grid(rows), 512, 0, a, s, what);
+  if (fits(2)) return launch(tree_attention_join<T, 4>, grid(rows), 256, 0, a, s, what);
+  if (fits(1)) return launch(tree_attention_join<T, 2>, grid(rows), 128, 0, a, s, what);
+  return launch(tree_attention_join<T, 1>, grid((rows + kJoinRows - 1) / kJoinRows), 64 * kJoinRows, 0, a, s, what);
 }
 
 }  // namespace

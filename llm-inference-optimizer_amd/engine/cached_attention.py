@@ -115,6 +115,7 @@ class CachedAttention(torch.nn.Module):
                 past_key_values=None, **kwargs):
         state = getattr(past_key_values, "mi355_cache", None)
         if state is None:
+            self._original.training = self.training  # not a registered child: train() and eval() pass it by
             return self._original(hidden_states=hidden_states, position_embeddings=position_embeddings,
                                   attention_mask=attention_mask, past_key_values=past_key_values, **kwargs)
         batch, tokens, _ = hidden_states.shape

@@ -1,4 +1,5 @@
 """What rotary positions, the cache and attention over it refuse before any GPU work, and their host-side parts."""
+import copy
 import ctypes
 import importlib
 
@@ -226,3 +227,17 @@ def test_rotary_that_changes_with_the_length_is_refused(pkg):
     pkg.patch_model_with_fused_kernels(model, fuse_attention=True)
     with pytest.raises(ValueError, match="dynamic"):
         pkg.DecoderCache.allocate(model, 1, 32, "int8")
+
+
+def test_patched_attention_follows_train_and_eval(pkg):
+    """With its own forward's dropout, parameter names and results unchanged."""
+    model = _tiny("Llama", attention_dropout=0.5).train()
+    names, ids = list(model.state_dict()), torch.arange(12)[None]
+    with torch.no_grad():
+        want = model.eval()(ids).logits
+        model.train()
+        pkg.patch_model_with_fused_kernels(model, patch_norm=False, patch_mlp=False, fuse_attention=True)
+        assert list(model.state_dict()) == names
+        assert not torch.equal(model(ids).logits, want)  # dropout
+        assert torch.equal(model.eval()(ids).logits, want)
+        assert torch.equal(copy.deepcopy(model)(ids).logits, want)

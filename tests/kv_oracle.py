@@ -2,8 +2,6 @@
 and the final rounding may differ from them by."""
 from __future__ import annotations
 
-import math
-
 import torch
 
 F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
@@ -153,7 +151,3 @@ def random_tree(batch, tokens, seed):
                 mask[b, i] = mask[b, int(torch.randint(max(0, i - 5), i, (1,), generator=g))]
             mask[b, i, i] = True
     return mask
-
-
-def default_scale(d):
-    return 1 / math.sqrt(d)

@@ -3,7 +3,6 @@ the decoded sequence into HF's DynamicCache: what the cache holds, the logits be
 import pytest
 import torch
 
-import kv_oracle as K
 from decode_check import compare_logits, reference_pass, sharpen_attention
 
 pytestmark = pytest.mark.gpu

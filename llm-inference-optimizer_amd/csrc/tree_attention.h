@@ -10,7 +10,6 @@ namespace mi355 {
 constexpr int kWaves = 4;            // of a workgroup
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLow = -3.4028235e38f;  // the running maximum before any score: the lowest number
-constexpr float kSlack = 8.0f;       // log2 of how far scores may pass it
 
 struct TreeArgs {
   KvCache c;
@@ -378,9 +377,26 @@ __device__ __forceinline__ uint32_t seen_slots(const TreeArgs& a, const Piece& p
   return (before | (t < p.fresh ? fresh & edge : 0u)) & ((there0 ? 0xfu : 0u) | (there1 ? 0xf0u : 0u));
 }
 
-// 16 query rows, one per column of the MFMA tiles: O^T in NV tiles, the running
-// maximum (the same in a column's four lanes) and this lane's part of the sum.
-template <int NV> struct Rows {
+// 16 query rows, one per column of the MFMA tiles: O^T in NV tiles, what the
+// exponents are relative to (log2; the same in a column's four lanes) and this
+// lane's part of the sum.  VT: the type of the weights' two parts.
+//
+// bf16 parts have fp32's exponents: `top` is the running maximum, which moves
+// only when a score passes it by 2^8.  fp16 parts end at 2^-24: relative to the
+// maximum, 17 nats down nothing would be left of a weight that the sum still
+// counts, and a slot that outweighs all others but has a small value (often the
+// first) makes such weights the result.  So there `top` follows the tiles, up
+// and down: it moves where a tile's largest weight would lie outside 2^7 ..
+// 2^15 (half the type's largest), to a whole number that puts it between 2^11
+// and 2^12.  Weights from 2^-8 on keep 16 bits, those below are off by 2^-25 at
+// most, that is 2^-32 of the tile's largest; o and sum are multiplied by powers
+// of 2, exactly.  The way down ends where the sum is 2^64 of a weight: o, of
+// values below 2^16, stays in range, and what is 2^-64 of the result is nothing
+// to 16-bit outputs.
+template <int NV, typename VT> struct Rows {
+  static constexpr bool FOLLOW = VT::code == MI355_F16;
+  static constexpr float kMost = FOLLOW ? 15.0f : 8.0f;  // log2 of the largest weight
+  static constexpr float kLeast = 7.0f, kRest = 12.0f, kMostSum = 64.0f;
   f32x4 o[NV];
   float top, sum;
 
@@ -396,13 +412,24 @@ template <int NV> struct Rows {
     return fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
                  fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
   }
-  // Whether a lane's largest score passes the maximum by more than the slack.
-  __device__ __forceinline__ bool passed(float most) const {
-    return __builtin_amdgcn_ballot_w64(most > top + kSlack) != 0;
+  // Whether a column's largest score, the largest of its lanes', asks for
+  // another `top`.  (A column that sees nothing of a tile asks, and keeps its own.)
+  __device__ __forceinline__ bool moves(float most) const {
+    const bool above = __builtin_amdgcn_ballot_w64(most > top + kMost) != 0;
+    if constexpr (!FOLLOW) return above;
+    uint64_t near = __builtin_amdgcn_ballot_w64(most >= top + kLeast);
+    near |= near >> 32;
+    near |= near >> 16;
+    return above || (near & 0xffff) != 0xffff;
   }
-  // Moves the maximum to the column's largest score.
-  __device__ __forceinline__ void raise(float most) {
-    const float now = fmaxf(top, max_quads(most));
+  // Moves `top` by the column's largest score.
+  __device__ __forceinline__ void move(float most) {
+    const float column = max_quads(most);
+    float now = fmaxf(top, column);
+    if constexpr (FOLLOW) {
+      const float least = top + __builtin_amdgcn_logf(sum_quads(sum)) - kMostSum;  // log2; -infinity without a sum
+      now = column >= kLow ? ceilf(fmaxf(column - kRest, least)) : top;
+    }
     const float f = __builtin_amdgcn_exp2f(top - now);
     top = now;
     sum *= f;
@@ -413,8 +440,8 @@ template <int NV> struct Rows {
   }
 
   // Scores of 8 slots (log2; -infinity where not seen) -> weights times the
-  // values' scales, as the two parts of a P^T operand of VT.
-  template <typename VT, bool SCALED>
+  // values' scales, as the two parts of a P^T operand.
+  template <bool SCALED>
   __device__ __forceinline__ void weights(const f32x4 (&sc)[2], const f32x4& vs0, const f32x4& vs1, bool masked,
                                           uint32_t seen, u32x4& hi, u32x4& lo) {
     // The score has been multiplied by the scale and rounded, as the maximum has:

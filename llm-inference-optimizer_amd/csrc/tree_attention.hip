@@ -27,8 +27,9 @@
 // times the key's scale.  Weights times the value's scale go to the second
 // product as two bf16 parts (fp16 for an fp16 cache), high and rest: 16
 // significant bits where one part would have 8.  It costs a second MFMA, of
-// which a decode step has plenty to spare.  The maximum moves only when a score
-// passes it by 2^8, so most tiles do not rescale O; weights then are at most 2^8.
+// which a decode step has plenty to spare.  What exponents are relative to moves
+// rarely, so most tiles do not rescale O (`Rows` has the rules, and what fp16's
+// short exponents ask for).
 //
 // Split: the tiles of all sequences, heads and row blocks form one line, of
 // which every workgroup takes an equal share, whatever the contexts' lengths;
@@ -92,7 +93,7 @@ __global__ __launch_bounds__(64 * kWaves, stream_waves(DP, MT)) void tree_attent
 
     u32x4 q[MT][NQ];
     int token[MT];
-    Rows<NV> rows[MT];
+    Rows<NV, VT> rows[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       load_queries<T, FMT>(a, p, m, q[m], token[m]);
@@ -157,9 +158,9 @@ __global__ __launch_bounds__(64 * kWaves, stream_waves(DP, MT)) void tree_attent
       u32x4 hi[MT], lo[MT];
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        const float most = Rows<NV>::largest(sc[m]);
-        if (rows[m].passed(most)) rows[m].raise(most);
-        rows[m].template weights<VT, SCALED>(sc[m], kv[0].vs, kv[1].vs, masked, seen[m], hi[m], lo[m]);
+        const float most = Rows<NV, VT>::largest(sc[m]);
+        if (rows[m].moves(most)) rows[m].move(most);
+        rows[m].template weights<SCALED>(sc[m], kv[0].vs, kv[1].vs, masked, seen[m], hi[m], lo[m]);
       }
 #pragma unroll
       for (int x = 0; x < NV; x += 2) {
@@ -305,7 +306,7 @@ __global__ __launch_bounds__(64 * kWaves, wide_groups(DP, MT)) void tree_attenti
 
     u32x4 q[MT][NQ];
     int token[MT];
-    Rows<NV> rows[MT];
+    Rows<NV, VT> rows[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       load_queries<T, FMT>(a, p, MT * wave + m, q[m], token[m]);
@@ -390,15 +391,15 @@ __global__ __launch_bounds__(64 * kWaves, wide_groups(DP, MT)) void tree_attenti
         }
       }
       float most[MT];
-      bool passed = false;
+      bool moves = false;
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        most[m] = fmaxf(Rows<NV>::largest(sc[0][m]), Rows<NV>::largest(sc[1][m]));
-        passed |= rows[m].passed(most[m]);
+        most[m] = fmaxf(Rows<NV, VT>::largest(sc[0][m]), Rows<NV, VT>::largest(sc[1][m]));
+        moves |= rows[m].moves(most[m]);
       }
-      if (passed) {
+      if (moves) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m) rows[m].raise(most[m]);
+        for (int m = 0; m < MT; ++m) rows[m].move(most[m]);
       }
       u32x4 hi[2][MT], lo[2][MT];
 #pragma unroll
@@ -410,8 +411,8 @@ __global__ __launch_bounds__(64 * kWaves, wide_groups(DP, MT)) void tree_attenti
         }
 #pragma unroll
         for (int m = 0; m < MT; ++m)
-          rows[m].template weights<VT, SCALED>(sc[pair][m], vs0, vs1, masked, seen[m] >> (8 * pair), hi[pair][m],
-                                               lo[pair][m]);
+          rows[m].template weights<SCALED>(sc[pair][m], vs0, vs1, masked, seen[m] >> (8 * pair), hi[pair][m],
+                                           lo[pair][m]);
       }
 #pragma unroll
       for (int x = 0; x < NV; ++x) {

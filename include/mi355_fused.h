@@ -412,7 +412,9 @@ int mi355_kv_cache_keep_fwd(const mi355_kv_cache* cache, const int32_t* seq_lens
  * (NULL: j <= t, a chain):
  *   S[s] = scale * q . K[s],  out = sum_s exp(S[s]) V[s] / sum_s exp(S[s])
  * over the slots it sees, with fp32 sums and one rounding.  What it does not
- * see has no influence, NaN and infinities included.  A token that sees
+ * see has no influence, NaN and infinities included.  An infinite 16-bit value
+ * that it sees makes its element infinite, however small its weight; a NaN, or
+ * both infinities, NaN; a value whose scale is not finite, all of them NaN.  A token that sees
  * nothing, and padding (t >= new_lens[b]; NULL: none), gets zeros, as does
  * one whose scores are all -infinity.
  *

@@ -467,6 +467,16 @@ template <int NV, typename VT> struct Rows {
     }
   }
 
+  // Whether a lane holds a NaN or an infinity of O.
+  __device__ __forceinline__ bool non_finite() const {
+    float zero[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < NV; ++x)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) zero[i] = __builtin_fmaf(o[x][i], 0.f, zero[i]);
+    return __builtin_amdgcn_ballot_w64(zero[0] + zero[1] + zero[2] + zero[3] != 0.f) != 0;
+  }
+
   // O of this lane's row to LDS or from it: row[NV (4 quad + i) + x].
   __device__ __forceinline__ void put(float* row, float f) const {
     const int quad = (threadIdx.x & 63) >> 4;
@@ -497,37 +507,70 @@ __device__ __forceinline__ void load_queries(const TreeArgs& a, const Piece& p, 
   }
 }
 
-// Adds the NaN and infinities that take_out_non_finite left out of the units
-// first, first + step, .. (slots) to the output rows [r0, r1) that see them:
-// rare, and slow.  In LDS, where rows and elements can be indexed; acc row 0 is
-// row r0.  Weights do not matter to them.
+// Sets the elements of the output rows [r0, r1) that see a NaN or an infinity
+// among the values of the tiles (of `slots` slots) first, first + step, .. to
+// the sum of those.  The second product cannot do it: it spreads a value to rows
+// that do not see it (take_out_non_finite), and an infinity times a weight's low
+// part, or a weight that is 0 in 32 bits, is NaN.  Weights do not matter to
+// them.  Rare; a lane for two elements, one look at the page per 16 slots, whose
+// loads go out together.  In LDS, where rows and elements can be indexed; acc
+// row 0 is row r0.
 template <typename T, int FMT, int PITCH>
-__device__ __forceinline__ void add_non_finite(const TreeArgs& a, const Piece& p, float (*acc)[PITCH], int r0, int r1,
+__device__ __forceinline__ void set_non_finite(const TreeArgs& a, const Piece& p, float (*acc)[PITCH], int r0, int r1,
                                                int first, int step, int slots) {
-  const int lane = threadIdx.x & 63;
-  for (; first < p.stop; first += step) {
+  // f(slot, which, value) of every NaN and infinity of elements e and e + 1 in
+  // slots [from, to)
+  const auto each = [&](int e, int from, int to, const auto& f) {
 #pragma unroll 1
-    for (int slot = first; slot < min(first + slots, p.stop); ++slot) {
-      const int64_t at = a.c.row(p.b, slot, p.h);
-      if (at < 0) continue;
+    for (int tile = first; tile < to; tile += step) {
 #pragma unroll 1
-      for (int e = lane; e < a.c.d; e += 64) {
-        float v;
-        if constexpr (FMT == KV_16BIT) {
-          v = load_elem<T>(a.c.v, at * a.c.d + e);
-        } else {
-          float f[4];
-          decode4<FMT>(static_cast<const uint8_t*>(a.c.v)[at * a.c.d + e], f);
-          v = f[0];
+      for (int unit = max(tile, from & ~15); unit < min(tile + slots, to); unit += 16) {
+        const int64_t at = a.c.row(p.b, unit, p.h);
+        if (at < 0) continue;
+        uint32_t two[16];  // a page has whole units
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int64_t i = (at + j) * a.c.d + e;
+          if constexpr (FMT == KV_16BIT) two[j] = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(a.c.v) + i);
+          else two[j] = *reinterpret_cast<const uint16_t*>(static_cast<const uint8_t*>(a.c.v) + i);
         }
-        if (v - v == 0.f) continue;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          float v[4];
+          if constexpr (FMT == KV_16BIT) {
+            const f32x2 w = widen2<T>(two[j]);
+            v[0] = w.x;
+            v[1] = w.y;
+          } else {
+            decode4<FMT>(two[j], v);
+          }
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            if (v[k] - v[k] != 0.f && unit + j >= from && unit + j < to) f(unit + j, k, v[k]);
+        }
+      }
+    }
+  };
+#pragma unroll 1
+  for (int e = 2 * (threadIdx.x & 63); e < a.c.d; e += 128) {
+    float context[2] = {0.f, 0.f};  // which every row sees
+    each(e, 0, min(p.len, p.stop), [&](int, int k, float v) { context[k] += v; });
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (context[k] != 0.f)
+        for (int r = r0; r < r1; ++r) acc[r - r0][e + k] = context[k];
+    if (p.stop <= p.len) continue;
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {  // what the product left goes first
+      each(e, p.len, p.stop, [&](int slot, int k, float v) {
 #pragma unroll 1
         for (int r = r0; r < r1; ++r) {
           const int t = (p.row0 + r) / a.group, i = slot - p.len;
-          const bool see = i < 0 || (t < p.fresh && (a.mask ? a.mask[p.b * a.mask_b + t * a.mask_t + i] != 0 : i <= t));
-          if (see) acc[r - r0][e] += v;
+          float* sum = &acc[r - r0][e + k];
+          if (t < p.fresh && (a.mask ? a.mask[p.b * a.mask_b + t * a.mask_t + i] != 0 : i <= t))
+            *sum = pass ? *sum + v : context[k] != 0.f ? *sum : 0.f;
         }
-      }
+      });
     }
   }
 }

@@ -41,8 +41,9 @@
 // the last slot in use (and is empty for a page that is not there), so that
 // loads beyond return zeros in hardware.  Slots that some rows see and others
 // do not (drafted tokens) keep NaN and infinities out of the second product,
-// which would spread them to every row; the rows that see them get them added
-// at the end.
+// which would spread them to every row; the elements that see them are set at
+// the end, as are those that 16-bit values made NaN or infinite.  (Codes have no
+// infinities; a scale that is not finite makes NaN of both parts, so of its row.)
 #include <type_traits>
 
 #include "tree_attention.h"
@@ -205,9 +206,10 @@ __global__ __launch_bounds__(64 * kWaves, stream_waves(DP, MT)) void tree_attent
     for (int m = 0; m < MT; ++m) {
       const int r = 16 * m + col;
       rows[m].put(joined[wave][r], __builtin_amdgcn_exp2f(rows[m].top - common(r)));
+      if constexpr (!SCALED) left_out |= rows[m].non_finite();
     }
-    if (left_out)
-      add_non_finite<T, FMT>(a, p, joined[wave], 0, p.rows, (share.t0 + wave) * TILE, kWaves * TILE, TILE);
+    if (__builtin_expect(left_out, false))
+      set_non_finite<T, FMT>(a, p, joined[wave], 0, p.rows, (share.t0 + wave) * TILE, kWaves * TILE, TILE);
     __syncthreads();
     for (int e = threadIdx.x; e < p.rows * (d / 4); e += 64 * kWaves) {
       const int r = e / (d / 4), c = 4 * (e - r * (d / 4));
@@ -430,6 +432,10 @@ __global__ __launch_bounds__(64 * kWaves, wide_groups(DP, MT)) void tree_attenti
     }
 
     // every wave has its rows to itself; through LDS for whole lines of stores
+    if constexpr (!SCALED) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m) left_out |= rows[m].non_finite();
+    }
     if (lane == 0) non_finite[wave] = left_out;
     const int64_t slot = share.slot();
     const bool cut = share.cut();
@@ -452,8 +458,8 @@ __global__ __launch_bounds__(64 * kWaves, wide_groups(DP, MT)) void tree_attenti
         }
       }
     }
-    if (uniform(non_finite[0] | non_finite[1] | non_finite[2] | non_finite[3]))
-      add_non_finite<T, FMT>(a, p, mine, r0, r1, share.t0 * TILE, TILE, TILE);
+    if (__builtin_expect(uniform(non_finite[0] | non_finite[1] | non_finite[2] | non_finite[3]), 0))
+      set_non_finite<T, FMT>(a, p, mine, r0, r1, share.t0 * TILE, TILE, TILE);
     constexpr int LINE = DP / 4;  // lanes of a row
     const int c = 4 * (lane % LINE);
     float* partial = a.partial + (slot * a.block_rows + r0) * d + c;
@@ -560,7 +566,21 @@ __global__ __launch_bounds__(64 * (WAVES == 1 ? kJoinRows : WAVES)) void tree_at
   const bool none = t >= s.fresh || total == 0.f;
   const int c = c0 + 128 * (lane / 32);  // lanes 32 - 63 write the second half
   if (c >= a.c.d) return;
-  const f32x4 o = lane < 32 ? v0 : v1;
+  f32x4 o = lane < 32 ? v0 : v1;
+  const f32x4 zero = o - o;
+  if (__builtin_expect(zero[0] + zero[1] + zero[2] + zero[3] != 0.f, false)) {
+    // a piece has a NaN or an infinity, which stays whatever the piece's factor:
+    // one that is 0 in 32 bits makes NaN of an infinity
+    f32x4 bad = {0.f, 0.f, 0.f, 0.f};
+    for (int w = w0; w <= w1; ++w) {
+      const int64_t at = (2 * static_cast<int64_t>(w) + (w * share >= first ? 0 : 1)) * block_rows + rr;
+      const f32x4 part = *reinterpret_cast<const f32x4*>(a.partial + at * a.c.d + c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bad[e] += part[e] - part[e] == 0.f ? 0.f : part[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = bad[e] == 0.f ? o[e] : bad[e];
+  }
   *reinterpret_cast<u32x2*>(static_cast<bits*>(a.out) + static_cast<int64_t>(qrow) * a.c.d + c) =
       none ? u32x2{0, 0} : u32x2{narrow2<T>(f32x2{o[0] * inv, o[1] * inv}), narrow2<T>(f32x2{o[2] * inv, o[3] * inv})};
 }

@@ -30,7 +30,9 @@ def tree_attention(q: torch.Tensor, cache: KVCache, seq_lens: torch.Tensor, *, n
 
     Returns softmax(scale * q K^T) V as [batch, tokens, q_heads, head_dim], fp32
     sums and one rounding to q's dtype.  Slots that a token does not see have no
-    influence, whatever they hold.  A token that sees nothing, and padding (t >=
+    influence, whatever they hold; an infinite 16-bit value that it sees
+    makes its element infinite, however small its weight, and a scale of codes
+    that is not finite makes all of its elements NaN.  A token that sees nothing, and padding (t >=
     ``new_lens[b]``), gets zeros."""
     if scale is None:
         scale = cache.k.shape[-1] ** -0.5

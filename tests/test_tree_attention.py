@@ -386,3 +386,76 @@ def test_small_weights_that_matter(pkg, cuda, dtype, pattern, nats, tokens, head
     want = K.attention(q, cache, [n], scale=1.0)
     K.close(pkg.tree_attention(q, cache, K.ints([n]), scale=1.0), *want)
     K.close(_without_workspace(q, cache, [n]), *want)
+
+
+def _expect_values(out, q, cache, lens, mask=None):
+    """Elements with a visible NaN or both infinities are NaN, those with one infinity are it, others as ever; codes
+    whose scale is not finite count as NaN."""
+    held = [t.clone() if t is not None else None for t in cache.tensors()]
+    k, v, _, ks, vs = held
+    codes = v.float()
+    bad = ~codes.isfinite() | (~vs.isfinite()[..., None] if vs is not None else False)
+    value = torch.where(codes.isfinite(), float("nan"), codes) if vs is not None else codes
+    (v.view(torch.uint8) if v.dtype == torch.float8_e4m3fn else v)[bad] = 0
+    if vs is not None:
+        vs[~vs.isfinite()] = 0
+    clean = type(cache)(*held)
+    want, bound = K.attention(q, clean, lens, mask=mask)
+    got = K.cpu(out)
+    batch, tokens, hq, _ = q.shape
+    special = torch.zeros(want.shape, dtype=torch.float32)
+    for b in range(batch):
+        for s in range(lens[b] + tokens):
+            at = K.place(cache, b, s)
+            row = torch.where(bad[at[0], :, at[1]], value[at[0], :, at[1]], 0.0).cpu()  # [kv_heads, d]
+            if not row.any():
+                continue
+            row = row.repeat_interleave(hq // row.shape[0], 0)
+            for t in range(tokens):
+                j = s - lens[b]
+                if j < 0 or (mask[b, t, j] if mask is not None else j <= t):
+                    special[b, t] += row
+    plain = special == 0
+    K.close(torch.where(plain, got, 0), torch.where(plain, want, 0.0), torch.where(plain, bound, 0.0))
+    assert torch.equal(got.float()[~plain].nan_to_num(12345.0, 1.0, -1.0), special[~plain].nan_to_num(12345.0, 1.0, -1.0))
+
+
+@pytest.mark.parametrize("kind,dtype", [("16bit", torch.float16), ("16bit", torch.bfloat16), ("int8", torch.float16),
+                                        ("e4m3", torch.bfloat16)])
+@pytest.mark.parametrize("tokens,heads,d", [(1, 4, 64), (1, 6, 128), (10, 6, 128), (20, 6, 64), (30, 8, 128), (12, 10, 256)])
+@pytest.mark.parametrize("length", [90, 2000])
+def test_visible_infinities(pkg, cuda, kind, dtype, tokens, heads, d, length):
+    """An infinite value that a row sees makes that element infinite -- in slots that all rows see as in drafted ones,
+    in one piece or many, at a large weight or a small one."""
+    lens = [length, length // 2]
+    cache, q = _case(pkg, kind, dtype, 2, tokens, heads, 2, d, 16, lens)
+    inf, nan = float("inf"), float("nan")
+    for b, s, e, x in [(0, 0, 0, inf), (0, length // 2, 1, -inf), (0, length - 1, 2, inf), (0, 3, 3, inf),
+                       (0, length - 20, 3, -inf), (0, 40, 4, nan), (0, length, 5, inf), (1, 7, d - 1, inf),
+                       (1, 7, d - 2, -inf), (1, length // 4, d - 1, inf)]:
+        page, at = K.place(cache, b, s)
+        if kind == "16bit":
+            cache.v[page, 1, at, e] = x
+        elif s % 2:  # the whole row
+            cache.v_scale[page, 1, at] = x
+        elif kind == "e4m3":
+            cache.v.view(torch.uint8)[page, 1, at, e] = 0x7f
+    mask = K.random_tree(2, tokens, 3)
+    out = pkg.tree_attention(q, cache, K.ints(lens), tree_mask=mask.to(cuda))
+    _expect_values(out, q, cache, lens, mask)
+
+
+@pytest.mark.parametrize("tokens", [1, 40])
+@pytest.mark.parametrize("nats", [60, 200])
+def test_a_visible_infinity_of_a_weight_that_vanishes(pkg, cuda, tokens, nats):
+    """The weight of the infinite value is beyond 32 bits of exponent (not beyond 64), in another piece than the rest."""
+    n = 3000
+    cache, q = _case(pkg, "16bit", torch.bfloat16, 1, tokens, 2, 1, 64, 32, [n])
+    q.zero_()
+    q[..., 0] = 8.0
+    cache.k.zero_()
+    for s in (5, 2900):
+        page, at = K.place(cache, 0, s)
+        cache.k[page, 0, at, 0] = -float(nats)  # 8 nats / sqrt(64)
+        cache.v[page, 0, at, s % 7] = float("inf")
+    _expect_values(pkg.tree_attention(q, cache, K.ints([n])), q, cache, [n])

@@ -313,7 +313,8 @@ int mi355_linear16_ws_fwd(const void* x, const void* weight, const void* bias, v
  *   y          [batch, tokens, heads, head_dim] of dtype, contiguous; must not
  *              overlap x.
  *   positions  int64 by two strides (0 for one row of positions for all).
- *   inv_freq   fp32 [R / 2]; R even, 0 <= R <= head_dim, R <= 256.
+ *   inv_freq   fp32 [R / 2]; R even, 0 <= R <= head_dim, R <= 256.  With R = 0
+ *              neither is read, and both may be NULL.
  *   batch * tokens < 2^24, heads <= 65535, head_dim < 2^20
  *   (MI355_ERR_UNSUPPORTED beyond).  Nothing to do for 0 elements.
  */

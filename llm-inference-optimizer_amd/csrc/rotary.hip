@@ -77,7 +77,8 @@ template <typename T> __global__ __launch_bounds__(256) void rotary_generic(Args
   __shared__ float cs[2 * kMaxPairs];
   const float* sn = cs + kMaxPairs;
   const int b = blockIdx.x / a.tokens, t = blockIdx.x - b * a.tokens;
-  rotary_angles(cs, a.rot, a.rot.positions[b * a.rot.pos_stride_b + t * a.rot.pos_stride_t], threadIdx.x, 256);
+  if (a.rot.rotary > 0)  // else there may be no positions
+    rotary_angles(cs, a.rot, a.rot.positions[b * a.rot.pos_stride_b + t * a.rot.pos_stride_t], threadIdx.x, 256);
   __syncthreads();
   const int half = a.rot.rotary / 2;
   for (int h = blockIdx.y * a.heads_per_wave; h < min(a.heads, (static_cast<int>(blockIdx.y) + 1) * a.heads_per_wave); ++h) {

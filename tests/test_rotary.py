@@ -99,3 +99,18 @@ def test_refusals(pkg, cuda):
             pkg.fused_rotary(*args)
     with pytest.raises(Exception, match="rotary_dim must be at most 256"):
         pkg.fused_rotary(torch.zeros((1, 1, 1, 300), device=cuda), p[:, :1], torch.zeros(129, device=cuda))
+
+
+@pytest.mark.parametrize("dtype,code", [(torch.float32, 0), (torch.float16, 1), (torch.bfloat16, 2)])
+@pytest.mark.parametrize("d,offset,tokens", [(7, 0, 3), (300, 1, 2), (2048, 0, 2), (64, 1, 1100), (64, 0, 3)])
+def test_nothing_to_rotate_needs_no_positions(pkg, cuda, dtype, code, d, offset, tokens):
+    """The C call with rotary_dim = 0, positions and inv_freq NULL: a copy, of whole packets and of odd rows."""
+    import importlib
+    L = importlib.import_module("llm-inference-optimizer_amd._lib")
+    assert (L.F32, L.F16, L.BF16)[code] == code
+    x = torch.randn(tokens * 3 * d + offset, generator=torch.Generator().manual_seed(d)).to(dtype).to(cuda)[offset:]
+    y = torch.empty((1, tokens, 3, d), dtype=dtype, device=cuda)
+    assert L.load().mi355_rotary_fwd(x.data_ptr(), y.data_ptr(), None, None, 1, tokens, 3, d, 0, 0, 3 * d, d, 0, 0, 1.0, 0,
+                                     code, L.stream_handle(y.device)) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(y.view(-1), x)

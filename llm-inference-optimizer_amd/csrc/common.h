@@ -420,6 +420,14 @@ __device__ __forceinline__ float load_dyn(const void* p, int64_t i, int dt) {
   return load_elem<F32>(p, i);
 }
 
+// Between what lanes of a wave write to LDS and what others of it read: the
+// operations of a wave are done in order, and the compiler keeps them so.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // ---------------------------------------------------------------------------
 // Host-side helpers shared by the launchers.
 // ---------------------------------------------------------------------------

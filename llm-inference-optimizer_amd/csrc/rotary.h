@@ -43,12 +43,6 @@ __device__ __forceinline__ void rotary_angles(float* cs, const RotaryArgs& a, in
     cs[kMaxPairs + j] = a.scale * s;
   }
 }
-// For one wave: LDS operations of a wave are done in order.
-__device__ __forceinline__ void wave_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
 
 // How a lane's packet of elements meets its pairs.
 enum RotaryMode {

@@ -208,8 +208,10 @@ __global__ __launch_bounds__(64 * kWaves, stream_waves(DP, MT)) void tree_attent
       rows[m].put(joined[wave][r], __builtin_amdgcn_exp2f(rows[m].top - common(r)));
       if constexpr (!SCALED) left_out |= rows[m].non_finite();
     }
-    if (__builtin_expect(left_out, false))
+    if (__builtin_expect(left_out, false)) {
+      wave_sync();
       set_non_finite<T, FMT>(a, p, joined[wave], 0, p.rows, (share.t0 + wave) * TILE, kWaves * TILE, TILE);
+    }
     __syncthreads();
     for (int e = threadIdx.x; e < p.rows * (d / 4); e += 64 * kWaves) {
       const int r = e / (d / 4), c = 4 * (e - r * (d / 4));
@@ -458,8 +460,11 @@ __global__ __launch_bounds__(64 * kWaves, wide_groups(DP, MT)) void tree_attenti
         }
       }
     }
-    if (__builtin_expect(uniform(non_finite[0] | non_finite[1] | non_finite[2] | non_finite[3]), 0))
+    wave_sync();
+    if (__builtin_expect(uniform(non_finite[0] | non_finite[1] | non_finite[2] | non_finite[3]), 0)) {
       set_non_finite<T, FMT>(a, p, mine, r0, r1, share.t0 * TILE, TILE, TILE);
+      wave_sync();
+    }
     constexpr int LINE = DP / 4;  // lanes of a row
     const int c = 4 * (lane % LINE);
     float* partial = a.partial + (slot * a.block_rows + r0) * d + c;

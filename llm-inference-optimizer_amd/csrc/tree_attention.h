@@ -253,7 +253,9 @@ template <typename T, int FMT, int DP, int AUX> struct UnitRegs {
     const int lane = threadIdx.x & 63, r = lane & 15, quad = lane >> 4;
     if constexpr (FMT != KV_16BIT)
       vs = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(u.vs, 16u * quad, 0, AUX));
-    const uint32_t first = NV * r < d ? static_cast<uint32_t>((4 * quad * d + NV * r) * ES) : kOob;
+    // beyond the unit in the last packet too: kOob and a packet would be 0
+    constexpr uint32_t kBeyond = VD > 4 ? kOob - 16 * (VD / 4 - 1) : kOob;
+    const uint32_t first = NV * r < d ? static_cast<uint32_t>((4 * quad * d + NV * r) * ES) : kBeyond;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int at = j * d * ES;  // uniform: the scalar offset of the load

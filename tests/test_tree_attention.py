@@ -459,3 +459,16 @@ def test_a_visible_infinity_of_a_weight_that_vanishes(pkg, cuda, tokens, nats):
         cache.k[page, 0, at, 0] = -float(nats)  # 8 nats / sqrt(64)
         cache.v[page, 0, at, s % 7] = float("inf")
     _expect_values(pkg.tree_attention(q, cache, K.ints([n])), q, cache, [n])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d", [144, 208, 240])
+@pytest.mark.parametrize("tokens,length", [(1, 40), (5, 600), (24, 600)])
+def test_non_finite_first_elements_of_heads_that_fill_no_tile(pkg, cuda, dtype, d, tokens, length):
+    """Lanes beyond the last element hold zeros, whatever the unit's first elements are."""
+    cache, q = _case(pkg, "16bit", dtype, 1, tokens, 4, 2, d, 16, [length])
+    for s, x in ((length // 3, float("inf")), (length, float("nan")), (length - 1, -float("inf"))):
+        page, at = K.place(cache, 0, s)
+        cache.v[page, 0, at, s % 8] = x
+    mask = K.random_tree(1, tokens, 3)
+    _expect_values(pkg.tree_attention(q, cache, K.ints([length]), tree_mask=mask.to(cuda)), q, cache, [length], mask)

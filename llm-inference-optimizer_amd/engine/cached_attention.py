@@ -99,6 +99,7 @@ class CachedAttention(torch.nn.Module):
 
     def __init__(self, orig_module: torch.nn.Module):
         super().__init__()
+        self.training = orig_module.training
         for name in _PARTS:
             setattr(self, name, getattr(orig_module, name))
         # plain attributes callers may read, and the forward for other caches; the

@@ -241,3 +241,13 @@ def test_patched_attention_follows_train_and_eval(pkg):
         assert not torch.equal(model(ids).logits, want)  # dropout
         assert torch.equal(model.eval()(ids).logits, want)
         assert torch.equal(copy.deepcopy(model)(ids).logits, want)
+
+
+def test_attention_patched_in_eval_mode_stays_there(pkg):
+    """A model that was in eval() before the patch does not start to drop attention weights."""
+    model, ids = _tiny("Llama", attention_dropout=0.5).eval(), torch.arange(12)[None]
+    with torch.no_grad():
+        want = model(ids).logits
+        pkg.patch_model_with_fused_kernels(model, patch_norm=False, patch_mlp=False, fuse_attention=True)
+        assert not any(m.training for m in model.modules())
+        assert torch.equal(model(ids).logits, want)

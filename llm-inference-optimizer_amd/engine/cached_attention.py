@@ -36,7 +36,13 @@ class DecoderCache:
     tensors -- ``lens`` (tokens in the cache, int32 [batch]), ``positions`` (of
     the step's tokens, int64 [batch, tokens]), ``new_lens`` and ``tree_mask`` (None,
     or of a draft).  HF's forward sees an empty cache of its own kind through
-    ``as_past()``: it builds no mask and no buffers for it."""
+    ``as_past()``: it builds no buffers for it.
+
+    What a token sees is said by these tensors alone: a padded batch, or any
+    attention mask but a causal one, is refused (padding goes behind a row's
+    tokens, with ``new_lens``).  ``unmasked``: set by a caller that passes the model
+    no mask, so that the one that HF may build needs no look, which waits for the
+    GPU."""
 
     def __init__(self, layers: list[KVCache], inv_freq: torch.Tensor, rotary_scale: float):
         self.layers = layers
@@ -45,7 +51,7 @@ class DecoderCache:
         batch = layers[0].page_table.shape[0]
         self.lens = torch.zeros((batch,), dtype=torch.int32, device=layers[0].k.device)
         self.positions = self.new_lens = self.tree_mask = None
-        self.prompt = False
+        self.prompt = self.unmasked = False
 
     @classmethod
     def allocate(cls, model, batch_size: int, max_len: int, kv_format: str, page_size: int | None = None):
@@ -94,6 +100,19 @@ def cacheable(module: torch.nn.Module) -> bool:
             and module.head_dim % 16 == 0 and module.head_dim <= 256)
 
 
+def plain_causal(mask: torch.Tensor) -> bool:
+    """Whether an attention mask, as attention modules get it (bool or additive
+    [batch, 1, tokens, tokens], or [batch, tokens] of the tokens that are there),
+    is that of a batch without padding."""
+    if mask.dim() == 2:
+        return bool((mask != 0).all())
+    tokens = mask.shape[-2]
+    if mask.shape[-1] != tokens:
+        return False
+    causal = torch.ones((tokens, tokens), dtype=torch.bool, device=mask.device).tril()
+    return bool(((mask if mask.dtype == torch.bool else mask == 0) == causal).all())
+
+
 class CachedAttention(torch.nn.Module):
     """Wraps an attention module's four projections (the same objects)."""
 
@@ -119,6 +138,9 @@ class CachedAttention(torch.nn.Module):
             self._original.training = self.training  # not a registered child: train() and eval() pass it by
             return self._original(hidden_states=hidden_states, position_embeddings=position_embeddings,
                                   attention_mask=attention_mask, past_key_values=past_key_values, **kwargs)
+        if attention_mask is not None and not state.unmasked and self.layer_idx == 0 and not plain_causal(attention_mask):
+            raise ValueError("the cache's attention takes no mask but a causal one: padding goes behind a row's tokens "
+                             "(DecoderCache.new_lens), a draft's tree into DecoderCache.tree_mask")
         batch, tokens, _ = hidden_states.shape
         q, k, v = (proj(hidden_states).view(batch, tokens, -1, self.head_dim)
                    for proj in (self.q_proj, self.k_proj, self.v_proj))

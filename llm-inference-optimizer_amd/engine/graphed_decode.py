@@ -86,6 +86,7 @@ class GraphedGreedyDecoder:
         n, t = self.batch_size, self.draft_tokens or 1
         # a draft's last nodes may lie behind the last token that is wanted
         self.cache = DecoderCache.allocate(self.model, n, self.max_cache_len + t - 1, kv_cache, page_size)
+        self.cache.unmasked = True
         self._past = self.cache.as_past()
         self._tok = torch.zeros((n, t), dtype=torch.long, device=self.device)
         self._pos_ids = torch.zeros((n, t), dtype=torch.long, device=self.device)

@@ -21,11 +21,14 @@
 //           slots is right.
 //
 // Measured: append of 3001 tokens of 4 sequences, half of them padding (28 + 2 x
-// 4 heads of 128, bf16 to e4m3, queries and keys rotated, 200 MB) 34.0 us, 5.9
-// TB/s; of 16 single tokens 4.6 us, of which a launch takes half.  Read of the
-// former (32 MB) 8.0 us, of one token 2.5.  Keep of up to 9 of 64 tokens of 128
-// sequences (8 heads of 16-bit values, 5 MB) 7.0 us: lengths, kept numbers, page
-// table, rows and stores are dependent trips to memory.
+// 4 heads of 128, bf16 to e4m3, queries and keys rotated, 194 MB) 33.7 us, 5.8
+// TB/s; of 16 single tokens 4.7 us: a launch, the position and slot, the page and
+// the row's store are trips that wait for each other.  Read of the former (32 MB)
+// 7.8 us, 4.1 TB/s: a lane's one packet waits for lengths, the page and the codes;
+// of one token 2.4.  Keep of up to 9 of 64 tokens of 128 sequences (8 heads of
+// 16-bit values, 5 MB) 6.9 us, of 4 sequences 3.6: five such trips, as it is
+// written -- kept_lens bounds the loop that loads `kept`, and the destination's
+// page is looked up behind the barrier.
 #include "kv_cache.h"
 #include "rotary.h"
 

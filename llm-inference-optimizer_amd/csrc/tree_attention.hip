@@ -8,8 +8,9 @@
 // rows of q, so it is bound by HBM: the T q_heads / kv_heads rows that share a
 // key/value head are taken together.
 //
-// Products on MFMA (v_mfma_f32_16x16x32), without LDS: a wave takes tiles of
-// 32 slots and computes
+// Products on MFMA (v_mfma_f32_16x16x32).  Up to 32 rows a wave makes its operands
+// in registers, without LDS (tree_attention_stream); for more rows the waves share
+// them through LDS (tree_attention_wide).  Of tiles of 32 slots a wave computes
 //   S^T = K Q^T   A = K: lane (r = l % 16, quad = l / 16) holds 8 elements of
 //                 the key in slot r of a 16-slot unit; B = Q^T: the lane's
 //                 column is query row l % 16.  A lane gets S of its query row
@@ -63,12 +64,18 @@ constexpr int stream_waves(int dp, int mt) {
 // tile, loads straight to MFMA operands.  The next tile's keys are loaded as soon
 // as this one's scores are taken, its values after the second product: the
 // registers hold one tile, and the other waves of the SIMD cover the rest.
-// Bound by HBM where contexts are long: 2 of 120011 slots (28 / 4 heads of 128,
-// e4m3, 253 MB) 47.4 us, 6.2 TB/s behind some 6 us of start and end; 32 ragged
-// ones to 6000 (int8, 114 MB) 27.8 us, 4.1 TB/s with that start; one context of 777 slots 7.0 us, all
-// of it latency.  Loads are non-temporal: 55.6 against 59.7 us with the join on
-// the long contexts, which pass through the caches, and 36.9 against 33.4 us on
-// the 114 MB where they are still there from the call before.
+// Bound by HBM where contexts are long: a call (with its join) over growing
+// contexts of 2 sequences (28 / 4 heads of 128) is a line of 5.9 TB/s for int8,
+// 6.0 for e4m3 and 6.6 for 16 bits that begins at 12 - 14 us: two launches, the
+// line of tiles, the first loads' trip and the join.  This kernel alone: 2 of
+// 120011 slots (e4m3, 253 MB) 49.8 us, 32 ragged ones to 6000 (int8, 114 MB)
+// 28.6, one of 777 7.0, all of it latency.  28 rows (4 tokens) over 8 contexts of
+// 4096 20.0 (int8, 35 MB) and 22.7 us (16 bits, 67 MB): short shares again, the
+// vector unit 39% and 29% busy, the matrix unit 9%.
+// Loads are non-temporal.  Against loads that stay in the caches, calls in a
+// graph over three caches in turn: 55.3 / 59.3 us for the 253 MB, 48.6 / 53.2 for
+// 225 MB of 16 bits; 35.0 / 34.6 for 116 MB of int8 and 30.2 / 28.3 for 67 MB, of
+// which some is still there from three calls before.
 template <typename T, int FMT, int DP, int MT>
 __global__ __launch_bounds__(64 * kWaves, stream_waves(DP, MT)) void tree_attention_stream(TreeArgs a) {
   typedef UnitRegs<T, FMT, DP, kStreamAux> Regs;  // the cache is read once
@@ -239,9 +246,9 @@ __global__ __launch_bounds__(64 * kWaves, stream_waves(DP, MT)) void tree_attent
 // bank twice.  Two tiles in LDS: while one is used, the next is written and the
 // one after it is on its way to registers; one barrier per tile.
 // 8 trees of 48 tokens over ragged contexts to 4100 (28 / 4 heads of 128, 16-bit,
-// 45 MB): 46.6 us for 13.2 GFLOP, 20 with the low parts of the weights: per SIMD
-// the matrix unit is busy 24% of the time and the vector unit 42% (exponentials,
-// the split of the weights, masks), with two waves to overlap them.
+// 45 MB): 49.6 us (fp16 52.2) for 13.2 GFLOP, 20 with the low parts of the weights:
+// per SIMD the matrix unit is busy 26% of the time and the vector unit 47%
+// (exponentials, the split of the weights, masks), with two waves to overlap them.
 constexpr int wide_groups(int dp, int mt) { return dp <= 64 && mt == 1 ? 3 : dp <= 128 ? 2 : 1; }  // of a CU
 
 template <typename T, int FMT, int DP, int MT>
@@ -601,22 +608,33 @@ Plan plan(const mi355_kv_cache& c, int64_t batch, int64_t tokens, int64_t q_head
   Plan p{};
   const int dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
   const int64_t rows = tokens * (q_heads / c.kv_heads);
-  // The stream kernel to 32 rows (8 contexts of 4096, D 128, stream / wide: 28
-  // rows of int8 28.3 / 30.2 us, of 16 bits 31.1 / 29.0; 56 rows of int8 in 64-row
-  // tiles of the stream kernel 50.8 / 31).  Wide: 16 rows per wave while one block
-  // holds them all, then 32 (336 rows, blocks of 128 / 64: 81 / 90 us for 8
-  // contexts of 4096 of int8, 64.6 / 66.2 us for ragged ones of 16 bits); 256-wide
-  // heads have the registers for 16.
+  // The stream kernel to 32 rows: calls in a graph, stream / wide in us, over 8
+  // contexts of 4096 (over 24 of 700 the same order):
+  //              28 rows, D 64   D 128         32 rows, D 256
+  //   int8       15.9 / 20.4     26.6 / 30.5   23.6 / 25.6
+  //   16 bits    16.6 / 18.9     29.6 / 29.4   28.2 / 25.4
+  //              56 rows, D 64   D 128         64 rows, D 256
+  //   int8       21.5 / 23.8     33.3 / 31.2   30.8 / 28.9
+  //   16 bits    22.3 / 22.5     38.5 / 30.3   35.6 / 28.0
+  // (e4m3 as int8): heads of 64 would take the stream kernel further, 16 bits of
+  // 256 the wide one earlier, by up to a tenth.  Wide: 16 rows per wave while one
+  // block holds them all, then 32 (336 rows of D 128, blocks of 128 / 64: 81 / 90
+  // us for 8 contexts of 4096 of int8, 64.6 / 66.2 us for ragged ones of 16 bits);
+  // 256-wide heads have the registers for 16.
   p.wide = rows > 32;
   p.mt = p.wide ? (rows <= 64 || dp == 256 ? 1 : 2) : (rows <= 16 ? 1 : 2);
   p.block_rows = 16 * p.mt * (p.wide ? kWaves : 1);
   p.blocks = static_cast<int>((rows + p.block_rows - 1) / p.block_rows);
   p.tile = p.wide ? kWideTile : kStreamTile;
   p.step = p.wide ? 1 : kWaves;  // tiles of a workgroup's step
-  // What a piece costs beside its tiles, in tiles.  Measured (stream, wide): 0, 0
-  // / 4, 2 / 8, 4 / 16, 6 tiles give 37.9 / 36.4 / 34.6 / 36.5 us for 32 ragged
-  // contexts to 6000, 14.2 / 10.6 / 9.8 / 9.6 us for one of 777 and 65.7 / 61.2
-  // / 60.3 / 62.1 us for 8 trees of 48.
+  // What a piece costs beside its tiles, in tiles.  Stream, 0 / 4 / 8 / 16: 32
+  // ragged contexts to 6000, D 128 37.6 / 35.3 / 35.0 / 35.7 us (int8) and 50.7 /
+  // 48.6 / 48.9 / 49.8 (16 bits), D 64 21.5 / 20.4 / 18.4 / 18.5 and 24.1 / 22.4 /
+  // 21.0 / 21.3, D 256 28.9 / 25.4 / 23.7 / 24.1 and 47.6 / 42.9 / 42.6 / 44.9; one
+  // of 777 slots 13.4 / 10.1 / 10.2 / 10.2.  Wide, 0 / 2 / 4 / 6: 8 trees of 48
+  // 64.4 / 60.0 / 59.1 / 59.9, 24 of 9 with D 64 25.6 / 24.6 / 24.8 / 24.5 (int8)
+  // and 25.0 / 23.5 / 23.5 / 23.4 (16 bits), 8 of 16 with D 256 36.6 / 32.2 / 31.9 /
+  // 32.2 and 36.8 / 32.1 / 31.8 / 32.7.
   p.pad = p.wide ? 4 : 8;
   const int64_t pieces = batch * c.kv_heads * p.blocks;
   const int64_t tiles = (c.table_width * c.page_size + p.tile - 1) / p.tile + p.pad;  // of the longest possible context
@@ -659,7 +677,10 @@ template <typename T> int tree_join(const TreeArgs& a, const Plan& p, hipStream_
   // the chip (8192 waves) holds them.  Against one wave per row: 56 rows of 96
   // pieces 55.9 / 73.5 us with the first kernel; 896 rows of 6 3.96 / 4.84 us
   // (4 waves / 1); 3024 rows of 16 7.2 / 7.9 (2 / 1; 8.7 with 4, 13.1 with 8);
-  // 10752 rows of 5 13.5 / 9.9 (2 / 1).
+  // 10752 rows of 5 13.5 / 9.9 (2 / 1).  Whole calls with 1 / 2 / 4 / 8 waves, of
+  // which the rule takes 8: 28 rows of 256 pieces with D 64 70.5 / 29.7 / 24.7 / 23.2
+  // us, 16 with D 256 71.5 / 32.8 / 27.8 / 26.3; 896 rows of 16 26.3 / 24.9 / 25.2 /
+  // 26.4, 1024 rows of 16 with D 256 32.3 / 30.1 / 29.9 / 31.8: there it is off by 6%.
   const auto fits = [&](int waves) { return pieces > 2 * waves && 2 * rows * waves <= 8192; };
   const auto grid = [&](int64_t groups) { return dim3(static_cast<unsigned>(groups)); };
   if (fits(4)) return launch(tree_attention_join<T, 8>, grid(rows), 512, 0, a, s, what);

@@ -52,7 +52,9 @@ class GraphedGreedyDecoder:
     one page per sequence without it).  The model's attention has to be patched
     (``patch_model_with_fused_kernels(model, fuse_attention=True)``).
     ``draft_tokens`` (2 .. 128, only with ``kv_cache``): nodes of the tree that a
-    step verifies; ``steps`` counts the steps of the last generation.  Tokens are
+    step verifies; ``steps`` counts the steps of the last generation.  They pay
+    for single sequences that repeat themselves; a batch takes the steps of its
+    slowest sequence, each with host work per sequence, and may get slower.  Tokens are
     those of greedy decoding up to rounding: a step of several tokens runs its
     projections in other shapes, so that near-ties may fall the other way."""
 

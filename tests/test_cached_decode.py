@@ -167,3 +167,25 @@ def test_refusals(pkg, cuda):
         dec.generate(_prompt(cuda, 2, 60), 5)
     windowed = _model(cuda, use_sliding_window=True, sliding_window=16, max_window_layers=0)
     assert pkg.patch_model_with_fused_kernels(windowed, fuse_attention=True)["attention"] == 0
+
+
+def test_a_ragged_prompt_over_a_used_cache(pkg, cuda):
+    """More tokens than tree_attention takes, padding behind the shorter row, over slots that hold NaN from before."""
+    model = _model(cuda)
+    pkg.patch_model_with_fused_kernels(model, fuse_attention=True)
+    cache = pkg.DecoderCache.allocate(model, 2, 256, "16bit")
+    for c in cache.layers:
+        c.k.fill_(float("nan"))
+        c.v.fill_(float("nan"))
+    ids, at = _prompt(cuda, 2, 200), torch.arange(200, device=cuda).expand(2, 200)
+    cache.positions, cache.prompt = at, True
+    cache.new_lens = torch.tensor([200, 150], dtype=torch.int32, device=cuda)
+    with torch.inference_mode():
+        logits = model(ids, past_key_values=cache.as_past(), position_ids=at, use_cache=True).logits.float()
+        whole = model(ids).logits.float()
+        short = model(ids[1:, :150]).logits.float()
+        cache.tree_mask = torch.zeros((2, 200, 200), dtype=torch.bool, device=cuda)
+        with pytest.raises(ValueError, match="a tree has at most 128"):
+            model(ids, past_key_values=cache.as_past(), position_ids=at, use_cache=True)
+    assert (logits[0] - whole[0]).abs().max().item() <= LOGIT_TOL["16bit"]
+    assert (logits[1, :150] - short[0]).abs().max().item() <= LOGIT_TOL["16bit"]

@@ -415,9 +415,9 @@ int mi355_kv_cache_keep_fwd(const mi355_kv_cache* cache, const int32_t* seq_lens
  * over the slots it sees, with fp32 sums and one rounding.  What it does not
  * see has no influence, NaN and infinities included.  An infinite 16-bit value
  * that it sees makes its element infinite, however small its weight; a NaN, or
- * both infinities, NaN; a value whose scale is not finite, all of them NaN.  A token that sees
- * nothing, and padding (t >= new_lens[b]; NULL: none), gets zeros, as does
- * one whose scores are all -infinity.
+ * both infinities, NaN; a value whose scale is not finite, all of them NaN.
+ * A token that sees nothing, and padding (t >= new_lens[b]; NULL: none), gets
+ * zeros, as does one whose scores are all -infinity.
  *
  *   q     [batch, tokens, q_heads, head_dim] of dtype (fp16, bf16) by three
  *         strides (batch, token, head), head_dim contiguous, rows 16-byte

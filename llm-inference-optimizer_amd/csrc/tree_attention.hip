@@ -71,7 +71,7 @@ constexpr int stream_waves(int dp, int mt) {
 // 120011 slots (e4m3, 253 MB) 49.8 us, 32 ragged ones to 6000 (int8, 114 MB)
 // 28.6, one of 777 7.0, all of it latency.  28 rows (4 tokens) over 8 contexts of
 // 4096 20.0 (int8, 35 MB) and 22.7 us (16 bits, 67 MB): short shares again, the
-// vector unit 39% and 29% busy, the matrix unit 9%.
+// vector unit 39% and 29% busy, the matrix unit 9% and 8%.
 // Loads are non-temporal.  Against loads that stay in the caches, calls in a
 // graph over three caches in turn: 55.3 / 59.3 us for the 253 MB, 48.6 / 53.2 for
 // 225 MB of 16 bits; 35.0 / 34.6 for 116 MB of int8 and 30.2 / 28.3 for 67 MB, of

@@ -40,6 +40,7 @@ class DecoderCache:
 
     ``prompt``: the cache is empty before the step, which may then have more tokens
     than ``tree_attention`` takes.
+
     What a token sees is said by these tensors alone: a padded batch, or any
     attention mask but a causal one, is refused (padding goes behind a row's
     tokens, with ``new_lens``).  ``unmasked``: set by a caller that passes the model
@@ -158,7 +159,7 @@ class CachedAttention(torch.nn.Module):
             if state.tree_mask is not None:
                 raise ValueError(f"a tree has at most {TREE_ATTENTION_MAX_TOKENS} tokens, got {tokens}")
             # zeros in the slots of padding, which hold what was there before: causal
-            # attention gives them no weight, and no weight times NaN is NaN
+            # attention gives them a weight of 0, and 0 times NaN is NaN
             end = state.lens + (tokens if state.new_lens is None else state.new_lens)
             k, v = kv_cache_read(cache, end, tokens, dtype=q.dtype)
             out = torch.nn.functional.scaled_dot_product_attention(q.transpose(1, 2), k, v, is_causal=True,

@@ -189,3 +189,15 @@ def test_a_ragged_prompt_over_a_used_cache(pkg, cuda):
             model(ids, past_key_values=cache.as_past(), position_ids=at, use_cache=True)
     assert (logits[0] - whole[0]).abs().max().item() <= LOGIT_TOL["16bit"]
     assert (logits[1, :150] - short[0]).abs().max().item() <= LOGIT_TOL["16bit"]
+
+
+@pytest.mark.parametrize("draft", [None, 6])
+def test_a_model_that_builds_masks(pkg, cuda, draft):
+    """HF's eager attention gets a causal mask with every step, which HF cannot build while a stream is captured."""
+    model = _model(cuda)
+    model.set_attn_implementation("eager")
+    pkg.patch_model_with_fused_kernels(model, fuse_attention=True)
+    ids = torch.cat((_prompt(cuda, 1, 40, period=7), _prompt(cuda, 1, 40, seed=13)))
+    dec = pkg.GraphedGreedyDecoder(model, 2, 120, use_graph=False, kv_cache="16bit", draft_tokens=draft)
+    out, logits = dec.generate(ids, 20, return_logits=True)
+    _check(pkg, model, dec, ids, out, logits, "16bit", f"eager draft {draft}")

@@ -2,8 +2,9 @@
  * mi355_fused.h -- C ABI of the MI355X (gfx950) fused RMSNorm and SiLU-and-mul
  * kernels, the fused gate/up projections, the weight-only int8 (W8A16)
  * linear with its quantiser, the 16-bit linear of the MLP's down projection,
- * and what lies between an attention block's projections: rotary positions, a
- * paged and quantised key/value cache, and attention over it.
+ * what lies between an attention block's projections (rotary positions, a
+ * paged and quantised key/value cache, and attention over it, shared prefixes
+ * among it), page tables made from lengths, and drawing the next tokens.
  *
  * The reference has no FFI: its boundary is a pair of Python launchers that
  * hand torch tensors to Triton kernels.  Each entry point below replaces one of
@@ -440,6 +441,110 @@ int mi355_tree_attention_fwd(const mi355_kv_cache* cache, const void* q, void* o
                              const uint8_t* tree_mask, int64_t mask_stride_b, int64_t mask_stride_t,
                              int64_t batch, int64_t tokens, int64_t q_heads, const int64_t* q_strides,
                              float scale, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Attention as mi355_tree_attention_fwd computes it, for a batch whose
+ * sequences share prefixes.  Sequence b is a member of group g if groups[g] <=
+ * b < groups[g + 1] (groups int32 [group_count + 1], ascending; NULL: groups of
+ * batch / group_count sequences each), and the slots below
+ *   shared_b = min(prefix_lens[g], seq_lens[b])
+ * are those that the page table names for the group's first sequence: they are
+ * read once for all members, whose own entries for them are not looked at.  From
+ * shared_b on a sequence's slots are its own.  A sequence of no group shares
+ * nothing; group_count 0 is allowed.  Group boundaries are clamped to
+ * [0, batch]; of descending ones, the first group that fits is taken.
+ *
+ * The other arguments, limits and rules (masks, padding, infinities) are those
+ * of mi355_tree_attention_fwd, the workspace's too.
+ */
+int64_t mi355_shared_prefix_attention_workspace(const mi355_kv_cache* cache, int64_t batch, int64_t tokens,
+                                                int64_t q_heads, int64_t group_count);
+int mi355_shared_prefix_attention_fwd(const mi355_kv_cache* cache, const void* q, void* out,
+                                      const int32_t* seq_lens, const int32_t* new_lens,
+                                      const int32_t* prefix_lens, const int32_t* groups, int64_t group_count,
+                                      const uint8_t* tree_mask, int64_t mask_stride_b, int64_t mask_stride_t,
+                                      int64_t batch, int64_t tokens, int64_t q_heads, const int64_t* q_strides,
+                                      float scale, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * A page table in which every sequence has pages for its slots below
+ * end_b = max(0, seq_lens[b]) + max(0, new_lens[b]) (new_lens NULL: 0):
+ *   need_b = ceil(end_b / page_size)
+ *   table_out[b, c] = page_table[b, c]  for c < need_b, where that names a page
+ *                   = a free page       for other c < need_b
+ *                   = -1                for c >= need_b
+ * Free are the pages that no entry of the first kind names: several sequences
+ * may name one page, and a page is free when none of them needs it any more
+ * (a sequence that ended has length 0).  Free pages are handed out in ascending
+ * order, to entries in the order of b, then c; when there are no more, -1.
+ * missing[b]: pages of need_b that sequence b did not get, those beyond the
+ * table's width among them.  The table is the only state.
+ *
+ *   Of the cache page_table, its sizes, pages and page_size are read; k, v and
+ *   scales may be NULL.  table_out int32 [batch, out_stride], out_stride >=
+ *   table_width: the cache's own table (with its stride), or memory that does
+ *   not overlap it.  missing int32 [batch].  batch < 2^24, batch * table_width
+ *   < 2^31, pages < 2^30 (MI355_ERR_UNSUPPORTED beyond).
+ *   workspace: at least mi355_kv_cache_reserve_workspace bytes of 16-byte
+ *   aligned device memory that no other work touches until the call's kernels
+ *   end (its contents need no preparation).
+ */
+int64_t mi355_kv_cache_reserve_workspace(const mi355_kv_cache* cache, int64_t batch);
+int mi355_kv_cache_reserve_fwd(const mi355_kv_cache* cache, const int32_t* seq_lens, const int32_t* new_lens,
+                               int32_t* table_out, int64_t out_stride, int32_t* missing, int64_t batch,
+                               void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Where the tokens of a packed batch go: new_lens[0] tokens of sequence 0, then
+ * new_lens[1] of sequence 1, ... (negative: 0).  For packed token j, token t of
+ * sequence b:
+ *   sequences[j] = b,  positions[j] = max(0, seq_lens[b]) + t
+ *   slots[j] = page * page_size + positions[j] % page_size with the page that
+ *              page_table names for the position, -1 where it names none
+ * Rows from the number of tokens on get slot -1, sequence -1 and position 0.
+ *
+ *   slots, positions int64 [tokens]; sequences int32 [tokens].  batch < 2^24,
+ *   tokens < 2^31 (MI355_ERR_UNSUPPORTED beyond).  Of the cache page_table, its
+ *   sizes, pages and page_size are read.  workspace: as for
+ *   mi355_kv_cache_reserve_fwd, of mi355_kv_slot_map_workspace bytes.
+ */
+int64_t mi355_kv_slot_map_workspace(int64_t batch);
+int mi355_kv_slot_map_fwd(const mi355_kv_cache* cache, const int32_t* seq_lens, const int32_t* new_lens,
+                          int64_t* slots, int32_t* sequences, int64_t* positions, int64_t batch, int64_t tokens,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Draws a token per row of logits x from the distribution that temperature,
+ * top-k, top-p and min-p leave, with one given uniform number u per row.
+ * With M the largest logit, w_i = exp((x_i - M) / temperature) and tokens ranked
+ * by x (equal ones by index), a token is kept if all of these hold:
+ *   its rank is below top_k                               (top_k <= 0: no limit)
+ *   the tokens ranked before it have less than top_p of
+ *   the weight of those that top_k keeps                  (top_p >= 1: no limit)
+ *   w_i >= min_p                                          (min_p <= 0: no limit)
+ * (the first is always kept).  tokens[r] is the first i, in the order of the
+ * vocabulary, up to which the kept weights sum to more than u times their total;
+ * logprobs[r] (NULL: not wanted) the logarithm of w_i / total, as which it was
+ * drawn.  temperature <= 0 (or NaN): the first token of rank 0, logarithm 0.
+ * u is clamped to [0, 1 - 2^-24], NaN to 0.  -infinity and NaN have weight 0;
+ * where the largest logit is +infinity, those that are have weight 1 and others
+ * 0.  A row without any other logit than -infinity and NaN gets token -1 and
+ * logarithm -infinity.  Weights and sums are of 64 bits.
+ *
+ *   logits      [rows, row_stride] of dtype (fp32, fp16, bf16), vocab elements
+ *               of each row contiguous, any alignment.  vocab < 2^20.
+ *   uniform     fp32 [rows].   tokens int64 [rows].   logprobs fp32 [rows].
+ *   temperature, top_p, min_p (fp32 [rows]) and top_k (int32 [rows]): a setting
+ *               per row, or NULL: the *_all value for every row.
+ *   rows < 2^20, row_stride >= vocab.  workspace: as for
+ *   mi355_kv_cache_reserve_fwd, of mi355_sample_tokens_workspace bytes.
+ */
+int64_t mi355_sample_tokens_workspace(int64_t rows, int64_t vocab);
+int mi355_sample_tokens_fwd(const void* logits, const float* uniform, int64_t* tokens, float* logprobs,
+                            const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                            float temperature_all, int32_t top_k_all, float top_p_all, float min_p_all,
+                            int64_t rows, int64_t vocab, int64_t row_stride, int dtype,
+                            void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -40,6 +40,12 @@ fuse_attention=True)`` installs ``CachedAttention``, with which
 ``GraphedGreedyDecoder(..., kv_cache="int8")`` decodes over such a cache, and
 with ``draft_tokens=n`` verifies drafted trees.
 
+For several continuations of a prompt: ``kv_cache_reserve`` and ``kv_slot_map``
+(page tables and slot maps from the requests' lengths),
+``shared_prefix_attention`` (a prefix read and computed once for all sequences
+that share it) and ``sample_tokens`` (temperature, top-k, top-p and min-p from
+given random numbers).
+
 The kernels live in ``libmi355_fused.so`` (gfx950 HIP, C ABI in
 ``include/mi355_fused.h``), built by ``build.py``.
 """
@@ -52,8 +58,11 @@ from .kernels.fused_rmsnorm_hip import fused_add_rmsnorm, fused_rmsnorm, naive_r
 from .kernels.fused_gate_up_hip import GATE_UP_MAX_ROWS, fused_gate_up_silu, naive_gate_up_silu_reference
 from .kernels.fused_swiglu_hip import fused_silu_mul, naive_silu_mul_reference
 from .kernels.kv_cache_hip import KV_FORMATS, KVCache, kv_cache_append, kv_cache_keep, kv_cache_read
+from .kernels.kv_pages_hip import kv_cache_reserve, kv_slot_map
 from .kernels.linear16_hip import LINEAR16_MAX_ROWS, linear16
 from .kernels.rotary_hip import fused_rotary, rotary_frequencies
+from .kernels.sampling_hip import sample_tokens
+from .kernels.shared_prefix_hip import shared_prefix_attention
 from .kernels.tree_attention_hip import TREE_ATTENTION_MAX_TOKENS, tree_attention
 from .kernels.w8a16_matmul_hip import fused_gate_up_silu_w8a16, quantize_int8_weight, w8a16_linear, w8a16_reference
 from .quantization.int8 import QuantizedLinearInt8, quantize_model_int8
@@ -67,5 +76,5 @@ __all__ = [
     "fused_gate_up_silu_w8a16", "linear16", "LINEAR16_MAX_ROWS",
     "fused_rotary", "rotary_frequencies", "KVCache", "KV_FORMATS", "kv_cache_append", "kv_cache_read",
     "kv_cache_keep", "tree_attention", "TREE_ATTENTION_MAX_TOKENS", "CachedAttention", "DecoderCache",
-    "ATTENTION_CLASS_NAMES",
+    "ATTENTION_CLASS_NAMES", "kv_cache_reserve", "kv_slot_map", "shared_prefix_attention", "sample_tokens",
 ]

@@ -30,7 +30,10 @@ EXPORTED_SYMBOLS = ("mi355_abi_version", "mi355_last_error", "mi355_rmsnorm_fwd"
                     "mi355_w8a16_linear_workspace", "mi355_w8a16_linear_ws_fwd", "mi355_linear16_workspace",
                     "mi355_linear16_ws_fwd", "mi355_rotary_fwd", "mi355_kv_cache_append_fwd",
                     "mi355_kv_cache_read_fwd", "mi355_kv_cache_keep_fwd", "mi355_tree_attention_workspace",
-                    "mi355_tree_attention_fwd")
+                    "mi355_tree_attention_fwd", "mi355_shared_prefix_attention_workspace",
+                    "mi355_shared_prefix_attention_fwd", "mi355_kv_cache_reserve_workspace",
+                    "mi355_kv_cache_reserve_fwd", "mi355_kv_slot_map_workspace", "mi355_kv_slot_map_fwd",
+                    "mi355_sample_tokens_workspace", "mi355_sample_tokens_fwd")
 
 # cache formats of the C ABI (enum mi355_kv_format)
 KV_16BIT, KV_INT8, KV_E4M3 = 0, 1, 2
@@ -106,8 +109,21 @@ def _declare(L: ctypes.CDLL, path: Path) -> ctypes.CDLL:
     L.mi355_tree_attention_workspace.restype = i64
     L.mi355_tree_attention_fwd.argtypes = [cache, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, strides, f32, i32, vp,
                                            i64, vp]
+    L.mi355_shared_prefix_attention_workspace.argtypes = [cache, i64, i64, i64, i64]
+    L.mi355_shared_prefix_attention_fwd.argtypes = [cache, vp, vp, vp, vp, vp, vp, i64, vp, i64, i64, i64, i64, i64,
+                                                    strides, f32, i32, vp, i64, vp]
+    L.mi355_kv_cache_reserve_workspace.argtypes = [cache, i64]
+    L.mi355_kv_cache_reserve_fwd.argtypes = [cache, vp, vp, vp, i64, vp, i64, vp, i64, vp]
+    L.mi355_kv_slot_map_workspace.argtypes = [i64]
+    L.mi355_kv_slot_map_fwd.argtypes = [cache, vp, vp, vp, vp, vp, i64, i64, vp, i64, vp]
+    L.mi355_sample_tokens_workspace.argtypes = [i64, i64]
+    L.mi355_sample_tokens_fwd.argtypes = [*[vp] * 8, f32, ctypes.c_int32, f32, f32, i64, i64, i64, i32, vp, i64, vp]
+    for name in ("mi355_shared_prefix_attention_workspace", "mi355_kv_cache_reserve_workspace",
+                 "mi355_kv_slot_map_workspace", "mi355_sample_tokens_workspace"):
+        getattr(L, name).restype = i64
     for name in ("mi355_rotary_fwd", "mi355_kv_cache_append_fwd", "mi355_kv_cache_read_fwd",
-                 "mi355_kv_cache_keep_fwd", "mi355_tree_attention_fwd"):
+                 "mi355_kv_cache_keep_fwd", "mi355_tree_attention_fwd", "mi355_shared_prefix_attention_fwd",
+                 "mi355_kv_cache_reserve_fwd", "mi355_kv_slot_map_fwd", "mi355_sample_tokens_fwd"):
         getattr(L, name).restype = i32
     ver = L.mi355_abi_version()
     if ver != ABI_VERSION:

@@ -1,6 +1,7 @@
 // C ABI entry points of rotary positions, the key/value cache and attention
 // over it (include/mi355_fused.h): argument validation.  Kernels and their
-// launchers live in rotary.hip, kv_cache.hip and tree_attention.hip.
+// launchers live in rotary.hip, kv_cache.hip, kv_pages.hip, tree_attention.hip
+// and shared_prefix.hip.
 #include "kv_cache.h"
 #include "rotary.h"
 
@@ -20,6 +21,20 @@ int tree_attention_launch(const mi355_kv_cache& cache, const void* q, void* out,
                           const int32_t* new_lens, const uint8_t* mask, int64_t mask_b, int64_t mask_t, int64_t batch,
                           int tokens, int q_heads, const int64_t* q_strides, float scale, int dtype, void* work,
                           int64_t work_bytes, hipStream_t stream);
+int64_t shared_prefix_workspace(const mi355_kv_cache& cache, int64_t batch, int64_t tokens, int64_t q_heads,
+                                int64_t group_count);
+int shared_prefix_launch(const mi355_kv_cache& cache, const void* q, void* out, const int32_t* lens,
+                         const int32_t* new_lens, const int32_t* prefix_lens, const int32_t* groups, int group_count,
+                         const uint8_t* mask, int64_t mask_b, int64_t mask_t, int64_t batch, int tokens, int q_heads,
+                         const int64_t* q_strides, float scale, int dtype, void* work, int64_t work_bytes,
+                         hipStream_t stream);
+int64_t kv_reserve_workspace(const mi355_kv_cache& cache, int64_t batch);
+int kv_reserve_launch(const mi355_kv_cache& cache, const int32_t* lens, const int32_t* new_lens, int32_t* out,
+                      int64_t out_stride, int32_t* missing, int64_t batch, void* work, hipStream_t stream);
+int64_t kv_slot_map_workspace(int64_t batch);
+int kv_slot_map_launch(const mi355_kv_cache& cache, const int32_t* lens, const int32_t* new_lens, int64_t* slots,
+                       int32_t* sequences, int64_t* positions, int64_t batch, int64_t tokens, void* work,
+                       hipStream_t stream);
 
 }  // namespace mi355
 
@@ -212,19 +227,21 @@ MI355_EXPORT int64_t mi355_tree_attention_workspace(const mi355_kv_cache* cache,
   return mi355::tree_attention_workspace(*cache, batch, tokens, q_heads);
 }
 
-MI355_EXPORT int mi355_tree_attention_fwd(const mi355_kv_cache* cache, const void* q, void* out,
-                                          const int32_t* seq_lens, const int32_t* new_lens, const uint8_t* tree_mask,
-                                          int64_t mask_stride_b, int64_t mask_stride_t, int64_t batch, int64_t tokens,
-                                          int64_t q_heads, const int64_t* q_strides, float scale, int dtype,
-                                          void* workspace, int64_t workspace_bytes, void* stream) {
-  static const char* fn = "mi355_tree_attention_fwd";
-  mi355::clear_error();
+namespace {
+
+// What both attentions check.  *empty: nothing to do.
+int check_attention(const char* fn, const mi355_kv_cache* cache, const void* q, const void* out, const int32_t* seq_lens,
+                    const void* tree_mask, int64_t mask_stride_b, int64_t mask_stride_t, int64_t batch, int64_t tokens,
+                    int64_t q_heads, const int64_t* q_strides, int dtype, const void* workspace,
+                    int64_t workspace_bytes, bool* empty) {
+  *empty = false;
   int st = check_cache(fn, cache);
   if (st == MI355_OK) st = check_dtype16(fn, dtype);
   if (st != MI355_OK) return st;
   if (batch < 0 || tokens < 0 || q_heads < 0) return bad(fn, "sizes out of range");
   if (q_heads % cache->kv_heads != 0) return bad(fn, "q_heads must be a multiple of kv_heads");
-  if (batch == 0 || tokens == 0 || q_heads == 0) return MI355_OK;
+  *empty = batch == 0 || tokens == 0 || q_heads == 0;
+  if (*empty) return MI355_OK;
   if (tokens > 128 || q_heads > 65535 || !product_below(batch, tokens * q_heads, kMaxRows))
     return beyond(fn, "size beyond the kernel's limits (tokens <= 128, q_heads <= 65535, "
                       "batch * tokens * q_heads < 2^24)");
@@ -235,9 +252,127 @@ MI355_EXPORT int mi355_tree_attention_fwd(const mi355_kv_cache* cache, const voi
     return beyond(fn, "q and out must be 16-byte aligned, the strides of q multiples of 8");
   if (workspace != nullptr && (!aligned16(workspace) || workspace_bytes < 0))
     return bad(fn, "the workspace must be 16-byte aligned and its size >= 0");
-  st = check_pools(fn, cache);
-  if (st != MI355_OK) return st;
+  return check_pools(fn, cache);
+}
+
+// The page table alone, and a workspace that the call cannot do without.
+int check_pages(const char* fn, const mi355_kv_cache* cache, const void* workspace, int64_t workspace_bytes,
+                int64_t needs) {
+  if (cache->page_table == nullptr) return bad(fn, "null pointer in the cache");
+  if (cache->pages < 1 || cache->table_width < 1) return bad(fn, "a cache without pages");
+  if (needs > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < needs)) {
+    set_error("%s: the workspace must be 16-byte aligned and of %lld bytes", fn, static_cast<ll>(needs));
+    return MI355_ERR_INVALID;
+  }
+  return MI355_OK;
+}
+
+}  // namespace
+
+MI355_EXPORT int mi355_tree_attention_fwd(const mi355_kv_cache* cache, const void* q, void* out,
+                                          const int32_t* seq_lens, const int32_t* new_lens, const uint8_t* tree_mask,
+                                          int64_t mask_stride_b, int64_t mask_stride_t, int64_t batch, int64_t tokens,
+                                          int64_t q_heads, const int64_t* q_strides, float scale, int dtype,
+                                          void* workspace, int64_t workspace_bytes, void* stream) {
+  static const char* fn = "mi355_tree_attention_fwd";
+  mi355::clear_error();
+  bool empty;
+  const int st = check_attention(fn, cache, q, out, seq_lens, tree_mask, mask_stride_b, mask_stride_t, batch, tokens,
+                                 q_heads, q_strides, dtype, workspace, workspace_bytes, &empty);
+  if (st != MI355_OK || empty) return st;
   return mi355::tree_attention_launch(*cache, q, out, seq_lens, new_lens, tree_mask, mask_stride_b, mask_stride_t,
                                       batch, static_cast<int>(tokens), static_cast<int>(q_heads), q_strides, scale,
                                       dtype, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+MI355_EXPORT int64_t mi355_shared_prefix_attention_workspace(const mi355_kv_cache* cache, int64_t batch,
+                                                             int64_t tokens, int64_t q_heads, int64_t group_count) {
+  static const char* fn = "mi355_shared_prefix_attention_workspace";
+  mi355::clear_error();
+  if (check_cache(fn, cache) != MI355_OK || batch < 1 || tokens < 1 || tokens > 128 || q_heads < 1 ||
+      q_heads > 65535 || q_heads % cache->kv_heads != 0 || !product_below(batch, tokens * q_heads, kMaxRows) ||
+      group_count < 0 || group_count > batch)
+    return 0;
+  return mi355::shared_prefix_workspace(*cache, batch, tokens, q_heads, group_count);
+}
+
+MI355_EXPORT int mi355_shared_prefix_attention_fwd(
+    const mi355_kv_cache* cache, const void* q, void* out, const int32_t* seq_lens, const int32_t* new_lens,
+    const int32_t* prefix_lens, const int32_t* groups, int64_t group_count, const uint8_t* tree_mask,
+    int64_t mask_stride_b, int64_t mask_stride_t, int64_t batch, int64_t tokens, int64_t q_heads,
+    const int64_t* q_strides, float scale, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  static const char* fn = "mi355_shared_prefix_attention_fwd";
+  mi355::clear_error();
+  bool empty;
+  const int st = check_attention(fn, cache, q, out, seq_lens, tree_mask, mask_stride_b, mask_stride_t, batch, tokens,
+                                 q_heads, q_strides, dtype, workspace, workspace_bytes, &empty);
+  if (st != MI355_OK) return st;
+  if (group_count < 0 || group_count > batch) return bad(fn, "group_count must be in [0, batch]");
+  if (empty) return MI355_OK;
+  if (group_count > 0 && prefix_lens == nullptr) return bad(fn, "null pointer");
+  if (group_count > 0 && groups == nullptr && batch % group_count != 0)
+    return bad(fn, "without groups, batch must be a multiple of group_count");
+  return mi355::shared_prefix_launch(*cache, q, out, seq_lens, new_lens, prefix_lens, groups,
+                                     static_cast<int>(group_count), tree_mask, mask_stride_b, mask_stride_t, batch,
+                                     static_cast<int>(tokens), static_cast<int>(q_heads), q_strides, scale, dtype,
+                                     workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+namespace {
+bool reserve_fits(const mi355_kv_cache* c, int64_t batch) {
+  return batch < kMaxRows && c->pages < (int64_t{1} << 30) && product_below(batch, c->table_width, int64_t{1} << 31);
+}
+}  // namespace
+
+MI355_EXPORT int64_t mi355_kv_cache_reserve_workspace(const mi355_kv_cache* cache, int64_t batch) {
+  mi355::clear_error();
+  if (check_cache("mi355_kv_cache_reserve_workspace", cache) != MI355_OK || batch < 1 || !reserve_fits(cache, batch))
+    return 0;
+  return mi355::kv_reserve_workspace(*cache, batch);
+}
+
+MI355_EXPORT int mi355_kv_cache_reserve_fwd(const mi355_kv_cache* cache, const int32_t* seq_lens,
+                                            const int32_t* new_lens, int32_t* table_out, int64_t out_stride,
+                                            int32_t* missing, int64_t batch, void* workspace, int64_t workspace_bytes,
+                                            void* stream) {
+  static const char* fn = "mi355_kv_cache_reserve_fwd";
+  mi355::clear_error();
+  int st = check_cache(fn, cache);
+  if (st != MI355_OK) return st;
+  if (batch < 0 || out_stride < cache->table_width) return bad(fn, "sizes out of range (out_stride >= table_width)");
+  if (batch == 0) return MI355_OK;
+  if (!reserve_fits(cache, batch))
+    return beyond(fn, "size beyond the kernel's limits (batch < 2^24, batch * table_width < 2^31, pages < 2^30)");
+  if (seq_lens == nullptr || table_out == nullptr || missing == nullptr) return bad(fn, "null pointer");
+  if (table_out == cache->page_table && batch > 1 && out_stride != cache->table_stride)
+    return bad(fn, "in place, out_stride must be the table's");
+  st = check_pages(fn, cache, workspace, workspace_bytes, mi355::kv_reserve_workspace(*cache, batch));
+  if (st != MI355_OK) return st;
+  return mi355::kv_reserve_launch(*cache, seq_lens, new_lens, table_out, out_stride, missing, batch, workspace,
+                                  static_cast<hipStream_t>(stream));
+}
+
+MI355_EXPORT int64_t mi355_kv_slot_map_workspace(int64_t batch) {
+  mi355::clear_error();
+  return batch < 1 || batch >= kMaxRows ? 0 : mi355::kv_slot_map_workspace(batch);
+}
+
+MI355_EXPORT int mi355_kv_slot_map_fwd(const mi355_kv_cache* cache, const int32_t* seq_lens, const int32_t* new_lens,
+                                       int64_t* slots, int32_t* sequences, int64_t* positions, int64_t batch,
+                                       int64_t tokens, void* workspace, int64_t workspace_bytes, void* stream) {
+  static const char* fn = "mi355_kv_slot_map_fwd";
+  mi355::clear_error();
+  int st = check_cache(fn, cache);
+  if (st != MI355_OK) return st;
+  if (batch < 0 || tokens < 0) return bad(fn, "sizes out of range");
+  if (tokens == 0) return MI355_OK;
+  if (batch >= kMaxRows || tokens >= (int64_t{1} << 31))
+    return beyond(fn, "size beyond the kernel's limits (batch < 2^24, tokens < 2^31)");
+  if (batch < 1) return bad(fn, "tokens of no sequence");
+  if (seq_lens == nullptr || new_lens == nullptr || slots == nullptr || sequences == nullptr || positions == nullptr)
+    return bad(fn, "null pointer");
+  st = check_pages(fn, cache, workspace, workspace_bytes, mi355::kv_slot_map_workspace(batch));
+  if (st != MI355_OK) return st;
+  return mi355::kv_slot_map_launch(*cache, seq_lens, new_lens, slots, sequences, positions, batch, tokens, workspace,
+                                   static_cast<hipStream_t>(stream));
 }

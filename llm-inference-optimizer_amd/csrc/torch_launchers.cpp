@@ -641,44 +641,195 @@ void kv_keep(const at::Tensor& ck, const at::Tensor& cv, const at::Tensor& table
   }
 }
 
+// Attention's arguments as both operators take them.
+struct Attention {
+  Cache cache;
+  int dev, code;
+  Heads4 h;
+  at::Tensor lens, fresh, mask;
+  Attention(const at::Tensor& q, const at::Tensor& ck, const at::Tensor& cv, const at::Tensor& table,
+            const OptTensor& ks, const OptTensor& vs, const at::Tensor& seq_lens, const OptTensor& new_lens,
+            const OptTensor& tree_mask)
+      : cache(cache_of(ck, cv, table, ks, vs)), dev(ck.get_device()), code(check_new("q", q, cache, dev)),
+        h(heads4("q", q, true)) {
+    if (h.d != cache.c.head_dim || h.heads % std::max<int64_t>(1, cache.c.kv_heads) != 0)
+      fail_assert("q has " + std::to_string(h.heads) + " heads of " + std::to_string(h.d) + ", the cache " +
+                  std::to_string(cache.c.kv_heads) + " of " + std::to_string(cache.c.head_dim));
+    if (table.size(0) != h.batch)
+      fail_assert("page_table has " + std::to_string(table.size(0)) + " sequences, q " + std::to_string(h.batch));
+    lens = lengths("seq_lens", seq_lens, h.batch, dev);
+    if (has(new_lens)) fresh = lengths("new_lens", *new_lens, h.batch, dev);
+    if (has(tree_mask)) {
+      mask = *tree_mask;
+      const bool fits = (mask.dim() == 2 || (mask.dim() == 3 && (mask.size(0) == h.batch || mask.size(0) == 1))) &&
+                        mask.size(-1) == h.tokens && mask.size(-2) == h.tokens;
+      if (!(mask.is_cuda() && mask.get_device() == dev && mask.scalar_type() == at::kBool && fits))
+        fail_assert("tree_mask must be bool [tokens, tokens] or [batch, tokens, tokens] on q's device, got " +
+                    dtype_str(mask.scalar_type()) + " " + shape_str(mask.sizes()));
+      if (mask.dim() == 2) mask = mask.unsqueeze(0);
+      if (mask.numel() && mask.stride(2) != 1 && mask.size(2) != 1) mask = mask.contiguous();
+    }
+  }
+  const uint8_t* mask_ptr() const { return mask.defined() ? static_cast<const uint8_t*>(ptr(mask)) : nullptr; }
+  int64_t mask_b() const { return mask.defined() && mask.size(0) > 1 ? mask.stride(0) : 0; }
+  int64_t mask_t() const { return mask.defined() && mask.size(1) > 1 ? mask.stride(1) : 0; }
+};
+
 at::Tensor tree_attention(const at::Tensor& q, const at::Tensor& ck, const at::Tensor& cv, const at::Tensor& table,
                           const OptTensor& ks, const OptTensor& vs, const at::Tensor& seq_lens,
                           const OptTensor& new_lens, const OptTensor& tree_mask, double scale) {
-  const Cache cache = cache_of(ck, cv, table, ks, vs);
-  const int dev = ck.get_device();
-  const int code = check_new("q", q, cache, dev);
-  const Heads4 h = heads4("q", q, true);
-  if (h.d != cache.c.head_dim || h.heads % std::max<int64_t>(1, cache.c.kv_heads) != 0)
-    fail_assert("q has " + std::to_string(h.heads) + " heads of " + std::to_string(h.d) + ", the cache " +
-                std::to_string(cache.c.kv_heads) + " of " + std::to_string(cache.c.head_dim));
-  if (table.size(0) != h.batch)
-    fail_assert("page_table has " + std::to_string(table.size(0)) + " sequences, q " + std::to_string(h.batch));
-  const at::Tensor lens = lengths("seq_lens", seq_lens, h.batch, dev);
-  const at::Tensor fresh = has(new_lens) ? lengths("new_lens", *new_lens, h.batch, dev) : at::Tensor();
-  at::Tensor mask;
-  if (has(tree_mask)) {
-    mask = *tree_mask;
-    const bool fits = (mask.dim() == 2 || (mask.dim() == 3 && (mask.size(0) == h.batch || mask.size(0) == 1))) &&
-                      mask.size(-1) == h.tokens && mask.size(-2) == h.tokens;
-    if (!(mask.is_cuda() && mask.get_device() == dev && mask.scalar_type() == at::kBool && fits))
-      fail_assert("tree_mask must be bool [tokens, tokens] or [batch, tokens, tokens] on q's device, got " +
-                  dtype_str(mask.scalar_type()) + " " + shape_str(mask.sizes()));
-    if (mask.dim() == 2) mask = mask.unsqueeze(0);
-    if (mask.numel() && mask.stride(2) != 1 && mask.size(2) != 1) mask = mask.contiguous();
-  }
+  const Attention a(q, ck, cv, table, ks, vs, seq_lens, new_lens, tree_mask);
+  const Heads4& h = a.h;
   at::Tensor out = at::empty(q.sizes(), q.options());
   if (out.numel()) {
-    Launch l(dev);
-    const at::Tensor work = workspace(mi355_tree_attention_workspace(&cache.c, h.batch, h.tokens, h.heads), q);
+    Launch l(a.dev);
+    const at::Tensor work = workspace(mi355_tree_attention_workspace(&a.cache.c, h.batch, h.tokens, h.heads), q);
     check("mi355_tree_attention_fwd",
-          mi355_tree_attention_fwd(&cache.c, ptr(h.t), ptr(out), ints(lens), ints(fresh),
-                                   mask.defined() ? static_cast<const uint8_t*>(ptr(mask)) : nullptr,
-                                   mask.defined() && mask.size(0) > 1 ? mask.stride(0) : 0,
-                                   mask.defined() && mask.size(1) > 1 ? mask.stride(1) : 0, h.batch, h.tokens, h.heads,
-                                   h.strides, static_cast<float>(scale), code,
+          mi355_tree_attention_fwd(&a.cache.c, ptr(h.t), ptr(out), ints(a.lens), ints(a.fresh), a.mask_ptr(), a.mask_b(),
+                                   a.mask_t(), h.batch, h.tokens, h.heads, h.strides, static_cast<float>(scale), a.code,
                                    work.defined() ? ptr(work) : nullptr, work.defined() ? work.numel() : 0, l.stream));
   }
   return out;
+}
+
+at::Tensor shared_prefix_attention(const at::Tensor& q, const at::Tensor& ck, const at::Tensor& cv,
+                                   const at::Tensor& table, const OptTensor& ks, const OptTensor& vs,
+                                   const at::Tensor& seq_lens, const at::Tensor& prefix_lens, const OptTensor& groups,
+                                   const OptTensor& new_lens, const OptTensor& tree_mask, double scale) {
+  const Attention a(q, ck, cv, table, ks, vs, seq_lens, new_lens, tree_mask);
+  const Heads4& h = a.h;
+  if (prefix_lens.dim() != 1) fail_assert("prefix_lens must be int32 [groups], got " + shape_str(prefix_lens.sizes()));
+  const int64_t count = prefix_lens.size(0);
+  const at::Tensor prefix = lengths("prefix_lens", prefix_lens, count, a.dev);
+  if (count > h.batch)
+    fail_assert("prefix_lens has " + std::to_string(count) + " groups, the batch " + std::to_string(h.batch) + " sequences");
+  at::Tensor starts;
+  if (has(groups)) starts = lengths("groups", *groups, count + 1, a.dev);
+  else if (count > 0 && h.batch % count != 0)
+    fail_assert("without groups, the batch of " + std::to_string(h.batch) + " must be a multiple of the " +
+                std::to_string(count) + " prefix_lens");
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  if (out.numel()) {
+    Launch l(a.dev);
+    const at::Tensor work =
+        workspace(mi355_shared_prefix_attention_workspace(&a.cache.c, h.batch, h.tokens, h.heads, count), q);
+    check("mi355_shared_prefix_attention_fwd",
+          mi355_shared_prefix_attention_fwd(&a.cache.c, ptr(h.t), ptr(out), ints(a.lens), ints(a.fresh), ints(prefix),
+                                            ints(starts), count, a.mask_ptr(), a.mask_b(), a.mask_t(), h.batch,
+                                            h.tokens, h.heads, h.strides, static_cast<float>(scale), a.code,
+                                            work.defined() ? ptr(work) : nullptr, work.defined() ? work.numel() : 0,
+                                            l.stream));
+  }
+  return out;
+}
+
+// ------------------------------------------------- page tables from lengths
+
+// Scratch memory that a call cannot do without.
+at::Tensor scratch(int64_t bytes, const at::Tensor& like) {
+  return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : at::Tensor();
+}
+
+std::tuple<at::Tensor, at::Tensor> kv_reserve(const at::Tensor& ck, const at::Tensor& cv, const at::Tensor& table,
+                                              const OptTensor& ks, const OptTensor& vs, const at::Tensor& seq_lens,
+                                              const OptTensor& new_lens, const OptTensor& out) {
+  const Cache cache = cache_of(ck, cv, table, ks, vs);
+  const int dev = ck.get_device();
+  const int64_t batch = table.size(0), width = table.size(1);
+  const at::Tensor lens = lengths("seq_lens", seq_lens, batch, dev);
+  const at::Tensor fresh = has(new_lens) ? lengths("new_lens", *new_lens, batch, dev) : at::Tensor();
+  const at::Tensor to = has(out) ? *out : table;
+  if (!(to.is_cuda() && to.get_device() == dev && to.scalar_type() == at::kInt && to.sizes() == table.sizes()))
+    fail_assert("out must be int32 " + shape_str(table.sizes()) + " on the cache's device, got " +
+                dtype_str(to.scalar_type()) + " " + shape_str(to.sizes()));
+  if (to.numel() && ((width > 1 && to.stride(1) != 1) || (batch > 1 && to.stride(0) < width)))
+    fail_assert(std::string(has(out) ? "out" : "page_table") + " must have contiguous rows that do not overlap");
+  at::Tensor missing = at::empty({batch}, table.options());
+  if (batch) {
+    // a table that overlaps the old one in any other way than being it would be read half written
+    const bool same = ptr(to) == ptr(cache.table) && (batch == 1 || to.stride(0) == cache.table.stride(0));
+    Cache from = cache;
+    if (!same && to.is_alias_of(cache.table)) {
+      from.table = cache.table.clone(at::MemoryFormat::Contiguous);
+      from.c.page_table = static_cast<const int32_t*>(ptr(from.table));
+      from.c.table_stride = width;
+    }
+    Launch l(dev);
+    const at::Tensor work = scratch(mi355_kv_cache_reserve_workspace(&from.c, batch), table);
+    check("mi355_kv_cache_reserve_fwd",
+          mi355_kv_cache_reserve_fwd(&from.c, ints(lens), ints(fresh), static_cast<int32_t*>(ptr(to)),
+                                     batch > 1 ? to.stride(0) : width, static_cast<int32_t*>(ptr(missing)), batch,
+                                     work.defined() ? ptr(work) : nullptr, work.defined() ? work.numel() : 0, l.stream));
+  }
+  return {to, missing};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> kv_slot_map(const at::Tensor& ck, const at::Tensor& cv,
+                                                           const at::Tensor& table, const OptTensor& ks,
+                                                           const OptTensor& vs, const at::Tensor& seq_lens,
+                                                           const at::Tensor& new_lens, int64_t tokens) {
+  const Cache cache = cache_of(ck, cv, table, ks, vs);
+  const int dev = ck.get_device();
+  if (tokens < 0) fail_assert("tokens must be >= 0");
+  const int64_t batch = table.size(0);
+  const at::Tensor lens = lengths("seq_lens", seq_lens, batch, dev), fresh = lengths("new_lens", new_lens, batch, dev);
+  const auto wide = table.options().dtype(at::kLong);
+  at::Tensor slots = at::empty({tokens}, wide), owners = at::empty({tokens}, table.options());
+  at::Tensor positions = at::empty({tokens}, wide);
+  if (tokens) {
+    Launch l(dev);
+    const at::Tensor work = scratch(mi355_kv_slot_map_workspace(batch), table);
+    check("mi355_kv_slot_map_fwd",
+          mi355_kv_slot_map_fwd(&cache.c, ints(lens), ints(fresh), static_cast<int64_t*>(ptr(slots)),
+                                static_cast<int32_t*>(ptr(owners)), static_cast<int64_t*>(ptr(positions)), batch, tokens,
+                                work.defined() ? ptr(work) : nullptr, work.defined() ? work.numel() : 0, l.stream));
+  }
+  return {slots, owners, positions};
+}
+
+// ----------------------------------------------------------- drawing tokens
+
+std::tuple<at::Tensor, OptTensor> sample(const at::Tensor& logits, const at::Tensor& uniform,
+                                         const OptTensor& temperature, double temperature_all, const OptTensor& top_k,
+                                         int64_t top_k_all, const OptTensor& top_p, double top_p_all,
+                                         const OptTensor& min_p, double min_p_all, bool logprobs) {
+  if (!logits.is_cuda()) fail_assert("logits must be a ROCm GPU tensor");
+  const int code = code_of(logits.scalar_type());
+  if (code < 0) fail_assert("unsupported dtype logits=" + dtype_str(logits.scalar_type()) + " (fp16, bf16, fp32)");
+  if (logits.dim() < 1 || logits.size(-1) < 1) fail_assert("logits must be [..., vocab], got " + shape_str(logits.sizes()));
+  const int dev = logits.get_device();
+  const int64_t vocab = logits.size(-1);
+  const at::IntArrayRef shape = logits.sizes().slice(0, logits.dim() - 1);
+  const at::Tensor x = matrix_rows(logits, vocab);
+  const int64_t rows = x.size(0);
+  const auto per_row = [&](const char* what, const at::Tensor& t, at::ScalarType type) {
+    if (!(t.is_cuda() && t.get_device() == dev && t.scalar_type() == type && t.sizes() == shape))
+      fail_assert(std::string(what) + " must be " + dtype_str(type) + " " + shape_str(shape) +
+                  " on the logits' device, got " + dtype_str(t.scalar_type()) + " " + shape_str(t.sizes()));
+    return t.contiguous();
+  };
+  const at::Tensor u = per_row("uniform", uniform, at::kFloat);
+  at::Tensor heat, k, p, least;
+  if (has(temperature)) heat = per_row("temperature", *temperature, at::kFloat);
+  if (has(top_k)) k = per_row("top_k", *top_k, at::kInt);
+  if (has(top_p)) p = per_row("top_p", *top_p, at::kFloat);
+  if (has(min_p)) least = per_row("min_p", *min_p, at::kFloat);
+  at::Tensor tokens = at::empty(shape, logits.options().dtype(at::kLong));
+  OptTensor logs;
+  if (logprobs) logs = at::empty(shape, logits.options().dtype(at::kFloat));
+  const auto floats = [](const at::Tensor& t) { return t.defined() ? static_cast<const float*>(ptr(t)) : nullptr; };
+  if (rows) {
+    Launch l(dev);
+    const at::Tensor work = scratch(mi355_sample_tokens_workspace(rows, vocab), logits);
+    const int32_t all = static_cast<int32_t>(std::min<int64_t>(std::max<int64_t>(top_k_all, 0), vocab));
+    check("mi355_sample_tokens_fwd",
+          mi355_sample_tokens_fwd(ptr(x), floats(u), static_cast<int64_t*>(ptr(tokens)),
+                                  logprobs ? static_cast<float*>(ptr(*logs)) : nullptr, floats(heat), ints(k), floats(p),
+                                  floats(least), static_cast<float>(temperature_all), all, static_cast<float>(top_p_all),
+                                  static_cast<float>(min_p_all), rows, vocab, rows > 1 ? x.stride(0) : vocab, code,
+                                  work.defined() ? ptr(work) : nullptr, work.defined() ? work.numel() : 0, l.stream));
+  }
+  return {tokens, logs};
 }
 
 }  // namespace
@@ -711,4 +862,14 @@ PYBIND11_MODULE(_mi355_torch, m) {
   m.def("tree_attention", &tree_attention, py::arg("q"), py::arg("cache_k"), py::arg("cache_v"),
         py::arg("page_table"), py::arg("k_scale"), py::arg("v_scale"), py::arg("seq_lens"), py::arg("new_lens"),
         py::arg("tree_mask"), py::arg("scale"));
+  m.def("shared_prefix_attention", &shared_prefix_attention, py::arg("q"), py::arg("cache_k"), py::arg("cache_v"),
+        py::arg("page_table"), py::arg("k_scale"), py::arg("v_scale"), py::arg("seq_lens"), py::arg("prefix_lens"),
+        py::arg("groups"), py::arg("new_lens"), py::arg("tree_mask"), py::arg("scale"));
+  m.def("kv_reserve", &kv_reserve, py::arg("cache_k"), py::arg("cache_v"), py::arg("page_table"), py::arg("k_scale"),
+        py::arg("v_scale"), py::arg("seq_lens"), py::arg("new_lens"), py::arg("out"));
+  m.def("kv_slot_map", &kv_slot_map, py::arg("cache_k"), py::arg("cache_v"), py::arg("page_table"), py::arg("k_scale"),
+        py::arg("v_scale"), py::arg("seq_lens"), py::arg("new_lens"), py::arg("tokens"));
+  m.def("sample", &sample, py::arg("logits"), py::arg("uniform"), py::arg("temperature"), py::arg("temperature_all"),
+        py::arg("top_k"), py::arg("top_k_all"), py::arg("top_p"), py::arg("top_p_all"), py::arg("min_p"),
+        py::arg("min_p_all"), py::arg("logprobs"));
 }

@@ -455,7 +455,8 @@ int mi355_tree_attention_fwd(const mi355_kv_cache* cache, const void* q, void* o
  * [0, batch]; of descending ones, the first group that fits is taken.
  *
  * The other arguments, limits and rules (masks, padding, infinities) are those
- * of mi355_tree_attention_fwd, the workspace's too.
+ * of mi355_tree_attention_fwd.  Without a workspace of the size asked for, a wave
+ * computes each query row by itself: right, and slow.
  */
 int64_t mi355_shared_prefix_attention_workspace(const mi355_kv_cache* cache, int64_t batch, int64_t tokens,
                                                 int64_t q_heads, int64_t group_count);

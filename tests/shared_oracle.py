@@ -9,10 +9,12 @@ from kv_oracle import cpu
 
 
 def members(batch, count, groups):
-    """[(first, size)] of the groups."""
+    """[(first, size)] of the groups; a boundary below an earlier one counts as that one."""
     if groups is None:
         return [(g * (batch // count), batch // count) for g in range(count)] if count else []
-    at = [max(0, min(int(g), batch)) for g in groups]
+    at = []
+    for g in groups:
+        at.append(max([max(0, min(int(g), batch)), *at]))
     return [(at[g], at[g + 1] - at[g]) for g in range(count)]
 
 

@@ -6,18 +6,34 @@
 
 namespace mi355 {
 
+// How a stretch of slots is worked on.  Up to 16 SM query rows: every wave takes
+// tiles of 32 slots for itself.  More: the waves take 16 MT rows each and share
+// tiles of 16 slots per wave through LDS.
+constexpr int kWaveSlots = 32;
+
+// What the line counts for a tile and, the first `pad` of it, for a piece's other
+// work: queries, first loads, sums to write and join.
+struct SharedCost {
+  int tile, pad;
+};
+
 struct SharedArgs {
-  TreeArgs t;             // lens, queries, mask, page numbers; partial, stats, starts of the pieces that are cut
+  TreeArgs t;             // lens, queries, mask, page numbers; partial and stats of the pieces that are cut
   const int32_t* prefix;  // [groups]
   const int32_t* bounds;  // [groups + 1], ascending: where groups begin; null: every `even` sequences
-  const int32_t* first;   // [batch]: the first sequence of a sequence's group, with bounds
-  const int32_t* shared;  // [batch]: its shared slots, with bounds
+  const int32_t* shared;  // [batch]: a sequence's shared slots, with bounds
   float* whole;           // [2][rows][d]: what one workgroup has of a prefix, of own slots
   float2* whole_stats;    // [2][rows]
+  int2* pieces;           // [2][rows]: where a row's first piece is, and how many there are
   int groups, even;
   int rows;               // of all sequences: batch tokens q_heads
   int mt_rows;            // tokens group: rows of a sequence and key/value head
+  int block_log;          // log2 of the rows of a block
+  int few;                // rows that every wave takes for itself
+  SharedCost many_cost, few_cost;
+  int least;              // a share has at least this
   uint32_t seq_mul, seq_shift, group_mul, group_shift;  // n / mt_rows = n * seq_mul >> seq_shift, likewise group
+  uint32_t even_mul, even_shift;
 };
 
 __device__ __forceinline__ int divide(int n, uint32_t mul, uint32_t shift) {
@@ -35,104 +51,119 @@ struct Lengths {
   }
 };
 
-// Slots that sequence b shares, and with whom, by lane.
-__device__ __forceinline__ int shared_of(const SharedArgs& a, int b, int len, int* first) {
-  *first = b;
-  if (a.bounds) {
-    *first = a.first[b];
-    return a.shared[b];
-  }
-  if (a.groups == 0) return 0;
-  const int g = b / a.even;
-  *first = g * a.even;
-  return max(0, min(a.prefix[g], len));
-}
-
 // A stretch of slots that some rows attend to: the prefix of group v, or the own
-// slots of sequence v - groups.  `tiles` per head and row block.
+// slots of sequence v - groups.
 struct Stretch {
-  int first, begin, end, rows, tiles, blocks;  // first: the sequence of row 0, whose page table counts
-  __device__ __forceinline__ int size(const TreeArgs& a) const { return tiles ? a.c.heads * blocks * (tiles + a.pad) : 0; }
+  int first, begin, end, rows;  // first: the sequence of row 0, whose page table counts
+  int base, slots;              // tiles of `slots` slots from `base` on, a multiple of 16
+  int tiles, blocks;            // per head and row block
+  SharedCost cost;
+  __device__ __forceinline__ int piece() const { return cost.pad + tiles * cost.tile; }
+  __device__ __forceinline__ int size(const TreeArgs& a) const { return tiles ? a.c.heads * blocks * piece() : 0; }
 };
-__device__ __forceinline__ Stretch stretch_of(const SharedArgs& s, int v) {
+
+// Reads stretch v with LOAD(pointer, index): vector loads of a lane's, all on
+// their way at once, or scalar ones.
+template <typename LOAD> __device__ __forceinline__ Stretch stretch_of(const SharedArgs& s, int v, const LOAD& load) {
   const TreeArgs& a = s.t;
-  Stretch r;
-  if (v < s.groups) {
-    const int g0 = s.bounds ? s.bounds[v] : v * s.even;
-    const int g1 = s.bounds ? s.bounds[v + 1] : g0 + s.even;
-    r.first = g0;
-    r.begin = 0;
-    r.end = max(0, min(s.prefix[v], a.c.capacity()));
-    r.rows = (g1 - g0) * s.mt_rows;
-    r.tiles = r.rows ? (r.end + a.tile - 1) / a.tile : 0;
-  } else {
-    const int b = v - s.groups;
-    const Lengths n(a, a.lens[b], a.new_lens ? a.new_lens[b] : a.tokens);
-    int first;
-    r.first = b;
-    r.begin = shared_of(s, b, n.len, &first);
-    r.end = n.end;
-    r.rows = s.mt_rows;
-    r.tiles = n.fresh && r.end > r.begin ? (r.end + a.tile - 1) / a.tile - r.begin / a.tile : 0;
+  const bool group = v < s.groups;
+  const int b = group ? 0 : v - s.groups;
+  const int g = group ? v : s.groups && !s.bounds ? divide(b, s.even_mul, s.even_shift) : 0;
+  const int len = load(a.lens, b), fresh = a.new_lens ? load(a.new_lens, b) : a.tokens;
+  const int prefix = s.groups ? load(s.prefix, g) : 0;
+  int g0 = g * s.even, g1 = g0 + s.even, shared = prefix;
+  if (s.bounds) {
+    g0 = load(s.bounds, g);
+    g1 = load(s.bounds, g + 1);
+    shared = load(s.shared, b);
   }
-  r.blocks = (r.rows + a.block_rows - 1) / a.block_rows;
+  const Lengths n(a, len, fresh);
+  Stretch r;
+  r.first = group ? g0 : b;
+  r.begin = group ? 0 : max(0, min(shared, n.len));
+  r.end = group ? max(0, min(prefix, a.c.capacity())) : n.end;
+  r.rows = group ? (g1 - g0) * s.mt_rows : s.mt_rows;
+  const bool few = r.rows <= s.few;
+  const int log = few ? 7 : 6;  // of the slots of a tile
+  static_assert(kWaves * kWaveSlots == 128 && kWaves * 16 == 64, "");
+  r.cost = few ? s.few_cost : s.many_cost;
+  r.base = r.begin & ~15;
+  r.slots = 1 << log;
+  const bool any = (group ? r.rows > 0 : n.fresh > 0) && r.end > r.begin;
+  r.tiles = any ? (r.end - r.base + r.slots - 1) >> log : 0;
+  r.blocks = few ? 1 : (r.rows + (1 << s.block_log) - 1) >> s.block_log;
   return r;
+}
+__device__ __forceinline__ Stretch lane_stretch(const SharedArgs& s, int v) {
+  return stretch_of(s, v, [](const int32_t* p, int i) { return p[i]; });
 }
 
 // A workgroup's share [at, last) of the line, piece by piece, in scalar
-// registers.  The first `pad` tiles of a piece stand for what it costs beside
-// its tiles.
+// registers.  A tile is in the share that its first unit is in.
 struct SharedShare {
   int at, last, first, size, place, count;
   int v, start;  // the stretch at hand and where it begins
-  // one piece: tiles [t0, t1) of rows row0 .. row0 + rows - 1
+  // one piece: tiles of slots [from, stop) for rows row0 .. row0 + rows - 1
   Stretch w;
-  int h, row0, rows, t0, t1, stop, width;
-  bool prefix, cut;
+  int h, row0, rows, from, stop, tiles, width;
+  int pieces;  // of the rows of a piece that begins here
+  bool prefix, few, cut, begins;
   const int32_t* table;
+
+  static constexpr int kHeld = 4;  // chunks of 64 stretches whose sizes stay in registers
 
   __device__ __forceinline__ explicit SharedShare(const SharedArgs& s) {
     const TreeArgs& a = s.t;
     const int lane = threadIdx.x & 63;
     count = s.groups + a.batch;
-    int total = 0;
-    int mine = 0;  // of the first 64 stretches, up to this lane's
-    for (int v0 = 0; v0 < count; v0 += 64) {
-      const int upto = wave_scan(v0 + lane < count ? stretch_of(s, v0 + lane).size(a) : 0);
-      if (v0 == 0) mine = upto;
-      total += __builtin_amdgcn_readlane(upto, 63);
+    int total = 0, held[kHeld];
+    const auto chunk = [&](int v0) {  // the running sum of 64 sizes
+      const int size = lane_stretch(s, min(v0 + lane, count - 1)).size(a);
+      return wave_scan(v0 + lane < count ? size : 0);
+    };
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      held[i] = 0;
+      if (64 * i < count) held[i] = chunk(64 * i);
     }
-    size = uniform(max(1, (total + a.grid - 1) / a.grid));
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) total += __builtin_amdgcn_readlane(held[i], 63);
+    for (int v0 = 64 * kHeld; v0 < count; v0 += 64) total += __builtin_amdgcn_readlane(chunk(v0), 63);
+    size = uniform(max(s.least, (total + a.grid - 1) / a.grid));
     place = uniform(line_place(a, blockIdx.x));
     at = first = uniform(min(place * size, total));
     last = uniform(min(at + size, total));
     v = count;
     start = total;
+    if (at == last) return;
     int before = 0;
-    for (int v0 = 0; v0 < count; v0 += 64) {
-      const int upto = before + (v0 ? wave_scan(v0 + lane < count ? stretch_of(s, v0 + lane).size(a) : 0) : mine);
-      if (blockIdx.x == 0 && threadIdx.x < 64 && v0 + lane < count) a.starts[1 + v0 + lane + 1] = upto;
-      const uint64_t past = __builtin_amdgcn_ballot_w64(upto > at);
-      if (past && v == count) {
+    const auto look = [&](int v0, int sum) {
+      const uint64_t past = __builtin_amdgcn_ballot_w64(before + sum > at);
+      if (past) {
         const int i = uniform(__builtin_ctzll(past));
-        start = uniform(i ? __builtin_amdgcn_readlane(upto, i - 1) : before);
+        start = uniform(before + (i ? __builtin_amdgcn_readlane(sum, i - 1) : 0));
         v = uniform(v0 + i);
-        if (blockIdx.x != 0) break;
       }
-      before = __builtin_amdgcn_readlane(upto, 63);
-    }
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-      a.starts[0] = size;
-      a.starts[1] = 0;
-    }
-    if (v < count) w = scalar_stretch(s, v);
+      before += __builtin_amdgcn_readlane(sum, 63);
+      return past != 0;
+    };
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (!found) found = look(64 * i, held[i]);
+    for (int v0 = 64 * kHeld; !found && v0 < count; v0 += 64) found = look(v0, chunk(v0));
+    w = scalar_stretch(s, v);
   }
   static __device__ __forceinline__ Stretch scalar_stretch(const SharedArgs& s, int v) {
-    Stretch r = stretch_of(s, v);
+    Stretch r = stretch_of(s, v, [](const int32_t* p, int i) { return scalar_load(p, i); });
     r.first = uniform(r.first);
     r.begin = uniform(r.begin);
     r.end = uniform(r.end);
     r.rows = uniform(r.rows);
+    r.base = uniform(r.base);
+    r.slots = uniform(r.slots);
+    r.cost.tile = uniform(r.cost.tile);
+    r.cost.pad = uniform(r.cost.pad);
     r.tiles = uniform(r.tiles);
     r.blocks = uniform(r.blocks);
     return r;
@@ -140,7 +171,7 @@ struct SharedShare {
   __device__ __forceinline__ bool next(const SharedArgs& s) {
     const TreeArgs& a = s.t;
     while (v < count && at < last) {
-      const int piece = w.tiles + a.pad;
+      const int piece = w.piece();
       const int hm = w.tiles ? uniform((at - start) / piece) : 0;
       if (w.tiles == 0 || hm >= a.c.heads * w.blocks) {
         start = uniform(start + w.size(a));
@@ -150,30 +181,39 @@ struct SharedShare {
       }
       const int v0 = uniform(at - start - hm * piece), v1 = uniform(min(piece, v0 + last - at));
       width = v1 - v0;
-      t0 = max(0, v0 - a.pad);
-      t1 = v1 - a.pad;
-      if (t1 <= t0) {  // the share ends before the piece's first tile
+      const int c = w.cost.tile;
+      const int t0 = uniform(max(0, v0 - w.cost.pad + c - 1) / c), t1 = uniform(max(0, v1 - w.cost.pad + c - 1) / c);
+      if (t1 <= t0) {  // no tile begins in this part
         done();
         continue;
       }
       cut = t0 > 0 || t1 < w.tiles;
+      begins = t0 == 0;
+      pieces = cut ? uniform((start + (hm + 1) * piece - c) / size) - place + 1 : 1;
       h = uniform(hm / w.blocks);
-      row0 = uniform((hm - h * w.blocks) * a.block_rows);
-      rows = uniform(min(a.block_rows, w.rows - row0));
+      row0 = uniform((hm - h * w.blocks) << s.block_log);
+      few = w.rows <= s.few;
+      rows = uniform(few ? w.rows : min(1 << s.block_log, w.rows - row0));
       prefix = v < s.groups;
-      const int base = w.begin / a.tile;  // own tiles begin where the prefix ends
-      t0 = uniform(t0 + base);
-      t1 = uniform(t1 + base);
-      stop = uniform(min(w.end, t1 * a.tile));
+      tiles = t1 - t0;
+      from = uniform(w.base + t0 * w.slots);
+      stop = uniform(min(w.end, w.base + t1 * w.slots));
       table = a.c.table + static_cast<int64_t>(w.first) * a.c.table_stride;
       return true;
     }
     return false;
   }
-  // where a piece that is cut goes in the workspace
-  __device__ __forceinline__ int64_t slot() const { return 2 * static_cast<int64_t>(place) + (at == first ? 0 : 1); }
+  // where a piece that is cut goes in the workspace; the pieces behind a row's
+  // first are the first of the workgroups that follow
+  __device__ __forceinline__ int slot() const { return 2 * place + (at == first ? 0 : 1); }
   __device__ __forceinline__ void done() { at = uniform(at + width); }
 };
+
+// The slots that sequence b shares, by lane.
+__device__ __forceinline__ int shared_of(const SharedArgs& s, int b, int len) {
+  if (s.bounds) return s.shared[b];
+  return s.groups ? max(0, min(s.prefix[divide(b, s.even_mul, s.even_shift)], len)) : 0;
+}
 
 // A query row of a piece, by lane.
 struct SharedRow {
@@ -193,8 +233,7 @@ struct SharedRow {
     const Lengths n(a, a.lens[b], a.new_lens ? a.new_lens[b] : a.tokens);
     len = n.len;
     fresh = r < p.rows ? n.fresh : 0;
-    int first;
-    limit = !p.prefix ? n.len : t < fresh ? shared_of(s, b, n.len, &first) : kAll;
+    limit = !p.prefix ? n.len : t < fresh ? shared_of(s, b, n.len) : kAll;
   }
   __device__ __forceinline__ int64_t out_row(const TreeArgs& a) const {
     return (static_cast<int64_t>(b) * a.tokens + t) * a.q_heads + hq;
@@ -259,16 +298,16 @@ __device__ __forceinline__ void shared_queries(const TreeArgs& a, const SharedRo
 // set_non_finite of the tree's attention has it); acc row 0 is row r0.  Rare.
 template <typename T, int FMT, int PITCH>
 __device__ __forceinline__ void set_shared_non_finite(const SharedArgs& s, const SharedShare& p, float (*acc)[PITCH], int r0,
-                                                      int r1, int first, int step, int slots) {
+                                                      int r1, int first, int step, int slots) {  // slots first .. + slots - 1, first + step .., ..
   const TreeArgs& a = s.t;
 #pragma unroll 1
   for (int e = threadIdx.x & 63; e < a.c.d; e += 64) {
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {  // what the product left goes first
 #pragma unroll 1
-      for (int tile = first; tile * slots < p.stop; tile += step) {
+      for (int tile = first; tile < p.stop; tile += step) {
 #pragma unroll 1
-        for (int slot = tile * slots; slot < min((tile + 1) * slots, p.stop); ++slot) {
+        for (int slot = tile; slot < min(tile + slots, p.stop); ++slot) {
           const int64_t at = a.c.row(p.w.first, slot, p.h);
           if (at < 0) continue;
           float v;

@@ -2,17 +2,42 @@
 // one given uniform number, for gfx950.
 //
 // Tokens are ranked by their logit, equal ones by index; what the filters keep is
-// a beginning of that order: all above a threshold and the first few equal to
-// it.  The threshold is found digit by digit from histograms of the logits as
-// ordered integers -- of counts for top-k, of weights for top-p, these as integer
-// multiples of 2^-43, whose sums do not depend on the order of the atomics.
+// a beginning of that order, told by its last token: a threshold of logits and,
+// among those equal to it, of indexes.
+//
+//   w_i = 2^((x_i - M) log2 e / T),   M the largest logit
+//
+// Weights and sums have 64 bits: a token next to the border of the cumulated
+// weights has to fall on the right side of it, whatever the order of the sums; in
+// 32 bits one draw in a hundred from 150000 tokens would not.
+//
+// sample_parts reads the logits once, in parts of 4096 on all compute units: each
+// part's largest logit and sum of weights, the largest logit of each block of
+// 512, and, for rows with filters, how many tokens and how much weight a part has
+// in bins a quarter of a power of 2 wide.  Then a workgroup per row draws: without
+// filters (sample_plain) from the part that the number falls into; with them
+// (sample_rows) it finds the bin that a threshold lies in, sorts that bin's tokens
+// (or those of a 256th of it), and adds the kept weights of the blocks.  Blocks
+// whose largest logit is below a threshold are not read again.
 #include "common.h"
 
 namespace mi355 {
 namespace {
 
-constexpr int kBlock = 1024, kBlockWaves = kBlock / 64;
+constexpr int kPart = 4096, kBlock = 512, kPartBlocks = kPart / kBlock;
+constexpr int kPartThreads = 256, kRowThreads = 1024, kRowWaves = kRowThreads / 64;
+constexpr int kBins = 256;          // the last holds all that is further down
+constexpr int kListed = 2048;       // tokens that a row's workgroup sorts
+constexpr int64_t kChunk = 1024;    // rows whose parts the workspace holds
+constexpr double kBinUnit = 524288.0;  // 2^19: the weights of a part's bin, largest 1 each, fit 32 bits
 constexpr double kUnit = 8796093022208.0;  // 2^43: sums of 2^20 weights fit 64 bits
+constexpr float kHottest = 1e30f;   // temperatures beyond (infinity) have no weight range to clamp to
+
+struct Part {
+  float top;   // largest logit; -infinity: nothing to draw
+  int32_t q;   // its bin
+  double sum;  // of weights relative to it
+};
 
 struct SampleArgs {
   const void* logits;
@@ -25,230 +50,828 @@ struct SampleArgs {
   float temperature_all;
   int32_t top_k_all;
   float top_p_all, min_p_all;
-  int64_t rows, stride;
-  int vocab;
+  int64_t row0, rows, stride;  // of a chunk
+  int vocab, parts;
+  bool aligned;                // rows start on 16 bytes
+  Part* part;                  // [rows][parts]
+  float* block_top;            // [rows][parts * kPartBlocks]
+  uint64_t* bins;              // [rows][parts][kBins]: count << 32 | weight
 };
 
-// Logits as integers in their order; those that are never drawn are 0.
-__device__ __forceinline__ uint32_t key_of(float x) {
-  if (!(x > -INFINITY)) return 0;
-  const uint32_t b = as_u32(x + 0.f);  // -0 counts as 0
+struct Settings {
+  float heat, top_p, min_p;
+  int top_k;
+  double c;  // log2 e / T
+  bool greedy, by_count, by_weight, by_least;
+  __device__ __forceinline__ Settings(const SampleArgs& a, int64_t row) {
+    heat = a.temperature ? a.temperature[row] : a.temperature_all;
+    top_k = a.top_k ? a.top_k[row] : a.top_k_all;
+    top_p = a.top_p ? a.top_p[row] : a.top_p_all;
+    min_p = a.min_p ? a.min_p[row] : a.min_p_all;
+    greedy = !(heat > 0.f);
+    c = 1.4426950408889634074 / static_cast<double>(heat);
+    by_count = !greedy && top_k > 0 && top_k < a.vocab;
+    by_weight = !greedy && top_p < 1.f;
+    by_least = !greedy && min_p > 0.f;
+  }
+  __device__ __forceinline__ bool filters() const { return by_count || by_weight || by_least; }
+  // The bin of a logit: a monotone function of it alone, a quarter of a power of 2 of
+  // weight wide.
+  __device__ __forceinline__ int bin(float x) const {
+    return static_cast<int>(fminf(fmaxf(floorf(height(x)), -1e9f), 1e9f));
+  }
+  __device__ __forceinline__ float height(float x) const { return x * (4.f * static_cast<float>(c)); }
+  // Which 256th of its bin: monotone too, as nothing but the product is rounded.
+  __device__ __forceinline__ int fine(float x) const {
+    const float y = height(x);
+    return min(static_cast<int>((y - floorf(y)) * 256.f), 255);  // NaN of an infinite height: 0
+  }
+};
+
+// 2^t for -1000 <= t <= 1/2: the polynomial of degree 9 that meets 2^f at the
+// Chebyshev nodes of [-1/2, 1/2], off by 1.9e-14 of it at most.
+__device__ __forceinline__ double exp2_64(double t) {
+  const double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are t, rounded
+  const double s = t + magic;
+  const double f = t - (s - magic);
+  double p = 1.0205905413765595e-07;
+  p = __builtin_fma(p, f, 1.325964524488711e-06);
+  p = __builtin_fma(p, f, 1.5252672924850737e-05);
+  p = __builtin_fma(p, f, 0.0001540343375125101);
+  p = __builtin_fma(p, f, 0.0013333558200794592);
+  p = __builtin_fma(p, f, 0.009618129193934313);
+  p = __builtin_fma(p, f, 0.05550410866465167);
+  p = __builtin_fma(p, f, 0.2402265069564034);
+  p = __builtin_fma(p, f, 0.6931471805599462);
+  p = __builtin_fma(p, f, 1.0000000000000135);
+  const uint64_t n = __builtin_bit_cast(uint64_t, s) << 52;
+  return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) + n);
+}
+
+// Weights relative to a largest logit.  A weight below 2^-1000 counts as that: next
+// to the largest, 1, it is nothing in 64 bits.  Only `exact` says whether there is
+// a weight at all.
+struct Weights {
+  double top, c, least;  // least: of x - top
+  float top32;
+  bool plain;
+  __device__ __forceinline__ Weights(const Settings& s, float top_) {
+    top32 = top_;
+    top = top_;
+    c = s.c;
+    least = -1000.0 / c;
+    plain = top_ < INFINITY && s.heat <= kHottest;
+  }
+  __device__ __forceinline__ double fast(float x) const {
+    return exp2_64(fmax(static_cast<double>(x) - top, least) * c);
+  }
+  __device__ __forceinline__ double exact(float x) const {
+    if (!(x > -INFINITY)) return 0.;
+    if (top32 == INFINITY) return x == INFINITY ? 1. : 0.;
+    const double t = (static_cast<double>(x) - top) * c;
+    return t < -1000. ? 0. : exp2_64(t);
+  }
+};
+
+__device__ __forceinline__ uint32_t key_of(float x) {  // in the logits' order; -0 counts as 0
+  const uint32_t b = as_u32(x + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t key) {
   return as_f32(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-template <typename V> __device__ __forceinline__ V block_sum(V v, V* part) {
+// Logits of block `block` of a row: 8 per lane, -infinity beyond the vocabulary and
+// for NaN.  index(e): their tokens.
+template <typename T> struct Block {
+  static constexpr int W = pack_width<T>::value;  // consecutive
+  float x[8];
+  int first;
+  static __device__ __forceinline__ int place(int e) {  // of element e, from the block's beginning
+    const int lane = threadIdx.x & 63;
+    return e / W * 64 * W + lane * W + e % W;
+  }
+  u32x4 raw[8 / W];
+  bool packets;  // whole ones: not a last one that ends within
+  __device__ __forceinline__ void load(const SampleArgs& a, int64_t row, int block) {
+    first = block * kBlock;
+    const typename T::bits* p = static_cast<const typename T::bits*>(a.logits) + row * a.stride;
+    packets = a.aligned && (first + kBlock <= a.vocab || a.vocab % W == 0);
+    if (packets) {
+      const rsrc_t r = make_rsrc(p, static_cast<uint32_t>(a.vocab) * sizeof(typename T::bits));
+#pragma unroll
+      for (int i = 0; i < 8 / W; ++i)
+        raw[i] = buf_load16_cached(r, static_cast<uint32_t>((first + place(W * i)) * sizeof(typename T::bits)));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = load_elem<T>(p, min(first + place(e), a.vocab - 1));
+    }
+  }
+  __device__ __forceinline__ void take(const SampleArgs& a) {
+    if (packets) {
+#pragma unroll
+      for (int i = 0; i < 8 / W; ++i) {
+        Packet<T> k{raw[i]};
+        float f[W];
+        k.unpack(f);
+#pragma unroll
+        for (int e = 0; e < W; ++e) x[W * i + e] = f[e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = fmaxf(x[e], -INFINITY);  // NaN
+    if (first + kBlock > a.vocab) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = first + place(e) < a.vocab ? x[e] : -INFINITY;
+    }
+  }
+  __device__ __forceinline__ int index(int e) const { return first + place(e); }
+};
+
+__device__ __forceinline__ float wave_max(float v) {
+  for (int m = 32; m; m >>= 1) v = fmaxf(v, __shfl_xor(v, m));
+  return v;
+}
+__device__ __forceinline__ double wave_sum(double v) {
   for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+  return v;
+}
+
+template <typename T> __global__ __launch_bounds__(kPartThreads) void sample_parts(SampleArgs a) {
+  constexpr int WAVES = kPartThreads / 64, OWN = kPartBlocks / WAVES;  // blocks of a wave
+  __shared__ unsigned long long bins[kBins];
+  __shared__ float tops[WAVES];
+  __shared__ double sums[WAVES];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  {
+    const int64_t item = blockIdx.x, r = item / a.parts, row = a.row0 + r;
+    const int part = static_cast<int>(item - r * a.parts);
+    Block<T> b[OWN];
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) b[i].load(a, row, part * kPartBlocks + wave * OWN + i);
+    const Settings s(a, row);
+    const bool filters = s.filters();
+    if (filters) bins[threadIdx.x] = 0;
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+      b[i].take(a);
+      float most = b[i].x[0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) most = fmaxf(most, b[i].x[e]);
+      most = wave_max(most);
+      if (lane == 0) a.block_top[(r * a.parts + part) * kPartBlocks + wave * OWN + i] = most;
+      top = fmaxf(top, most);
+    }
+    if (lane == 0) tops[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, tops[w]);
+    const int q = s.bin(top);
+    double sum = 0.;
+    if (!s.greedy && top > -INFINITY) {
+      const Weights w(s, top);
+      const auto each = [&](const auto& weight) {
+#pragma unroll
+        for (int i = 0; i < OWN; ++i)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum += weight(b[i].x[e]);
+      };
+      const auto binned = [&](float x, double v) {
+        if (x > -INFINITY) {
+          const int l = min(q - s.bin(x), kBins - 1);
+          // v times the unit, rounded, in the low bits
+          const uint64_t fixed = __builtin_bit_cast(uint64_t, __builtin_fma(v, kBinUnit, 4503599627370496.0));
+          atomicAdd(&bins[l], (1ull << 32) | static_cast<uint32_t>(fixed));
+        }
+        return v;
+      };
+      if (w.plain && !filters) each([&](float x) { return w.fast(x); });
+      else if (w.plain) each([&](float x) { return binned(x, w.fast(x)); });
+      else each([&](float x) { const double v = w.exact(x); return filters ? binned(x, v) : v; });
+      sum = wave_sum(sum);
+    }
+    if (lane == 0) sums[wave] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      double all = sums[0];
+      for (int w = 1; w < WAVES; ++w) all += sums[w];
+      a.part[r * a.parts + part] = Part{top, q, top > -INFINITY ? all : 0.};
+    }
+    if (filters) a.bins[(r * a.parts + part) * kBins + threadIdx.x] = bins[threadIdx.x];
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------ a row
+
+struct RowShared {
+  uint64_t list[kListed];
+  double weight[kListed];      // of blocks: 2048 of them hold 2^20 tokens
+  double parts[kRowWaves + 1];
+  double bin_weight[kBins];
+  uint32_t bin_count[kBins];
+  unsigned long long radix[kBins];
+  int count, found, last;
+  uint32_t digit;
+  uint64_t upto;
+  double chosen;
+};
+
+// Sums of v over the threads before this one and it; *all: over all threads.
+__device__ __forceinline__ double block_scan(double v, double* parts, double* all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int step = 1; step < 64; step *= 2) {
+    const double add = __shfl_up(v, step);
+    if (lane >= step) v += add;
+  }
+  if (lane == 63) parts[wave] = v;
   __syncthreads();
-  V sum = part[0];
-  for (int w = 1; w < kBlockWaves; ++w) sum += part[w];
+  double before = 0., total = 0.;
+  for (int w = 0; w < kRowWaves; ++w) {
+    if (w == wave) before = total;
+    total += parts[w];
+  }
+  __syncthreads();
+  *all = total;
+  return before + v;
+}
+__device__ __forceinline__ double block_sum(double v, double* parts) {
+  v = wave_sum(v);
+  if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double sum = 0.;
+  for (int w = 0; w < kRowWaves; ++w) sum += parts[w];
   __syncthreads();
   return sum;
 }
 
-template <typename T> struct Row {
-  const SampleArgs& a;
-  int64_t base;
-  uint32_t top;      // key of the largest logit
-  double peak, heat; // its value, the temperature
-  __device__ __forceinline__ uint32_t key(int i) const { return key_of(load_elem<T>(a.logits, base + i)); }
-  __device__ __forceinline__ double weight(uint32_t k) const {
-    if (k == 0) return 0.;
-    if (top == key_of(INFINITY)) return k == top ? 1. : 0.;
-    return exp((static_cast<double>(value_of(k)) - peak) / heat);
+// What a row's workgroup begins with: thread t's part and the row's largest logit.
+struct RowStart {
+  Part mine;
+  float top;
+  __device__ __forceinline__ RowStart(const SampleArgs& a, int64_t r, double* parts) {
+    mine = static_cast<int>(threadIdx.x) < a.parts ? a.part[r * a.parts + threadIdx.x] : Part{-INFINITY, 0, 0.};
+    top = wave_max(mine.top);
+    if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = top;
+    __syncthreads();
+    for (int w = 0; w < kRowWaves; ++w) top = fmaxf(top, static_cast<float>(parts[w]));
+    __syncthreads();
   }
 };
 
-// The key at which the count (WEIGHTS: the weights) of the ranked tokens reaches
-// `want`: f(key) of all above it is below want.  *above: theirs.
-template <bool WEIGHTS, typename T>
-__device__ uint32_t cross(const Row<T>& r, uint64_t want, uint64_t* above, uint64_t* bins) {
-  uint32_t prefix = 0, mask = 0;
-  uint64_t before = 0;
-  __shared__ uint32_t digit;
-  __shared__ uint64_t upto;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256; i += kBlock) bins[i] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < r.a.vocab; i += kBlock) {
-      const uint32_t k = r.key(i);
-      if (k == 0 || (k & mask) != prefix) continue;
-      const uint64_t v = WEIGHTS ? static_cast<uint64_t>(r.weight(k) * kUnit + 0.5) : 1;
-      atomicAdd(reinterpret_cast<unsigned long long*>(&bins[k >> shift & 255]), static_cast<unsigned long long>(v));
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      uint64_t s = before;
-      int found = 0, lowest = 0;
-      for (int i = 255; i >= 0; --i) {
-        if (bins[i] == 0) continue;
-        lowest = i;
-        if (s + bins[i] >= want) {
-          found = 1;
-          break;
-        }
-        s += bins[i];
-      }
-      if (!found) s -= bins[lowest];  // fewer than wanted: the last
-      digit = lowest;
-      upto = s;
-    }
-    __syncthreads();
-    prefix |= digit << shift;
-    mask |= 255u << shift;
-    before = upto;
-    __syncthreads();
-  }
-  *above = before;
-  return prefix;
+__device__ __forceinline__ void write(const SampleArgs& a, int64_t row, int token, double p) {
+  a.tokens[row] = token;
+  if (a.logprobs) a.logprobs[row] = p > 0. ? static_cast<float>(log(p)) : -INFINITY;
 }
 
-template <typename T> __global__ __launch_bounds__(kBlock) void sample_rows(SampleArgs a) {
-  __shared__ uint64_t bins[256];
-  __shared__ double parts[kBlockWaves];
-  __shared__ int ints[kBlockWaves];
-  __shared__ double scan[kBlock];
-  const int64_t row = blockIdx.x;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  Row<T> r{a, row * a.stride, 0, 0, 0};
-  const float heat = a.temperature ? a.temperature[row] : a.temperature_all;
-  const int top_k = a.top_k ? a.top_k[row] : a.top_k_all;
-  const float top_p = a.top_p ? a.top_p[row] : a.top_p_all, min_p = a.min_p ? a.min_p[row] : a.min_p_all;
-  const float u = fminf(fmaxf(a.uniform[row], 0.f), 0.99999994f);
-
-  uint32_t top = 0;
-  for (int i = threadIdx.x; i < a.vocab; i += kBlock) top = max(top, r.key(i));
-  for (int m = 32; m; m >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), m)));
-  if (lane == 0) bins[wave] = top;
+// The first of `n` threads' tokens (thread t's is first + t) that goes beyond
+// `goal`, `before` being what the tokens before them weigh; without one, by
+// rounding at the end, the last that weighs anything.
+__device__ __forceinline__ void draw_from(const SampleArgs& a, int64_t row, double v, int token, double goal, double before,
+                                          double total, int* found, double* parts) {
+  if (threadIdx.x == 0) found[0] = 0x7fffffff, found[1] = -1;
+  double sum;
+  const double upto = before + block_scan(v, parts, &sum);
+  if (v > 0. && upto > goal) atomicMin(&found[0], token);
+  if (v > 0.) atomicMax(&found[1], token);
   __syncthreads();
-  for (int w = 0; w < kBlockWaves; ++w) top = max(top, static_cast<uint32_t>(bins[w]));
+  if (v > 0. && token == (found[0] == 0x7fffffff ? found[1] : found[0])) write(a, row, token, v / total);
+}
+
+// Rows without filters, and greedy ones: true if this was one.
+template <typename T>
+__device__ __forceinline__ bool draw_plain(const SampleArgs& a, const Settings& s, const RowStart& start, const Weights& w,
+                                           int64_t r, int64_t row, double u, int (&found)[2], double* parts,
+                                           double* chosen, double* total) {
+  const int blocks = (a.vocab + kBlock - 1) / kBlock;
+  const float* block_top = a.block_top + r * a.parts * kPartBlocks;
+  if (!(start.top > -INFINITY)) {
+    if (threadIdx.x == 0) write(a, row, -1, 0.);
+    return true;
+  }
+  if (threadIdx.x == 0) found[0] = 0x7fffffff, found[1] = -1;
+  if (s.greedy) {  // the first token of the first block that has the largest logit
+    __syncthreads();
+    for (int b = threadIdx.x; b < blocks; b += kRowThreads)
+      if (block_top[b] == start.top) atomicMin(&found[0], b);
+    __syncthreads();
+    const int i = found[0] * kBlock + threadIdx.x;
+    __syncthreads();
+    const bool hit = threadIdx.x < kBlock && i < a.vocab && load_elem<T>(a.logits, row * a.stride + i) == start.top;
+    draw_from(a, row, hit ? 1. : 0., i, 0., 0., 1., found, parts);
+    return true;
+  }
+  // weights of the parts relative to the row's largest logit
+  const double weight = start.mine.sum > 0. ? start.mine.sum * w.exact(start.mine.top) : 0.;
+  const double upto = block_scan(weight, parts, total);
+  if (s.filters()) return false;
+  const double goal = u * *total;
+  if (weight > 0.) {
+    if (upto > goal) atomicMin(&found[0], static_cast<int>(threadIdx.x));
+    atomicMax(&found[1], static_cast<int>(threadIdx.x));
+  }
   __syncthreads();
-  if (top == 0) {
-    if (threadIdx.x == 0) {
-      a.tokens[row] = -1;
-      if (a.logprobs) a.logprobs[row] = -INFINITY;
-    }
-    return;
-  }
-  r.top = top;
-  r.peak = value_of(top);
-  r.heat = heat;
-  const bool greedy = !(heat > 0.f);
-
-  // what is kept: keys above `edge`, the first `ties` tokens of that key, weights from `least` on
-  uint32_t edge = 0;
-  int64_t ties = 0;
-  if (greedy) {
-    edge = top;
-    ties = 1;
-  } else {
-    double total = 0;
-    if (top_k > 0 && top_k < a.vocab) {
-      uint64_t above;
-      edge = cross<false>(r, top_k, &above, bins);
-      ties = top_k - static_cast<int64_t>(above);
-    }
-    if (top_p < 1.f) {
-      for (int i = threadIdx.x; i < a.vocab; i += kBlock) {
-        const uint32_t k = r.key(i);
-        if (k > edge) total += r.weight(k);
+  const int at = found[0] == 0x7fffffff ? found[1] : found[0];
+  if (static_cast<int>(threadIdx.x) == at) *chosen = upto - weight;
+  // four tokens per thread, then one of them
+  float x[4];
+  double v[4], sum = 0.;
+  const int first = at * kPart + 4 * static_cast<int>(threadIdx.x);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    x[e] = fmaxf(load_elem<T>(a.logits, row * a.stride + min(first + e, a.vocab - 1)), -INFINITY);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) sum += v[e] = first + e < a.vocab ? w.exact(x[e]) : 0.;
+  __syncthreads();
+  double before = *chosen, all;
+  if (threadIdx.x == 0) found[0] = 0x7fffffff, found[1] = -1;
+  before += block_scan(sum, parts, &all) - sum;
+  int token = -1, last = -1;
+  double of_token = 0., of_last = 0.;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    before += v[e];
+    if (v[e] > 0.) {
+      last = first + e;
+      of_last = v[e];
+      if (before > goal && token < 0) {
+        token = first + e;
+        of_token = v[e];
       }
-      total = block_sum(total, parts) + static_cast<double>(ties) * r.weight(edge);
-      const double need = static_cast<double>(top_p) * total;
-      uint64_t above;
-      const uint32_t at = cross<true>(r, max(uint64_t{1}, static_cast<uint64_t>(ceil(need * kUnit))), &above, bins);
-      const double before = static_cast<double>(above) / kUnit, w = r.weight(at);
-      int64_t m = w > 0 ? static_cast<int64_t>(fmin(ceil((need - before) / w), 1e9)) : 1;
-      m = max(m, int64_t{1});
-      if (at == edge) ties = min(ties, m);
-      else if (at > edge) edge = at, ties = m;
     }
   }
-  const double least = !greedy && min_p > 0.f ? min_p : 0.;
+  if (token >= 0) atomicMin(&found[0], token);
+  if (last >= 0) atomicMax(&found[1], last);
+  __syncthreads();
+  if (found[0] == 0x7fffffff ? last >= 0 && last == found[1] : token >= 0 && token == found[0])
+    write(a, row, found[0] == 0x7fffffff ? last : token, (found[0] == 0x7fffffff ? of_last : of_token) / *total);
+  return true;
+}
 
-  // the order of the vocabulary, twice: the kept weights' total, then the first token beyond u of it
-  double total = 0, goal = 0;
-  int last = -1;  // the last kept token so far
-  for (int pass = 0; pass < 2; ++pass) {
-    int64_t equal = 0;  // tokens of key `edge` so far
-    double before = 0;
-    for (int i0 = 0; i0 < a.vocab; i0 += kBlock) {
-      const int i = i0 + threadIdx.x;
-      const uint32_t k = i < a.vocab ? r.key(i) : 0;
-      const bool tie = k != 0 && k == edge;
-      const uint64_t all = __builtin_amdgcn_ballot_w64(tie);
-      if (lane == 0) ints[wave] = __popcll(all);
-      __syncthreads();
-      int64_t rank = equal + __popcll(all & ((uint64_t{1} << lane) - 1));
-      for (int w = 0; w < kBlockWaves; ++w) {
-        if (w < wave) rank += ints[w];
-        equal += ints[w];
-      }
-      double v = k > edge || (tie && rank < ties) ? r.weight(k) : 0.;
-      if (v < least && k != top) v = 0;
-      if (k == top && (k > edge || rank < ties)) v = 1;
-      scan[threadIdx.x] = v;
-      __syncthreads();
-      for (int step = 1; step < kBlock; step *= 2) {
-        const double add = static_cast<int>(threadIdx.x) >= step ? scan[threadIdx.x - step] : 0.;
-        __syncthreads();
-        scan[threadIdx.x] += add;
-        __syncthreads();
-      }
-      const double upto = before + scan[threadIdx.x];
-      if (pass == 1) {
-        const bool hit = v > 0 && upto > goal;
-        const bool other = v > 0;
-        const uint64_t hits = __builtin_amdgcn_ballot_w64(hit), others = __builtin_amdgcn_ballot_w64(other);
-        if (lane == 0) {
-          ints[wave] = hits ? i0 + 64 * wave + __builtin_ctzll(hits) : -1;
-          bins[wave] = others ? i0 + 64 * wave + 63 - __builtin_clzll(others) : 0xffffffffu;
+template <typename T> __global__ __launch_bounds__(kRowThreads) void sample_plain(SampleArgs a) {
+  __shared__ double parts[kRowWaves + 1], chosen;
+  __shared__ int found[2];
+  const int64_t r = blockIdx.x, row = a.row0 + r;
+  const Settings s(a, row);
+  const double u = static_cast<double>(fminf(fmaxf(a.uniform[row], 0.f), 0.99999994f));
+  const RowStart start(a, r, parts);
+  const Weights w(s, start.top);
+  double total;
+  draw_plain<T>(a, s, start, w, r, row, u, found, parts, &chosen, &total);
+}
+
+// Sorts list[0, n) upwards; n a power of 2, entries beyond the last ~0.
+__device__ __forceinline__ void sort(uint64_t* list, int n) {
+  const bool one = n <= 128;  // one wave's work
+  const int threads = one ? 64 : kRowThreads;
+  if (!one || threadIdx.x < 64) {
+    for (int size = 2; size <= n; size *= 2)
+      for (int step = size / 2; step; step /= 2) {
+        for (int i = threadIdx.x; i < n / 2; i += threads) {
+          const int at = 2 * i - (i & (step - 1)), other = at + step;
+          const uint64_t x = list[at], y = list[other];
+          if ((x > y) == ((at & size) == 0)) {
+            list[at] = y;
+            list[other] = x;
+          }
         }
-        __syncthreads();
-        int found = -1;
-        for (int w = kBlockWaves - 1; w >= 0; --w) {
-          if (ints[w] >= 0) found = ints[w];
-        }
-        for (int w = 0; w < kBlockWaves; ++w)
-          if (bins[w] != 0xffffffffu) last = static_cast<int>(bins[w]);
-        if (found >= 0) {
-          last = found;
-          break;
-        }
+        if (one) wave_sync();
+        else __syncthreads();
       }
-      before += scan[kBlock - 1];
-      __syncthreads();
+  }
+  __syncthreads();
+}
+__device__ __forceinline__ int power_of_2(int n) { return n <= 2 ? 2 : 1 << (32 - __builtin_clz(n - 1)); }
+
+// Kept are logits above `edge`, and of those equal to it the tokens up to `last`.
+struct Kept {
+  uint32_t edge;  // key
+  int last;
+  __device__ __forceinline__ bool has(float x, int i) const {
+    const uint32_t k = key_of(x);
+    return x > -INFINITY && (k > edge || (k == edge && i <= last));
+  }
+};
+
+// A bin, or the 256ths of it from `low` to `high`.
+struct Range {
+  int bin, low, high;
+};
+
+template <typename T> struct RowWork {
+  const SampleArgs& a;
+  RowShared& l;
+  const Settings& s;
+  const Weights& w;
+  int64_t row;
+  const float* block_top;
+  int blocks, q_top;
+
+  // f(logits of a block, its number), a wave per block, for the blocks of whose
+  // largest logit wanted(it) holds; the next block's logits are on their way.
+  template <typename WANTED, typename F> __device__ __forceinline__ void each_block(const WANTED& wanted, const F& f) const {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int b0 = wave; b0 < blocks; b0 += 64 * kRowWaves) {
+      const int mine = b0 + kRowWaves * lane;
+      const float top = mine < blocks ? block_top[mine] : -INFINITY;
+      uint64_t todo = __builtin_amdgcn_ballot_w64(top > -INFINITY && wanted(top));
+      Block<T> next;
+      int at = 0;
+      const auto take = [&] {
+        at = b0 + kRowWaves * __builtin_ctzll(todo);
+        todo &= todo - 1;
+        next.load(a, row, at);
+      };
+      bool more = todo != 0;
+      if (more) take();
+      while (more) {
+        Block<T> b = next;
+        const int number = at;
+        more = todo != 0;
+        if (more) take();
+        b.take(a);
+        f(b, number);
+      }
+    }
+  }
+
+  // Of the tokens in a range: the list of them (false: it does not hold them), or
+  // (COUNT) how many and how much weight each 256th has.  *above: what those in
+  // higher ranges weigh.
+  template <bool COUNT> __device__ bool look(const Range& range, double* above) {
+    const int lane = threadIdx.x & 63;
+    if (threadIdx.x == 0) l.count = 0;
+    if (COUNT && threadIdx.x < kBins) {
+      l.bin_count[threadIdx.x] = 0;
+      l.radix[threadIdx.x] = 0;
     }
     __syncthreads();
-    if (pass == 0) {
-      total = before;
-      goal = static_cast<double>(u) * total;
+    double sum = 0.;
+    each_block([&](float top) { return s.bin(top) >= range.bin; }, [&](const Block<T>& b, int) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = b.x[e];
+        const int q = s.bin(x), fine = s.fine(x);
+        if (!(x > -INFINITY) || q < range.bin || (q == range.bin && fine < range.low)) continue;
+        const bool in = q == range.bin && fine <= range.high;
+        if (COUNT || !in) {
+          const double v = w.exact(x);
+          if (!in) sum += v;
+          else {
+            atomicAdd(&l.bin_count[255 - fine], 1u);
+            atomicAdd(&l.radix[255 - fine], static_cast<unsigned long long>(v * kUnit + 0.5));
+          }
+        }
+        if (!COUNT && in) {
+          const int i = atomicAdd(&l.count, 1);
+          if (i < kListed) l.list[i] = static_cast<uint64_t>(~key_of(x)) << 32 | static_cast<uint32_t>(b.index(e));
+        }
+      }
+    });
+    *above = block_sum(sum, l.parts);
+    if constexpr (COUNT) {
+      if (threadIdx.x < kBins) l.bin_weight[threadIdx.x] = static_cast<double>(l.radix[threadIdx.x]) / kUnit;
+      __syncthreads();
+      return true;
+    } else {
+      const int count = l.count;
+      if (count > kListed) return false;
+      const int n = power_of_2(count);
+      for (int i = count + threadIdx.x; i < n; i += kRowThreads) l.list[i] = ~uint64_t{0};
+      __syncthreads();
+      sort(l.list, n);
+      return true;
+    }
+    (void)lane;
+  }
+
+  // The first bin at which the count (weight) of the bins up to it, `before` ahead of
+  // the first, reaches `want`; the last without one.  *upto: before that bin.
+  __device__ __forceinline__ int reaches(double want, bool by_count, double before, double* upto) {
+    const int lane = threadIdx.x & 63;
+    if (threadIdx.x < 64) {
+      double own = 0.;
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) own += by_count ? static_cast<double>(l.bin_count[4 * lane + i]) : l.bin_weight[4 * lane + i];
+      double sum = own;
+      for (int step = 1; step < 64; step *= 2) {
+        const double add = __shfl_up(sum, step);
+        if (lane >= step) sum += add;
+      }
+      sum += before;
+      const uint64_t past = __builtin_amdgcn_ballot_w64(sum >= want);
+      if (lane == (past ? __builtin_ctzll(past) : 63)) {
+        double at = sum - own;
+        int bin = 4 * lane;
+#pragma unroll 1
+        for (;; ++bin) {
+          const double v = by_count ? static_cast<double>(l.bin_count[bin]) : l.bin_weight[bin];
+          if (at + v >= want || bin == 4 * lane + 3) break;
+          at += v;
+        }
+        l.found = past ? bin : kBins - 1;
+        l.chosen = at;
+      }
+    }
+    __syncthreads();
+    const int bin = l.found;
+    *upto = l.chosen;
+    __syncthreads();
+    return bin;
+  }
+
+  // The last ranked token before which less than `want` lies (by_count: tokens,
+  // else weight), and the kept weight up to it.  False if lists do not hold what
+  // has to be sorted for it, or bins, whose weights are rounded, do not say where.
+  __device__ __forceinline__ bool threshold(double want, bool by_count, Kept* kept, double* weight) {
+    double ahead, above;
+    const int b = reaches(want, by_count, 0., &ahead);
+    if (b == kBins - 1) return false;
+#pragma unroll 1
+    for (int step = 0; step < (by_count ? 1 : 3); ++step) {  // rounded weights: perhaps the bin next to it
+      const int g = step == 0 ? b : step == 1 ? b - 1 : b + 1;
+      if (g < 0 || g >= kBins - 1) continue;
+      Range range{q_top - g, 0, 255};
+      bool listed = l.bin_count[g] <= static_cast<uint32_t>(kListed);
+      __syncthreads();
+      if (!listed) {  // a 256th of the bin, and a little more
+        look<true>(range, &above);
+        double before = ahead;
+        const int f = reaches(want, by_count, by_count ? ahead : above, &before);
+        ahead = before;  // of a count: up to this 256th
+        range.low = max(0, 255 - f - (by_count ? 0 : 1));
+        range.high = min(255, 255 - f + (by_count ? 0 : 1));
+      }
+      listed = look<false>(range, &above);
+      const int count = l.count;
+      if (!listed || count == 0) {
+        if (range.low == 0 && range.high == 255) continue;
+        return false;  // the bins are not the row's any more
+      }
+      const int i = 2 * threadIdx.x;
+      double w2[2], all;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        w2[e] = i + e < count ? w.exact(value_of(~static_cast<uint32_t>(l.list[i + e] >> 32))) : 0.;
+      const double upto1 = block_scan(w2[0] + w2[1], l.parts, &all), upto0 = upto1 - w2[1];
+      if (threadIdx.x == 0) l.found = -1;
+      __syncthreads();
+      int at;
+      if (by_count) {
+        at = min(static_cast<int>(want - ahead), count) - 1;
+      } else {
+        if (above < want && above + all >= want) {
+          if (i < count && above + (upto0 - w2[0]) < want) atomicMax(&l.found, i);
+          if (i + 1 < count && above + upto0 < want) atomicMax(&l.found, i + 1);
+        }
+        __syncthreads();
+        at = l.found;
+      }
+      if (at >= 0) {
+        if (i <= at && at <= i + 1) {
+          l.chosen = above + (at == i ? upto0 : upto1);
+          l.upto = l.list[at];
+        }
+        __syncthreads();
+        *weight = l.chosen;
+        *kept = Kept{~static_cast<uint32_t>(l.upto >> 32), static_cast<int>(l.upto)};
+        __syncthreads();
+        return true;
+      }
+      if (range.low != 0 || range.high != 255) return false;
+      __syncthreads();
+    }
+    return false;
+  }
+
+  // As threshold, digit by digit over all tokens that are kept so far.
+  __device__ __forceinline__ Kept by_digits(double need, bool by_count, const Kept& within) {
+    uint32_t prefix = 0, mask = 0;
+    uint64_t before = 0;
+    const double unit = by_count ? 1. : kUnit;
+    const uint64_t want = max(uint64_t{1}, static_cast<uint64_t>(ceil(need * unit)));
+#pragma unroll 1
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      if (threadIdx.x < 256) l.radix[threadIdx.x] = 0;
+      __syncthreads();
+      each_block([&](float top) { return key_of(top) >= max(within.edge, prefix); }, [&](const Block<T>& b, int) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t k = key_of(b.x[e]);
+          if (!within.has(b.x[e], b.index(e)) || (k & mask) != prefix) continue;
+          atomicAdd(&l.radix[k >> shift & 255],
+                    by_count ? 1ull : static_cast<unsigned long long>(w.exact(b.x[e]) * kUnit + 0.5));
+        }
+      });
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        uint64_t sum = before;
+        int lowest = 0;
+        bool found = false;
+#pragma unroll 1
+        for (int i = 255; i >= 0 && !found; --i) {
+          if (l.radix[i] == 0) continue;
+          lowest = i;
+          if (sum + l.radix[i] >= want) found = true;
+          else sum += l.radix[i];
+        }
+        if (!found) sum -= l.radix[lowest];  // fewer than wanted: the last
+        l.digit = lowest;
+        l.upto = sum;
+      }
+      __syncthreads();
+      prefix |= l.digit << shift;
+      mask |= 255u << shift;
+      before = l.upto;
+      __syncthreads();
+    }
+    // of the tokens equal to it, in order, as many as are needed
+    const double each = by_count ? 1. : w.exact(value_of(prefix));
+    const double left = need - static_cast<double>(before) / unit;
+    const int ties = each > 0. ? max(1, static_cast<int>(fmin(ceil(left / each), 1e9))) : 1;
+    if (threadIdx.x == 0) l.last = -1;
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      int seen = 0;
+#pragma unroll 1
+      for (int i0 = 0; i0 < a.vocab && seen < ties; i0 += 64) {
+        const int i = i0 + threadIdx.x;
+        const float x = i < a.vocab ? load_elem<T>(a.logits, row * a.stride + i) : -INFINITY;
+        const bool tie = x > -INFINITY && key_of(x) == prefix && within.has(x, i);
+        const uint64_t all = __builtin_amdgcn_ballot_w64(tie);
+        const int rank = seen + __popcll(all & ((uint64_t{1} << threadIdx.x) - 1));
+        if (tie && rank < ties) atomicMax(&l.last, i);
+        seen += __popcll(all);
+      }
+    }
+    __syncthreads();
+    return Kept{prefix, l.last};
+  }
+
+  // Weights of the blocks' kept tokens, in l.weight; their sum.
+  __device__ __forceinline__ double weigh(const Kept& kept, double least) {
+    for (int b = threadIdx.x; b < blocks; b += kRowThreads) l.weight[b] = 0.;
+    __syncthreads();
+    each_block([&](float top) { return key_of(top) >= kept.edge; }, [&](const Block<T>& b, int number) {
+      double sum = 0.;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (!kept.has(b.x[e], b.index(e))) continue;
+        const double v = w.exact(b.x[e]);
+        if (v >= least || b.x[e] == w.top32) sum += v;
+      }
+      sum = wave_sum(sum);
+      if ((threadIdx.x & 63) == 0) l.weight[number] = sum;
+    });
+    __syncthreads();
+    double all;
+    const int i = 2 * threadIdx.x;
+    const double w0 = i < blocks ? l.weight[i] : 0., w1 = i + 1 < blocks ? l.weight[i + 1] : 0.;
+    const double upto = block_scan(w0 + w1, l.parts, &all);
+    if (i < blocks) l.weight[i] = upto - w1;  // up to a block, and it
+    if (i + 1 < blocks) l.weight[i + 1] = upto;
+    __syncthreads();
+    return all;
+  }
+};
+
+template <typename T> __global__ __launch_bounds__(kRowThreads) void sample_rows(SampleArgs a) {
+  __shared__ RowShared l;
+  __shared__ int found[2];
+  const int64_t r = blockIdx.x, row = a.row0 + r;
+  const Settings s(a, row);
+  const double u = static_cast<double>(fminf(fmaxf(a.uniform[row], 0.f), 0.99999994f));
+  const RowStart start(a, r, l.parts);
+  const Weights w(s, start.top);
+  double total;
+  if (draw_plain<T>(a, s, start, w, r, row, u, found, l.parts, &l.chosen, &total)) return;
+  const int blocks = (a.vocab + kBlock - 1) / kBlock;
+  const Part* part = a.part + r * a.parts;
+  RowWork<T> work{a, l, s, w, row, a.block_top + r * a.parts * kPartBlocks, blocks, s.bin(start.top)};
+
+  // the row's bins, by four groups of threads: a part's bin g - shift is the row's bin g
+  {
+    const int g = threadIdx.x & (kBins - 1), group = threadIdx.x / kBins;
+    uint32_t count = 0;
+    double weight = 0.;
+    for (int p = group; p < a.parts; p += kRowThreads / kBins) {
+      const Part other = part[p];
+      if (!(other.sum > 0.)) continue;
+      const int64_t i = g - (static_cast<int64_t>(work.q_top) - other.q);
+      if (i < 0 || i >= kBins - 1) continue;
+      const uint64_t v = a.bins[(r * a.parts + p) * kBins + i];
+      count += static_cast<uint32_t>(v >> 32);
+      weight += static_cast<double>(static_cast<uint32_t>(v)) * (w.exact(other.top) / kBinUnit);
+    }
+    if (threadIdx.x < kBins) l.bin_count[g] = 0;
+    __syncthreads();
+    if (g < kBins - 1) atomicAdd(&l.bin_count[g], count);
+    for (int k = 0; k < kRowThreads / kBins; ++k) {  // in order
+      if (group == k) l.bin_weight[g] = g == kBins - 1 ? 0. : k ? l.bin_weight[g] + weight : weight;
+      __syncthreads();
     }
   }
-  if (threadIdx.x == 0) {
-    a.tokens[row] = last;
-    if (a.logprobs) a.logprobs[row] = static_cast<float>(log((greedy ? 1. : r.weight(r.key(last))) / total));
+  // thresholds one by one; for both, the second from the row's bins again
+  Kept kept{0, 0x7fffffff};
+  double base = total;
+  uint32_t bin_count = 0;
+  double bin_weight = 0.;
+  if (threadIdx.x < kBins) {
+    bin_count = l.bin_count[threadIdx.x];
+    bin_weight = l.bin_weight[threadIdx.x];
   }
+#pragma unroll 1
+  for (int round = 0; round < 2; ++round) {
+    const bool by_count = round == 0;
+    if (!(by_count ? s.by_count : s.by_weight)) continue;
+    const double want = by_count ? static_cast<double>(s.top_k) : static_cast<double>(s.top_p) * base;
+    Kept k;
+    double weight;
+    if (work.threshold(want, by_count, &k, &weight)) {
+      base = weight;
+      if (k.edge > kept.edge || (k.edge == kept.edge && k.last < kept.last)) kept = k;
+    } else {
+      kept = work.by_digits(want, by_count, kept);
+      if (by_count && s.by_weight) base = work.weigh(kept, 0.);
+    }
+    __syncthreads();
+    if (threadIdx.x < kBins) {
+      l.bin_count[threadIdx.x] = bin_count;
+      l.bin_weight[threadIdx.x] = bin_weight;
+    }
+    __syncthreads();
+  }
+  const double least = s.by_least ? static_cast<double>(s.min_p) : 0.;
+  const double all = work.weigh(kept, least), goal = u * all;
+  // the first block beyond the goal; without one, by rounding, the last that weighs anything
+  if (threadIdx.x == 0) found[0] = 0x7fffffff, found[1] = -1;
+  __syncthreads();
+  for (int b = threadIdx.x; b < blocks; b += kRowThreads) {
+    const double upto = l.weight[b], before = b ? l.weight[b - 1] : 0.;
+    if (upto > before) {
+      if (upto > goal) atomicMin(&found[0], b);
+      atomicMax(&found[1], b);
+    }
+  }
+  __syncthreads();
+  const int block = found[0] == 0x7fffffff ? found[1] : found[0];
+  const int i = block * kBlock + threadIdx.x;  // a thread per token
+  double v = 0.;
+  if (threadIdx.x < kBlock && i < a.vocab) {
+    const float x = fmaxf(load_elem<T>(a.logits, row * a.stride + i), -INFINITY);
+    if (kept.has(x, i)) {
+      v = w.exact(x);
+      if (v < least && x != w.top32) v = 0.;
+    }
+  }
+  __syncthreads();
+  draw_from(a, row, v, i, goal, block ? l.weight[block - 1] : 0., all, found, l.parts);
 }
+
+int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
+int64_t part_count(int64_t vocab) { return (vocab + kPart - 1) / kPart; }
 
 }  // namespace
 
-int64_t sample_workspace(int64_t, int64_t) { return 0; }
+int64_t sample_workspace(int64_t rows, int64_t vocab) {
+  const int64_t n = (rows < kChunk ? rows : kChunk) * part_count(vocab);
+  return up16(n * sizeof(Part)) + up16(n * kPartBlocks * 4) + n * kBins * 8;
+}
 
 int sample_launch(const void* logits, const float* uniform, int64_t* tokens, float* logprobs, const float* temperature,
                   const int32_t* top_k, const float* top_p, const float* min_p, float temperature_all, int32_t top_k_all,
-                  float top_p_all, float min_p_all, int64_t rows, int vocab, int64_t stride, int dtype, void*,
+                  float top_p_all, float min_p_all, int64_t rows, int vocab, int64_t stride, int dtype, void* work,
                   hipStream_t stream) {
-  const SampleArgs a{logits, uniform, tokens, logprobs, temperature, top_k, top_p, min_p, temperature_all, top_k_all,
-                     top_p_all, min_p_all, rows, stride, vocab};
-  const dim3 grid(static_cast<unsigned>(rows));
+  SampleArgs a{logits, uniform, tokens, logprobs, temperature, top_k, top_p, min_p, temperature_all, top_k_all,
+               top_p_all, min_p_all, 0, 0, stride, vocab, static_cast<int>(part_count(vocab)), false, nullptr, nullptr,
+               nullptr};
+  const int64_t es = dtype == MI355_F32 ? 4 : 2;
+  a.aligned = aligned16(logits) && (rows == 1 || stride * es % 16 == 0);
+  const int64_t n = (rows < kChunk ? rows : kChunk) * a.parts;
+  uint8_t* at = static_cast<uint8_t*>(work);
+  a.part = reinterpret_cast<Part*>(at);
+  at += up16(n * sizeof(Part));
+  a.block_top = reinterpret_cast<float*>(at);
+  at += up16(n * kPartBlocks * 4);
+  a.bins = reinterpret_cast<uint64_t*>(at);
   static const char* what = "sample_tokens launch";
-  if (dtype == MI355_F32) return launch(sample_rows<F32>, grid, kBlock, 0, a, stream, what);
-  if (dtype == MI355_F16) return launch(sample_rows<F16>, grid, kBlock, 0, a, stream, what);
-  return launch(sample_rows<BF16>, grid, kBlock, 0, a, stream, what);
+  // known here: no row has filters
+  const bool plain = top_k == nullptr && top_p == nullptr && min_p == nullptr && temperature == nullptr &&
+                     (!(temperature_all > 0.f) ||
+                      ((top_k_all <= 0 || top_k_all >= vocab) && !(top_p_all < 1.f) && !(min_p_all > 0.f)));
+  const auto run = [&](auto* parts, auto* draw) {
+    const int st = launch(parts, dim3(static_cast<unsigned>(a.rows * a.parts)), kPartThreads, 0, a, stream, what);
+    return st != MI355_OK ? st : launch(draw, dim3(static_cast<unsigned>(a.rows)), kRowThreads, 0, a, stream, what);
+  };
+  for (a.row0 = 0; a.row0 < rows; a.row0 += kChunk) {
+    a.rows = rows - a.row0 < kChunk ? rows - a.row0 : kChunk;
+    const int st = dtype == MI355_F32   ? run(sample_parts<F32>, plain ? sample_plain<F32> : sample_rows<F32>)
+                   : dtype == MI355_F16 ? run(sample_parts<F16>, plain ? sample_plain<F16> : sample_rows<F16>)
+                                        : run(sample_parts<BF16>, plain ? sample_plain<BF16> : sample_rows<BF16>);
+    if (st != MI355_OK) return st;
+  }
+  return MI355_OK;
 }
 
 }  // namespace mi355

@@ -13,12 +13,13 @@
 //
 // sample_parts reads the logits once, in parts of 4096 on all compute units: each
 // part's largest logit and sum of weights, the largest logit of each block of
-// 512, and, for rows with filters, how many tokens and how much weight a part has
-// in bins a quarter of a power of 2 wide.  Then a workgroup per row draws: without
-// filters (sample_plain) from the part that the number falls into; with them
-// (sample_rows) it finds the bin that a threshold lies in, sorts that bin's tokens
-// (or those of a 256th of it), and adds the kept weights of the blocks.  Blocks
-// whose largest logit is below a threshold are not read again.
+// 512, and, for rows with filters, how much weight (and for top-k, how many
+// tokens) a part has in bins a quarter of a power of 2 wide.  Then a workgroup per
+// row draws: without filters (sample_plain) from the part that the number falls
+// into.  With them (sample_rows) a threshold's bin is known from the bins; that
+// bin's tokens are sorted, which is the one other time that a row is read, and
+// only blocks that reach up to it; and what is kept of a part is the sum of its
+// bins above and of the sorted tokens before the threshold.
 #include "common.h"
 
 namespace mi355 {
@@ -27,10 +28,11 @@ namespace {
 constexpr int kPart = 4096, kBlock = 512, kPartBlocks = kPart / kBlock;
 constexpr int kPartThreads = 256, kRowThreads = 1024, kRowWaves = kRowThreads / 64;
 constexpr int kBins = 256;          // the last holds all that is further down
-constexpr int kListed = 2048;       // tokens that a row's workgroup sorts
+constexpr int kListed = 8192;       // tokens that a row's workgroup sorts
 constexpr int64_t kChunk = 1024;    // rows whose parts the workspace holds
-constexpr double kBinUnit = 524288.0;  // 2^19: the weights of a part's bin, largest 1 each, fit 32 bits
-constexpr double kUnit = 8796093022208.0;  // 2^43: sums of 2^20 weights fit 64 bits
+// Weights in integers, whose sums do not depend on the atomics' order: 4096 of a
+// part, 2^20 of a row fit 64 bits.
+constexpr double kBinUnit = 0x1p50, kUnit = 0x1p43;
 constexpr float kHottest = 1e30f;   // temperatures beyond (infinity) have no weight range to clamp to
 
 struct Part {
@@ -55,7 +57,8 @@ struct SampleArgs {
   bool aligned;                // rows start on 16 bytes
   Part* part;                  // [rows][parts]
   float* block_top;            // [rows][parts * kPartBlocks]
-  uint64_t* bins;              // [rows][parts][kBins]: count << 32 | weight
+  uint64_t* bins;              // [rows][parts][kBins]: weights relative to the part's largest, of kBinUnit
+  uint32_t* counts;            // [rows][parts][kBins], of rows with top-k
 };
 
 struct Settings {
@@ -78,13 +81,7 @@ struct Settings {
   // The bin of a logit: a monotone function of it alone, a quarter of a power of 2 of
   // weight wide.
   __device__ __forceinline__ int bin(float x) const {
-    return static_cast<int>(fminf(fmaxf(floorf(height(x)), -1e9f), 1e9f));
-  }
-  __device__ __forceinline__ float height(float x) const { return x * (4.f * static_cast<float>(c)); }
-  // Which 256th of its bin: monotone too, as nothing but the product is rounded.
-  __device__ __forceinline__ int fine(float x) const {
-    const float y = height(x);
-    return min(static_cast<int>((y - floorf(y)) * 256.f), 255);  // NaN of an infinite height: 0
+    return static_cast<int>(fminf(fmaxf(floorf(x * (4.f * static_cast<float>(c))), -1e9f), 1e9f));
   }
 };
 
@@ -200,6 +197,7 @@ __device__ __forceinline__ double wave_sum(double v) {
 template <typename T> __global__ __launch_bounds__(kPartThreads) void sample_parts(SampleArgs a) {
   constexpr int WAVES = kPartThreads / 64, OWN = kPartBlocks / WAVES;  // blocks of a wave
   __shared__ unsigned long long bins[kBins];
+  __shared__ uint32_t counts[kBins];
   __shared__ float tops[WAVES];
   __shared__ double sums[WAVES];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -211,7 +209,7 @@ template <typename T> __global__ __launch_bounds__(kPartThreads) void sample_par
     for (int i = 0; i < OWN; ++i) b[i].load(a, row, part * kPartBlocks + wave * OWN + i);
     const Settings s(a, row);
     const bool filters = s.filters();
-    if (filters) bins[threadIdx.x] = 0;
+    if (filters) bins[threadIdx.x] = counts[threadIdx.x] = 0;
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < OWN; ++i) {
@@ -240,9 +238,10 @@ template <typename T> __global__ __launch_bounds__(kPartThreads) void sample_par
       const auto binned = [&](float x, double v) {
         if (x > -INFINITY) {
           const int l = min(q - s.bin(x), kBins - 1);
-          // v times the unit, rounded, in the low bits
-          const uint64_t fixed = __builtin_bit_cast(uint64_t, __builtin_fma(v, kBinUnit, 4503599627370496.0));
-          atomicAdd(&bins[l], (1ull << 32) | static_cast<uint32_t>(fixed));
+          // v times the unit, rounded, in the low 52 bits
+          const uint64_t fixed = __builtin_bit_cast(uint64_t, __builtin_fma(v, kBinUnit, 0x1p52)) & 0xfffffffffffffull;
+          atomicAdd(&bins[l], static_cast<unsigned long long>(fixed));
+          if (s.by_count) atomicAdd(&counts[l], 1u);
         }
         return v;
       };
@@ -259,6 +258,7 @@ template <typename T> __global__ __launch_bounds__(kPartThreads) void sample_par
       a.part[r * a.parts + part] = Part{top, q, top > -INFINITY ? all : 0.};
     }
     if (filters) a.bins[(r * a.parts + part) * kBins + threadIdx.x] = bins[threadIdx.x];
+    if (s.by_count) a.counts[(r * a.parts + part) * kBins + threadIdx.x] = counts[threadIdx.x];
     __syncthreads();
   }
 }
@@ -266,12 +266,14 @@ template <typename T> __global__ __launch_bounds__(kPartThreads) void sample_par
 // ------------------------------------------------------------------ a row
 
 struct RowShared {
-  uint64_t list[kListed];
-  double weight[kListed];      // of blocks: 2048 of them hold 2^20 tokens
+  uint64_t list[kListed];      // sorted: key inverted, token
+  double weight[2048];         // of blocks: these hold 2^20 tokens
   double parts[kRowWaves + 1];
   double bin_weight[kBins];
   uint32_t bin_count[kBins];
   unsigned long long radix[kBins];
+  double part_unit[256];       // weight of a part's bins' unit
+  int part_shift[256];         // the row's bin g is the part's bin g - shift
   int count, found, last;
   uint32_t digit;
   uint64_t upto;
@@ -339,6 +341,47 @@ __device__ __forceinline__ void draw_from(const SampleArgs& a, int64_t row, doub
   if (v > 0. && token == (found[0] == 0x7fffffff ? found[1] : found[0])) write(a, row, token, v / total);
 }
 
+// Draws from the tokens of a part that keeps(logit, token) holds for; *chosen: what
+// the parts before it weigh.
+template <typename T, typename KEEPS>
+__device__ __forceinline__ void draw_part(const SampleArgs& a, int64_t row, int part, double goal, double total,
+                                          const Weights& w, const KEEPS& keeps, int (&found)[2], double* parts,
+                                          double* chosen) {
+  // four tokens per thread, then one of them
+  float x[4];
+  double v[4], sum = 0.;
+  const int first = part * kPart + 4 * static_cast<int>(threadIdx.x);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    x[e] = fmaxf(load_elem<T>(a.logits, row * a.stride + min(first + e, a.vocab - 1)), -INFINITY);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) sum += v[e] = first + e < a.vocab && keeps(x[e], first + e) ? w.exact(x[e]) : 0.;
+  __syncthreads();
+  double before = *chosen, all;
+  if (threadIdx.x == 0) found[0] = 0x7fffffff, found[1] = -1;
+  before += block_scan(sum, parts, &all) - sum;
+  int token = -1, last = -1;
+  double of_token = 0., of_last = 0.;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    before += v[e];
+    if (v[e] > 0.) {
+      last = first + e;
+      of_last = v[e];
+      if (before > goal && token < 0) {
+        token = first + e;
+        of_token = v[e];
+      }
+    }
+  }
+  if (token >= 0) atomicMin(&found[0], token);
+  if (last >= 0) atomicMax(&found[1], last);
+  __syncthreads();
+  const bool end = found[0] == 0x7fffffff;  // by rounding: the last that weighs anything
+  if (end ? last >= 0 && last == found[1] : token >= 0 && token == found[0])
+    write(a, row, end ? last : token, (end ? of_last : of_token) / total);
+}
+
 // Rows without filters, and greedy ones: true if this was one.
 template <typename T>
 __device__ __forceinline__ bool draw_plain(const SampleArgs& a, const Settings& s, const RowStart& start, const Weights& w,
@@ -374,38 +417,7 @@ __device__ __forceinline__ bool draw_plain(const SampleArgs& a, const Settings& 
   __syncthreads();
   const int at = found[0] == 0x7fffffff ? found[1] : found[0];
   if (static_cast<int>(threadIdx.x) == at) *chosen = upto - weight;
-  // four tokens per thread, then one of them
-  float x[4];
-  double v[4], sum = 0.;
-  const int first = at * kPart + 4 * static_cast<int>(threadIdx.x);
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    x[e] = fmaxf(load_elem<T>(a.logits, row * a.stride + min(first + e, a.vocab - 1)), -INFINITY);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) sum += v[e] = first + e < a.vocab ? w.exact(x[e]) : 0.;
-  __syncthreads();
-  double before = *chosen, all;
-  if (threadIdx.x == 0) found[0] = 0x7fffffff, found[1] = -1;
-  before += block_scan(sum, parts, &all) - sum;
-  int token = -1, last = -1;
-  double of_token = 0., of_last = 0.;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    before += v[e];
-    if (v[e] > 0.) {
-      last = first + e;
-      of_last = v[e];
-      if (before > goal && token < 0) {
-        token = first + e;
-        of_token = v[e];
-      }
-    }
-  }
-  if (token >= 0) atomicMin(&found[0], token);
-  if (last >= 0) atomicMax(&found[1], last);
-  __syncthreads();
-  if (found[0] == 0x7fffffff ? last >= 0 && last == found[1] : token >= 0 && token == found[0])
-    write(a, row, found[0] == 0x7fffffff ? last : token, (found[0] == 0x7fffffff ? of_last : of_token) / *total);
+  draw_part<T>(a, row, at, goal, *total, w, [](float, int) { return true; }, found, parts, chosen);
   return true;
 }
 
@@ -454,11 +466,6 @@ struct Kept {
   }
 };
 
-// A bin, or the 256ths of it from `low` to `high`.
-struct Range {
-  int bin, low, high;
-};
-
 template <typename T> struct RowWork {
   const SampleArgs& a;
   RowShared& l;
@@ -496,80 +503,58 @@ template <typename T> struct RowWork {
     }
   }
 
-  // Of the tokens in a range: the list of them (false: it does not hold them), or
-  // (COUNT) how many and how much weight each 256th has.  *above: what those in
-  // higher ranges weigh.
-  template <bool COUNT> __device__ bool look(const Range& range, double* above) {
-    const int lane = threadIdx.x & 63;
+  // Sorts the tokens of the row's bins [low, high]; false if there are too many.
+  __device__ __forceinline__ bool look(int low, int high) {
     if (threadIdx.x == 0) l.count = 0;
-    if (COUNT && threadIdx.x < kBins) {
-      l.bin_count[threadIdx.x] = 0;
-      l.radix[threadIdx.x] = 0;
-    }
     __syncthreads();
-    double sum = 0.;
-    each_block([&](float top) { return s.bin(top) >= range.bin; }, [&](const Block<T>& b, int) {
+    const int q_low = q_top - high, q_high = q_top - low;
+    each_block([&](float top) { return s.bin(top) >= q_low; }, [&](const Block<T>& b, int) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float x = b.x[e];
-        const int q = s.bin(x), fine = s.fine(x);
-        if (!(x > -INFINITY) || q < range.bin || (q == range.bin && fine < range.low)) continue;
-        const bool in = q == range.bin && fine <= range.high;
-        if (COUNT || !in) {
-          const double v = w.exact(x);
-          if (!in) sum += v;
-          else {
-            atomicAdd(&l.bin_count[255 - fine], 1u);
-            atomicAdd(&l.radix[255 - fine], static_cast<unsigned long long>(v * kUnit + 0.5));
-          }
-        }
-        if (!COUNT && in) {
-          const int i = atomicAdd(&l.count, 1);
-          if (i < kListed) l.list[i] = static_cast<uint64_t>(~key_of(x)) << 32 | static_cast<uint32_t>(b.index(e));
-        }
+        const int q = s.bin(x);
+        if (q < q_low || q > q_high || !(x > -INFINITY)) continue;
+        const int i = atomicAdd(&l.count, 1);
+        if (i < kListed) l.list[i] = static_cast<uint64_t>(~key_of(x)) << 32 | static_cast<uint32_t>(b.index(e));
       }
     });
-    *above = block_sum(sum, l.parts);
-    if constexpr (COUNT) {
-      if (threadIdx.x < kBins) l.bin_weight[threadIdx.x] = static_cast<double>(l.radix[threadIdx.x]) / kUnit;
-      __syncthreads();
-      return true;
-    } else {
-      const int count = l.count;
-      if (count > kListed) return false;
-      const int n = power_of_2(count);
-      for (int i = count + threadIdx.x; i < n; i += kRowThreads) l.list[i] = ~uint64_t{0};
-      __syncthreads();
-      sort(l.list, n);
-      return true;
-    }
-    (void)lane;
+    __syncthreads();
+    const int count = l.count;
+    if (count > kListed) return false;
+    const int n = power_of_2(count);
+    for (int i = count + threadIdx.x; i < n; i += kRowThreads) l.list[i] = ~uint64_t{0};
+    __syncthreads();
+    sort(l.list, n);
+    return true;
+  }
+  __device__ __forceinline__ double listed(int i) const {
+    return w.exact(value_of(~static_cast<uint32_t>(l.list[i] >> 32)));
   }
 
-  // The first bin at which the count (weight) of the bins up to it, `before` ahead of
-  // the first, reaches `want`; the last without one.  *upto: before that bin.
-  __device__ __forceinline__ int reaches(double want, bool by_count, double before, double* upto) {
+  // The first bin at which the count (weight) of the bins up to it reaches `want`; the
+  // last without one.  *upto: of the bins before it.
+  __device__ __forceinline__ int reaches(double want, bool by_count, double* upto) {
     const int lane = threadIdx.x & 63;
     if (threadIdx.x < 64) {
-      double own = 0.;
-#pragma unroll 1
-      for (int i = 0; i < 4; ++i) own += by_count ? static_cast<double>(l.bin_count[4 * lane + i]) : l.bin_weight[4 * lane + i];
-      double sum = own;
+      double own[4], sum = 0.;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        sum += own[i] = by_count ? static_cast<double>(l.bin_count[4 * lane + i]) : l.bin_weight[4 * lane + i];
+      double at = -sum;
       for (int step = 1; step < 64; step *= 2) {
         const double add = __shfl_up(sum, step);
         if (lane >= step) sum += add;
       }
-      sum += before;
+      at += sum;
       const uint64_t past = __builtin_amdgcn_ballot_w64(sum >= want);
       if (lane == (past ? __builtin_ctzll(past) : 63)) {
-        double at = sum - own;
         int bin = 4 * lane;
-#pragma unroll 1
-        for (;; ++bin) {
-          const double v = by_count ? static_cast<double>(l.bin_count[bin]) : l.bin_weight[bin];
-          if (at + v >= want || bin == 4 * lane + 3) break;
-          at += v;
-        }
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+          if (bin == 4 * lane + i && at + own[i] < want) {
+            at += own[i];
+            ++bin;
+          }
         l.found = past ? bin : kBins - 1;
         l.chosen = at;
       }
@@ -580,69 +565,75 @@ template <typename T> struct RowWork {
     __syncthreads();
     return bin;
   }
+  __device__ __forceinline__ double weight_before(int bin) {  // of the bins
+    const int lane = threadIdx.x & 63;
+    double sum = 0.;
+    for (int i = lane; i < bin; i += 64) sum += l.bin_weight[i];
+    return wave_sum(sum);
+  }
 
-  // The last ranked token before which less than `want` lies (by_count: tokens,
-  // else weight), and the kept weight up to it.  False if lists do not hold what
-  // has to be sorted for it, or bins, whose weights are rounded, do not say where.
-  __device__ __forceinline__ bool threshold(double want, bool by_count, Kept* kept, double* weight) {
-    double ahead, above;
-    const int b = reaches(want, by_count, 0., &ahead);
-    if (b == kBins - 1) return false;
-#pragma unroll 1
-    for (int step = 0; step < (by_count ? 1 : 3); ++step) {  // rounded weights: perhaps the bin next to it
-      const int g = step == 0 ? b : step == 1 ? b - 1 : b + 1;
-      if (g < 0 || g >= kBins - 1) continue;
-      Range range{q_top - g, 0, 255};
-      bool listed = l.bin_count[g] <= static_cast<uint32_t>(kListed);
-      __syncthreads();
-      if (!listed) {  // a 256th of the bin, and a little more
-        look<true>(range, &above);
-        double before = ahead;
-        const int f = reaches(want, by_count, by_count ? ahead : above, &before);
-        ahead = before;  // of a count: up to this 256th
-        range.low = max(0, 255 - f - (by_count ? 0 : 1));
-        range.high = min(255, 255 - f + (by_count ? 0 : 1));
-      }
-      listed = look<false>(range, &above);
-      const int count = l.count;
-      if (!listed || count == 0) {
-        if (range.low == 0 && range.high == 255) continue;
-        return false;  // the bins are not the row's any more
-      }
-      const int i = 2 * threadIdx.x;
-      double w2[2], all;
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        w2[e] = i + e < count ? w.exact(value_of(~static_cast<uint32_t>(l.list[i + e] >> 32))) : 0.;
-      const double upto1 = block_scan(w2[0] + w2[1], l.parts, &all), upto0 = upto1 - w2[1];
-      if (threadIdx.x == 0) l.found = -1;
-      __syncthreads();
-      int at;
-      if (by_count) {
-        at = min(static_cast<int>(want - ahead), count) - 1;
-      } else {
-        if (above < want && above + all >= want) {
-          if (i < count && above + (upto0 - w2[0]) < want) atomicMax(&l.found, i);
-          if (i + 1 < count && above + upto0 < want) atomicMax(&l.found, i + 1);
-        }
-        __syncthreads();
-        at = l.found;
-      }
-      if (at >= 0) {
-        if (i <= at && at <= i + 1) {
-          l.chosen = above + (at == i ? upto0 : upto1);
-          l.upto = l.list[at];
-        }
-        __syncthreads();
-        *weight = l.chosen;
-        *kept = Kept{~static_cast<uint32_t>(l.upto >> 32), static_cast<int>(l.upto)};
-        __syncthreads();
-        return true;
-      }
-      if (range.low != 0 || range.high != 255) return false;
-      __syncthreads();
+  enum Rule { COUNT, WEIGHT, LEAST };
+  // The last ranked token that a rule keeps, and the kept weight up to it: the rank
+  // below `want`; less than `want` before it; a weight of `want`.  bins: in which
+  // first and last bin it was looked for, which the list holds then.  False if that
+  // does not say it.
+  __device__ __forceinline__ bool threshold(Rule rule, double want, Kept* kept, double* weight, int (&bins)[2]) {
+    double ahead = 0.;
+    int low, high;
+    if (rule == LEAST) {  // its logit in 32 bits may be in a bin next to its own
+      const int q = s.bin(static_cast<float>(w.top + log2(want) / s.c));
+      low = max(0, q_top - q - 1);
+      high = q_top - q + 1;
+    } else {
+      low = high = reaches(want, rule == COUNT, &ahead);
     }
-    return false;
+    if (high < 0 || high >= kBins - 1) return false;
+    if (low != bins[0] || high != bins[1]) {
+      bins[0] = low;
+      bins[1] = high;
+      if (!look(low, high)) {
+        bins[0] = -1;
+        return false;
+      }
+    }
+    const int count = l.count;
+    const double above = weight_before(low);
+    double before = above;
+    if (threadIdx.x == 0) l.found = -1;
+    __syncthreads();
+    bool done = false;
+#pragma unroll 1
+    for (int i0 = 0; i0 < count && !done; i0 += kRowThreads) {
+      const int i = i0 + threadIdx.x;
+      const double v = i < count ? listed(i) : 0.;
+      double all;
+      const double upto = before + block_scan(v, l.parts, &all);
+      bool is = false;  // the last that is kept
+      if (i < count) {
+        if (rule == COUNT) is = ahead + i + 1 == want;
+        else if (rule == WEIGHT) is = upto - v < want && (upto >= want || i == count - 1);
+        else is = v >= want && (i == count - 1 || listed(i + 1) < want);
+      }
+      if (is) {
+        l.found = i;
+        l.chosen = upto;
+        l.upto = l.list[i];
+      }
+      __syncthreads();
+      done = l.found >= 0;
+      before += all;
+    }
+    if (!done) {
+      if (rule != LEAST || count == 0) return false;
+      // none of these bins: their first token is the first that is not kept
+      *weight = above;
+      *kept = Kept{~static_cast<uint32_t>(l.list[0] >> 32), -1};
+      return true;
+    }
+    *weight = l.chosen;
+    *kept = Kept{~static_cast<uint32_t>(l.upto >> 32), static_cast<int>(l.upto)};
+    __syncthreads();
+    return true;
   }
 
   // As threshold, digit by digit over all tokens that are kept so far.
@@ -711,7 +702,7 @@ template <typename T> struct RowWork {
 
   // Weights of the blocks' kept tokens, in l.weight; their sum.
   __device__ __forceinline__ double weigh(const Kept& kept, double least) {
-    for (int b = threadIdx.x; b < blocks; b += kRowThreads) l.weight[b] = 0.;
+    for (int b = threadIdx.x; b < 2048; b += kRowThreads) l.weight[b] = 0.;
     __syncthreads();
     each_block([&](float top) { return key_of(top) >= kept.edge; }, [&](const Block<T>& b, int number) {
       double sum = 0.;
@@ -750,59 +741,104 @@ template <typename T> __global__ __launch_bounds__(kRowThreads) void sample_rows
   const Part* part = a.part + r * a.parts;
   RowWork<T> work{a, l, s, w, row, a.block_top + r * a.parts * kPartBlocks, blocks, s.bin(start.top)};
 
-  // the row's bins, by four groups of threads: a part's bin g - shift is the row's bin g
+  if (start.mine.sum > 0.) {
+    l.part_unit[threadIdx.x] = w.exact(start.mine.top) / kBinUnit;
+    // beyond all bins where the part has nothing in them
+    l.part_shift[threadIdx.x] = static_cast<int>(min(static_cast<int64_t>(work.q_top) - start.mine.q, int64_t{kBins}));
+  } else if (static_cast<int>(threadIdx.x) < a.parts) {
+    l.part_unit[threadIdx.x] = 0.;
+    l.part_shift[threadIdx.x] = kBins;
+  }
+  if (threadIdx.x < kBins) l.bin_count[threadIdx.x] = 0;
+  __syncthreads();
+  const uint64_t* bins = a.bins + r * a.parts * kBins;
+  const uint32_t* counts = a.counts + r * a.parts * kBins;
   {
+    // the row's bins, by four groups of threads; the last is nobody's
     const int g = threadIdx.x & (kBins - 1), group = threadIdx.x / kBins;
     uint32_t count = 0;
     double weight = 0.;
+#pragma unroll 4
     for (int p = group; p < a.parts; p += kRowThreads / kBins) {
-      const Part other = part[p];
-      if (!(other.sum > 0.)) continue;
-      const int64_t i = g - (static_cast<int64_t>(work.q_top) - other.q);
-      if (i < 0 || i >= kBins - 1) continue;
-      const uint64_t v = a.bins[(r * a.parts + p) * kBins + i];
-      count += static_cast<uint32_t>(v >> 32);
-      weight += static_cast<double>(static_cast<uint32_t>(v)) * (w.exact(other.top) / kBinUnit);
+      const int i = g - l.part_shift[p];
+      if (i < 0 || g == kBins - 1) continue;
+      if (s.by_count) count += counts[p * kBins + i];
+      weight += static_cast<double>(bins[p * kBins + i]) * l.part_unit[p];
     }
-    if (threadIdx.x < kBins) l.bin_count[g] = 0;
+    if (s.by_count) atomicAdd(&l.bin_count[g], count);
+    l.weight[threadIdx.x] = weight;
     __syncthreads();
-    if (g < kBins - 1) atomicAdd(&l.bin_count[g], count);
-    for (int k = 0; k < kRowThreads / kBins; ++k) {  // in order
-      if (group == k) l.bin_weight[g] = g == kBins - 1 ? 0. : k ? l.bin_weight[g] + weight : weight;
-      __syncthreads();
-    }
-  }
-  // thresholds one by one; for both, the second from the row's bins again
-  Kept kept{0, 0x7fffffff};
-  double base = total;
-  uint32_t bin_count = 0;
-  double bin_weight = 0.;
-  if (threadIdx.x < kBins) {
-    bin_count = l.bin_count[threadIdx.x];
-    bin_weight = l.bin_weight[threadIdx.x];
-  }
-#pragma unroll 1
-  for (int round = 0; round < 2; ++round) {
-    const bool by_count = round == 0;
-    if (!(by_count ? s.by_count : s.by_weight)) continue;
-    const double want = by_count ? static_cast<double>(s.top_k) : static_cast<double>(s.top_p) * base;
-    Kept k;
-    double weight;
-    if (work.threshold(want, by_count, &k, &weight)) {
-      base = weight;
-      if (k.edge > kept.edge || (k.edge == kept.edge && k.last < kept.last)) kept = k;
-    } else {
-      kept = work.by_digits(want, by_count, kept);
-      if (by_count && s.by_weight) base = work.weigh(kept, 0.);
-    }
-    __syncthreads();
-    if (threadIdx.x < kBins) {
-      l.bin_count[threadIdx.x] = bin_count;
-      l.bin_weight[threadIdx.x] = bin_weight;
-    }
+    if (threadIdx.x < kBins) l.bin_weight[g] = (weight + l.weight[g + kBins]) + (l.weight[g + 2 * kBins] + l.weight[g + 3 * kBins]);
     __syncthreads();
   }
   const double least = s.by_least ? static_cast<double>(s.min_p) : 0.;
+  Kept kept{0, 0x7fffffff};
+  int at_bin[2] = {-1, -1};  // of `kept`: the list's bins when it was found
+  int listed[2] = {-1, -1};
+  double base = total;
+  bool known = true;  // that is what is kept
+  typedef RowWork<T> Work;
+#pragma unroll 1
+  for (int i = 0; i < 3; ++i) {
+    const typename Work::Rule rule = i == 0 ? Work::COUNT : i == 1 ? Work::WEIGHT : Work::LEAST;
+    if (!(i == 0 ? s.by_count : i == 1 ? s.by_weight : s.by_least)) continue;
+    const double want = i == 0 ? static_cast<double>(s.top_k) : i == 1 ? static_cast<double>(s.top_p) * base : least;
+    Kept k;
+    double weight;
+    if (known && work.threshold(rule, want, &k, &weight, listed)) {
+      if (k.edge > kept.edge || (k.edge == kept.edge && k.last < kept.last)) {
+        kept = k;
+        base = weight;
+        at_bin[0] = listed[0];
+        at_bin[1] = listed[1];
+      }
+    } else if (i < 2) {
+      known = false;
+      kept = work.by_digits(want, i == 0, kept);
+      if (i == 0 && s.by_weight) base = work.weigh(kept, 0.);
+    } else {
+      known = false;
+    }
+    __syncthreads();
+  }
+  if (known) {
+    if (listed[0] != at_bin[0] || listed[1] != at_bin[1]) work.look(at_bin[0], at_bin[1]);  // it held them
+    // what is kept of each part: its bins above the list's, and of the list
+    if (threadIdx.x < 256) l.radix[threadIdx.x] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < l.count; i += kRowThreads) {
+      const int token = static_cast<int>(l.list[i]);
+      const uint32_t key = ~static_cast<uint32_t>(l.list[i] >> 32);
+      if (key > kept.edge || (key == kept.edge && token <= kept.last))
+        atomicAdd(&l.radix[token / kPart], static_cast<unsigned long long>(work.listed(i) * kUnit + 0.5));
+    }
+    for (int p = threadIdx.x >> 6; p < a.parts; p += kRowWaves) {
+      unsigned long long sum = 0;  // exactly
+      const int end = at_bin[0] - l.part_shift[p];
+      for (int i = threadIdx.x & 63; i < end; i += 64) sum += bins[p * kBins + i];
+      for (int m = 32; m; m >>= 1) sum += __shfl_xor(sum, m);
+      if ((threadIdx.x & 63) == 0) l.weight[p] = static_cast<double>(sum) * l.part_unit[p];
+    }
+    __syncthreads();
+    const double v = static_cast<int>(threadIdx.x) < a.parts
+                         ? l.weight[threadIdx.x] + static_cast<double>(l.radix[threadIdx.x]) / kUnit : 0.;
+    double all;
+    const double upto = block_scan(v, l.parts, &all), goal = u * all;
+    if (threadIdx.x == 0) found[0] = 0x7fffffff, found[1] = -1;
+    __syncthreads();
+    if (v > 0.) {
+      if (upto > goal) atomicMin(&found[0], static_cast<int>(threadIdx.x));
+      atomicMax(&found[1], static_cast<int>(threadIdx.x));
+    }
+    __syncthreads();
+    const int at = found[0] == 0x7fffffff ? found[1] : found[0];
+    if (static_cast<int>(threadIdx.x) == at) l.chosen = upto - v;
+    draw_part<T>(a, row, at, goal, all, w, [&](float x, int i) { return kept.has(x, i); }, found, l.parts, &l.chosen);
+    return;
+  }
+
+  // Too many tokens in one bin (equal ones, or weights that hardly differ): the
+  // kept weights block by block
   const double all = work.weigh(kept, least), goal = u * all;
   // the first block beyond the goal; without one, by rounding, the last that weighs anything
   if (threadIdx.x == 0) found[0] = 0x7fffffff, found[1] = -1;
@@ -836,7 +872,7 @@ int64_t part_count(int64_t vocab) { return (vocab + kPart - 1) / kPart; }
 
 int64_t sample_workspace(int64_t rows, int64_t vocab) {
   const int64_t n = (rows < kChunk ? rows : kChunk) * part_count(vocab);
-  return up16(n * sizeof(Part)) + up16(n * kPartBlocks * 4) + n * kBins * 8;
+  return up16(n * sizeof(Part)) + up16(n * kPartBlocks * 4) + n * kBins * 12;
 }
 
 int sample_launch(const void* logits, const float* uniform, int64_t* tokens, float* logprobs, const float* temperature,
@@ -845,7 +881,7 @@ int sample_launch(const void* logits, const float* uniform, int64_t* tokens, flo
                   hipStream_t stream) {
   SampleArgs a{logits, uniform, tokens, logprobs, temperature, top_k, top_p, min_p, temperature_all, top_k_all,
                top_p_all, min_p_all, 0, 0, stride, vocab, static_cast<int>(part_count(vocab)), false, nullptr, nullptr,
-               nullptr};
+               nullptr, nullptr};
   const int64_t es = dtype == MI355_F32 ? 4 : 2;
   a.aligned = aligned16(logits) && (rows == 1 || stride * es % 16 == 0);
   const int64_t n = (rows < kChunk ? rows : kChunk) * a.parts;
@@ -855,6 +891,7 @@ int sample_launch(const void* logits, const float* uniform, int64_t* tokens, flo
   a.block_top = reinterpret_cast<float*>(at);
   at += up16(n * kPartBlocks * 4);
   a.bins = reinterpret_cast<uint64_t*>(at);
+  a.counts = reinterpret_cast<uint32_t*>(at + n * kBins * 8);
   static const char* what = "sample_tokens launch";
   // known here: no row has filters
   const bool plain = top_k == nullptr && top_p == nullptr && min_p == nullptr && temperature == nullptr &&

@@ -354,6 +354,20 @@ __device__ __forceinline__ float wave_allreduce_sum(float v) {
   return v;
 }
 
+template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_add(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+// Sum of v over this lane and those before it.
+__device__ __forceinline__ int wave_scan(int v) {
+  v = dpp_add<0x111, 0xf>(v);  // row_shr:1
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  v = dpp_add<0x118, 0xf>(v);
+  v = dpp_add<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+  v = dpp_add<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
 // fp32 silu(g) * u with one rounding left to the caller.
 //   sigmoid(g) = 1 / (1 + exp(-g));  exp via v_exp_f32 (2^x) on -g*log2(e),
 //   reciprocal via v_rcp_f32.  g -> -inf gives exp -> inf, rcp -> 0 and the

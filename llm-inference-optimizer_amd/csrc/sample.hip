@@ -26,9 +26,9 @@ namespace mi355 {
 namespace {
 
 constexpr int kPart = 4096, kBlock = 512, kPartBlocks = kPart / kBlock;
-constexpr int kPartThreads = 256, kRowThreads = 1024, kRowWaves = kRowThreads / 64;
+constexpr int kPartThreads = 256, kRowThreads = 512, kRowWaves = kRowThreads / 64;
 constexpr int kBins = 256;          // the last holds all that is further down
-constexpr int kListed = 8192;       // tokens that a row's workgroup sorts
+constexpr int kListed = 8192, kPicked = 512;  // tokens that a row's workgroup lists, and sorts of them
 constexpr int64_t kChunk = 1024;    // rows whose parts the workspace holds
 // Weights in integers, whose sums do not depend on the atomics' order: 4096 of a
 // part, 2^20 of a row fit 64 bits.
@@ -266,15 +266,19 @@ template <typename T> __global__ __launch_bounds__(kPartThreads) void sample_par
 // ------------------------------------------------------------------ a row
 
 struct RowShared {
-  uint64_t list[kListed];      // sorted: key inverted, token
+  uint64_t list[kListed];      // tokens of some bins: key inverted, token
   double weight[2048];         // of blocks: these hold 2^20 tokens
   double parts[kRowWaves + 1];
-  double bin_weight[kBins];
-  uint32_t bin_count[kBins];
+  double bin_weight[kBins], bin_ranks[kBins];  // the row's
+  double steps[kBins], ranks[kBins];           // of a part of the list
   unsigned long long radix[kBins];
+  uint32_t step_count[kBins];
   double part_unit[256];       // weight of a part's bins' unit
   int part_shift[256];         // the row's bin g is the part's bin g - shift
-  int count, found, last;
+  uint64_t picked[kPicked];    // sorted: of the list, the tokens that a threshold is among
+  int count, found, last, picked_count;
+  float above;                 // the least logit above the list's bins
+  unsigned long long low, high;
   uint32_t digit;
   uint64_t upto;
   double chosen;
@@ -347,15 +351,16 @@ template <typename T, typename KEEPS>
 __device__ __forceinline__ void draw_part(const SampleArgs& a, int64_t row, int part, double goal, double total,
                                           const Weights& w, const KEEPS& keeps, int (&found)[2], double* parts,
                                           double* chosen) {
-  // four tokens per thread, then one of them
-  float x[4];
-  double v[4], sum = 0.;
-  const int first = part * kPart + 4 * static_cast<int>(threadIdx.x);
+  // some tokens per thread, then one of them
+  constexpr int OWN = kPart / kRowThreads;
+  float x[OWN];
+  double v[OWN], sum = 0.;
+  const int first = part * kPart + OWN * static_cast<int>(threadIdx.x);
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
+  for (int e = 0; e < OWN; ++e)
     x[e] = fmaxf(load_elem<T>(a.logits, row * a.stride + min(first + e, a.vocab - 1)), -INFINITY);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) sum += v[e] = first + e < a.vocab && keeps(x[e], first + e) ? w.exact(x[e]) : 0.;
+  for (int e = 0; e < OWN; ++e) sum += v[e] = first + e < a.vocab && keeps(x[e], first + e) ? w.exact(x[e]) : 0.;
   __syncthreads();
   double before = *chosen, all;
   if (threadIdx.x == 0) found[0] = 0x7fffffff, found[1] = -1;
@@ -363,7 +368,7 @@ __device__ __forceinline__ void draw_part(const SampleArgs& a, int64_t row, int 
   int token = -1, last = -1;
   double of_token = 0., of_last = 0.;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 0; e < OWN; ++e) {
     before += v[e];
     if (v[e] > 0.) {
       last = first + e;
@@ -476,70 +481,102 @@ template <typename T> struct RowWork {
   int blocks, q_top;
 
   // f(logits of a block, its number), a wave per block, for the blocks of whose
-  // largest logit wanted(it) holds; the next block's logits are on their way.
-  template <typename WANTED, typename F> __device__ __forceinline__ void each_block(const WANTED& wanted, const F& f) const {
+  // largest logit wanted(it) holds; the next AHEAD blocks' logits are on their way.
+  template <int AHEAD, typename WANTED, typename F>
+  __device__ __forceinline__ void each_block(const WANTED& wanted, const F& f) const {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int b0 = wave; b0 < blocks; b0 += 64 * kRowWaves) {
       const int mine = b0 + kRowWaves * lane;
       const float top = mine < blocks ? block_top[mine] : -INFINITY;
       uint64_t todo = __builtin_amdgcn_ballot_w64(top > -INFINITY && wanted(top));
-      Block<T> next;
-      int at = 0;
-      const auto take = [&] {
-        at = b0 + kRowWaves * __builtin_ctzll(todo);
+      Block<T> b[AHEAD];
+      int number[AHEAD];
+      const auto fetch = [&](int i) {
+        number[i] = todo ? b0 + kRowWaves * __builtin_ctzll(todo) : -1;
         todo &= todo - 1;
-        next.load(a, row, at);
+        if (number[i] >= 0) b[i].load(a, row, number[i]);
       };
-      bool more = todo != 0;
-      if (more) take();
-      while (more) {
-        Block<T> b = next;
-        const int number = at;
-        more = todo != 0;
-        if (more) take();
-        b.take(a);
-        f(b, number);
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) fetch(i);
+      bool any = true;
+#pragma unroll 1
+      while (any) {
+        any = false;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+          if (number[i] < 0) continue;
+          any = true;
+          b[i].take(a);
+          f(b[i], number[i]);
+          fetch(i);
+        }
       }
     }
   }
 
-  // Sorts the tokens of the row's bins [low, high]; false if there are too many.
+  // The least logit of bin q or a higher one: its neighbours are looked at by 64
+  // lanes.  False where it is not near q's quotient (bins at the ends of all).
+  __device__ __forceinline__ bool least_of(int q, float* x) const {
+    const float about = static_cast<float>(static_cast<double>(q) / (4. * s.c));
+    if (!(fabsf(about) < 1e37f)) return false;
+    const int lane = threadIdx.x & 63;
+    const float mine = value_of(key_of(about) + static_cast<uint32_t>(lane - 32));
+    const uint64_t from = __builtin_amdgcn_ballot_w64(s.bin(mine) >= q);
+    if (from == 0 || (from & 1)) return false;
+    *x = __shfl(mine, __builtin_ctzll(from));
+    return true;
+  }
+
+  // Lists the tokens of the row's bins [low, high]; false if there are too many.
   __device__ __forceinline__ bool look(int low, int high) {
-    if (threadIdx.x == 0) l.count = 0;
-    __syncthreads();
     const int q_low = q_top - high, q_high = q_top - low;
-    each_block([&](float top) { return s.bin(top) >= q_low; }, [&](const Block<T>& b, int) {
+    float from, to;  // as logits
+    if (!least_of(q_low, &from)) return false;
+    if (low == 0) to = INFINITY;
+    else if (!least_of(q_high + 1, &to)) return false;
+    const bool open = low == 0;
+    if (threadIdx.x == 0) {
+      l.count = 0;
+      l.above = to;
+    }
+    __syncthreads();
+    each_block<4>([&](float top) { return top >= from; }, [&](const Block<T>& b, int) {
+      uint32_t in = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) in |= b.x[e] >= from && (open || b.x[e] < to) ? 1u << e : 0u;
+      if (!__builtin_amdgcn_ballot_w64(in != 0)) return;
+      const int own = __popc(in), upto = wave_scan(own);
+      int at = 0;
+      if ((threadIdx.x & 63) == 63) at = atomicAdd(&l.count, upto);
+      at = __builtin_amdgcn_readlane(at, 63) + upto - own;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float x = b.x[e];
-        const int q = s.bin(x);
-        if (q < q_low || q > q_high || !(x > -INFINITY)) continue;
-        const int i = atomicAdd(&l.count, 1);
-        if (i < kListed) l.list[i] = static_cast<uint64_t>(~key_of(x)) << 32 | static_cast<uint32_t>(b.index(e));
+        if ((in >> e & 1) && at < kListed)
+          l.list[at] = static_cast<uint64_t>(~key_of(b.x[e])) << 32 | static_cast<uint32_t>(b.index(e));
+        at += in >> e & 1;
       }
     });
     __syncthreads();
-    const int count = l.count;
-    if (count > kListed) return false;
-    const int n = power_of_2(count);
-    for (int i = count + threadIdx.x; i < n; i += kRowThreads) l.list[i] = ~uint64_t{0};
-    __syncthreads();
-    sort(l.list, n);
-    return true;
+    return l.count <= kListed;
   }
-  __device__ __forceinline__ double listed(int i) const {
-    return w.exact(value_of(~static_cast<uint32_t>(l.list[i] >> 32)));
+  __device__ __forceinline__ float logit(uint64_t entry) const { return value_of(~static_cast<uint32_t>(entry >> 32)); }
+  // The `count` entries at l.picked, sorted.
+  __device__ __forceinline__ void sort_picked(int count) {
+    const int n = power_of_2(count);
+    for (int i = count + threadIdx.x; i < n; i += kRowThreads) l.picked[i] = ~uint64_t{0};
+    __syncthreads();
+    sort(l.picked, n);
   }
 
-  // The first bin at which the count (weight) of the bins up to it reaches `want`; the
-  // last without one.  *upto: of the bins before it.
-  __device__ __forceinline__ int reaches(double want, bool by_count, double* upto) {
+  // The first of 256 at which the sum up to it reaches `want`; the last without one.
+  // *upto: the sum before it.
+  __device__ __forceinline__ int reaches(double want, const double* sums, double* upto) {
     const int lane = threadIdx.x & 63;
     if (threadIdx.x < 64) {
       double own[4], sum = 0.;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        sum += own[i] = by_count ? static_cast<double>(l.bin_count[4 * lane + i]) : l.bin_weight[4 * lane + i];
+        sum += own[i] = sums[4 * lane + i];
       double at = -sum;
       for (int step = 1; step < 64; step *= 2) {
         const double add = __shfl_up(sum, step);
@@ -585,7 +622,7 @@ template <typename T> struct RowWork {
       low = max(0, q_top - q - 1);
       high = q_top - q + 1;
     } else {
-      low = high = reaches(want, rule == COUNT, &ahead);
+      low = high = reaches(want, rule == COUNT ? l.bin_ranks : l.bin_weight, &ahead);
     }
     if (high < 0 || high >= kBins - 1) return false;
     if (low != bins[0] || high != bins[1]) {
@@ -597,39 +634,118 @@ template <typename T> struct RowWork {
       }
     }
     const int count = l.count;
-    const double above = weight_before(low);
-    double before = above;
+    double above = weight_before(low);
+    if (rule == LEAST) {  // how many of them is what is wanted
+      if (threadIdx.x == 0) l.found = 0;
+      __syncthreads();
+      int some = 0;
+#pragma unroll 1
+      for (int i = threadIdx.x; i < count; i += kRowThreads) some += w.exact(logit(l.list[i])) >= want ? 1 : 0;
+      some = __builtin_amdgcn_readlane(wave_scan(some), 63);
+      if ((threadIdx.x & 63) == 0) atomicAdd(&l.found, some);
+      __syncthreads();
+      some = l.found;
+      __syncthreads();
+      if (some == 0) {  // all that are above them
+        *weight = above;
+        *kept = Kept{key_of(l.above), 0x7fffffff};
+        if (low == 0) return false;  // not: the largest weighs 1
+        return true;
+      }
+      want = some;
+      ahead = 0.;
+    }
+    // the 256th of the entries' range that it is in, again and again
+    unsigned long long from = 0, to = ~0ull;
+    int picked = count;
+#pragma unroll 1
+    while (picked > kPicked) {
+      if (threadIdx.x < kBins) {
+        l.radix[threadIdx.x] = 0;
+        l.step_count[threadIdx.x] = 0;
+      }
+      if (threadIdx.x == 0) {
+        l.low = ~0ull;
+        l.high = 0;
+      }
+      __syncthreads();
+      unsigned long long least = ~0ull, most = 0;
+#pragma unroll 1
+      for (int i = threadIdx.x; i < count; i += kRowThreads) {
+        const unsigned long long e = l.list[i];
+        if (e < from || e > to) continue;
+        least = min(least, e);
+        most = max(most, e);
+      }
+      for (int m = 32; m; m >>= 1) {
+        least = min(least, __shfl_xor(least, m));
+        most = max(most, __shfl_xor(most, m));
+      }
+      if ((threadIdx.x & 63) == 0) {
+        atomicMin(&l.low, least);
+        atomicMax(&l.high, most);
+      }
+      __syncthreads();
+      from = l.low;
+      to = l.high;
+      const int shift = max(0, 56 - __builtin_clzll(to - from));
+#pragma unroll 1
+      for (int i = threadIdx.x; i < count; i += kRowThreads) {
+        const unsigned long long e = l.list[i];
+        if (e < from || e > to) continue;
+        const int step = static_cast<int>((e - from) >> shift);
+        atomicAdd(&l.radix[step], static_cast<unsigned long long>(w.exact(logit(e)) * kUnit + 0.5));
+        atomicAdd(&l.step_count[step], 1u);
+      }
+      __syncthreads();
+      if (threadIdx.x < kBins) {
+        l.steps[threadIdx.x] = static_cast<double>(l.radix[threadIdx.x]) / kUnit;
+        l.ranks[threadIdx.x] = l.step_count[threadIdx.x];
+      }
+      __syncthreads();
+      double before;
+      const int step = reaches(rule == WEIGHT ? want - above : want - ahead, rule == WEIGHT ? l.steps : l.ranks, &before);
+      if (l.step_count[step] == 0) return false;
+      double ranks = 0., weights = 0.;  // of the steps before it
+      for (int i = threadIdx.x & 63; i < step; i += 64) {
+        ranks += l.ranks[i];
+        weights += l.steps[i];
+      }
+      ahead += wave_sum(ranks);
+      above += wave_sum(weights);
+      picked = static_cast<int>(l.step_count[step]);
+      from += static_cast<unsigned long long>(step) << shift;
+      to = min(to, from + ((1ull << shift) - 1));
+      __syncthreads();
+    }
+    if (threadIdx.x == 0) l.picked_count = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int i = threadIdx.x; i < count; i += kRowThreads) {
+      const unsigned long long e = l.list[i];
+      if (e >= from && e <= to) l.picked[atomicAdd(&l.picked_count, 1)] = e;
+    }
+    __syncthreads();
+    sort_picked(picked);
     if (threadIdx.x == 0) l.found = -1;
     __syncthreads();
-    bool done = false;
-#pragma unroll 1
-    for (int i0 = 0; i0 < count && !done; i0 += kRowThreads) {
-      const int i = i0 + threadIdx.x;
-      const double v = i < count ? listed(i) : 0.;
+    {
+      const int i = threadIdx.x;
+      const double v = i < picked ? w.exact(logit(l.picked[i])) : 0.;
       double all;
-      const double upto = before + block_scan(v, l.parts, &all);
+      const double upto = above + block_scan(v, l.parts, &all);
       bool is = false;  // the last that is kept
-      if (i < count) {
-        if (rule == COUNT) is = ahead + i + 1 == want;
-        else if (rule == WEIGHT) is = upto - v < want && (upto >= want || i == count - 1);
-        else is = v >= want && (i == count - 1 || listed(i + 1) < want);
+      if (i < picked) {
+        is = rule == WEIGHT ? upto - v < want && (upto >= want || i == picked - 1) : ahead + i + 1 == want;
       }
       if (is) {
         l.found = i;
         l.chosen = upto;
-        l.upto = l.list[i];
+        l.upto = l.picked[i];
       }
       __syncthreads();
-      done = l.found >= 0;
-      before += all;
     }
-    if (!done) {
-      if (rule != LEAST || count == 0) return false;
-      // none of these bins: their first token is the first that is not kept
-      *weight = above;
-      *kept = Kept{~static_cast<uint32_t>(l.list[0] >> 32), -1};
-      return true;
-    }
+    if (l.found < 0) return false;
     *weight = l.chosen;
     *kept = Kept{~static_cast<uint32_t>(l.upto >> 32), static_cast<int>(l.upto)};
     __syncthreads();
@@ -646,7 +762,7 @@ template <typename T> struct RowWork {
     for (int shift = 24; shift >= 0; shift -= 8) {
       if (threadIdx.x < 256) l.radix[threadIdx.x] = 0;
       __syncthreads();
-      each_block([&](float top) { return key_of(top) >= max(within.edge, prefix); }, [&](const Block<T>& b, int) {
+      each_block<1>([&](float top) { return key_of(top) >= max(within.edge, prefix); }, [&](const Block<T>& b, int) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const uint32_t k = key_of(b.x[e]);
@@ -704,7 +820,7 @@ template <typename T> struct RowWork {
   __device__ __forceinline__ double weigh(const Kept& kept, double least) {
     for (int b = threadIdx.x; b < 2048; b += kRowThreads) l.weight[b] = 0.;
     __syncthreads();
-    each_block([&](float top) { return key_of(top) >= kept.edge; }, [&](const Block<T>& b, int number) {
+    each_block<1>([&](float top) { return key_of(top) >= kept.edge; }, [&](const Block<T>& b, int number) {
       double sum = 0.;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -716,12 +832,14 @@ template <typename T> struct RowWork {
       if ((threadIdx.x & 63) == 0) l.weight[number] = sum;
     });
     __syncthreads();
-    double all;
-    const int i = 2 * threadIdx.x;
-    const double w0 = i < blocks ? l.weight[i] : 0., w1 = i + 1 < blocks ? l.weight[i + 1] : 0.;
-    const double upto = block_scan(w0 + w1, l.parts, &all);
-    if (i < blocks) l.weight[i] = upto - w1;  // up to a block, and it
-    if (i + 1 < blocks) l.weight[i + 1] = upto;
+    double all, sum = 0.;
+    constexpr int OWN = 2048 / kRowThreads;
+    const int first = OWN * threadIdx.x;
+#pragma unroll 1
+    for (int e = 0; e < OWN; ++e) sum += l.weight[first + e];
+    double upto = block_scan(sum, l.parts, &all) - sum;
+#pragma unroll 1
+    for (int e = 0; e < OWN; ++e) l.weight[first + e] = upto += l.weight[first + e];  // up to a block, and it
     __syncthreads();
     return all;
   }
@@ -749,26 +867,39 @@ template <typename T> __global__ __launch_bounds__(kRowThreads) void sample_rows
     l.part_unit[threadIdx.x] = 0.;
     l.part_shift[threadIdx.x] = kBins;
   }
-  if (threadIdx.x < kBins) l.bin_count[threadIdx.x] = 0;
   __syncthreads();
   const uint64_t* bins = a.bins + r * a.parts * kBins;
   const uint32_t* counts = a.counts + r * a.parts * kBins;
   {
-    // the row's bins, by four groups of threads; the last is nobody's
+    // the row's bins, by two groups of threads; the last is nobody's
     const int g = threadIdx.x & (kBins - 1), group = threadIdx.x / kBins;
     uint32_t count = 0;
     double weight = 0.;
-#pragma unroll 4
-    for (int p = group; p < a.parts; p += kRowThreads / kBins) {
-      const int i = g - l.part_shift[p];
-      if (i < 0 || g == kBins - 1) continue;
-      if (s.by_count) count += counts[p * kBins + i];
-      weight += static_cast<double>(bins[p * kBins + i]) * l.part_unit[p];
+    for (int p0 = group; p0 < a.parts; p0 += 8 * (kRowThreads / kBins)) {
+      uint64_t v[8];
+      uint32_t n[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {  // all on their way at once
+        const int p = p0 + e * (kRowThreads / kBins), i = p < a.parts ? g - l.part_shift[p] : -1;
+        const bool in = i >= 0 && g != kBins - 1;
+        v[e] = in ? bins[p * kBins + i] : 0;
+        n[e] = in && s.by_count ? counts[p * kBins + i] : 0;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int p = min(p0 + e * (kRowThreads / kBins), a.parts - 1);
+        count += n[e];
+        weight += static_cast<double>(v[e]) * l.part_unit[p];
+      }
     }
-    if (s.by_count) atomicAdd(&l.bin_count[g], count);
     l.weight[threadIdx.x] = weight;
+    l.weight[kRowThreads + threadIdx.x] = count;
     __syncthreads();
-    if (threadIdx.x < kBins) l.bin_weight[g] = (weight + l.weight[g + kBins]) + (l.weight[g + 2 * kBins] + l.weight[g + 3 * kBins]);
+    static_assert(kRowThreads == 2 * kBins, "groups of threads");
+    if (threadIdx.x < kBins) {
+      l.bin_weight[g] = weight + l.weight[g + kBins];
+      l.bin_ranks[g] = count + l.weight[kRowThreads + g + kBins];
+    }
     __syncthreads();
   }
   const double least = s.by_least ? static_cast<double>(s.min_p) : 0.;
@@ -810,13 +941,15 @@ template <typename T> __global__ __launch_bounds__(kRowThreads) void sample_rows
       const int token = static_cast<int>(l.list[i]);
       const uint32_t key = ~static_cast<uint32_t>(l.list[i] >> 32);
       if (key > kept.edge || (key == kept.edge && token <= kept.last))
-        atomicAdd(&l.radix[token / kPart], static_cast<unsigned long long>(work.listed(i) * kUnit + 0.5));
+        atomicAdd(&l.radix[token / kPart], static_cast<unsigned long long>(w.exact(work.logit(l.list[i])) * kUnit + 0.5));
     }
     for (int p = threadIdx.x >> 6; p < a.parts; p += kRowWaves) {
       unsigned long long sum = 0;  // exactly
-      const int end = at_bin[0] - l.part_shift[p];
-      for (int i = threadIdx.x & 63; i < end; i += 64) sum += bins[p * kBins + i];
-      for (int m = 32; m; m >>= 1) sum += __shfl_xor(sum, m);
+      const int end = at_bin[0] - l.part_shift[p], lane = threadIdx.x & 63;
+#pragma unroll
+      for (int i = 0; i < kBins; i += 64) sum += i + lane < end ? bins[p * kBins + i + lane] : 0;
+      if (__builtin_amdgcn_ballot_w64(sum != 0))
+        for (int m = 32; m; m >>= 1) sum += __shfl_xor(sum, m);
       if ((threadIdx.x & 63) == 0) l.weight[p] = static_cast<double>(sum) * l.part_unit[p];
     }
     __syncthreads();

@@ -63,20 +63,6 @@ struct Seq {
   }
 };
 
-template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_add(int v) {
-  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
-}
-// Sum of v over this lane and those before it.
-__device__ __forceinline__ int wave_scan(int v) {
-  v = dpp_add<0x111, 0xf>(v);  // row_shr:1
-  v = dpp_add<0x112, 0xf>(v);
-  v = dpp_add<0x114, 0xf>(v);
-  v = dpp_add<0x118, 0xf>(v);
-  v = dpp_add<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
-  v = dpp_add<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
-  return v;
-}
-
 // The line of tiles: sequence b has Seq::tiles of them for each of its heads
 // and row blocks, head and block outermost.
 struct Line {

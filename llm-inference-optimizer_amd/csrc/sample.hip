@@ -54,7 +54,6 @@ struct SampleArgs {
   float top_p_all, min_p_all;
   int64_t row0, rows, stride;  // of a chunk
   int vocab, parts;
-  bool aligned;                // rows start on 16 bytes
   Part* part;                  // [rows][parts]
   float* block_top;            // [rows][parts * kPartBlocks]
   uint64_t* bins;              // [rows][parts][kBins]: weights relative to the part's largest, of kBinUnit
@@ -138,34 +137,32 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return as_f32(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// Logits of block `block` of a row: 8 per lane, -infinity beyond the vocabulary and
-// for NaN.  index(e): their tokens.
-template <typename T> struct Block {
-  static constexpr int W = pack_width<T>::value;  // consecutive
-  float x[8];
+// Logits of block `block` of a row: 8 per lane, -infinity beyond the vocabulary.
+// PACKETS: rows start on 16 bytes and hold whole packets of 16.
+template <typename T, bool PACKETS> struct Block {
+  static constexpr int W = PACKETS ? pack_width<T>::value : 1;  // consecutive
   int first;
+  u32x4 raw[PACKETS ? 8 / W : 1];
+  float elem[PACKETS ? 1 : 8];
   static __device__ __forceinline__ int place(int e) {  // of element e, from the block's beginning
     const int lane = threadIdx.x & 63;
     return e / W * 64 * W + lane * W + e % W;
   }
-  u32x4 raw[8 / W];
-  bool packets;  // whole ones: not a last one that ends within
   __device__ __forceinline__ void load(const SampleArgs& a, int64_t row, int block) {
     first = block * kBlock;
     const typename T::bits* p = static_cast<const typename T::bits*>(a.logits) + row * a.stride;
-    packets = a.aligned && (first + kBlock <= a.vocab || a.vocab % W == 0);
-    if (packets) {
+    if constexpr (PACKETS) {
       const rsrc_t r = make_rsrc(p, static_cast<uint32_t>(a.vocab) * sizeof(typename T::bits));
 #pragma unroll
       for (int i = 0; i < 8 / W; ++i)
         raw[i] = buf_load16_cached(r, static_cast<uint32_t>((first + place(W * i)) * sizeof(typename T::bits)));
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = load_elem<T>(p, min(first + place(e), a.vocab - 1));
+      for (int e = 0; e < 8; ++e) elem[e] = load_elem<T>(p, min(first + place(e), a.vocab - 1));
     }
   }
-  __device__ __forceinline__ void take(const SampleArgs& a) {
-    if (packets) {
+  __device__ __forceinline__ void take(const SampleArgs& a, float (&x)[8]) const {
+    if constexpr (PACKETS) {
 #pragma unroll
       for (int i = 0; i < 8 / W; ++i) {
         Packet<T> k{raw[i]};
@@ -174,9 +171,10 @@ template <typename T> struct Block {
 #pragma unroll
         for (int e = 0; e < W; ++e) x[W * i + e] = f[e];
       }
-    }
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = fmaxf(x[e], -INFINITY);  // NaN
+      for (int e = 0; e < 8; ++e) x[e] = elem[e];
+    }
     if (first + kBlock > a.vocab) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = first + place(e) < a.vocab ? x[e] : -INFINITY;
@@ -194,7 +192,7 @@ __device__ __forceinline__ double wave_sum(double v) {
   return v;
 }
 
-template <typename T> __global__ __launch_bounds__(kPartThreads) void sample_parts(SampleArgs a) {
+template <typename T, bool PACKETS> __global__ __launch_bounds__(kPartThreads) void sample_parts(SampleArgs a) {
   constexpr int WAVES = kPartThreads / 64, OWN = kPartBlocks / WAVES;  // blocks of a wave
   __shared__ unsigned long long bins[kBins];
   __shared__ uint32_t counts[kBins];
@@ -204,7 +202,8 @@ template <typename T> __global__ __launch_bounds__(kPartThreads) void sample_par
   {
     const int64_t item = blockIdx.x, r = item / a.parts, row = a.row0 + r;
     const int part = static_cast<int>(item - r * a.parts);
-    Block<T> b[OWN];
+    Block<T, PACKETS> b[OWN];
+    float x[OWN][8];
 #pragma unroll
     for (int i = 0; i < OWN; ++i) b[i].load(a, row, part * kPartBlocks + wave * OWN + i);
     const Settings s(a, row);
@@ -213,10 +212,10 @@ template <typename T> __global__ __launch_bounds__(kPartThreads) void sample_par
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < OWN; ++i) {
-      b[i].take(a);
-      float most = b[i].x[0];
+      b[i].take(a, x[i]);
+      float most = -INFINITY;  // NaN is no largest
 #pragma unroll
-      for (int e = 1; e < 8; ++e) most = fmaxf(most, b[i].x[e]);
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, x[i][e]);
       most = wave_max(most);
       if (lane == 0) a.block_top[(r * a.parts + part) * kPartBlocks + wave * OWN + i] = most;
       top = fmaxf(top, most);
@@ -233,7 +232,7 @@ template <typename T> __global__ __launch_bounds__(kPartThreads) void sample_par
 #pragma unroll
         for (int i = 0; i < OWN; ++i)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) sum += weight(b[i].x[e]);
+          for (int e = 0; e < 8; ++e) sum += weight(x[i][e]);
       };
       const auto binned = [&](float x, double v) {
         if (x > -INFINITY) {
@@ -471,7 +470,7 @@ struct Kept {
   }
 };
 
-template <typename T> struct RowWork {
+template <typename T, bool PACKETS> struct RowWork {
   const SampleArgs& a;
   RowShared& l;
   const Settings& s;
@@ -481,34 +480,32 @@ template <typename T> struct RowWork {
   int blocks, q_top;
 
   // f(logits of a block, its number), a wave per block, for the blocks of whose
-  // largest logit wanted(it) holds; the next AHEAD blocks' logits are on their way.
-  template <int AHEAD, typename WANTED, typename F>
+  // largest logit wanted(it) holds; the logits of GROUP blocks are on their way at
+  // once (without branches between the loads, so that each waits for its own).
+  template <int GROUP, typename WANTED, typename F>
   __device__ __forceinline__ void each_block(const WANTED& wanted, const F& f) const {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int b0 = wave; b0 < blocks; b0 += 64 * kRowWaves) {
       const int mine = b0 + kRowWaves * lane;
       const float top = mine < blocks ? block_top[mine] : -INFINITY;
       uint64_t todo = __builtin_amdgcn_ballot_w64(top > -INFINITY && wanted(top));
-      Block<T> b[AHEAD];
-      int number[AHEAD];
-      const auto fetch = [&](int i) {
-        number[i] = todo ? b0 + kRowWaves * __builtin_ctzll(todo) : -1;
-        todo &= todo - 1;
-        if (number[i] >= 0) b[i].load(a, row, number[i]);
-      };
-#pragma unroll
-      for (int i = 0; i < AHEAD; ++i) fetch(i);
-      bool any = true;
 #pragma unroll 1
-      while (any) {
-        any = false;
+      while (todo) {
+        Block<T, PACKETS> b[GROUP];
+        int number[GROUP], n = 0;
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-          if (number[i] < 0) continue;
-          any = true;
-          b[i].take(a);
-          f(b[i], number[i]);
-          fetch(i);
+        for (int i = 0; i < GROUP; ++i) {  // the last one again where there are fewer
+          number[i] = todo ? b0 + kRowWaves * __builtin_ctzll(todo) : number[i ? i - 1 : 0];
+          n += todo ? 1 : 0;
+          todo &= todo - 1;
+          b[i].load(a, row, number[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < GROUP; ++i) {
+          if (i >= n) break;
+          float x[8];
+          b[i].take(a, x);
+          f(b[i], x, number[i]);
         }
       }
     }
@@ -540,10 +537,10 @@ template <typename T> struct RowWork {
       l.above = to;
     }
     __syncthreads();
-    each_block<4>([&](float top) { return top >= from; }, [&](const Block<T>& b, int) {
+    each_block<4>([&](float top) { return top >= from; }, [&](const auto& b, const float (&x)[8], int) {
       uint32_t in = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) in |= b.x[e] >= from && (open || b.x[e] < to) ? 1u << e : 0u;
+      for (int e = 0; e < 8; ++e) in |= x[e] >= from && (open || x[e] < to) ? 1u << e : 0u;
       if (!__builtin_amdgcn_ballot_w64(in != 0)) return;
       const int own = __popc(in), upto = wave_scan(own);
       int at = 0;
@@ -552,7 +549,7 @@ template <typename T> struct RowWork {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         if ((in >> e & 1) && at < kListed)
-          l.list[at] = static_cast<uint64_t>(~key_of(b.x[e])) << 32 | static_cast<uint32_t>(b.index(e));
+          l.list[at] = static_cast<uint64_t>(~key_of(x[e])) << 32 | static_cast<uint32_t>(b.index(e));
         at += in >> e & 1;
       }
     });
@@ -762,13 +759,13 @@ template <typename T> struct RowWork {
     for (int shift = 24; shift >= 0; shift -= 8) {
       if (threadIdx.x < 256) l.radix[threadIdx.x] = 0;
       __syncthreads();
-      each_block<1>([&](float top) { return key_of(top) >= max(within.edge, prefix); }, [&](const Block<T>& b, int) {
+      each_block<1>([&](float top) { return key_of(top) >= max(within.edge, prefix); }, [&](const auto& b, const float (&x)[8], int) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const uint32_t k = key_of(b.x[e]);
-          if (!within.has(b.x[e], b.index(e)) || (k & mask) != prefix) continue;
+          const uint32_t k = key_of(x[e]);
+          if (!within.has(x[e], b.index(e)) || (k & mask) != prefix) continue;
           atomicAdd(&l.radix[k >> shift & 255],
-                    by_count ? 1ull : static_cast<unsigned long long>(w.exact(b.x[e]) * kUnit + 0.5));
+                    by_count ? 1ull : static_cast<unsigned long long>(w.exact(x[e]) * kUnit + 0.5));
         }
       });
       __syncthreads();
@@ -820,13 +817,13 @@ template <typename T> struct RowWork {
   __device__ __forceinline__ double weigh(const Kept& kept, double least) {
     for (int b = threadIdx.x; b < 2048; b += kRowThreads) l.weight[b] = 0.;
     __syncthreads();
-    each_block<1>([&](float top) { return key_of(top) >= kept.edge; }, [&](const Block<T>& b, int number) {
+    each_block<1>([&](float top) { return key_of(top) >= kept.edge; }, [&](const auto& b, const float (&x)[8], int number) {
       double sum = 0.;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        if (!kept.has(b.x[e], b.index(e))) continue;
-        const double v = w.exact(b.x[e]);
-        if (v >= least || b.x[e] == w.top32) sum += v;
+        if (!kept.has(x[e], b.index(e))) continue;
+        const double v = w.exact(x[e]);
+        if (v >= least || x[e] == w.top32) sum += v;
       }
       sum = wave_sum(sum);
       if ((threadIdx.x & 63) == 0) l.weight[number] = sum;
@@ -845,7 +842,7 @@ template <typename T> struct RowWork {
   }
 };
 
-template <typename T> __global__ __launch_bounds__(kRowThreads) void sample_rows(SampleArgs a) {
+template <typename T, bool PACKETS> __global__ __launch_bounds__(kRowThreads) void sample_rows(SampleArgs a) {
   __shared__ RowShared l;
   __shared__ int found[2];
   const int64_t r = blockIdx.x, row = a.row0 + r;
@@ -857,7 +854,7 @@ template <typename T> __global__ __launch_bounds__(kRowThreads) void sample_rows
   if (draw_plain<T>(a, s, start, w, r, row, u, found, l.parts, &l.chosen, &total)) return;
   const int blocks = (a.vocab + kBlock - 1) / kBlock;
   const Part* part = a.part + r * a.parts;
-  RowWork<T> work{a, l, s, w, row, a.block_top + r * a.parts * kPartBlocks, blocks, s.bin(start.top)};
+  RowWork<T, PACKETS> work{a, l, s, w, row, a.block_top + r * a.parts * kPartBlocks, blocks, s.bin(start.top)};
 
   if (start.mine.sum > 0.) {
     l.part_unit[threadIdx.x] = w.exact(start.mine.top) / kBinUnit;
@@ -908,7 +905,7 @@ template <typename T> __global__ __launch_bounds__(kRowThreads) void sample_rows
   int listed[2] = {-1, -1};
   double base = total;
   bool known = true;  // that is what is kept
-  typedef RowWork<T> Work;
+  typedef RowWork<T, PACKETS> Work;
 #pragma unroll 1
   for (int i = 0; i < 3; ++i) {
     const typename Work::Rule rule = i == 0 ? Work::COUNT : i == 1 ? Work::WEIGHT : Work::LEAST;
@@ -1013,10 +1010,10 @@ int sample_launch(const void* logits, const float* uniform, int64_t* tokens, flo
                   float top_p_all, float min_p_all, int64_t rows, int vocab, int64_t stride, int dtype, void* work,
                   hipStream_t stream) {
   SampleArgs a{logits, uniform, tokens, logprobs, temperature, top_k, top_p, min_p, temperature_all, top_k_all,
-               top_p_all, min_p_all, 0, 0, stride, vocab, static_cast<int>(part_count(vocab)), false, nullptr, nullptr,
+               top_p_all, min_p_all, 0, 0, stride, vocab, static_cast<int>(part_count(vocab)), nullptr, nullptr,
                nullptr, nullptr};
   const int64_t es = dtype == MI355_F32 ? 4 : 2;
-  a.aligned = aligned16(logits) && (rows == 1 || stride * es % 16 == 0);
+  const bool packets = aligned16(logits) && vocab * es % 16 == 0 && (rows == 1 || stride * es % 16 == 0);
   const int64_t n = (rows < kChunk ? rows : kChunk) * a.parts;
   uint8_t* at = static_cast<uint8_t*>(work);
   a.part = reinterpret_cast<Part*>(at);
@@ -1036,9 +1033,15 @@ int sample_launch(const void* logits, const float* uniform, int64_t* tokens, flo
   };
   for (a.row0 = 0; a.row0 < rows; a.row0 += kChunk) {
     a.rows = rows - a.row0 < kChunk ? rows - a.row0 : kChunk;
-    const int st = dtype == MI355_F32   ? run(sample_parts<F32>, plain ? sample_plain<F32> : sample_rows<F32>)
-                   : dtype == MI355_F16 ? run(sample_parts<F16>, plain ? sample_plain<F16> : sample_rows<F16>)
-                                        : run(sample_parts<BF16>, plain ? sample_plain<BF16> : sample_rows<BF16>);
+    int st;
+    const auto typed = [&](auto t) {
+      typedef decltype(t) T;
+      if (packets) return run(sample_parts<T, true>, plain ? sample_plain<T> : sample_rows<T, true>);
+      return run(sample_parts<T, false>, plain ? sample_plain<T> : sample_rows<T, false>);
+    };
+    if (dtype == MI355_F32) st = typed(F32{});
+    else if (dtype == MI355_F16) st = typed(F16{});
+    else st = typed(BF16{});
     if (st != MI355_OK) return st;
   }
   return MI355_OK;

@@ -265,7 +265,7 @@ template <typename T, bool PACKETS> __global__ __launch_bounds__(kPartThreads) v
 // ------------------------------------------------------------------ a row
 
 struct RowShared {
-  uint64_t list[kListed];      // tokens of some bins: key inverted, token
+  uint64_t list[kListed + 64]; // tokens of some bins: key inverted, token
   double weight[2048];         // of blocks: these hold 2^20 tokens
   double parts[kRowWaves + 1];
   double bin_weight[kBins], bin_ranks[kBins];  // the row's
@@ -479,11 +479,11 @@ template <typename T, bool PACKETS> struct RowWork {
   const float* block_top;
   int blocks, q_top;
 
-  // f(logits of a block, its number), a wave per block, for the blocks of whose
-  // largest logit wanted(it) holds; the logits of GROUP blocks are on their way at
-  // once (without branches between the loads, so that each waits for its own).
+  // f(blocks, their logits, how many), a wave per block, for the blocks of whose
+  // largest logit wanted(it) holds, in groups whose logits are on their way at once
+  // (without branches between the loads, so that each waits for its own).
   template <int GROUP, typename WANTED, typename F>
-  __device__ __forceinline__ void each_block(const WANTED& wanted, const F& f) const {
+  __device__ __forceinline__ void each_group(const WANTED& wanted, const F& f) const {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int b0 = wave; b0 < blocks; b0 += 64 * kRowWaves) {
       const int mine = b0 + kRowWaves * lane;
@@ -492,23 +492,25 @@ template <typename T, bool PACKETS> struct RowWork {
 #pragma unroll 1
       while (todo) {
         Block<T, PACKETS> b[GROUP];
-        int number[GROUP], n = 0;
+        float x[GROUP][8];
+        int number = 0, n = 0;
 #pragma unroll
         for (int i = 0; i < GROUP; ++i) {  // the last one again where there are fewer
-          number[i] = todo ? b0 + kRowWaves * __builtin_ctzll(todo) : number[i ? i - 1 : 0];
+          number = todo ? b0 + kRowWaves * __builtin_ctzll(todo) : number;
           n += todo ? 1 : 0;
           todo &= todo - 1;
-          b[i].load(a, row, number[i]);
+          b[i].load(a, row, number);
         }
 #pragma unroll
-        for (int i = 0; i < GROUP; ++i) {
-          if (i >= n) break;
-          float x[8];
-          b[i].take(a, x);
-          f(b[i], x, number[i]);
-        }
+        for (int i = 0; i < GROUP; ++i) b[i].take(a, x[i]);
+        f(b, x, n);
       }
     }
+  }
+  // f(block, its logits, its number), one by one.
+  template <typename WANTED, typename F>
+  __device__ __forceinline__ void each_block(const WANTED& wanted, const F& f) const {
+    each_group<1>(wanted, [&](const auto& b, const float (&x)[1][8], int) { f(b[0], x[0], b[0].first / kBlock); });
   }
 
   // The least logit of bin q or a higher one: its neighbours are looked at by 64
@@ -537,20 +539,31 @@ template <typename T, bool PACKETS> struct RowWork {
       l.above = to;
     }
     __syncthreads();
-    each_block<4>([&](float top) { return top >= from; }, [&](const auto& b, const float (&x)[8], int) {
+    const int lane = threadIdx.x & 63;
+    each_group<4>([&](float top) { return top >= from; }, [&](const auto& b, const float (&x)[4][8], int n) {
       uint32_t in = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) in |= x[e] >= from && (open || x[e] < to) ? 1u << e : 0u;
-      if (!__builtin_amdgcn_ballot_w64(in != 0)) return;
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) in |= x[i][e] >= from && (open || x[i][e] < to) ? 1u << (8 * i + e) : 0u;
+      in = n < 4 ? in & ((1u << 8 * n) - 1) : in;
+      const uint64_t some = __builtin_amdgcn_ballot_w64(in != 0);
+      if (!some) return;
       const int own = __popc(in), upto = wave_scan(own);
       int at = 0;
-      if ((threadIdx.x & 63) == 63) at = atomicAdd(&l.count, upto);
+      if (lane == 63) at = atomicAdd(&l.count, upto);
       at = __builtin_amdgcn_readlane(at, 63) + upto - own;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if ((in >> e & 1) && at < kListed)
-          l.list[at] = static_cast<uint64_t>(~key_of(x[e])) << 32 | static_cast<uint32_t>(b.index(e));
-        at += in >> e & 1;
+      for (int i = 0; i < 4; ++i) {
+        if (!__builtin_amdgcn_ballot_w64((in >> 8 * i & 0xff) != 0)) continue;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          // without a branch: what is not listed goes to the lane's place behind the list
+          const bool is = in >> (8 * i + e) & 1;
+          l.list[is && at < kListed ? at : kListed + lane] =
+              static_cast<uint64_t>(~key_of(x[i][e])) << 32 | static_cast<uint32_t>(b[i].index(e));
+          at += is ? 1 : 0;
+        }
       }
     });
     __syncthreads();
@@ -759,7 +772,7 @@ template <typename T, bool PACKETS> struct RowWork {
     for (int shift = 24; shift >= 0; shift -= 8) {
       if (threadIdx.x < 256) l.radix[threadIdx.x] = 0;
       __syncthreads();
-      each_block<1>([&](float top) { return key_of(top) >= max(within.edge, prefix); }, [&](const auto& b, const float (&x)[8], int) {
+      each_block([&](float top) { return key_of(top) >= max(within.edge, prefix); }, [&](const auto& b, const float (&x)[8], int) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const uint32_t k = key_of(x[e]);
@@ -817,7 +830,7 @@ template <typename T, bool PACKETS> struct RowWork {
   __device__ __forceinline__ double weigh(const Kept& kept, double least) {
     for (int b = threadIdx.x; b < 2048; b += kRowThreads) l.weight[b] = 0.;
     __syncthreads();
-    each_block<1>([&](float top) { return key_of(top) >= kept.edge; }, [&](const auto& b, const float (&x)[8], int number) {
+    each_block([&](float top) { return key_of(top) >= kept.edge; }, [&](const auto& b, const float (&x)[8], int number) {
       double sum = 0.;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {

@@ -64,8 +64,9 @@ def test_shared_prefix_empty_is_noop(L, lib):
     (dict(cache=dict(pages=1 << 30)), -2, "limits"), (dict(batch=1 << 20, cache=dict(table_width=1 << 11, table_stride=1 << 11), stride=1 << 11), -2, "limits"),
     (dict(lens=0), -1, "null"), (dict(out=0), -1, "null"), (dict(missing=0), -1, "null"),
     (dict(out=P, stride=9), -1, "in place"), (dict(cache=dict(page_table=0), out=P + 64), -1, "null"),
-    (dict(cache=dict(pages=0)), -1, "without pages"), (dict(work=None), -1, "workspace"), (dict(work=P + 4), -1, "workspace"),
-    (dict(bytes=16), -1, "workspace"), (dict(cache=dict(page_size=20)), -2, "page_size")])
+    (dict(cache=dict(pages=0)), -1, "without pages"), (dict(cache=dict(pages=10 ** 6), work=None), -1, "workspace"),
+    (dict(batch=2000, work=P + 4), -1, "workspace"), (dict(batch=5000, bytes=16), -1, "workspace"),
+    (dict(cache=dict(page_size=20)), -2, "page_size")])
 def test_reserve_abi_rejects(L, lib, kw, code, message):
     a = dict(lens=P, out=P + 4096, stride=8, missing=P, batch=3, work=P, bytes=1 << 30, cache={})
     a.update(kw)
@@ -77,7 +78,7 @@ def test_reserve_abi_rejects(L, lib, kw, code, message):
     (dict(batch=-1), -1, "sizes"), (dict(tokens=-1), -1, "sizes"), (dict(batch=1 << 24), -2, "limits"),
     (dict(tokens=1 << 31), -2, "limits"), (dict(batch=0), -1, "no sequence"), (dict(lens=0), -1, "null"),
     (dict(new=0), -1, "null"), (dict(slots=0), -1, "null"), (dict(cache=dict(page_table=0)), -1, "null"),
-    (dict(cache=dict(table_width=0)), -1, "without pages"), (dict(work=P + 8), -1, "workspace")])
+    (dict(cache=dict(table_width=0)), -1, "without pages"), (dict(batch=5000, work=P + 8), -1, "workspace")])
 def test_slot_map_abi_rejects(L, lib, kw, code, message):
     a = dict(lens=P, new=P, slots=P, batch=3, tokens=5, work=P, bytes=1 << 20, cache={})
     a.update(kw)

@@ -44,7 +44,8 @@ For several continuations of a prompt: ``kv_cache_reserve`` and ``kv_slot_map``
 (page tables and slot maps from the requests' lengths),
 ``shared_prefix_attention`` (a prefix read and computed once for all sequences
 that share it) and ``sample_tokens`` (temperature, top-k, top-p and min-p from
-given random numbers).
+given random numbers).  ``GraphedSamplingDecoder`` decodes on them, n samples of
+each prompt, the whole step in one graph.
 
 The kernels live in ``libmi355_fused.so`` (gfx950 HIP, C ABI in
 ``include/mi355_fused.h``), built by ``build.py``.
@@ -54,6 +55,7 @@ from .engine.fused_norm_activation_patch import (DECODER_LAYER_CLASS_NAMES, MLP_
                                                  FusedDecoderLayer, FusedMLP, FusedRMSNorm,
                                                  patch_model_with_fused_kernels)
 from .engine.graphed_decode import GraphedGreedyDecoder
+from .engine.graphed_sampling import GraphedSamplingDecoder
 from .kernels.fused_rmsnorm_hip import fused_add_rmsnorm, fused_rmsnorm, naive_rmsnorm_reference
 from .kernels.fused_gate_up_hip import GATE_UP_MAX_ROWS, fused_gate_up_silu, naive_gate_up_silu_reference
 from .kernels.fused_swiglu_hip import fused_silu_mul, naive_silu_mul_reference
@@ -77,4 +79,5 @@ __all__ = [
     "fused_rotary", "rotary_frequencies", "KVCache", "KV_FORMATS", "kv_cache_append", "kv_cache_read",
     "kv_cache_keep", "tree_attention", "TREE_ATTENTION_MAX_TOKENS", "CachedAttention", "DecoderCache",
     "ATTENTION_CLASS_NAMES", "kv_cache_reserve", "kv_slot_map", "shared_prefix_attention", "sample_tokens",
+    "GraphedSamplingDecoder",
 ]

@@ -327,7 +327,8 @@ struct RowStart {
 
 __device__ __forceinline__ void write(const SampleArgs& a, int64_t row, int token, double p) {
   a.tokens[row] = token;
-  if (a.logprobs) a.logprobs[row] = p > 0. ? static_cast<float>(log(p)) : -INFINITY;
+  // sums of rounded weights may be a last bit below one of them
+  if (a.logprobs) a.logprobs[row] = p > 0. ? static_cast<float>(log(fmin(p, 1.))) : -INFINITY;
 }
 
 // The first of `n` threads' tokens (thread t's is first + t) that goes beyond

@@ -22,6 +22,7 @@ from __future__ import annotations
 import torch
 
 from ..kernels.kv_cache_hip import KVCache, kv_cache_append, kv_cache_keep, kv_cache_read
+from ..kernels.shared_prefix_hip import shared_prefix_attention
 from ..kernels.tree_attention_hip import TREE_ATTENTION_MAX_TOKENS, tree_attention
 
 __all__ = ["CachedAttention", "DecoderCache", "ATTENTION_CLASS_NAMES"]
@@ -38,6 +39,10 @@ class DecoderCache:
     or of a draft).  HF's forward sees an empty cache of its own kind through
     ``as_past()``: it builds no buffers for it.
 
+    ``shared_prefix`` (None, or int32 [groups]): every batch / groups sequences share
+    that many of their first slots, which ``shared_prefix_attention`` then reads and
+    computes once for all of them.
+
     ``prompt``: the cache is empty before the step, which may then have more tokens
     than ``tree_attention`` takes.
 
@@ -53,12 +58,13 @@ class DecoderCache:
         self.rotary_scale = rotary_scale
         batch = layers[0].page_table.shape[0]
         self.lens = torch.zeros((batch,), dtype=torch.int32, device=layers[0].k.device)
-        self.positions = self.new_lens = self.tree_mask = None
+        self.positions = self.new_lens = self.tree_mask = self.shared_prefix = None
         self.prompt = self.unmasked = False
 
     @classmethod
-    def allocate(cls, model, batch_size: int, max_len: int, kv_format: str, page_size: int | None = None):
-        """For an HF causal LM whose attention modules are ``CachedAttention``."""
+    def allocate(cls, model, batch_size: int, max_len: int, kv_format: str, page_size: int | None = None,
+                 pages: int | None = None):
+        """For an HF causal LM whose attention modules are ``CachedAttention``.  pages: as in ``KVCache.allocate``."""
         blocks = [layer.self_attn for layer in model.model.layers]
         if not all(isinstance(b, CachedAttention) for b in blocks):
             raise ValueError("kv_cache needs the model's attention patched: "
@@ -69,7 +75,7 @@ class DecoderCache:
                              "would keep old ones")
         p = next(model.parameters())
         layers = [KVCache.allocate(batch_size, max_len, b.k_proj.out_features // b.head_dim, b.head_dim, kv_format,
-                                   p.dtype, p.device, page_size) for b in blocks]
+                                   p.dtype, p.device, page_size, pages) for b in blocks]
         table = layers[0].page_table
         for c in layers:
             c.page_table = table
@@ -150,7 +156,10 @@ class CachedAttention(torch.nn.Module):
         cache = state.layers[self.layer_idx]
         q = kv_cache_append(cache, k, v, state.lens, new_lens=state.new_lens, q=q, positions=state.positions,
                             inv_freq=state.inv_freq, scale=state.rotary_scale)
-        if tokens <= TREE_ATTENTION_MAX_TOKENS:
+        if state.shared_prefix is not None and tokens <= TREE_ATTENTION_MAX_TOKENS:
+            out = shared_prefix_attention(q, cache, state.lens, state.shared_prefix, new_lens=state.new_lens,
+                                          tree_mask=state.tree_mask, scale=self.scaling)
+        elif tokens <= TREE_ATTENTION_MAX_TOKENS:
             out = tree_attention(q, cache, state.lens, new_lens=state.new_lens, tree_mask=state.tree_mask,
                                  scale=self.scaling)
         elif not state.prompt:

@@ -45,11 +45,12 @@ class KVCache:
     @classmethod
     def allocate(cls, batch: int, max_len: int, kv_heads: int, head_dim: int, kv_format: str = "int8",
                  dtype: torch.dtype = torch.float16, device: torch.device | str = "cuda",
-                 page_size: int | None = None) -> "KVCache":
+                 page_size: int | None = None, pages: int | None = None) -> "KVCache":
         """An empty cache of ``max_len`` slots (rounded up to whole pages) for
         each of ``batch`` sequences, its pages in order; one page per sequence
-        without ``page_size``.  kv_format: "16bit" (of ``dtype``), "int8" or
-        "e4m3"."""
+        without ``page_size``.  With ``pages``, a pool of that many and a table
+        without any, which ``kv_cache_reserve`` hands out.  kv_format: "16bit" (of
+        ``dtype``), "int8" or "e4m3"."""
         if kv_format not in KV_FORMATS:
             raise ValueError(f"unknown kv_format {kv_format!r} ({', '.join(KV_FORMATS)})")
         if page_size is None:
@@ -58,13 +59,18 @@ class KVCache:
             raise ValueError("page_size and head_dim must be multiples of 16, head_dim at most 256 "
                              f"(got {page_size}, {head_dim})")
         per = max(1, -(-max_len // page_size))
-        shape = (batch * per, kv_heads, page_size, head_dim)
+        if pages is not None and pages < 1:
+            raise ValueError(f"a pool has at least one page, got {pages}")
+        shape = (batch * per if pages is None else pages, kv_heads, page_size, head_dim)
         quantised = kv_format != "16bit"
         pools = [torch.zeros(shape, dtype=torch.uint8 if quantised else dtype, device=device) for _ in range(2)]
         if quantised:
             pools = [p.view(KV_FORMATS[kv_format]) for p in pools]
         scales = [torch.zeros(shape[:3], dtype=torch.float32, device=device) if quantised else None for _ in range(2)]
-        table = torch.arange(batch * per, dtype=torch.int32, device=device).view(batch, per)
+        if pages is None:
+            table = torch.arange(batch * per, dtype=torch.int32, device=device).view(batch, per)
+        else:
+            table = torch.full((batch, per), -1, dtype=torch.int32, device=device)
         return cls(*pools, table, *scales)
 
     @property

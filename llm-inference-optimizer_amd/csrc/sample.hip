@@ -28,7 +28,7 @@ namespace {
 constexpr int kPart = 4096, kBlock = 512, kPartBlocks = kPart / kBlock;
 constexpr int kPartThreads = 256, kRowThreads = 512, kRowWaves = kRowThreads / 64;
 constexpr int kBins = 256;          // the last holds all that is further down
-constexpr int kListed = 8192, kPicked = 512;  // tokens that a row's workgroup lists, and sorts of them
+constexpr int kListed = 8192, kPicked = 256;  // tokens that a row's workgroup lists, and sorts of them
 constexpr int64_t kChunk = 1024;    // rows whose parts the workspace holds
 // Weights in integers, whose sums do not depend on the atomics' order: 4096 of a
 // part, 2^20 of a row fit 64 bits.
@@ -274,7 +274,9 @@ struct RowShared {
   uint32_t step_count[kBins];
   double part_unit[256];       // weight of a part's bins' unit
   int part_shift[256];         // the row's bin g is the part's bin g - shift
-  uint64_t picked[kPicked];    // sorted: of the list, the tokens that a threshold is among
+  alignas(16) uint64_t picked[kPicked];
+  uint64_t sorted[kPicked];  // of the list, the tokens that a threshold is among
+  int place[kPicked];
   int count, found, last, picked_count;
   float above;                 // the least logit above the list's bins
   unsigned long long low, high;
@@ -438,29 +440,6 @@ template <typename T> __global__ __launch_bounds__(kRowThreads) void sample_plai
   draw_plain<T>(a, s, start, w, r, row, u, found, parts, &chosen, &total);
 }
 
-// Sorts list[0, n) upwards; n a power of 2, entries beyond the last ~0.
-__device__ __forceinline__ void sort(uint64_t* list, int n) {
-  const bool one = n <= 128;  // one wave's work
-  const int threads = one ? 64 : kRowThreads;
-  if (!one || threadIdx.x < 64) {
-    for (int size = 2; size <= n; size *= 2)
-      for (int step = size / 2; step; step /= 2) {
-        for (int i = threadIdx.x; i < n / 2; i += threads) {
-          const int at = 2 * i - (i & (step - 1)), other = at + step;
-          const uint64_t x = list[at], y = list[other];
-          if ((x > y) == ((at & size) == 0)) {
-            list[at] = y;
-            list[other] = x;
-          }
-        }
-        if (one) wave_sync();
-        else __syncthreads();
-      }
-  }
-  __syncthreads();
-}
-__device__ __forceinline__ int power_of_2(int n) { return n <= 2 ? 2 : 1 << (32 - __builtin_clz(n - 1)); }
-
 // Kept are logits above `edge`, and of those equal to it the tokens up to `last`.
 struct Kept {
   uint32_t edge;  // key
@@ -480,9 +459,9 @@ template <typename T, bool PACKETS> struct RowWork {
   const float* block_top;
   int blocks, q_top;
 
-  // f(blocks, their logits, how many), a wave per block, for the blocks of whose
-  // largest logit wanted(it) holds, in groups whose logits are on their way at once
-  // (without branches between the loads, so that each waits for its own).
+  // f(blocks, how many), a wave per block, for the blocks of whose largest logit
+  // wanted(it) holds, in groups of which the next is on its way (without branches
+  // between a group's loads, so that each waits for its own).
   template <int GROUP, typename WANTED, typename F>
   __device__ __forceinline__ void each_group(const WANTED& wanted, const F& f) const {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -490,28 +469,40 @@ template <typename T, bool PACKETS> struct RowWork {
       const int mine = b0 + kRowWaves * lane;
       const float top = mine < blocks ? block_top[mine] : -INFINITY;
       uint64_t todo = __builtin_amdgcn_ballot_w64(top > -INFINITY && wanted(top));
-#pragma unroll 1
-      while (todo) {
-        Block<T, PACKETS> b[GROUP];
-        float x[GROUP][8];
+      Block<T, PACKETS> b[GROUP], next[GROUP];
+      const auto load = [&](Block<T, PACKETS> (&to)[GROUP]) {
         int number = 0, n = 0;
 #pragma unroll
         for (int i = 0; i < GROUP; ++i) {  // the last one again where there are fewer
           number = todo ? b0 + kRowWaves * __builtin_ctzll(todo) : number;
           n += todo ? 1 : 0;
           todo &= todo - 1;
-          b[i].load(a, row, number);
+          to[i].load(a, row, number);
         }
+        return n;
+      };
+      if (!todo) continue;
+      int n = load(b);
+#pragma unroll 1
+      for (;;) {
+        int more = 0;
+        if (todo) more = load(next);
+        f(b, n);
+        if (!more) break;
+        n = more;
 #pragma unroll
-        for (int i = 0; i < GROUP; ++i) b[i].take(a, x[i]);
-        f(b, x, n);
+        for (int i = 0; i < GROUP; ++i) b[i] = next[i];
       }
     }
   }
   // f(block, its logits, its number), one by one.
   template <typename WANTED, typename F>
   __device__ __forceinline__ void each_block(const WANTED& wanted, const F& f) const {
-    each_group<1>(wanted, [&](const auto& b, const float (&x)[1][8], int) { f(b[0], x[0], b[0].first / kBlock); });
+    each_group<1>(wanted, [&](const auto& b, int) {
+      float x[8];
+      b[0].take(a, x);
+      f(b[0], x, b[0].first / kBlock);
+    });
   }
 
   // The least logit of bin q or a higher one: its neighbours are looked at by 64
@@ -530,53 +521,94 @@ template <typename T, bool PACKETS> struct RowWork {
   // Lists the tokens of the row's bins [low, high]; false if there are too many.
   __device__ __forceinline__ bool look(int low, int high) {
     const int q_low = q_top - high, q_high = q_top - low;
-    float from, to;  // as logits
+    float from, to = INFINITY;  // as logits, both of them in
     if (!least_of(q_low, &from)) return false;
-    if (low == 0) to = INFINITY;
-    else if (!least_of(q_high + 1, &to)) return false;
-    const bool open = low == 0;
-    if (threadIdx.x == 0) {
-      l.count = 0;
-      l.above = to;
+    if (low > 0) {
+      float above;
+      if (!least_of(q_high + 1, &above)) return false;
+      if (threadIdx.x == 0) l.above = above;
+      to = value_of(key_of(above) - 1);
     }
+    if (threadIdx.x == 0) l.count = 0;
     __syncthreads();
     const int lane = threadIdx.x & 63;
-    each_group<4>([&](float top) { return top >= from; }, [&](const auto& b, const float (&x)[4][8], int n) {
-      uint32_t in = 0;
+    constexpr int GROUP = 8;
+    each_group<GROUP>([&](float top) { return top >= from; }, [&](const auto& b, int n) {
+      uint64_t in = 0;  // bit 8 i + e: block i's element e
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < GROUP; ++i) {
+        float x[8];
+        b[i].take(a, x);
+        uint32_t of = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) in |= x[i][e] >= from && (open || x[i][e] < to) ? 1u << (8 * i + e) : 0u;
-      in = n < 4 ? in & ((1u << 8 * n) - 1) : in;
-      const uint64_t some = __builtin_amdgcn_ballot_w64(in != 0);
-      if (!some) return;
-      const int own = __popc(in), upto = wave_scan(own);
+        for (int e = 7; e >= 0; --e) of = 2 * of + (__builtin_amdgcn_fmed3f(x[e], from, to) == x[e] ? 1 : 0);
+        in |= static_cast<uint64_t>(i < n ? of : 0) << 8 * i;
+      }
+      if (!__builtin_amdgcn_ballot_w64(in != 0)) return;
+      const int own = __popcll(in), upto = wave_scan(own);
       int at = 0;
       if (lane == 63) at = atomicAdd(&l.count, upto);
       at = __builtin_amdgcn_readlane(at, 63) + upto - own;
+      // few lanes have more than one or two: their numbers, and the logits afterwards
+      while (in) {
+        const int e = __builtin_ctzll(in);
+        int first = b[0].first;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (!__builtin_amdgcn_ballot_w64((in >> 8 * i & 0xff) != 0)) continue;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          // without a branch: what is not listed goes to the lane's place behind the list
-          const bool is = in >> (8 * i + e) & 1;
-          l.list[is && at < kListed ? at : kListed + lane] =
-              static_cast<uint64_t>(~key_of(x[i][e])) << 32 | static_cast<uint32_t>(b[i].index(e));
-          at += is ? 1 : 0;
-        }
+        for (int i = 1; i < GROUP; ++i) first = e >> 3 == i ? b[i].first : first;
+        if (at < kListed) l.list[at] = static_cast<uint32_t>(first + b[0].place(e & 7));
+        ++at;
+        in &= in - 1;
       }
     });
     __syncthreads();
-    return l.count <= kListed;
+    const int count = l.count;
+    if (count > kListed) return false;
+    constexpr int OWN = 8;  // on their way at once
+#pragma unroll 1
+    for (int i0 = threadIdx.x; i0 < count; i0 += OWN * kRowThreads) {
+      uint32_t token[OWN];
+      float x[OWN];
+#pragma unroll
+      for (int e = 0; e < OWN; ++e) token[e] = static_cast<uint32_t>(l.list[min(i0 + e * kRowThreads, count - 1)]);
+#pragma unroll
+      for (int e = 0; e < OWN; ++e) x[e] = load_elem<T>(a.logits, row * a.stride + token[e]);
+#pragma unroll
+      for (int e = 0; e < OWN; ++e)
+        if (i0 + e * kRowThreads < count) l.list[i0 + e * kRowThreads] = static_cast<uint64_t>(~key_of(x[e])) << 32 | token[e];
+    }
+    __syncthreads();
+    return true;
   }
   __device__ __forceinline__ float logit(uint64_t entry) const { return value_of(~static_cast<uint32_t>(entry >> 32)); }
-  // The `count` entries at l.picked, sorted.
+  // The `count` entries at l.picked in order, at l.sorted: each one's place is how
+  // many are before it, which the threads of an entry count a share each of.
   __device__ __forceinline__ void sort_picked(int count) {
-    const int n = power_of_2(count);
-    for (int i = count + threadIdx.x; i < n; i += kRowThreads) l.picked[i] = ~uint64_t{0};
+    constexpr int SHARES = kRowThreads / kPicked;
+    const int e = threadIdx.x % kPicked, share = threadIdx.x / kPicked;
+    if (share == 0) {
+      l.place[e] = 0;
+      if (e >= count) l.picked[e] = ~uint64_t{0};
+    }
     __syncthreads();
-    sort(l.picked, n);
+    const uint64_t mine = l.picked[e];
+    int before = 0;
+    constexpr int AT_ONCE = 4;  // pairs
+#pragma unroll 1
+    for (int i0 = 2 * share; i0 < count; i0 += 2 * SHARES * AT_ONCE) {
+      ulonglong2 other[AT_ONCE];
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i)
+        other[i] = *reinterpret_cast<const ulonglong2*>(&l.picked[(i0 + 2 * SHARES * i) % kPicked]);
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const int more = (other[i].x < mine ? 1 : 0) + (other[i].y < mine ? 1 : 0);
+        before += i0 + 2 * SHARES * i < kPicked ? more : 0;
+      }
+    }
+    atomicAdd(&l.place[e], before);
+    __syncthreads();
+    if (share == 0 && e < count) l.sorted[l.place[e]] = mine;
+    __syncthreads();
   }
 
   // The first of 256 at which the sum up to it reaches `want`; the last without one.
@@ -622,8 +654,8 @@ template <typename T, bool PACKETS> struct RowWork {
 
   enum Rule { COUNT, WEIGHT, LEAST };
   // The last ranked token that a rule keeps, and the kept weight up to it: the rank
-  // below `want`; less than `want` before it; a weight of `want`.  bins: in which
-  // first and last bin it was looked for, which the list holds then.  False if that
+  // below `want`; less than `want` before it; a weight of `want`.  bins: the first and
+  // last bin that the list holds, its own among them.  False if that
   // does not say it.
   __device__ __forceinline__ bool threshold(Rule rule, double want, Kept* kept, double* weight, int (&bins)[2]) {
     double ahead = 0.;
@@ -634,16 +666,22 @@ template <typename T, bool PACKETS> struct RowWork {
       high = q_top - q + 1;
     } else {
       low = high = reaches(want, rule == COUNT ? l.bin_ranks : l.bin_weight, &ahead);
+      // few: all up to it, among which the other rules find theirs
+      if (rule == COUNT && ahead + l.bin_ranks[high] <= kPicked) {
+        low = 0;
+        ahead = 0.;
+      }
     }
     if (high < 0 || high >= kBins - 1) return false;
-    if (low != bins[0] || high != bins[1]) {
+    if (low < bins[0] || high > bins[1]) {
       bins[0] = low;
       bins[1] = high;
       if (!look(low, high)) {
-        bins[0] = -1;
+        bins[0] = kBins;
         return false;
       }
     }
+    low = bins[0];
     const int count = l.count;
     double above = weight_before(low);
     if (rule == LEAST) {  // how many of them is what is wanted
@@ -742,7 +780,7 @@ template <typename T, bool PACKETS> struct RowWork {
     __syncthreads();
     {
       const int i = threadIdx.x;
-      const double v = i < picked ? w.exact(logit(l.picked[i])) : 0.;
+      const double v = i < picked ? w.exact(logit(l.sorted[i])) : 0.;
       double all;
       const double upto = above + block_scan(v, l.parts, &all);
       bool is = false;  // the last that is kept
@@ -752,7 +790,7 @@ template <typename T, bool PACKETS> struct RowWork {
       if (is) {
         l.found = i;
         l.chosen = upto;
-        l.upto = l.picked[i];
+        l.upto = l.sorted[i];
       }
       __syncthreads();
     }
@@ -884,23 +922,28 @@ template <typename T, bool PACKETS> __global__ __launch_bounds__(kRowThreads) vo
   {
     // the row's bins, by two groups of threads; the last is nobody's
     const int g = threadIdx.x & (kBins - 1), group = threadIdx.x / kBins;
+    constexpr int AT_ONCE = 8;
     uint32_t count = 0;
     double weight = 0.;
-    for (int p0 = group; p0 < a.parts; p0 += 8 * (kRowThreads / kBins)) {
-      uint64_t v[8];
-      uint32_t n[8];
+    for (int p0 = group; p0 < a.parts; p0 += AT_ONCE * (kRowThreads / kBins)) {
+      uint64_t v[AT_ONCE];
+      uint32_t n[AT_ONCE];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {  // all on their way at once
-        const int p = p0 + e * (kRowThreads / kBins), i = p < a.parts ? g - l.part_shift[p] : -1;
-        const bool in = i >= 0 && g != kBins - 1;
-        v[e] = in ? bins[p * kBins + i] : 0;
-        n[e] = in && s.by_count ? counts[p * kBins + i] : 0;
+      for (int e = 0; e < AT_ONCE; ++e) {  // all on their way at once, without branches
+        const int p = min(p0 + e * (kRowThreads / kBins), a.parts - 1);
+        v[e] = bins[p * kBins + max(g - l.part_shift[p], 0)];
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
+      for (int e = 0; e < AT_ONCE; ++e) {
         const int p = min(p0 + e * (kRowThreads / kBins), a.parts - 1);
-        count += n[e];
-        weight += static_cast<double>(v[e]) * l.part_unit[p];
+        n[e] = s.by_count ? counts[p * kBins + max(g - l.part_shift[p], 0)] : 0;
+      }
+#pragma unroll
+      for (int e = 0; e < AT_ONCE; ++e) {
+        const int p = p0 + e * (kRowThreads / kBins), last = min(p, a.parts - 1);
+        const bool in = p < a.parts && g >= l.part_shift[last] && g != kBins - 1;
+        count += in ? n[e] : 0;
+        weight += in ? static_cast<double>(v[e]) * l.part_unit[last] : 0.;
       }
     }
     l.weight[threadIdx.x] = weight;
@@ -916,7 +959,7 @@ template <typename T, bool PACKETS> __global__ __launch_bounds__(kRowThreads) vo
   const double least = s.by_least ? static_cast<double>(s.min_p) : 0.;
   Kept kept{0, 0x7fffffff};
   int at_bin[2] = {-1, -1};  // of `kept`: the list's bins when it was found
-  int listed[2] = {-1, -1};
+  int listed[2] = {kBins, -1};
   double base = total;
   bool known = true;  // that is what is kept
   typedef RowWork<T, PACKETS> Work;
@@ -954,14 +997,26 @@ template <typename T, bool PACKETS> __global__ __launch_bounds__(kRowThreads) vo
       if (key > kept.edge || (key == kept.edge && token <= kept.last))
         atomicAdd(&l.radix[token / kPart], static_cast<unsigned long long>(w.exact(work.logit(l.list[i])) * kUnit + 0.5));
     }
-    for (int p = threadIdx.x >> 6; p < a.parts; p += kRowWaves) {
-      unsigned long long sum = 0;  // exactly
-      const int end = at_bin[0] - l.part_shift[p], lane = threadIdx.x & 63;
+    constexpr int AT_ONCE = 4;
+#pragma unroll 1
+    for (int p0 = threadIdx.x >> 6; p0 < a.parts; p0 += AT_ONCE * kRowWaves) {
+      unsigned long long sum[AT_ONCE] = {};  // exactly
+      const int lane = threadIdx.x & 63;
 #pragma unroll
-      for (int i = 0; i < kBins; i += 64) sum += i + lane < end ? bins[p * kBins + i + lane] : 0;
-      if (__builtin_amdgcn_ballot_w64(sum != 0))
-        for (int m = 32; m; m >>= 1) sum += __shfl_xor(sum, m);
-      if ((threadIdx.x & 63) == 0) l.weight[p] = static_cast<double>(sum) * l.part_unit[p];
+      for (int e = 0; e < AT_ONCE; ++e) {
+        const int p = min(p0 + e * kRowWaves, a.parts - 1), end = at_bin[0] - l.part_shift[p];
+#pragma unroll
+        for (int i = 0; i < kBins; i += 64) {
+          const uint64_t v = bins[p * kBins + i + lane];
+          sum[e] += i + lane < end ? v : 0;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < AT_ONCE; ++e) {
+        const int p = p0 + e * kRowWaves;
+        for (int m = 32; m; m >>= 1) sum[e] += __shfl_xor(sum[e], m);
+        if (lane == 0 && p < a.parts) l.weight[p] = static_cast<double>(sum[e]) * l.part_unit[p];
+      }
     }
     __syncthreads();
     const double v = static_cast<int>(threadIdx.x) < a.parts

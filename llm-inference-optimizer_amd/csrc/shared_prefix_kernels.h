@@ -49,16 +49,14 @@ __device__ __forceinline__ void split_weights(const f32x4 (&w)[2], u32x4& hi, u3
   }
 }
 
-// Scores of 32 slots for 16 rows (q . k, without the scale) -> weights times the
-// values' scales, as the two parts of a P^T operand.  f: the scores' factors.
-// Where all rows see all slots the weights are computed at once, relative to the
-// maximum so far, and only if one of them asks for another maximum (false) are the
-// scores looked at.
-template <int NV, typename VT, bool SCALED>
-__device__ __forceinline__ bool weights_at_once(Rows<NV, VT>& rows, f32x4 (&sc)[2], const f32x4 (&f)[2],
-                                                const f32x4 (&vs)[2], u32x4& hi, u32x4& lo) {
+// Weights of 32 slots for 16 rows from their scores (q . k, without the scale; f:
+// the scores' factors), relative to the maximum so far; the largest of a lane's.
+// Where all rows see all slots, and none of the weights asks for another maximum,
+// they are the weights.
+template <int NV, typename VT>
+__device__ __forceinline__ float weights_at_once(const Rows<NV, VT>& rows, const f32x4 (&sc)[2], const f32x4 (&f)[2],
+                                                 f32x4 (&w)[2]) {
   float most = 0.f;
-  f32x4 w[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -66,15 +64,20 @@ __device__ __forceinline__ bool weights_at_once(Rows<NV, VT>& rows, f32x4 (&sc)[
       w[u][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][j], f[u][j], -rows.top));
       most = fmaxf(most, w[u][j]);
     }
-  if (weights_move<VT>(most)) return false;
+  return most;
+}
+// Adds them to the rows' sums; times the values' scales they are the two parts of
+// a P^T operand.
+template <int NV, typename VT, bool SCALED>
+__device__ __forceinline__ void take_weights(Rows<NV, VT>& rows, f32x4 (&w)[2], const f32x4 (&vs)[2], u32x4& hi, u32x4& lo) {
   rows.sum += ((w[0][0] + w[0][1]) + (w[0][2] + w[0][3])) + ((w[1][0] + w[1][1]) + (w[1][2] + w[1][3]));
   if constexpr (SCALED) {
     w[0] *= vs[0];
     w[1] *= vs[1];
   }
   split_weights<VT>(w, hi, lo);
-  return true;
 }
+// The same with masks and another maximum where it is asked for.
 template <int NV, typename VT, bool SCALED>
 __device__ __forceinline__ void weights_by_maximum(Rows<NV, VT>& rows, f32x4 (&sc)[2], const f32x4 (&f)[2],
                                                    const f32x4 (&vs)[2], bool masked, uint32_t seen, u32x4& hi,
@@ -220,52 +223,67 @@ template <typename T, int FMT, int DP, int MT, int SM> struct SharedTiles {
         page_ahead = page(i + 3, all_ahead);
       }
       if (!work) continue;
+      // Two pairs of units: the weights of one, on the vector units, may be computed
+      // between the products of the other, on the matrix units.
+      static_assert(PAIRS == 2, "the order of the steps below");
+      f32x4 sc[PAIRS][MT][2], w[MT][2], f[2], vs[2];
+      float most[MT];
+      const auto scores = [&](int pair) {
 #pragma unroll
-      for (int pair = 0; pair < PAIRS; ++pair) {
-        f32x4 sc[MT][2];
-        const auto scores = [&] {
+        for (int m = 0; m < MT; ++m) sc[pair][m][0] = sc[pair][m][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int m = 0; m < MT; ++m) sc[m][0] = sc[m][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int n = 0; n < NQ; ++n) {
+          const u32x4 k0 = st.k[pair][0][n][lane], k1 = st.k[pair][1][n][lane];
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) {
-            const u32x4 k0 = st.k[pair][0][n][lane], k1 = st.k[pair][1][n][lane];
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-              sc[m][0] = mfma16<T>(k0, q[m][n], sc[m][0]);
-              sc[m][1] = mfma16<T>(k1, q[m][n], sc[m][1]);
-            }
+          for (int m = 0; m < MT; ++m) {
+            sc[pair][m][0] = mfma16<T>(k0, q[m][n], sc[pair][m][0]);
+            sc[pair][m][1] = mfma16<T>(k1, q[m][n], sc[pair][m][1]);
           }
-        };
-        f32x4 f[2] = {{a.scale, a.scale, a.scale, a.scale}, {a.scale, a.scale, a.scale, a.scale}};
-        f32x4 vs[2] = {{1.f, 1.f, 1.f, 1.f}, {1.f, 1.f, 1.f, 1.f}};
-        if constexpr (SCALED) {
+        }
+      };
+      const auto weights = [&](int pair) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < 2; ++u) {
+          f[u] = f32x4{a.scale, a.scale, a.scale, a.scale};
+          vs[u] = f32x4{1.f, 1.f, 1.f, 1.f};
+          if constexpr (SCALED) {
             f[u] *= *reinterpret_cast<const f32x4*>(&st.ks[32 * pair + 16 * u + 4 * quad]);
             vs[u] = *reinterpret_cast<const f32x4*>(&st.vs[32 * pair + 16 * u + 4 * quad]);
           }
         }
-        u32x4 hi[MT], lo[MT];
-        scores();
+#pragma unroll
+        for (int m = 0; m < MT; ++m) most[m] = weights_at_once(rows[m], sc[pair][m], f, w[m]);
+      };
+      u32x4 hi[MT], lo[MT];
+      // masks, or another maximum
+      const auto look = [&](int pair) {
+        bool move = masked;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) move |= weights_move<VT>(most[m]);
+        if (!move) {
+#pragma unroll
+          for (int m = 0; m < MT; ++m) take_weights<NV, VT, SCALED>(rows[m], w[m], vs, hi[m], lo[m]);
+          return;
+        }
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          if (masked || !weights_at_once<NV, VT, SCALED>(rows[m], sc[m], f, vs, hi[m], lo[m])) {
-            uint32_t seen = 0xff;
-            if (masked) {
-              const int slot = p.from + i * TILE + 32 * pair;
-              const int n = p.stop > slot ? (p.stop - slot + 15) / 16 : 0;
-              // a tile with a unit that is not there is looked up anew
-              uint32_t there = n > 1 ? 3u : n;
-              if (there) {
-                const bool in0 = a.c.row(p.w.first, slot, p.h) >= 0;
-                const bool in1 = n > 1 && a.c.row(p.w.first, slot + 16, p.h) >= 0;
-                there = (in0 ? 1u : 0u) | (in1 ? 2u : 0u);
-              }
-              seen = shared_seen(a, p, row[m], slot, there);
+          uint32_t seen = 0xff;
+          if (masked) {
+            const int slot = p.from + i * TILE + 32 * pair;
+            const int n = p.stop > slot ? (p.stop - slot + 15) / 16 : 0;
+            // a tile with a unit that is not there is looked up anew
+            uint32_t there = n > 1 ? 3u : n;
+            if (there) {
+              const bool in0 = a.c.row(p.w.first, slot, p.h) >= 0;
+              const bool in1 = n > 1 && a.c.row(p.w.first, slot + 16, p.h) >= 0;
+              there = (in0 ? 1u : 0u) | (in1 ? 2u : 0u);
             }
-            weights_by_maximum<NV, VT, SCALED>(rows[m], sc[m], f, vs, masked, seen, hi[m], lo[m]);
+            seen = shared_seen(a, p, row[m], slot, there);
           }
+          weights_by_maximum<NV, VT, SCALED>(rows[m], sc[pair][m], f, vs, masked, seen, hi[m], lo[m]);
         }
+      };
+      const auto sums = [&](int pair) {
 #pragma unroll
         for (int x = 0; x < NV; ++x) {
           const u32x4 v = *reinterpret_cast<const u32x4*>(&st.v[pair][x][lane][0]);
@@ -274,7 +292,19 @@ template <typename T, int FMT, int DP, int MT, int SM> struct SharedTiles {
 #pragma unroll
           for (int m = 0; m < MT; ++m) rows[m].o[x] = mfma16<VT>(v, lo[m], rows[m].o[x]);
         }
-      }
+      };
+      // Both pairs' scores first where registers allow it (codes' scales take more of
+      // them): 128 rows under 32768 slots of bf16 149 us instead of 156, but 40
+      // sequences of e4m3 70 instead of 64.
+      scores(0);
+      if constexpr (!SCALED) scores(1);
+      weights(0);
+      look(0);
+      sums(0);
+      if constexpr (SCALED) scores(1);
+      weights(1);
+      look(1);
+      sums(1);
     }
 
     // every wave has its rows to itself; through LDS for whole lines of stores

@@ -353,7 +353,8 @@ template <typename T, typename KEEPS>
 __device__ __forceinline__ void draw_part(const SampleArgs& a, int64_t row, int part, double goal, double total,
                                           const Weights& w, const KEEPS& keeps, int (&found)[2], double* parts,
                                           double* chosen) {
-  // some tokens per thread, then one of them
+  // some tokens per thread, then one of them; part < 0 (nothing weighs anything) cannot be
+  part = max(part, 0);
   constexpr int OWN = kPart / kRowThreads;
   float x[OWN];
   double v[OWN], sum = 0.;
@@ -532,7 +533,7 @@ template <typename T, bool PACKETS> struct RowWork {
     if (threadIdx.x == 0) l.count = 0;
     __syncthreads();
     const int lane = threadIdx.x & 63;
-    constexpr int GROUP = 8;
+    constexpr int GROUP = PACKETS && sizeof(typename T::bits) == 2 ? 6 : 4;  // and the next: more take registers that are not there
     each_group<GROUP>([&](float top) { return top >= from; }, [&](const auto& b, int n) {
       uint64_t in = 0;  // bit 8 i + e: block i's element e
 #pragma unroll

@@ -5,7 +5,10 @@
 // taking the k-th page that nobody keeps.  Bound by launches and by the trips of
 // loads that wait for each other: a table is read and written once, 8 bytes per
 // entry.  Tables of a decode step are one workgroup's work (kv_reserve_one), its
-// pages a bit each in LDS; larger ones take four launches.
+// pages a bit each in LDS; larger ones take four launches.  32 sequences of up to
+// 4001 tokens, 64 a page: 4.1 us, 8.5 with the launch, where the four launches take
+// 17.  4096 sequences of up to 8300 tokens, 16 a page: 30 us, of which clear 2,
+// mark 9, list 3 and assign 16; its 9.6 MB would take 2 us at a copy's rate.
 #include "kv_cache.h"
 
 namespace mi355 {
@@ -297,7 +300,9 @@ template <typename E> __device__ __forceinline__ int sequence_of(const E* ends, 
 }
 
 // Up to 4096 sequences: every workgroup sums their lengths for itself, for 2048
-// tokens, two neighbours per thread and store.
+// tokens, two neighbours per thread and store.  16 sequences of 8 tokens: 3.1 us, 8.5
+// with the launch; 300 prompts of 2.3 million tokens: 19 us, 2.4 TB/s written, where
+// a launch for the sums and one for the rows take 23.
 constexpr int kSlotBatch = 4096, kSlotTokens = 2048;
 
 __global__ __launch_bounds__(kBlock) void kv_slot_rows(SlotsArgs a) {

@@ -93,7 +93,17 @@ __device__ __forceinline__ void weights_by_maximum(Rows<NV, VT>& rows, f32x4 (&s
 }
 
 // One pass over this workgroup's pieces of the line.  Products on MFMA with the
-// layouts of tree_attention.hip.
+// layouts of tree_attention.hip; weights in two parts of 16 bits, so that they are
+// off by 2^-17 and not by 2^-9, which takes half as many products again.
+//
+// Many rows are bound by the vector units (an exponential and a dozen further
+// operations per score), the loads of operands from LDS and the matrix units, which
+// overlap little: 28 query heads' 128 sequences under 32768 slots of bf16 take 149
+// us, of which the products alone are 60 and the fixed work about 35.  Few rows, and
+// short prefixes, are bound by that fixed work: a piece waits for its page numbers,
+// then for its first tiles, 4 to 10 us, whatever its length.  32 sequences under
+// 8011 slots of int8 and 700 of their own: 31 us; 40 with drafts of 6 tokens under 5
+// prefixes of up to 3003 slots of e4m3: 64; 4 under 700: 13.
 template <typename T, int FMT, int DP, int MT, int SM> struct SharedTiles {
   typedef UnitRegs<T, FMT, DP, 0> Regs;  // row blocks of a head meet its cache in the L2
   static constexpr int WAVES = kWaves, NV = Regs::NV, NQ = DP / 32, PITCH = DP + 4;
@@ -346,7 +356,7 @@ template <typename T, int FMT, int DP, int MT, int SM> struct SharedTiles {
 
   // Tiles of 32 slots for up to 16 SM rows: a wave for itself, loads straight to
   // operands, as tree_attention_stream does; the waves join in LDS.
-  static __device__ void few(const SharedArgs& s, const SharedShare& p, Lds& lds, float (&note)[2][WAVES],
+  static __device__ void few(const SharedArgs& s, const SharedShare& p, Lds& lds,
                              float (&tops)[WAVES][16 * SM], float (&sums)[WAVES][16 * SM],
                              int64_t (&out_row)[WAVES][16 * (MT > SM ? MT : SM)]) {
     const TreeArgs& a = s.t;
@@ -504,12 +514,15 @@ __global__ __launch_bounds__(64 * kWaves, shared_groups(DP)) void shared_prefix_
   __shared__ int64_t out_row[K::WAVES][16 * (MT > SM ? MT : SM)];  // where a row's sums go, in rows
   SharedShare p(s);
   while (p.next(s)) {
-    if (p.few) K::few(s, p, lds, note, tops, sums, out_row);
+    if (p.few) K::few(s, p, lds, tops, sums, out_row);
     else K::many(s, p, lds, note, out_row);
     p.done();
   }
 }
 
+// Bound by three trips of loads that wait for each other (where the pieces are,
+// their sums, the row's end): 48 rows 4 us, 896 rows of some 30 pieces 7, 9600 rows 10.
+//
 // Adds the pieces of one query row, those of the prefix and its own, in order:
 // lanes 0 - 31 and 32 - 63 of each of WAVES waves take every 2 WAVES-th piece with
 // a running maximum, 4 (and, beyond 128, 4 more) elements per lane.
@@ -657,6 +670,7 @@ template <typename T> int shared_prefix_run(const SharedArgs& a, const SharedPla
   static const char* what = "shared_prefix_attention join launch";
   const auto grid = [&](int64_t groups) { return dim3(static_cast<unsigned>(groups)); };
   const int64_t rows = a.rows;
+  // as many waves a row as the card has room for at once
   if (8 * rows <= 8192) return launch(shared_prefix_join<T, 8>, grid(rows), 512, 0, a, s, what);
   if (2 * rows <= 8192) return launch(shared_prefix_join<T, 2>, grid(rows), 128, 0, a, s, what);
   return launch(shared_prefix_join<T, 1>, grid((rows + kSharedJoinRows - 1) / kSharedJoinRows), 64 * kSharedJoinRows, 0, a,

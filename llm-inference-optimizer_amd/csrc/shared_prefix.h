@@ -280,16 +280,24 @@ __device__ __forceinline__ uint32_t shared_seen(const TreeArgs& a, const SharedS
   return (below | (row.t < row.fresh ? fresh & edge : 0u)) & own & there;
 }
 
-// Q^T operands of a lane's row.
-template <typename T, int FMT, int NQ>
+// Q^T operands of a lane's row.  AHEAD: loaded before the row's length is here,
+// which takes registers.
+template <typename T, int FMT, bool AHEAD, int NQ>
 __device__ __forceinline__ void shared_queries(const TreeArgs& a, const SharedRow& row, u32x4 (&q)[NQ]) {
   typedef typename T::bits bits;
   const int quad = (threadIdx.x & 63) >> 4;
   const bits* from = static_cast<const bits*>(a.q) + row.b * a.qb + row.t * a.qt + row.hq * a.qh;
+  const auto is = [&](int n) { return row.t < row.fresh && key_element<FMT>(n, quad) < a.c.d; };
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     const int e = key_element<FMT>(n, quad);
-    q[n] = row.t < row.fresh && e < a.c.d ? *reinterpret_cast<const u32x4*>(from + e) : u32x4{0, 0, 0, 0};
+    if constexpr (AHEAD) q[n] = *reinterpret_cast<const u32x4*>(from + (e < a.c.d ? e : 0));
+    else q[n] = is(n) ? *reinterpret_cast<const u32x4*>(from + e) : u32x4{0, 0, 0, 0};
+  }
+  if constexpr (AHEAD) {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+      if (!is(n)) q[n] = u32x4{0, 0, 0, 0};
   }
 }
 

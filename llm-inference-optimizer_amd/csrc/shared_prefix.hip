@@ -166,9 +166,15 @@ bool plan(const mi355_kv_cache& c, int64_t batch, int64_t tokens, int64_t q_head
   const int dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
   const int64_t rows = tokens * (q_heads / c.kv_heads);                         // of a sequence
   const int64_t group_rows = groups ? (batch + groups - 1) / groups * rows : rows;  // on average
-  p.mt = group_rows <= 16 * kWaves || dp == 256 ? 1 : 2;
   p.sm = rows <= 16 ? 1 : 2;
   p.grid = cus * shared_groups(dp);
+  // Blocks of 128 rows, which read a tile half as often as those of 64, unless a
+  // workgroup has few of them: then the sums to write and join, 64 KB a piece, count.
+  // 32 sequences under 8011 slots (2 of 128 a workgroup): 64 rows 28.8 + 6.2 us, 128
+  // rows 30.0 + 7.4; 40 under 3003, drafts (9): 92.9 + 8.5, 66.8 + 10.3; 128 under
+  // 32768 (28): 217 + 7.6, 148 + 9.5.
+  const int64_t all_tiles = c.kv_heads * groups * ((group_rows + 127) / 128) * (c.table_width * c.page_size / 64);
+  p.mt = group_rows <= 16 * kWaves || dp == 256 || all_tiles < 4 * p.grid ? 1 : 2;
   a.few = 16 * p.sm;
   a.block_log = 0;
   while ((1 << a.block_log) < 16 * p.mt * kWaves) ++a.block_log;

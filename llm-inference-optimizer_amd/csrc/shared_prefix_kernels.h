@@ -149,17 +149,17 @@ template <typename T, int FMT, int DP, int MT, int SM> struct SharedTiles {
     const int wave = uniform(threadIdx.x >> 6);
     const int d = a.c.d;
     int pages = load_pages(a, p, p.from), pages_ahead = -1, held = 0;
-    // page of this wave's unit of tile i; all: whether every unit of the tile is there
+    // page of this wave's unit of tile i; there: a bit for each unit of the tile that is there
     constexpr int HELD = 64 / WAVES;  // tiles whose pages 64 lanes hold
-    const auto page = [&](int i, bool& all) {
+    constexpr uint32_t UNITS = (1u << WAVES) - 1;
+    const auto page = [&](int i, uint32_t& there) {
       if (i - held >= HELD) {
         pages = pages_ahead;
         held += HELD;
       }
       if (i - held == HELD - 2) pages_ahead = load_pages(a, p, p.from + (held + HELD) * TILE);
       const int at = WAVES * (i - held);
-      constexpr uint32_t units = (1u << WAVES) - 1;
-      all = (static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(pages >= 0) >> at) & units) == units;
+      there = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(pages >= 0) >> at) & UNITS;
       return __builtin_amdgcn_readlane(pages, at + wave);
     };
     Regs kv;
@@ -168,10 +168,11 @@ template <typename T, int FMT, int DP, int MT, int SM> struct SharedTiles {
       kv.load_keys(u, d);
       kv.load_values(u, d);
     };
-    bool all, all_ahead, left_out = false;
-    const int page0 = page(0, all);
+    bool left_out = false;
+    uint32_t there, there_ahead;
+    const int page0 = page(0, there);
     load(0, page0);
-    int page_ahead = page(1, all_ahead);
+    int page_ahead = page(1, there_ahead);
 
     u32x4 q[MT][NQ];
     SharedRow row[MT];
@@ -180,7 +181,7 @@ template <typename T, int FMT, int DP, int MT, int SM> struct SharedTiles {
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       row[m] = SharedRow(s, p, 16 * (MT * wave + m) + col);
-      shared_queries<T, FMT>(a, row[m], q[m]);
+      shared_queries<T, FMT, MT == 1>(a, row[m], q[m]);
       rows[m].clear();
       below = min(below, row[m].limit);
     }
@@ -191,12 +192,12 @@ template <typename T, int FMT, int DP, int MT, int SM> struct SharedTiles {
     for (int w = 0; w < WAVES; ++w) below = min(below, __builtin_bit_cast(int, note[0][w]));
     below = uniform(below);
     // a tile that not every row sees whole
-    const auto edge = [&](int i, bool whole) {
-      return !whole || p.from + (i + 1) * TILE > min(below, p.stop) || p.from + i * TILE < p.w.begin;
+    const auto edge = [&](int i, uint32_t units) {
+      return units != UNITS || p.from + (i + 1) * TILE > min(below, p.stop) || p.from + i * TILE < p.w.begin;
     };
-    const auto put = [&](int i, bool whole) {
+    const auto put = [&](int i, uint32_t units) {
       Stage& st = lds.stage[i & 1];
-      if (edge(i, whole)) left_out |= kv.take_out_non_finite();
+      if (edge(i, units)) left_out |= kv.take_out_non_finite();
 #pragma unroll
       for (int n = 0; n < NQ; ++n) st.k[wave >> 1][wave & 1][n][lane] = kv.keys(n);
 #pragma unroll
@@ -213,24 +214,25 @@ template <typename T, int FMT, int DP, int MT, int SM> struct SharedTiles {
         }
       }
     };
-    put(0, all);
-    bool all_now = all;  // of the tile in LDS
+    put(0, there);
+    uint32_t there_next = there;  // of the tile in LDS
     load(1, page_ahead);
-    all = all_ahead;
-    page_ahead = page(2, all_ahead);
+    there = there_ahead;
+    page_ahead = page(2, there_ahead);
     const bool work = 16 * MT * wave < p.rows;  // else this wave only loads
 
 #pragma unroll 1
     for (int i = 0; i < p.tiles; ++i) {
       __syncthreads();
       const Stage& st = lds.stage[i & 1];
-      const bool masked = edge(i, all_now);
+      const uint32_t there_now = there_next;
+      const bool masked = edge(i, there_now);
       if (i + 1 < p.tiles) {
-        put(i + 1, all);
-        all_now = all;
+        put(i + 1, there);
+        there_next = there;
         load(i + 2, page_ahead);
-        all = all_ahead;
-        page_ahead = page(i + 3, all_ahead);
+        there = there_ahead;
+        page_ahead = page(i + 3, there_ahead);
       }
       if (!work) continue;
       // Two pairs of units: the weights of one, on the vector units, may be computed
@@ -280,15 +282,7 @@ template <typename T, int FMT, int DP, int MT, int SM> struct SharedTiles {
           uint32_t seen = 0xff;
           if (masked) {
             const int slot = p.from + i * TILE + 32 * pair;
-            const int n = p.stop > slot ? (p.stop - slot + 15) / 16 : 0;
-            // a tile with a unit that is not there is looked up anew
-            uint32_t there = n > 1 ? 3u : n;
-            if (there) {
-              const bool in0 = a.c.row(p.w.first, slot, p.h) >= 0;
-              const bool in1 = n > 1 && a.c.row(p.w.first, slot + 16, p.h) >= 0;
-              there = (in0 ? 1u : 0u) | (in1 ? 2u : 0u);
-            }
-            seen = shared_seen(a, p, row[m], slot, there);
+            seen = shared_seen(a, p, row[m], slot, there_now >> (2 * pair) & 3);
           }
           weights_by_maximum<NV, VT, SCALED>(rows[m], sc[pair][m], f, vs, masked, seen, hi[m], lo[m]);
         }
@@ -386,7 +380,7 @@ template <typename T, int FMT, int DP, int MT, int SM> struct SharedTiles {
 #pragma unroll
     for (int m = 0; m < SM; ++m) {
       row[m] = SharedRow(s, p, 16 * m + col);
-      shared_queries<T, FMT>(a, row[m], q[m]);
+      shared_queries<T, FMT, MT == 1>(a, row[m], q[m]);
       rows[m].clear();
       below = min(below, row[m].limit);
     }

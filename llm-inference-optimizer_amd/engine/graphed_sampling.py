@@ -3,7 +3,8 @@
 ``GraphedSamplingDecoder`` keeps every prompt's keys and values once.  Its step
 
     kv_cache_reserve (a page for the sequences that enter a new one) -> forward, in every layer kv_cache_append and
-    shared_prefix_attention (the prompt read and computed once for all of its continuations) -> sample_tokens
+    shared_prefix_attention (the prompt read and computed once for all of its continuations; of short ones
+    tree_attention) -> sample_tokens
 
 reads and writes static tensors only, so that all of it is one graph: the page table grows, tokens are drawn and fed
 back on the GPU, and the host adds a step's random numbers.  (The greedy decoder's argmax has to stay outside; the
@@ -22,6 +23,13 @@ from .cached_attention import DecoderCache
 
 __all__ = ["GraphedSamplingDecoder"]
 
+# What a layer's tree_attention has to read of the prompts, each once per continuation, from which on
+# shared_prefix_attention is the faster: it has two kinds of pieces to start and to join.  In a graph, int8, 128-wide
+# heads, us of shared_prefix_attention and tree_attention: 12 / 2 heads, 1 x 8 continuations of 1024 tokens (4 MB) 16.1
+# and 10.5; 1 x 32 of 4096 (69 MB) 24.9 and 23.3; 4 x 8 of 4096 (69) 23.2 and 24.7; 4 x 16 of 8192 (277) 32.4 and 60.5;
+# 28 / 4 heads, 4 x 8 of 1024 (35) 22.4 and 19.9; of 2048 (69) 24.4 and 26.7.
+_SHARED_BYTES = 64 << 20
+
 
 class GraphedSamplingDecoder:
     """Sampled generation for an HF causal LM whose attention is patched (``patch_model_with_fused_kernels(model,
@@ -30,18 +38,20 @@ class GraphedSamplingDecoder:
     ``kv_cache``: "16bit", "int8" or "e4m3", in pages of ``page_size`` slots.  ``pages``: how many the pool holds; a
     generation of ``new`` tokens takes ``pages_needed(prompt length, new)`` of them, far fewer than the default, which
     is enough for sequences of ``max_cache_len`` tokens that share nothing.  ``temperature``, ``top_k``, ``top_p`` and
-    ``min_p`` as in ``sample_tokens``: numbers, or tensors that broadcast to [batch_size, samples].  ``use_graph=False``
-    runs the same step eagerly."""
+    ``min_p`` as in ``sample_tokens``: numbers, or tensors that broadcast to [batch_size, samples].  ``share_prefix``:
+    whether attention reads a prompt once for all of its continuations (``shared_prefix_attention``) or for each
+    (``tree_attention``); None: whichever is faster at the prompt's length.  ``use_graph=False`` runs the same step
+    eagerly."""
 
     def __init__(self, model, batch_size: int, samples: int, max_cache_len: int, *, kv_cache: str = "16bit",
                  page_size: int = 64, pages: int | None = None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
-                 use_graph: bool = True):
+                 share_prefix: bool | None = None, use_graph: bool = True):
         if batch_size < 1 or samples < 1:
             raise ValueError(f"batch_size and samples must be at least 1, got {batch_size} and {samples}")
         self.model = model
         self.device = next(model.parameters()).device
         self.batch_size, self.samples, self.max_cache_len = batch_size, samples, max_cache_len
-        self.page_size, self.use_graph = page_size, use_graph
+        self.page_size, self.share_prefix, self.use_graph = page_size, share_prefix, use_graph
         rows = batch_size * samples
         self.pages = rows * -(-max_cache_len // page_size) if pages is None else pages
         self.settings = {name: self._per_row(value, torch.int32 if name == "top_k" else torch.float32)
@@ -55,7 +65,6 @@ class GraphedSamplingDecoder:
                                           for c in self.cache.layers], self.cache.inv_freq, self.cache.rotary_scale)
         self.prompt_cache.unmasked = self.prompt_cache.prompt = True
         self._prefix = torch.zeros((batch_size,), dtype=torch.int32, device=self.device)
-        self.cache.shared_prefix = self._prefix
         self._past, self._prompt_past = self.cache.as_past(), self.prompt_cache.as_past()
         self._one = torch.ones((rows,), dtype=torch.int32, device=self.device)
         self._missing = torch.zeros((rows,), dtype=torch.int32, device=self.device)
@@ -63,7 +72,7 @@ class GraphedSamplingDecoder:
         self._pos = torch.zeros((rows, 1), dtype=torch.long, device=self.device)
         self._uniform = torch.zeros((rows,), dtype=torch.float32, device=self.device)
         self._log = torch.zeros((rows,), dtype=torch.float32, device=self.device)
-        self._graph = None
+        self._graph, self._graphs = None, {}
 
     def _per_row(self, value, dtype):
         if not torch.is_tensor(value):
@@ -75,6 +84,13 @@ class GraphedSamplingDecoder:
         shared = prompt_len // self.page_size
         end = -(-(prompt_len + new_tokens - 1) // self.page_size)
         return self.batch_size * (shared + self.samples * (end - shared))
+
+    def _shares(self, length: int) -> bool:
+        if self.share_prefix is not None:
+            return self.share_prefix
+        c = self.cache.layers[0]
+        token = 2 * c.k.shape[1] * (c.k.shape[3] * c.k.element_size() + (4 if c.k_scale is not None else 0))
+        return self.samples > 1 and self.batch_size * self.samples * length * token >= _SHARED_BYTES
 
     def _sample(self, logits: torch.Tensor) -> None:
         """Draws the rows' next tokens into the step's inputs."""
@@ -137,6 +153,9 @@ class GraphedSamplingDecoder:
                         t = t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t
                         t[to // page, :, to % page] = t[source // page, :, source % page]
         self._prefix.fill_(shared * page)
+        shares = self._shares(length)
+        c.shared_prefix = self._prefix if shares else None
+        self._graph = self._graphs.get(shares)
         self._pos.fill_(length)
         return logits
 
@@ -174,6 +193,7 @@ class GraphedSamplingDecoder:
                 else:
                     if self._graph is None:
                         self._capture()
+                        self._graphs[self.cache.shared_prefix is not None] = self._graph
                     self._graph.replay()
             out[:, i] = self._tok[:, 0]
             logs[:, i] = self._log

@@ -155,3 +155,35 @@ def test_refusals(pkg, cuda):
         with pytest.raises(ValueError):
             call()
     assert math.isfinite(float(dec.generate(ids, 5, return_logprobs=True)[1].sum()))
+
+
+@pytest.mark.parametrize("kind", ["16bit", "int8"])
+def test_prompts_read_once_or_for_each_sample(pkg, cuda, kind):
+    """Both attentions draw from the model, and a decoder follows the prompt's length from one to the other and back."""
+    model = _model(cuda)
+    pkg.patch_model_with_fused_kernels(model, fuse_attention=True, fuse_residual=True)
+    u = torch.rand((2, 5, 40), generator=torch.Generator().manual_seed(71))
+    outs = {}
+    for share in (True, False):
+        dec = pkg.GraphedSamplingDecoder(model, 2, 5, 260, kv_cache=kind, page_size=32, temperature=0.8, share_prefix=share)
+        for length in (77, 200):
+            ids = _prompt(cuda, 2, length)
+            out, logs = dec.generate(ids, 40, uniform=u, return_logprobs=True)
+            assert (dec.cache.shared_prefix is not None) == share
+            want = torch.log_softmax(_reference(model, ids, out) / 0.8, -1).gather(-1, out[:, :, length:, None])[..., 0]
+            assert (logs - want).abs().max().item() <= 2 * LOGIT_TOL[kind] / 0.8
+            outs[share, length] = out
+    dec = pkg.GraphedSamplingDecoder(model, 2, 5, 260, kv_cache=kind, page_size=32, temperature=0.8)
+    dec._shares = lambda length: length > 100
+    for length in (77, 200, 77):
+        assert torch.equal(dec.generate(_prompt(cuda, 2, length), 40, uniform=u), outs[length > 100, length])
+    assert len(dec._graphs) == 2
+
+
+def test_which_attention(pkg, cuda):
+    """The rule: what the prompts' continuations would read, keys and values of 2 heads of 64 with scales, 272 bytes a token."""
+    model = _model(cuda)
+    pkg.patch_model_with_fused_kernels(model, fuse_attention=True)
+    dec = pkg.GraphedSamplingDecoder(model, 4, 16, 4096, kv_cache="int8", pages=64)
+    assert not dec._shares(64 * 2 ** 20 // (64 * 272) - 1) and dec._shares(64 * 2 ** 20 // (64 * 272) + 1)
+    assert not pkg.GraphedSamplingDecoder(model, 64, 1, 4096, kv_cache="int8", pages=64)._shares(4096)

@@ -38,7 +38,7 @@ constexpr int kPart = 4096, kBlock = 512, kPartBlocks = kPart / kBlock;
 constexpr int kPartThreads = 256, kRowThreads = 512, kRowWaves = kRowThreads / 64;
 constexpr int kBins = 256;          // the last holds all that is further down
 constexpr int kListed = 8192, kPicked = 256;  // tokens that a row's workgroup lists, and sorts of them
-constexpr int64_t kChunk = 1024;    // rows whose parts the workspace holds
+constexpr int64_t kChunkParts = 32768;  // parts that the workspace holds, of whole rows: 100 MB
 // Weights in integers, whose sums do not depend on the atomics' order: 4096 of a
 // part, 2^20 of a row fit 64 bits.
 constexpr double kBinUnit = 0x1p50, kUnit = 0x1p43;
@@ -1077,11 +1077,15 @@ template <typename T, bool PACKETS> __global__ __launch_bounds__(kRowThreads) vo
 
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 int64_t part_count(int64_t vocab) { return (vocab + kPart - 1) / kPart; }
+int64_t chunk_rows(int64_t rows, int64_t vocab) {
+  const int64_t most = kChunkParts / part_count(vocab);
+  return rows < most ? rows : most;
+}
 
 }  // namespace
 
 int64_t sample_workspace(int64_t rows, int64_t vocab) {
-  const int64_t n = (rows < kChunk ? rows : kChunk) * part_count(vocab);
+  const int64_t n = chunk_rows(rows, vocab) * part_count(vocab);
   return up16(n * sizeof(Part)) + up16(n * kPartBlocks * 4) + n * kBins * 12;
 }
 
@@ -1094,7 +1098,7 @@ int sample_launch(const void* logits, const float* uniform, int64_t* tokens, flo
                nullptr, nullptr};
   const int64_t es = dtype == MI355_F32 ? 4 : 2;
   const bool packets = aligned16(logits) && vocab * es % 16 == 0 && (rows == 1 || stride * es % 16 == 0);
-  const int64_t n = (rows < kChunk ? rows : kChunk) * a.parts;
+  const int64_t chunk = chunk_rows(rows, vocab), n = chunk * a.parts;
   uint8_t* at = static_cast<uint8_t*>(work);
   a.part = reinterpret_cast<Part*>(at);
   at += up16(n * sizeof(Part));
@@ -1111,8 +1115,8 @@ int sample_launch(const void* logits, const float* uniform, int64_t* tokens, flo
     const int st = launch(parts, dim3(static_cast<unsigned>(a.rows * a.parts)), kPartThreads, 0, a, stream, what);
     return st != MI355_OK ? st : launch(draw, dim3(static_cast<unsigned>(a.rows)), kRowThreads, 0, a, stream, what);
   };
-  for (a.row0 = 0; a.row0 < rows; a.row0 += kChunk) {
-    a.rows = rows - a.row0 < kChunk ? rows - a.row0 : kChunk;
+  for (a.row0 = 0; a.row0 < rows; a.row0 += chunk) {
+    a.rows = rows - a.row0 < chunk ? rows - a.row0 : chunk;
     int st;
     const auto typed = [&](auto t) {
       typedef decltype(t) T;

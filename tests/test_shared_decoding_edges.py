@@ -26,6 +26,20 @@ def test_more_rows_than_the_workspace_holds(pkg, cuda):
     assert torch.equal(tokens[1024:], pkg.sample_tokens(x[1024:].to(cuda), u[1024:].to(cuda)))
 
 
+@pytest.mark.parametrize("rows,vocab", [(32768 + 5, 40), (2 * 128 + 3, 2 ** 20 - 8)])
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=9, top_p=0.9)], ids=str)
+def test_rows_beyond_one_pass(pkg, cuda, rows, vocab, settings):
+    """More 4096ths of rows than 32768: rows are taken in turns, and draw what they draw alone."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    x = (torch.randn((rows, vocab), generator=g, device=cuda) * 3).half()
+    u = torch.rand((rows,), generator=g, device=cuda)
+    tokens = pkg.sample_tokens(x, u, **settings)
+    for first, last in ((0, 100), (100, 129), (rows // 2, rows // 2 + 9), (rows - 9, rows)):
+        assert torch.equal(tokens[first:last], pkg.sample_tokens(x[first:last], u[first:last], **settings))
+    at = [0, 127, 128, rows - 6, rows - 1]
+    _check(pkg, cuda, x[at].cpu(), u[at].cpu(), **settings)
+
+
 @pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("vocab", [2 ** 20 - 1, 2 ** 20 - 16])
 def test_the_largest_vocabulary(pkg, cuda, kind, vocab):

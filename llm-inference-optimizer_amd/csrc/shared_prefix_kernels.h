@@ -102,8 +102,8 @@ __device__ __forceinline__ void weights_by_maximum(Rows<NV, VT>& rows, f32x4 (&s
 // us, of which the products alone are 60 and the fixed work about 35.  Few rows, and
 // short prefixes, are bound by that fixed work: a piece waits for its page numbers,
 // then for its first tiles, 4 to 10 us, whatever its length.  32 sequences under
-// 8011 slots of int8 and 700 of their own: 31 us; 40 with drafts of 6 tokens under 5
-// prefixes of up to 3003 slots of e4m3: 64; 4 under 700: 13.
+// 8011 slots of int8 and 700 of their own: 29 us; 40 with drafts of 6 tokens under 5
+// prefixes of up to 3003 slots of e4m3: 65; 4 under 700: 12.
 template <typename T, int FMT, int DP, int MT, int SM> struct SharedTiles {
   typedef UnitRegs<T, FMT, DP, 0> Regs;  // row blocks of a head meet its cache in the L2
   static constexpr int WAVES = kWaves, NV = Regs::NV, NQ = DP / 32, PITCH = DP + 4;
@@ -515,7 +515,7 @@ __global__ __launch_bounds__(64 * kWaves, shared_groups(DP)) void shared_prefix_
 }
 
 // Bound by three trips of loads that wait for each other (where the pieces are,
-// their sums, the row's end): 48 rows 4 us, 896 rows of some 30 pieces 7, 9600 rows 10.
+// their sums, the row's end): 48 rows 4 us, 896 rows of some 30 pieces 6, 9600 rows 10.
 //
 // Adds the pieces of one query row, those of the prefix and its own, in order:
 // lanes 0 - 31 and 32 - 63 of each of WAVES waves take every 2 WAVES-th piece with

@@ -25,7 +25,10 @@ def shared_prefix_attention(q: torch.Tensor, cache: KVCache, seq_lens: torch.Ten
 
     The other arguments and the result are those of ``tree_attention``: q [batch, tokens, q_heads, head_dim], at most
     ``TREE_ATTENTION_MAX_TOKENS`` new tokens per sequence, which are in the cache already, behind ``seq_lens[b]`` others
-    (the prefix among them)."""
+    (the prefix among them).
+
+    Where all members' page tables name the prefix's pages, ``tree_attention`` computes the same, and is faster while it
+    would read less than about 64 MB of prefixes, once for each member."""
     if scale is None:
         scale = cache.k.shape[-1] ** -0.5
     return _lib.ext().shared_prefix_attention(q, cache.k, cache.v, cache.page_table, cache.k_scale, cache.v_scale,

@@ -169,11 +169,12 @@ bool plan(const mi355_kv_cache& c, int64_t batch, int64_t tokens, int64_t q_head
   p.sm = rows <= 16 ? 1 : 2;
   p.grid = cus * shared_groups(dp);
   // Blocks of 128 rows, which read a tile half as often as those of 64, unless a
-  // workgroup has few of them: then the sums to write and join, 64 KB a piece, count.
+  // workgroup has few tiles: then the sums to write and join, 64 KB a piece, count.
   // 32 sequences under 8011 slots (2 of 128 a workgroup): 64 rows 28.8 + 6.2 us, 128
   // rows 30.0 + 7.4; 40 under 3003, drafts (9): 92.9 + 8.5, 66.8 + 10.3; 128 under
   // 32768 (28): 217 + 7.6, 148 + 9.5.
-  const int64_t all_tiles = c.kv_heads * groups * ((group_rows + 127) / 128) * (c.table_width * c.page_size / 64);
+  const int64_t of_128 = groups * ((group_rows + 127) / 128) + (rows > 32 ? batch * ((rows + 127) / 128) : 0);
+  const int64_t all_tiles = c.kv_heads * of_128 * (c.table_width * c.page_size / 64);
   p.mt = group_rows <= 16 * kWaves || dp == 256 || all_tiles < 4 * p.grid ? 1 : 2;
   a.few = 16 * p.sm;
   a.block_log = 0;

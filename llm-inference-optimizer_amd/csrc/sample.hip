@@ -532,13 +532,12 @@ template <typename T, bool PACKETS> struct RowWork {
   // Lists the tokens of the row's bins [low, high]; false if there are too many.
   __device__ __forceinline__ bool look(int low, int high) {
     const int q_low = q_top - high, q_high = q_top - low;
-    float from, to = INFINITY;  // as logits, both of them in
+    const bool open = low == 0;
+    float from, to = INFINITY;  // as logits
     if (!least_of(q_low, &from)) return false;
-    if (low > 0) {
-      float above;
-      if (!least_of(q_high + 1, &above)) return false;
-      if (threadIdx.x == 0) l.above = above;
-      to = value_of(key_of(above) - 1);
+    if (!open) {
+      if (!least_of(q_high + 1, &to)) return false;
+      if (threadIdx.x == 0) l.above = to;
     }
     if (threadIdx.x == 0) l.count = 0;
     __syncthreads();
@@ -552,7 +551,7 @@ template <typename T, bool PACKETS> struct RowWork {
         b[i].take(a, x);
         uint32_t of = 0;
 #pragma unroll
-        for (int e = 7; e >= 0; --e) of = 2 * of + (__builtin_amdgcn_fmed3f(x[e], from, to) == x[e] ? 1 : 0);
+        for (int e = 7; e >= 0; --e) of = 2 * of + ((x[e] >= from) & ((x[e] < to) | open) ? 1 : 0);
         in |= static_cast<uint64_t>(i < n ? of : 0) << 8 * i;
       }
       if (!__builtin_amdgcn_ballot_w64(in != 0)) return;

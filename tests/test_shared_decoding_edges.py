@@ -119,3 +119,18 @@ def test_more_groups_than_threads(pkg, cuda):
     cache, q, lens, starts = _setup(pkg, "int8", F16, (2, 1, 64), sizes, prefix, own, 1, 16, 67)
     out = pkg.shared_prefix_attention(q, cache, ints(lens), ints(prefix), ints(starts))
     close(out, *attention(q, cache, lens, prefix, starts))
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("settings", [dict(top_k=360), dict(top_k=400, temperature=0.7), dict(top_p=0.5), dict(top_p=0.6, temperature=2.0),
+                                      dict(min_p=0.58), dict(top_k=900, top_p=0.55)], ids=str)
+def test_thresholds_right_below_zeros(pkg, cuda, kind, settings):
+    """Bins of logits end at 0: zeros of both signs belong to the one above."""
+    g = torch.Generator().manual_seed(73)
+    x = torch.full((4, 3000), -3.0)
+    x[:, :300] = 0.0
+    x[:, 300:400] = -0.0
+    x[:, 400:900] = -0.002 - 0.1 * torch.rand((4, 500), generator=g)
+    x[:, 900:910] = 0.5
+    x = x[:, torch.randperm(3000, generator=g)]
+    _check(pkg, cuda, x.to(TYPES[kind]), torch.rand((4,), generator=g), **settings)

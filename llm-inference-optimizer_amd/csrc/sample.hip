@@ -30,13 +30,13 @@
 // nucleus, sharp and flat, 37 for 256 rows of 32000 with settings of their own, 18
 // for 512 without filters.
 #include "common.h"
+#include "sample_bins.h"
 
 namespace mi355 {
 namespace {
 
 constexpr int kPart = 4096, kBlock = 512, kPartBlocks = kPart / kBlock;
 constexpr int kPartThreads = 256, kRowThreads = 512, kRowWaves = kRowThreads / 64;
-constexpr int kBins = 256;          // the last holds all that is further down
 constexpr int kListed = 8192, kPicked = 256;  // tokens that a row's workgroup lists, and sorts of them
 constexpr int64_t kChunkParts = 32768;  // parts that the workspace holds, of whole rows: 100 MB
 // Weights in integers, whose sums do not depend on the atomics' order: 4096 of a
@@ -86,11 +86,7 @@ struct Settings {
     by_least = !greedy && min_p > 0.f;
   }
   __device__ __forceinline__ bool filters() const { return by_count || by_weight || by_least; }
-  // The bin of a logit: a monotone function of it alone, a quarter of a power of 2 of
-  // weight wide.
-  __device__ __forceinline__ int bin(float x) const {
-    return static_cast<int>(fminf(fmaxf(floorf(x * (4.f * static_cast<float>(c))), -1e9f), 1e9f));
-  }
+  __device__ __forceinline__ int bin(float x) const { return bin_of(x, bins_per_unit(c)); }
 };
 
 // 2^t for -1000 <= t <= 1/2: 1 + f g(f), with the polynomial g of degree 8 that meets
@@ -246,7 +242,7 @@ template <typename T, bool PACKETS> __global__ __launch_bounds__(kPartThreads) v
       };
       const auto binned = [&](float x, double v) {
         if (x > -INFINITY) {
-          const int l = min(q - s.bin(x), kBins - 1);
+          const int l = bin_in_part(q, s.bin(x));
           // v times the unit, rounded, in the low 52 bits
           const uint64_t fixed = __builtin_bit_cast(uint64_t, __builtin_fma(v, kBinUnit, 0x1p52)) & 0xfffffffffffffull;
           atomicAdd(&bins[l], static_cast<unsigned long long>(fixed));
@@ -921,7 +917,7 @@ template <typename T, bool PACKETS> __global__ __launch_bounds__(kRowThreads) vo
   if (start.mine.sum > 0.) {
     l.part_unit[threadIdx.x] = w.exact(start.mine.top) / kBinUnit;
     // beyond all bins where the part has nothing in them
-    l.part_shift[threadIdx.x] = static_cast<int>(min(static_cast<int64_t>(work.q_top) - start.mine.q, int64_t{kBins}));
+    l.part_shift[threadIdx.x] = shift_of_part(work.q_top, start.mine.q);
   } else if (static_cast<int>(threadIdx.x) < a.parts) {
     l.part_unit[threadIdx.x] = 0.;
     l.part_shift[threadIdx.x] = kBins;

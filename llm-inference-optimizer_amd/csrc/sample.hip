@@ -39,9 +39,11 @@ constexpr int kPart = 4096, kBlock = 512, kPartBlocks = kPart / kBlock;
 constexpr int kPartThreads = 256, kRowThreads = 512, kRowWaves = kRowThreads / 64;
 constexpr int kListed = 8192, kPicked = 256;  // tokens that a row's workgroup lists, and sorts of them
 constexpr int64_t kChunkParts = 32768;  // parts that the workspace holds, of whole rows: 100 MB
-// Weights in integers, whose sums do not depend on the atomics' order: 4096 of a
-// part, 2^20 of a row fit 64 bits.
-constexpr double kBinUnit = 0x1p50, kUnit = 0x1p43;
+// Weights in whole numbers, whose sums do not depend on the atomics' order: 4096 of a
+// part's, 2^20 of a row's fit 64 bits.  The row's are in two words, of 2^-43 and 2^-86
+// (Fixed): a light token's weight may be little next to the first word's unit, but
+// thousands of them are not, and with a small random number one of them is drawn.
+constexpr double kBinUnit = 0x1p51, kUnit = 0x1p43;
 constexpr float kHottest = 1e30f;   // temperatures beyond (infinity) have no weight range to clamp to
 
 struct Part {
@@ -132,6 +134,20 @@ struct Weights {
     if (top32 == INFINITY) return x == INFINITY ? 1. : 0.;
     const double t = (static_cast<double>(x) - top) * c;
     return t < -1000. ? 0. : exp2_64(t);
+  }
+};
+
+// A weight from 0 to 1 in two words, and what sums of them are.
+struct Fixed {
+  unsigned long long high, low;  // low: with a sign
+  __device__ __forceinline__ explicit Fixed(double v) {
+    const double a = __builtin_fma(v, kUnit, 0x1p52);  // rounded to whole numbers, which its low bits hold
+    const double b = __builtin_fma(__builtin_fma(v, kUnit, -(a - 0x1p52)), kUnit, 0x1.8p52);
+    high = __builtin_bit_cast(uint64_t, a) - __builtin_bit_cast(uint64_t, 0x1p52);
+    low = __builtin_bit_cast(uint64_t, b) - __builtin_bit_cast(uint64_t, 0x1.8p52);
+  }
+  static __device__ __forceinline__ double value(unsigned long long high, unsigned long long low) {
+    return (static_cast<double>(high) + static_cast<double>(static_cast<int64_t>(low)) / kUnit) / kUnit;
   }
 };
 
@@ -244,6 +260,7 @@ template <typename T, bool PACKETS> __global__ __launch_bounds__(kPartThreads) v
         if (x > -INFINITY) {
           const int l = bin_in_part(q, s.bin(x));
           // v times the unit, rounded, in the low 52 bits
+          static_assert(kBinUnit <= 0x1p51, "2^52 more has the same exponent");
           const uint64_t fixed = __builtin_bit_cast(uint64_t, __builtin_fma(v, kBinUnit, 0x1p52)) & 0xfffffffffffffull;
           atomicAdd(&bins[l], static_cast<unsigned long long>(fixed));
           if (s.by_count) atomicAdd(&counts[l], 1u);
@@ -276,7 +293,7 @@ struct RowShared {
   double parts[kRowWaves + 1];
   double bin_weight[kBins], bin_ranks[kBins];  // the row's
   double steps[kBins], ranks[kBins];           // of a part of the list
-  unsigned long long radix[kBins];
+  unsigned long long radix[kBins], radix_low[kBins];  // Fixed sums; of counts the first alone
   uint32_t step_count[kBins];
   double part_unit[256];       // weight of a part's bins' unit
   int part_shift[256];         // the row's bin g is the part's bin g - shift
@@ -585,6 +602,12 @@ template <typename T, bool PACKETS> struct RowWork {
     __syncthreads();
     return true;
   }
+  // to one of l.radix
+  __device__ __forceinline__ void add(int at, double v) const {
+    const Fixed f(v);
+    atomicAdd(&l.radix[at], f.high);
+    atomicAdd(&l.radix_low[at], f.low);
+  }
   __device__ __forceinline__ float logit(uint64_t entry) const { return value_of(~static_cast<uint32_t>(entry >> 32)); }
   // The `count` entries at l.picked in order, at l.sorted: each one's place is how
   // many are before it, which the threads of an entry count a share each of.
@@ -716,7 +739,7 @@ template <typename T, bool PACKETS> struct RowWork {
 #pragma unroll 1
     while (picked > kPicked) {
       if (threadIdx.x < kBins) {
-        l.radix[threadIdx.x] = 0;
+        l.radix[threadIdx.x] = l.radix_low[threadIdx.x] = 0;
         l.step_count[threadIdx.x] = 0;
       }
       if (threadIdx.x == 0) {
@@ -749,12 +772,12 @@ template <typename T, bool PACKETS> struct RowWork {
         const unsigned long long e = l.list[i];
         if (e < from || e > to) continue;
         const int step = static_cast<int>((e - from) >> shift);
-        atomicAdd(&l.radix[step], static_cast<unsigned long long>(w.exact(logit(e)) * kUnit + 0.5));
+        add(step, w.exact(logit(e)));
         atomicAdd(&l.step_count[step], 1u);
       }
       __syncthreads();
       if (threadIdx.x < kBins) {
-        l.steps[threadIdx.x] = static_cast<double>(l.radix[threadIdx.x]) / kUnit;
+        l.steps[threadIdx.x] = Fixed::value(l.radix[threadIdx.x], l.radix_low[threadIdx.x]);
         l.ranks[threadIdx.x] = l.step_count[threadIdx.x];
       }
       __syncthreads();
@@ -810,47 +833,44 @@ template <typename T, bool PACKETS> struct RowWork {
   // As threshold, digit by digit over all tokens that are kept so far.
   __device__ __forceinline__ Kept by_digits(double need, bool by_count, const Kept& within) {
     uint32_t prefix = 0, mask = 0;
-    uint64_t before = 0;
-    const double unit = by_count ? 1. : kUnit;
-    const uint64_t want = max(uint64_t{1}, static_cast<uint64_t>(ceil(need * unit)));
+    double before = 0.;
 #pragma unroll 1
     for (int shift = 24; shift >= 0; shift -= 8) {
-      if (threadIdx.x < 256) l.radix[threadIdx.x] = 0;
+      if (threadIdx.x < 256) l.radix[threadIdx.x] = l.radix_low[threadIdx.x] = 0;
       __syncthreads();
       each_block([&](float top) { return key_of(top) >= max(within.edge, prefix); }, [&](const auto& b, const float (&x)[8], int) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const uint32_t k = key_of(x[e]);
           if (!within.has(x[e], b.index(e)) || (k & mask) != prefix) continue;
-          atomicAdd(&l.radix[k >> shift & 255],
-                    by_count ? 1ull : static_cast<unsigned long long>(w.exact(x[e]) * kUnit + 0.5));
+          if (by_count) atomicAdd(&l.radix[k >> shift & 255], 1ull);
+          else add(k >> shift & 255, w.exact(x[e]));
         }
       });
       __syncthreads();
       if (threadIdx.x == 0) {
-        uint64_t sum = before;
+        double sum = before, ahead = before;  // ahead: of the digits above the lowest so far
         int lowest = 0;
-        bool found = false;
 #pragma unroll 1
-        for (int i = 255; i >= 0 && !found; --i) {
-          if (l.radix[i] == 0) continue;
+        for (int i = 255; i >= 0; --i) {
+          if (l.radix[i] == 0 && l.radix_low[i] == 0) continue;
           lowest = i;
-          if (sum + l.radix[i] >= want) found = true;
-          else sum += l.radix[i];
+          ahead = sum;
+          sum += by_count ? static_cast<double>(l.radix[i]) : Fixed::value(l.radix[i], l.radix_low[i]);
+          if (sum >= need) break;  // without one, the last
         }
-        if (!found) sum -= l.radix[lowest];  // fewer than wanted: the last
         l.digit = lowest;
-        l.upto = sum;
+        l.chosen = ahead;
       }
       __syncthreads();
       prefix |= l.digit << shift;
       mask |= 255u << shift;
-      before = l.upto;
+      before = l.chosen;
       __syncthreads();
     }
     // of the tokens equal to it, in order, as many as are needed
     const double each = by_count ? 1. : w.exact(value_of(prefix));
-    const double left = need - static_cast<double>(before) / unit;
+    const double left = need - before;
     const int ties = each > 0. ? max(1, static_cast<int>(fmin(ceil(left / each), 1e9))) : 1;
     if (threadIdx.x == 0) l.last = -1;
     __syncthreads();
@@ -995,13 +1015,13 @@ template <typename T, bool PACKETS> __global__ __launch_bounds__(kRowThreads) vo
   if (known) {
     if (listed[0] != at_bin[0] || listed[1] != at_bin[1]) work.look(at_bin[0], at_bin[1]);  // it held them
     // what is kept of each part: its bins above the list's, and of the list
-    if (threadIdx.x < 256) l.radix[threadIdx.x] = 0;
+    if (threadIdx.x < 256) l.radix[threadIdx.x] = l.radix_low[threadIdx.x] = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < l.count; i += kRowThreads) {
       const int token = static_cast<int>(l.list[i]);
       const uint32_t key = ~static_cast<uint32_t>(l.list[i] >> 32);
       if (key > kept.edge || (key == kept.edge && token <= kept.last))
-        atomicAdd(&l.radix[token / kPart], static_cast<unsigned long long>(w.exact(work.logit(l.list[i])) * kUnit + 0.5));
+        work.add(token / kPart, w.exact(work.logit(l.list[i])));
     }
     constexpr int AT_ONCE = 4;
 #pragma unroll 1
@@ -1026,7 +1046,7 @@ template <typename T, bool PACKETS> __global__ __launch_bounds__(kRowThreads) vo
     }
     __syncthreads();
     const double v = static_cast<int>(threadIdx.x) < a.parts
-                         ? l.weight[threadIdx.x] + static_cast<double>(l.radix[threadIdx.x]) / kUnit : 0.;
+                         ? l.weight[threadIdx.x] + Fixed::value(l.radix[threadIdx.x], l.radix_low[threadIdx.x]) : 0.;
     double all;
     const double upto = block_scan(v, l.parts, &all), goal = u * all;
     if (threadIdx.x == 0) found[0] = 0x7fffffff, found[1] = -1;

@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+from shared_oracle import sample
 from test_sampling import TYPES, _check, _logits
 
 pytestmark = pytest.mark.gpu
@@ -28,3 +29,43 @@ def test_infinite_temperature_and_infinite_logits(pkg, cuda, kind, vocab):
         _check(pkg, cuda, x, u, temperature=math.inf, **settings)
         mixed = torch.tensor([math.inf, 1.0, math.inf, math.inf, 0.5, 0.0])
         _check(pkg, cuda, x, u, temperature=mixed, **settings)
+
+
+@pytest.mark.parametrize("kind", ["fp16", "fp32"])
+def test_light_tokens_in_earlier_parts(pkg, cuda, kind):
+    """Weights of 2^-58 of the largest, kept by top-k and before it: random numbers of 0 and 2^-100 draw the first of them."""
+    x = torch.full((3, 9000), -200.0)
+    x[:, 8500:8510] = torch.linspace(7.0, 8.0, 10)
+    x[:, 5] = 4.0
+    x[:, 4097] = 4.125
+    x[:, 6000:6025] = 3.875
+    x = x.to(TYPES[kind])
+    u = torch.tensor([0.0, 2.0 ** -100, 2.0 ** -57])
+    for settings in (dict(top_k=20), dict(top_k=12), dict(top_k=300)):
+        tokens, logs = pkg.sample_tokens(x.to(cuda), u.to(cuda), temperature=0.1, return_logprobs=True, **settings)
+        # borders are 2^-58 of the total apart, and at least a tenth of that from these numbers
+        want = [sample(x[r], u[r].item(), temperature=0.1, **settings)[:2] for r in range(3)]
+        assert [w[0] for w in want] == [5, 5, 4097] and tokens.tolist() == [5, 5, 4097]
+        assert all(abs(float(got) - w[1]) <= abs(w[1]) * 2.0 ** -24 * 1.0001 + 2.0 ** -40 for got, w in zip(logs, want))
+
+
+def _tail(count, units, vocab, seed):
+    """One logit of 0 and `count` light ones, whose weights are units[0] to units[1] times 2^-43."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.full((1, vocab), -math.inf)
+    at = torch.randperm(vocab, generator=g)[:count + 1]
+    x[0, at[0]] = 0.0
+    w = (units[0] + (units[1] - units[0]) * torch.rand((count,), generator=g).double()) * 2.0 ** -43
+    x[0, at[1:]] = torch.log(w).float()
+    return x
+
+
+@pytest.mark.parametrize("count,units,vocab,top_p,u,seed", [
+    (8000, (512.40, 512.49), 12000, 1 - 2.0 ** -24, 1 - 2.0 ** -24, 2),  # a list of them
+    (8000, (512.40, 512.49), 12000, 1 - 2.0 ** -24, 1 - 2.0 ** -23, 2),
+    (40000, (50.40, 50.49), 50001, 1 - 2.0 ** -23, 1 - 2.0 ** -24, 1),   # more than a list holds
+    (40000, (50.40, 50.49), 50001, 1 - 2.0 ** -23, 1 - 2.0 ** -24, 3)])
+def test_sums_of_light_tokens(pkg, cuda, count, units, vocab, top_p, u, seed):
+    """Thresholds and draws among tokens that weigh a few times 2^-43 of the largest each: rounded to that, their sums would
+    be off by many of them."""
+    _check(pkg, cuda, _tail(count, units, vocab, seed), torch.tensor([u]), top_p=top_p)

@@ -523,14 +523,14 @@ int mi355_kv_slot_map_fwd(const mi355_kv_cache* cache, const int32_t* seq_lens, 
  *   the tokens ranked before it have less than top_p of
  *   the weight of those that top_k keeps                  (top_p >= 1: no limit)
  *   w_i >= min_p                                          (min_p <= 0: no limit)
- * (the first is always kept).  tokens[r] is the first i, in the order of the
- * vocabulary, up to which the kept weights sum to more than u times their total;
- * logprobs[r] (NULL: not wanted) the logarithm of w_i / total, as which it was
- * drawn.  temperature <= 0 (or NaN): the first token of rank 0, logarithm 0.
- * u is clamped to [0, 1 - 2^-24], NaN to 0.  -infinity and NaN have weight 0;
- * where the largest logit is +infinity, those that are have weight 1 and others
- * 0.  A row without any other logit than -infinity and NaN gets token -1 and
- * logarithm -infinity.  Weights and sums are of 64 bits.
+ * (the first is always kept, alone if min_p > 1).  tokens[r] is the first i, in
+ * the order of the vocabulary, up to which the kept weights sum to more than u
+ * times their total; logprobs[r] (NULL: not wanted) the logarithm of w_i / total,
+ * as which it was drawn.  temperature <= 0 (or NaN): the first token of rank 0,
+ * logarithm 0.  u is clamped to [0, 1 - 2^-24], NaN to 0.  -infinity and NaN have
+ * weight 0; where the largest logit is +infinity, those that are have weight 1 and
+ * others 0.  A row without any other logit than -infinity and NaN gets token -1
+ * and logarithm -infinity.  Weights and sums are of 64 bits.
  *
  *   logits      [rows, row_stride] of dtype (fp32, fp16, bf16), vocab elements
  *               of each row contiguous, any alignment.  vocab < 2^20.

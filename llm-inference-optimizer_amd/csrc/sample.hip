@@ -81,6 +81,10 @@ struct Settings {
     top_k = a.top_k ? a.top_k[row] : a.top_k_all;
     top_p = a.top_p ? a.top_p[row] : a.top_p_all;
     min_p = a.min_p ? a.min_p[row] : a.min_p_all;
+    if (min_p > 1.f) {  // no token weighs that much: the first of rank 0 alone
+      top_k = 1;
+      min_p = 0.f;
+    }
     greedy = !(heat > 0.f);
     c = 1.4426950408889634074 / static_cast<double>(heat);
     by_count = !greedy && top_k > 0 && top_k < a.vocab;
@@ -901,7 +905,7 @@ template <typename T, bool PACKETS> struct RowWork {
       for (int e = 0; e < 8; ++e) {
         if (!kept.has(x[e], b.index(e))) continue;
         const double v = w.exact(x[e]);
-        if (v >= least || x[e] == w.top32) sum += v;
+        if (v >= least) sum += v;
       }
       sum = wave_sum(sum);
       if ((threadIdx.x & 63) == 0) l.weight[number] = sum;
@@ -1083,7 +1087,7 @@ template <typename T, bool PACKETS> __global__ __launch_bounds__(kRowThreads) vo
     const float x = fmaxf(load_elem<T>(a.logits, row * a.stride + i), -INFINITY);
     if (kept.has(x, i)) {
       v = w.exact(x);
-      if (v < least && x != w.top32) v = 0.;
+      if (v < least) v = 0.;
     }
   }
   __syncthreads();

@@ -69,3 +69,17 @@ def test_sums_of_light_tokens(pkg, cuda, count, units, vocab, top_p, u, seed):
     """Thresholds and draws among tokens that weigh a few times 2^-43 of the largest each: rounded to that, their sums would
     be off by many of them."""
     _check(pkg, cuda, _tail(count, units, vocab, seed), torch.tensor([u]), top_p=top_p)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_least_weights_above_the_largest(pkg, cuda, kind):
+    """A min-p above 1 keeps the first of the largest logits alone, as a top-k of 1 does."""
+    x, u = _logits(6, 9000, TYPES[kind], 97)
+    x[:, [100, 5000, 8999]] = 50.0
+    x[4, [7, 70]] = math.inf
+    x[5] = 2.0
+    u[:] = 0.999
+    least = torch.tensor([1.0, 1.0000001, 1.5, math.inf, 2.0, 3.0])
+    for settings in (dict(), dict(top_k=2), dict(top_p=0.9), dict(temperature=math.inf), dict(temperature=0.3, top_k=500, top_p=0.5)):
+        tokens = _check(pkg, cuda, x, u, min_p=least, **settings)
+        assert tokens[1:].tolist() == [100, 100, 100, 7, 0]

@@ -330,15 +330,6 @@ __device__ __forceinline__ double block_scan(double v, double* parts, double* al
   *all = total;
   return before + v;
 }
-__device__ __forceinline__ double block_sum(double v, double* parts) {
-  v = wave_sum(v);
-  if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = v;
-  __syncthreads();
-  double sum = 0.;
-  for (int w = 0; w < kRowWaves; ++w) sum += parts[w];
-  __syncthreads();
-  return sum;
-}
 
 // What a row's workgroup begins with: thread t's part and the row's largest logit.
 struct RowStart {
@@ -935,7 +926,6 @@ template <typename T, bool PACKETS> __global__ __launch_bounds__(kRowThreads) vo
   double total;
   if (draw_plain<T>(a, s, start, w, r, row, u, found, l.parts, &l.chosen, &total)) return;
   const int blocks = (a.vocab + kBlock - 1) / kBlock;
-  const Part* part = a.part + r * a.parts;
   RowWork<T, PACKETS> work{a, l, s, w, row, a.block_top + r * a.parts * kPartBlocks, blocks, s.bin(start.top)};
 
   if (start.mine.sum > 0.) {

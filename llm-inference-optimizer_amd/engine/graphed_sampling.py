@@ -38,10 +38,10 @@ class GraphedSamplingDecoder:
     ``kv_cache``: "16bit", "int8" or "e4m3", in pages of ``page_size`` slots.  ``pages``: how many the pool holds; a
     generation of ``new`` tokens takes ``pages_needed(prompt length, new)`` of them, far fewer than the default, which
     is enough for sequences of ``max_cache_len`` tokens that share nothing.  ``temperature``, ``top_k``, ``top_p`` and
-    ``min_p`` as in ``sample_tokens``: numbers, or tensors that broadcast to [batch_size, samples].  ``share_prefix``:
-    whether attention reads a prompt once for all of its continuations (``shared_prefix_attention``) or for each
-    (``tree_attention``); None: whichever is faster at the prompt's length.  ``use_graph=False`` runs the same step
-    eagerly."""
+    ``min_p`` as in ``sample_tokens``: numbers, or tensors that broadcast to [batch_size, samples], which are copied.
+    ``share_prefix``: whether attention reads a prompt once for all of its continuations (``shared_prefix_attention``)
+    or for each (``tree_attention``); None: whichever is faster at the prompt's length.  ``use_graph=False`` runs the
+    same step eagerly."""
 
     def __init__(self, model, batch_size: int, samples: int, max_cache_len: int, *, kv_cache: str = "16bit",
                  page_size: int = 64, pages: int | None = None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
@@ -77,7 +77,8 @@ class GraphedSamplingDecoder:
     def _per_row(self, value, dtype):
         if not torch.is_tensor(value):
             return value
-        return value.to(device=self.device, dtype=dtype).expand(self.batch_size, self.samples).contiguous().view(-1)
+        own = torch.empty((self.batch_size, self.samples), dtype=dtype, device=self.device)
+        return own.copy_(value.detach().expand_as(own)).view(-1)
 
     def pages_needed(self, prompt_len: int, new_tokens: int) -> int:
         """Pages of a generation: the prompts', and what each continuation has for itself."""

@@ -1,0 +1,25 @@
+"""What GraphedSamplingDecoder does with the settings that it is given, and with logits that leave nothing to draw."""
+
+import pytest
+import torch
+from test_sampling_decode import _model, _prompt
+
+pytest.importorskip("transformers")
+
+
+@pytest.mark.gpu
+def test_settings_are_the_decoder_s_own(pkg, cuda):
+    """Tensors that already have the step's shape and type are copied: writing to them later changes nothing."""
+    model = _model(cuda)
+    pkg.patch_model_with_fused_kernels(model, fuse_attention=True)
+    given = dict(temperature=torch.full((2, 3), 0.7, device=cuda), top_k=torch.full((2, 3), 40, dtype=torch.int32, device=cuda),
+                 top_p=torch.full((2, 3), 0.95, device=cuda), min_p=torch.full((2, 3), 0.01, device=cuda))
+    dec = pkg.GraphedSamplingDecoder(model, 2, 3, 64, page_size=16, **given)
+    ids = _prompt(cuda, 2, 20)
+    u = torch.rand((2, 3, 20), generator=torch.Generator().manual_seed(7))
+    want = dec.generate(ids, 20, uniform=u)
+    given["temperature"].fill_(0.0)
+    given["top_k"].fill_(1)
+    given["top_p"].fill_(0.0)
+    given["min_p"].fill_(1.0)
+    assert torch.equal(dec.generate(ids, 20, uniform=u), want)

@@ -78,6 +78,8 @@ class GraphedSamplingDecoder:
         if not torch.is_tensor(value):
             return value
         own = torch.empty((self.batch_size, self.samples), dtype=dtype, device=self.device)
+        if dtype == torch.int32 and value.dtype == torch.int64:  # in 32 bits 2^32 + 1 would be another limit
+            value = value.clamp(0, 2 ** 31 - 1)
         return own.copy_(value.detach().expand_as(own)).view(-1)
 
     def pages_needed(self, prompt_len: int, new_tokens: int) -> int:

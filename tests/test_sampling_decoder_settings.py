@@ -1,5 +1,4 @@
 """What GraphedSamplingDecoder does with the settings that it is given, and with logits that leave nothing to draw."""
-
 import pytest
 import torch
 from test_sampling_decode import _model, _prompt
@@ -23,3 +22,14 @@ def test_settings_are_the_decoder_s_own(pkg, cuda):
     given["top_p"].fill_(0.0)
     given["min_p"].fill_(1.0)
     assert torch.equal(dec.generate(ids, 20, uniform=u), want)
+
+
+@pytest.mark.gpu
+def test_limits_beyond_32_bits_are_none(pkg, cuda):
+    model = _model(cuda)
+    pkg.patch_model_with_fused_kernels(model, fuse_attention=True)
+    ids = _prompt(cuda, 1, 20)
+    u = torch.rand((1, 3, 10), generator=torch.Generator().manual_seed(9))
+    out = [pkg.GraphedSamplingDecoder(model, 1, 3, 64, page_size=16, top_k=torch.tensor(k)).generate(ids, 10, uniform=u)
+           for k in (0, 2 ** 32 + 1, -2 ** 32 + 1, 2 ** 31)]
+    assert all(torch.equal(o, out[0]) for o in out)

@@ -18,7 +18,7 @@ import torch
 
 from ..kernels.kv_cache_hip import KVCache
 from ..kernels.kv_pages_hip import kv_cache_reserve, kv_slot_map
-from ..kernels.sampling_hip import sample_tokens
+from ..kernels.sampling_hip import sample_tokens, sampling_settings
 from .cached_attention import DecoderCache
 
 __all__ = ["GraphedSamplingDecoder"]
@@ -48,6 +48,7 @@ class GraphedSamplingDecoder:
                  share_prefix: bool | None = None, use_graph: bool = True):
         if batch_size < 1 or samples < 1:
             raise ValueError(f"batch_size and samples must be at least 1, got {batch_size} and {samples}")
+        sampling_settings(temperature, top_k, top_p, min_p)
         self.model = model
         self.device = next(model.parameters()).device
         self.batch_size, self.samples, self.max_cache_len = batch_size, samples, max_cache_len

@@ -21,6 +21,15 @@ def _setting(name: str, value, low: float, high: float):
     return None, value
 
 
+def sampling_settings(temperature, top_k, top_p, min_p):
+    """The four as ``_setting`` has them; ValueError for a number that ``sample_tokens`` does not take."""
+    heat = _setting("temperature", temperature, 0.0, math.inf)
+    k = _setting("top_k", top_k, 0, 2 ** 31 - 1)
+    if int(k[1]) != k[1]:
+        raise ValueError(f"top_k must be a whole number, got {top_k!r}")
+    return heat, k, _setting("top_p", top_p, 0.0, 1.0), _setting("min_p", min_p, 0.0, 1.0)
+
+
 def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: float | torch.Tensor = 1.0,
                   top_k: int | torch.Tensor = 0, top_p: float | torch.Tensor = 1.0, min_p: float | torch.Tensor = 0.0,
                   return_logprobs: bool = False):
@@ -39,12 +48,7 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: f
     vocabulary, at which their cumulated probability exceeds ``uniform``.  A temperature of 0 takes the first of the
     largest logits.  Probabilities and their sums are held in 64 bits.  -infinity and NaN are never drawn; a row of
     nothing else gets -1 (and a logarithm of -infinity)."""
-    heat, heat_all = _setting("temperature", temperature, 0.0, math.inf)
-    if not torch.is_tensor(top_k) and int(top_k) != top_k:
-        raise ValueError(f"top_k must be a whole number, got {top_k!r}")
-    k, k_all = _setting("top_k", top_k, 0, 2 ** 31 - 1)
-    p, p_all = _setting("top_p", top_p, 0.0, 1.0)
-    least, least_all = _setting("min_p", min_p, 0.0, 1.0)
+    (heat, heat_all), (k, k_all), (p, p_all), (least, least_all) = sampling_settings(temperature, top_k, top_p, min_p)
     tokens, logs = _lib.ext().sample(logits, uniform, heat, heat_all, k, int(k_all), p, p_all, least, least_all,
                                      return_logprobs)
     return (tokens, logs) if return_logprobs else tokens

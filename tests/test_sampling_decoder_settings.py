@@ -1,9 +1,19 @@
 """What GraphedSamplingDecoder does with the settings that it is given, and with logits that leave nothing to draw."""
+import math
+
 import pytest
 import torch
 from test_sampling_decode import _model, _prompt
 
 pytest.importorskip("transformers")
+
+
+@pytest.mark.parametrize("settings", [dict(temperature=-0.1), dict(temperature=math.nan), dict(top_k=-1), dict(top_k=1.5),
+                                      dict(top_k=math.inf), dict(top_p=1.01), dict(top_p=math.nan), dict(min_p=-0.1),
+                                      dict(min_p=None)], ids=str)
+def test_numbers_are_checked_before_anything_else(pkg, settings):
+    with pytest.raises(ValueError, match=next(iter(settings))):
+        pkg.GraphedSamplingDecoder(None, 1, 2, 64, **settings)
 
 
 @pytest.mark.gpu

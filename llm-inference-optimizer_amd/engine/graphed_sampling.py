@@ -69,6 +69,7 @@ class GraphedSamplingDecoder:
         self._past, self._prompt_past = self.cache.as_past(), self.prompt_cache.as_past()
         self._one = torch.ones((rows,), dtype=torch.int32, device=self.device)
         self._missing = torch.zeros((rows,), dtype=torch.int32, device=self.device)
+        self._drawn = torch.zeros((rows,), dtype=torch.long, device=self.device)  # below 0: a draw gave no token
         self._tok = torch.zeros((rows, 1), dtype=torch.long, device=self.device)
         self._pos = torch.zeros((rows, 1), dtype=torch.long, device=self.device)
         self._uniform = torch.zeros((rows,), dtype=torch.float32, device=self.device)
@@ -99,7 +100,8 @@ class GraphedSamplingDecoder:
     def _sample(self, logits: torch.Tensor) -> None:
         """Draws the rows' next tokens into the step's inputs."""
         tokens, logs = sample_tokens(logits, self._uniform, return_logprobs=True, **self.settings)
-        self._tok.copy_(tokens.clamp_(min=0).unsqueeze(1))  # logits that are all NaN: no token
+        torch.minimum(self._drawn, tokens, out=self._drawn)  # -1 where all logits are NaN: generate tells it
+        self._tok.copy_(tokens.clamp_(min=0).unsqueeze(1))
         self._log.copy_(logs)
 
     def _step(self) -> None:
@@ -112,7 +114,7 @@ class GraphedSamplingDecoder:
         self._sample(out.logits[:, -1])
 
     def _capture(self) -> None:
-        state = (self.cache.lens, self._pos, self._tok, self._log, self._missing, self.table)
+        state = (self.cache.lens, self._pos, self._tok, self._log, self._missing, self._drawn, self.table)
         held = [t.clone() for t in state]
         side = torch.cuda.Stream(device=self.device)
         side.wait_stream(torch.cuda.current_stream(self.device))
@@ -133,6 +135,7 @@ class GraphedSamplingDecoder:
         self.table.fill_(-1)
         c.lens.zero_()
         self._missing.zero_()
+        self._drawn.zero_()
         new = torch.zeros((n, m), dtype=torch.int32, device=self.device)
         new[:, 0] = length
         kv_cache_reserve(c.layers[0], c.lens, new.view(-1))
@@ -168,7 +171,8 @@ class GraphedSamplingDecoder:
                  generator: torch.Generator | None = None, return_logprobs: bool = False):
         """input_ids [batch_size, length] -> [batch_size, samples, length + max_new_tokens]; with ``return_logprobs``
         also the logarithm of the probability that each new token was drawn with.  ``uniform``: the random numbers
-        (float32 [batch_size, samples, max_new_tokens]); without it ``torch.rand``'s, from ``generator``."""
+        (float32 [batch_size, samples, max_new_tokens]); without it ``torch.rand``'s, from ``generator``.  RuntimeError
+        if a row's logits were all NaN or -infinity, so that there was no token to draw."""
         n, length = input_ids.shape
         m, rows = self.samples, self.batch_size * self.samples
         if n != self.batch_size:
@@ -203,5 +207,7 @@ class GraphedSamplingDecoder:
             logs[:, i] = self._log
         if bool((self._missing > 0).any()):
             raise RuntimeError("the cache's pool ran out of pages")
+        if bool((self._drawn < 0).any()):
+            raise RuntimeError("a row's logits left no token to draw: they were all NaN or -infinity")
         ids = torch.cat((input_ids.unsqueeze(1).expand(n, m, length), out.view(shape)), 2)
         return (ids, logs.view(shape)) if return_logprobs else ids

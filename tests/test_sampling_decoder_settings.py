@@ -43,3 +43,23 @@ def test_limits_beyond_32_bits_are_none(pkg, cuda):
     out = [pkg.GraphedSamplingDecoder(model, 1, 3, 64, page_size=16, top_k=torch.tensor(k)).generate(ids, 10, uniform=u)
            for k in (0, 2 ** 32 + 1, -2 ** 32 + 1, 2 ** 31)]
     assert all(torch.equal(o, out[0]) for o in out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("use_graph", [True, False])
+def test_nothing_to_draw(pkg, cuda, use_graph):
+    """Logits that are all NaN end a generation with an error, not with tokens; the next generation is as before."""
+    model = _model(cuda)
+    pkg.patch_model_with_fused_kernels(model, fuse_attention=True)
+    dec = pkg.GraphedSamplingDecoder(model, 2, 3, 64, page_size=16, use_graph=use_graph)
+    ids = _prompt(cuda, 2, 20)
+    u = torch.rand((2, 3, 8), generator=torch.Generator().manual_seed(3))
+    want = dec.generate(ids, 8, uniform=u)
+    with torch.no_grad():
+        held = model.model.norm.weight.clone()
+        model.model.norm.weight.fill_(math.nan)
+        for new in (1, 8):
+            with pytest.raises(RuntimeError, match="draw"):
+                dec.generate(ids, new, uniform=u[:, :, :new])
+        model.model.norm.weight.copy_(held)
+    assert torch.equal(dec.generate(ids, 8, uniform=u), want)

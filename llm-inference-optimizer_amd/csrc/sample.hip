@@ -25,10 +25,19 @@
 // us, 3.9 TB/s) and by the weights' 64-bit arithmetic and the bins' atomics with them
 // (64 rows of bf16: 20 us).  A row's workgroup is bound by trips of loads that wait
 // for each other, some 1.5 us each: settings and parts 2 us, bins 4, the list 4 for
-// a sharp row and 17 for a flat one, narrowing it 5 a step, kept parts 5, the
-// drawing 3: 25 us for one row of 151936 with top-k and top-p, 55 for 64 rows of a
-// nucleus, sharp and flat, 37 for 256 rows of 32000 with settings of their own, 18
+// a sharp row and 17 for a flat one, narrowing it 5 to 7 a step, kept parts 5, the
+// drawing 3: 25 us for one row of 151936 with top-k and top-p, 60 for 64 rows of a
+// nucleus, sharp and flat, 39 for 256 rows of 32000 with settings of their own, 18
 // for 512 without filters.
+//
+// Not every threshold is in a bin that is short enough to list: at low temperatures,
+// and where a mask leaves fewer tokens than top-k, the last one kept is in the last
+// bin; flat rows have more than 8192 tokens in one.  Then the row's workgroup goes
+// over the row for every digit of the threshold (by_digits) and a wave over it for
+// the equal logits, which is slower than all else here by a factor of 10 to 40.
+// One row of 151936 bf16, and 64 of them, us: top-k 50 at temperature 0.1 654, 870
+// (with top-p 937, 1420); top-p 0.9 at temperature 2 902, 1117; 5 tokens left and
+// top-k 20 640, 903.
 #include "common.h"
 #include "sample_bins.h"
 

@@ -47,7 +47,11 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: f
     with probabilities after dividing the logits by ``temperature``; the token is the first, in the order of the
     vocabulary, at which their cumulated probability exceeds ``uniform``.  A temperature of 0 takes the first of the
     largest logits.  Probabilities and their sums are held in 64 bits.  -infinity and NaN are never drawn; a row of
-    nothing else gets -1 (and a logarithm of -infinity)."""
+    nothing else gets -1 (and a logarithm of -infinity).
+
+    Rows of 151936 take 30 to 90 us, but about a millisecond where the last token that ``top_k`` keeps has less than
+    2^-63 of the largest's probability (low temperatures, masks that leave fewer tokens), or a limit of many tokens
+    falls into a flat part of the row (high temperatures, a ``top_p`` near 1)."""
     (heat, heat_all), (k, k_all), (p, p_all), (least, least_all) = sampling_settings(temperature, top_k, top_p, min_p)
     tokens, logs = _lib.ext().sample(logits, uniform, heat, heat_all, k, int(k_all), p, p_all, least, least_all,
                                      return_logprobs)
